@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("NA2D_LIB", os.path.join(_PKG_DIR, "libna2d.so"))
 
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 PATH_AUTO, PATH_SIMT, PATH_TENSOR = 0, 1, 2
+ACT_NONE, ACT_SILU = 0, 1
 
 ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_WINDOW, ERR_CUDA = -1, -2, -3, -4
 ERR_NO_DEVICE, ERR_TOO_LARGE, ERR_KERNEL_WAIT = -5, -6, -7
@@ -43,6 +44,41 @@ class Args(C.Structure):
                 ("d_o", TensorDesc), ("d_q", TensorDesc), ("d_k", TensorDesc), ("d_v", TensorDesc),
                 ("lse", C.c_void_p), ("delta", C.c_void_p),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class Heads(C.Structure):
+    """Mirror of ``na2d_heads``: a (B, heads, T, C) operand."""
+    _fields_ = [("ptr", C.c_void_p), ("stride_b", C.c_int64), ("stride_n", C.c_int64), ("stride_t", C.c_int64)]
+
+
+class AttentionArgs(C.Structure):
+    """Mirror of ``na2d_attention_args``."""
+    _fields_ = [("struct_size", C.c_size_t), *[(n, C.c_int) for n in ("B", "N", "Nk", "Tq", "Tk", "C", "dtype", "path", "device", "causal")],
+                ("scale", C.c_float), ("stream", C.c_void_p),
+                *[(n, Heads) for n in ("q", "k", "v", "o", "d_o", "d_q", "d_k", "d_v")],
+                ("key_lengths", C.c_void_p), ("lse", C.c_void_p), ("delta", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class Pixels(C.Structure):
+    """Mirror of ``na2d_pixels``: a (B, P, C) map."""
+    _fields_ = [("ptr", C.c_void_p), ("stride_b", C.c_int64), ("stride_p", C.c_int64)]
+
+
+class NormArgs(C.Structure):
+    """Mirror of ``na2d_norm_args``."""
+    _fields_ = [("struct_size", C.c_size_t), *[(n, C.c_int) for n in ("B", "C", "groups", "dtype", "param_dtype", "activation", "device")],
+                ("eps", C.c_float), ("P", C.c_int64), ("stream", C.c_void_p), ("x", Pixels), ("d_y", Pixels),
+                *[(n, C.c_void_p) for n in ("y", "d_x", "weight", "bias", "d_weight", "d_bias", "mean", "rstd", "workspace")],
+                ("workspace_bytes", C.c_size_t)]
+
+
+class RotaryArgs(C.Structure):
+    """Mirror of ``na2d_rotary_args``."""
+    _fields_ = [("struct_size", C.c_size_t),
+                *[(n, C.c_int) for n in ("B", "N", "Nk", "T", "C", "dims", "dtype", "interleaved", "inverse", "index_64", "device")],
+                ("stream", C.c_void_p), ("q", Heads), ("k", Heads), ("out_q", C.c_void_p), ("out_k", C.c_void_p),
+                ("table", C.c_void_p), ("table_rows", C.c_int64), ("index", C.c_void_p)]
 
 
 OP_2D, OP_1D = 0, 1
@@ -79,6 +115,14 @@ SIGNATURES = {
     "na2d_qk_backward": (C.c_int, [C.c_void_p] * 5 + _PAIR),
     "na2d_av_forward": (C.c_int, [C.c_void_p] * 3 + _PAIR),
     "na2d_av_backward": (C.c_int, [C.c_void_p] * 5 + _PAIR),
+    "na2d_attention_forward": (C.c_int, [C.POINTER(AttentionArgs)]),
+    "na2d_attention_backward": (C.c_int, [C.POINTER(AttentionArgs)]),
+    "na2d_attention_workspace": (C.c_size_t, [C.POINTER(AttentionArgs), C.c_int]),
+    "na2d_group_norm_forward": (C.c_int, [C.POINTER(NormArgs)]),
+    "na2d_group_norm_backward": (C.c_int, [C.POINTER(NormArgs)]),
+    "na2d_group_norm_workspace": (C.c_size_t, [C.POINTER(NormArgs), C.c_int]),
+    "na2d_rotary": (C.c_int, [C.POINTER(RotaryArgs)]),
+    "na2d_rotary_table": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_double, C.c_void_p, C.c_int, C.c_void_p]),
     "na2d_check": (C.c_int, [C.c_int, C.c_void_p]),
     "na2d_poll": (C.c_int, [C.c_int, C.c_void_p]),
     "na2d_selftest_wait_timeout": (C.c_int, [C.c_int, C.c_void_p, C.c_uint]),
@@ -111,6 +155,9 @@ def _load_torch_ext():
     from . import _na2d_torch
     _na2d_torch.bind_abi(*(C.cast(fn, C.c_void_p).value
                            for fn in (lib.na2d_forward_ex, lib.na2d_backward_ex, lib.na2d_backward_workspace, lib.na2d_poll)))
+    _na2d_torch.bind_block_abi(*(C.cast(fn, C.c_void_p).value for fn in (
+        lib.na2d_attention_forward, lib.na2d_attention_backward, lib.na2d_attention_workspace, lib.na2d_group_norm_forward,
+        lib.na2d_group_norm_backward, lib.na2d_group_norm_workspace, lib.na2d_rotary, lib.na2d_poll)))
     return _na2d_torch
 
 

@@ -3,9 +3,10 @@
     python e_natten_b200/build.py [--force] [--verbose]
 
 The library is plain CUDA C++ behind a C ABI (include/na2d.h); it needs no framework headers.
-Its kernels are compiled as eleven translation units in parallel (the API with the SIMT kernels, the
-tiled CUDA-core kernels once per element type, the fp32 box kernels, and each of the three tcgen05 kernel families once per
-16-bit element type) and linked into one shared object.  The Python package's extension module
+Its kernels are compiled as seventeen translation units in parallel (the API with the SIMT kernels, the
+tiled CUDA-core kernels once per element type, the fp32 box kernels, each of the three tcgen05 kernel families once per
+16-bit element type, attention over all keys on tensor cores once per 16-bit type, on CUDA cores and its entry points, group norm and
+rotary positions) and linked into one shared object.  The Python package's extension module
 (_na2d_torch.so, host code over PyTorch's C++ API) is compiled beside it with g++; it belongs to one
 PyTorch and one Python version and is compiled again when either changes.
 """
@@ -37,6 +38,12 @@ UNITS = [
     ("na2d_tc_dq.cu", ["-DNA2D_TC_DT=2"], "na2d_tc_dq_f16.o"),
     ("na2d_tc_dkdv.cu", ["-DNA2D_TC_DT=1"], "na2d_tc_dkdv_bf16.o"),
     ("na2d_tc_dkdv.cu", ["-DNA2D_TC_DT=2"], "na2d_tc_dkdv_f16.o"),
+    ("na2d_attn_tc.cu", ["-DNA2D_TC_DT=1"], "na2d_attn_tc_bf16.o"),
+    ("na2d_attn_tc.cu", ["-DNA2D_TC_DT=2"], "na2d_attn_tc_f16.o"),
+    ("na2d_attn_simt.cu", [], "na2d_attn_simt.o"),
+    ("na2d_attn_api.cu", [], "na2d_attn_api.o"),
+    ("na2d_norm.cu", [], "na2d_norm.o"),
+    ("na2d_rotary.cu", [], "na2d_rotary.o"),
 ]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 
@@ -48,12 +55,14 @@ def _nvcc() -> str:
     return exe
 
 
-EXT_SOURCE = "na2d_torch.cpp"
+EXT_SOURCES = ("na2d_torch.cpp", "na2d_torch_block.cpp")
+EXT_HEADERS = ("na2d_torch.h",)
 
 
 def _deps(ext: bool):
     """Sources of the extension module, or of the library."""
-    names = [EXT_SOURCE] if ext else [f for f in os.listdir(CSRC) if f != EXT_SOURCE]
+    own = EXT_SOURCES + EXT_HEADERS
+    names = own if ext else [f for f in os.listdir(CSRC) if f not in own]
     deps = [os.path.join(CSRC, f) for f in names]
     deps.append(os.path.join(os.path.dirname(PKG_DIR), "include", "na2d.h"))
     return [d for d in deps if os.path.isfile(d)]
@@ -91,14 +100,20 @@ def _compile_torch_ext():
     """The Python extension module over PyTorch's C++ API (host code only)."""
     import torch
     from torch.utils import cpp_extension
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DNA2D_EXT_TAG="{_ext_tag()}"',
-           *[f"-isystem{p}" for p in (*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"])],
-           os.path.join(CSRC, EXT_SOURCE), "-o", EXT_PATH,
-           *[f"-L{p}" for p in cpp_extension.library_paths("cuda")],
-           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    return os.path.basename(EXT_PATH), proc.returncode, proc.stdout + proc.stderr, " ".join(cmd)
+    compiler = shutil.which("g++") or "g++"
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DNA2D_EXT_TAG="{_ext_tag()}"',
+             *[f"-isystem{p}" for p in (*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"])]]
+    objects = [os.path.join(OBJ_DIR, os.path.splitext(source)[0] + ".o") for source in EXT_SOURCES]
+    commands = [[compiler, *flags, "-c", os.path.join(CSRC, source), "-o", obj] for source, obj in zip(EXT_SOURCES, objects)]
+    with concurrent.futures.ThreadPoolExecutor(len(commands)) as pool:
+        done = list(pool.map(lambda cmd: subprocess.run(cmd, capture_output=True, text=True), commands))
+    if all(proc.returncode == 0 for proc in done):
+        commands.append([compiler, "-shared", *objects, "-o", EXT_PATH, *[f"-L{p}" for p in cpp_extension.library_paths("cuda")],
+                         "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
+        done.append(subprocess.run(commands[-1], capture_output=True, text=True))
+    return (os.path.basename(EXT_PATH), max(proc.returncode for proc in done), "".join(proc.stdout + proc.stderr for proc in done),
+            "; ".join(" ".join(cmd) for cmd in commands))
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags=(), lib_path: str = LIB_PATH) -> str:

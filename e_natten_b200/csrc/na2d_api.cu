@@ -12,6 +12,7 @@
 
 #include "../../include/na2d.h"
 #include "na2d_delta.cuh"
+#include "na2d_host.h"
 #include "na2d_index.cuh"
 #include "na2d_simt.cuh"
 #include "na2d_tc_entry.h"
@@ -45,23 +46,7 @@ int tc_fail(const char* what) {
         if (e__ != cudaSuccess) return cuda_fail(e__, #call);  \
     } while (0)
 
-// Makes `device` current for the scope and restores the previous device afterwards.
-// cudaSetDevice is called even when `device` already is the thread's current device: a thread that
-// has made no runtime call yet (an autograd worker thread, for one) reports device 0 as current
-// without having its context bound, and the driver call that encodes tensor maps needs a bound
-// context.
-struct DeviceScope {
-    int prev = -1;
-    cudaError_t err = cudaSuccess;
-    explicit DeviceScope(int device) {
-        err = cudaGetDevice(&prev);
-        if (err == cudaSuccess) err = cudaSetDevice(device);
-    }
-    ~DeviceScope() {
-        int cur = -1;
-        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-    }
-};
+using na2d_host::DeviceScope;
 
 constexpr int kMaxDevices = 64;
 
@@ -701,14 +686,29 @@ int pair_inverse(const PairProblem& p, const void* attn, const void* x, void* ou
 
 }  // namespace
 
+namespace na2d_host {
+
+int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
+int launch_fail(const char* what) { return ::tc_fail(what); }
+int check_device(int device) { return ::check_device(device); }
+int error_state(int device, const na2d_ptx::ErrorState** out) {
+    Errors err;
+    const int rc = ::error_state(device, &err);
+    if (rc == NA2D_OK) *out = err.device;
+    return rc;
+}
+void count_launches(int n) { g_launches.fetch_add(n); }
+
+}  // namespace na2d_host
+
 extern "C" {
 
-int na2d_version(void) { return 200; }
+int na2d_version(void) { return 300; }
 
 const char* na2d_strerror(int status) {
     switch (status) {
         case NA2D_OK: return "ok";
-        case NA2D_ERR_BAD_ARG: return "bad argument (null pointer, non-positive size, even kernel size, bad scale or bad row view)";
+        case NA2D_ERR_BAD_ARG: return "bad argument (null pointer, non-positive size, even kernel size, bad scale, row view or division of heads or channels)";
         case NA2D_ERR_UNSUPPORTED: return "unsupported dtype, head dim, kernel size or tensor layout for the requested path";
         case NA2D_ERR_WINDOW: return "grid side smaller than the kernel size, or key band does not cover the query band's windows";
         case NA2D_ERR_CUDA: return "CUDA call failed (see na2d_last_cuda_error)";

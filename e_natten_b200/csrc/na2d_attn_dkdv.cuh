@@ -1,0 +1,480 @@
+// Attention over all keys, key half of the backward, on tcgen05 (bf16 / fp16, head dims up to 128).
+//
+//     S^T = K Q_c^T,  dP^T = V dO_c^T                      (tensor memory, fp32)
+//     P^T = exp(S^T - lse),  dS^T = P^T (dP^T - delta)     (softmax warps)
+//     dV += P^T dO_c,  dK += dS^T Q_c                      (P^T, dS^T from tensor memory, 16 bit)
+// over the query chunks of every head that shares the key head, accumulated in tensor memory: no atomics, and the order of the sums is
+// the same in every call.  P and dS are rounded once to 16 bits for their products.
+//
+// Persistent, one CTA per SM, one tile of 128 keys (row r of every MMA) at a time, queries in chunks of 128.  All 512 columns of
+// tensor memory are in use, S^T and dP^T having one buffer each; the two halves of a chunk's arithmetic take turns with the MMAs:
+//     softmax   P(n)         | dS(n)        | P(n+1)        | dS(n+1)
+//     tensor          dP(n)  | dV(n) S(n+1) | dK(n) dP(n+1) | dV(n+1) ...
+// Few keys and many queries: the chunks of a tile are cut into `splits` parts, whose fp32 sums go to a workspace and are added by
+// attn_sum_kernel.
+//   warps 0-7   softmax: warps w and w + 4 share 32 keys and take 64 queries each;
+//   warp 8      producer of the Q / dO chunks and of the chunks' lse and delta;  warp 11  producer of the K, V tile;
+//   warp 9      MMA issue;  warps 12-15 epilogue.
+#pragma once
+
+#include "na2d_attn_dq.cuh"
+
+namespace na2d_attn {
+
+struct KeyCut {
+    int key_tiles;
+    int splits;
+    int items;
+    float* part_dk;         // (splits, B, Nk, Tk, C), where splits > 1
+    float* part_dv;
+};
+
+// One item: chunks [first, first + n) of those that see a key tile.
+struct KeyItem {
+    int b, m, k0, count, split;
+    int lo, per_head;       // the tile's chunks: query tiles lo .. lo + per_head - 1 of each (group of) heads
+    int first, n;
+    __device__ __forceinline__ KeyItem(const Geom& g, const KeyCut& cut, int item) {
+        split = item % cut.splits;
+        const int rest = item / cut.splits;
+        // (with a causal mask the first tiles are the longer ones)
+        const int tile = g.causal ? rest / g.units : rest % cut.key_tiles, unit = g.causal ? rest % g.units : rest / cut.key_tiles;
+        b = unit / g.Nk;
+        m = unit - b * g.Nk;
+        k0 = tile * kRows;
+        count = key_count(g, b);
+        const int t_min = g.causal ? max(k0 + g.Tq - count, 0) : 0;        // the first token that sees the tile
+        lo = t_min / kRows;
+        per_head = k0 < count && t_min < g.Tq ? g.tiles_t - lo : 0;
+        const long long all = (long long)per_head * (g.tiles / g.tiles_t);
+        first = (int)(all * split / cut.splits);
+        n = (int)(all * (split + 1) / cut.splits) - first;
+    }
+    // first head and token of the i-th chunk
+    __device__ __forceinline__ void chunk(const Geom& g, int i, int& h0, int& t0) const {
+        const int th = (first + i) / per_head;
+        h0 = m * g.G + th * g.hp;
+        t0 = (lo + first + i - th * per_head) * kRows;
+    }
+};
+
+template <int D>
+struct KeyCfg : TileCfg<D> {
+    using T = TileCfg<D>;
+    static constexpr int NST = D == 128 ? 2 : 4;                         // chunks of Q and dO
+    static constexpr int OUT_BYTES = 4 * 2 * OutStage<32>::BYTES;
+    static constexpr int X_BYTES = NST * 2 * kRows * 4;                  // [ring slot]{-lse * log2(e), -delta}[row]
+    static constexpr int SMEM = 2 * T::BYTES + 2 * NST * T::BYTES + OUT_BYTES + X_BYTES + 512 /*barriers*/ + 1024 /*alignment*/;
+    static constexpr int TMEM_S = 0, TMEM_DP = 128, TMEM_DV = 256, TMEM_DK = 384;
+    static_assert(SMEM <= kSmemLimit, "dK/dV kernel shared memory");
+};
+
+// P for its product, times 2^kShift: in fp16 the weights of long sequences would fall among the subnormal numbers.
+template <typename DT> struct Weight {
+    static constexpr float kShift = IsBf16<DT>::value ? 0.f : 6.f, kUnit = IsBf16<DT>::value ? 1.f : 1.f / 64.f;
+};
+
+template <typename DT, int D>
+__global__ void __launch_bounds__(512, 1)
+attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                 const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                 const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv, const float* __restrict__ lse,
+                 const float* __restrict__ delta, const ErrorState* __restrict__ errors, const Geom g, const KeyCut cut) {
+    using C = KeyCfg<D>;
+    constexpr int NST = C::NST;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sK = smem;
+    uint8_t* sV = sK + C::BYTES;
+    uint8_t* sQ = sV + C::BYTES;                          // NST x Q chunk
+    uint8_t* sG = sQ + NST * C::BYTES;                    // NST x dO chunk
+    uint8_t* sOut = sG + NST * C::BYTES;
+    float* s_x = reinterpret_cast<float*>(sOut + C::OUT_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_x + C::X_BYTES / 4);
+    uint64_t* kv_full = bars;                //     TMA -> MMA
+    uint64_t* kv_empty = bars + 1;           //     MMA (commit) -> TMA
+    uint64_t* acc_full = bars + 2;           //     MMA (commit) -> epilogue
+    uint64_t* acc_free = bars + 3;           //     epilogue -> MMA
+    uint64_t* s_full = bars + 4;             //     MMA (commit) -> softmax
+    uint64_t* p_full = bars + 5;             //     softmax -> MMA
+    uint64_t* dp_full = bars + 6;            //     MMA (commit) -> softmax
+    uint64_t* ds_full = bars + 7;            //     softmax -> MMA
+    uint64_t* qd_full = bars + 8;            // [4] TMA -> MMA
+    uint64_t* qd_empty = bars + 12;          // [4] MMA (commit) -> TMA
+    uint64_t* x_full = bars + 16;            // [4] producer -> MMA (and through it softmax): lse and delta
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+    const WaitCtx wctx{reinterpret_cast<WaitState*>(bars + 21)};
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        wait_state_init(wctx.st, errors, kWaitLimitNs);
+        mbar_init(kv_full, 1);
+        mbar_init(kv_empty, 1);
+        mbar_init(acc_full, 1);
+        mbar_init(acc_free, 4);
+        mbar_init(s_full, 1);
+        mbar_init(p_full, 8);
+        mbar_init(dp_full, 1);
+        mbar_init(ds_full, 8);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(qd_full + i, 1);
+            mbar_init(qd_empty + i, 1);
+            mbar_init(x_full + i, 1);
+        }
+        mbar_fence_init();
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_do);
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+        tma_prefetch_desc(&tm_dk);
+        tma_prefetch_desc(&tm_dv);
+    }
+    // Rows of a chunk that no copy writes (several heads of few tokens that do not fill 128 rows) are contraction rows all the same.
+    if (g.hp * g.tt < kRows) {
+        for (int i = tid; i < 2 * NST * C::BYTES / 16; i += 512) na2d_tc::st_shared_v4(smem_u32(sQ) + 16 * i, 0u, 0u, 0u, 0u);
+        fence_proxy_async();
+    }
+    after_previous_grid();
+    if (warp == 0) {
+        __syncwarp();
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    next_grid_may_start();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 8) {
+        // ------------------------------------------------------------------ producer of the Q / dO chunks
+        reg_dec<kDkvRegsCtl>();
+        LoadTracker lt(bars);
+        Ring ring;
+        for (int item = blockIdx.x; item < cut.items && lt.ok; item += gridDim.x) {
+            const KeyItem k(g, cut, item);
+            for (int i = 0; i < k.n; ++i) {
+                int h0, t0;
+                k.chunk(g, i, h0, t0);
+                float x_lse[4], x_delta[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {                // (read ahead of the wait for a free slot)
+                    const int r = lane + 32 * u, h = g.hp == 1 ? 0 : r / g.tt, t = t0 + r - h * g.tt;
+                    x_lse[u] = -CUDART_INF_F;
+                    x_delta[u] = 0.f;
+                    if (h < g.hp && t < g.Tq) {
+                        const size_t at = row_index(g, k.b, h0 + h, t);
+                        x_lse[u] = lse[at];
+                        x_delta[u] = delta[at];
+                    }
+                }
+                if (!lt.acquire_warp(qd_empty + ring.at, ring.phase ^ 1, wctx)) break;
+                if (lane == 0) {
+                    lt.arm(qd_full + ring.at, ring.phase, 2 * C::load_bytes(g.hp * g.tt));
+#pragma unroll
+                    for (int s = 0; s < C::NS; ++s) {
+                        tma_load_5d(sQ + ring.at * C::BYTES + s * C::SLAB, &tm_q, qd_full + ring.at, s * 64, t0, h0, k.b, 0);
+                        tma_load_5d(sG + ring.at * C::BYTES + s * C::SLAB, &tm_do, qd_full + ring.at, s * 64, t0, h0, k.b, 0);
+                    }
+                }
+                float* x = s_x + ring.at * 2 * kRows;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    // rows that see nothing, or are none: weights of exp2(-infinity)
+                    x[lane + 32 * u] = x_lse[u] == -CUDART_INF_F ? -CUDART_INF_F : Weight<DT>::kShift - x_lse[u] * kLog2e;
+                    x[kRows + lane + 32 * u] = -x_delta[u] * Weight<DT>::kUnit;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(x_full + ring.at);
+                ring.next(NST);
+            }
+        }
+        if (lane == 0) lt.drain(wctx);
+    } else if (warp == 11) {
+        // ------------------------------------------------------------------ producer of the K, V tile
+        reg_dec<kDkvRegsCtl>();
+        if (lane == 0) {
+            LoadTracker lt(bars);
+            uint32_t it = 0;
+            for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
+                const KeyItem k(g, cut, item);
+                if (k.n == 0) continue;
+                if (!lt.acquire(kv_empty, (it & 1) ^ 1, wctx)) break;
+                lt.arm(kv_full, it & 1, 2 * C::BYTES);
+#pragma unroll
+                for (int s = 0; s < C::NS; ++s) {
+                    tma_load_5d(sK + s * C::SLAB, &tm_k, kv_full, s * 64, k.k0, k.m, k.b, 0);
+                    tma_load_5d(sV + s * C::SLAB, &tm_v, kv_full, s * 64, k.k0, k.m, k.b, 0);
+                }
+                ++it;
+            }
+            lt.drain(wctx);
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------------------ MMA issue
+        reg_dec<kDkvRegsCtl>();
+        constexpr uint32_t idesc_s = umma_idesc(kRows, kRows, IsBf16<DT>::value, IsBf16<DT>::value, false, false);
+        constexpr uint32_t idesc_o = umma_idesc(kRows, D, IsBf16<DT>::value, IsBf16<DT>::value, false, true);
+        constexpr uint32_t hi = smem_desc_hi(C::ATOM, C::SWZ);
+        const uint32_t k_lo = smem_desc_lo(smem_u32(sK), 16), v_lo = smem_desc_lo(smem_u32(sV), 16);
+        const uint32_t q_lo0 = smem_desc_lo(smem_u32(sQ), 16), g_lo0 = smem_desc_lo(smem_u32(sG), 16);
+        const uint32_t qm_lo0 = smem_desc_lo(smem_u32(sQ), C::SLAB), gm_lo0 = smem_desc_lo(smem_u32(sG), C::SLAB);
+        auto product = [&](uint32_t t_d, uint32_t a_lo, uint32_t b_lo) {          // D = A B^T of two K-major operands
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                constexpr int kPerSlab = C::SLAB_C / 16;
+                const int at = (((kk / kPerSlab) * C::SLAB) >> 4) + 2 * (kk % kPerSlab);
+                umma_ss(t_d, desc64(hi, a_lo + at), desc64(hi, b_lo + at), idesc_s, kk > 0);
+            }
+        };
+        // D += A B, A the 16-bit pairs over a softmax warp's half of t_a's columns, B a chunk
+        auto gather = [&](uint32_t t_d, uint32_t t_a, uint32_t b_lo, uint32_t accumulate) {
+#pragma unroll
+            for (int kk = 0; kk < kRows / 16; ++kk)
+                umma_ts(t_d, t_a + (kk / 4) * 64 + (kk % 4) * 8, desc64(hi, b_lo + ((kk * 16 * C::ROWB) >> 4)), idesc_o,
+                        accumulate | (kk > 0));
+        };
+        Ring rs, ro;                          // places of the chunks that S and the outputs are at
+        uint32_t no = 0, it = 0;
+        auto scores = [&]() {
+            mbar_wait(qd_full + rs.at, rs.phase, wctx, kErrLoadWait);
+            mbar_wait(x_full + rs.at, rs.phase, wctx, kErrLoadWait);
+            tc_fence_after();
+            if (elect_one()) {
+                product(tmem_base + C::TMEM_S, k_lo, q_lo0 + rs.at * (C::BYTES >> 4));
+                umma_commit(s_full);
+            }
+            __syncwarp();
+        };
+        auto grads = [&](bool last) {
+            if (elect_one()) {
+                product(tmem_base + C::TMEM_DP, v_lo, g_lo0 + rs.at * (C::BYTES >> 4));
+                umma_commit(dp_full);
+                if (last) umma_commit(kv_empty);
+            }
+            __syncwarp();
+            rs.next(NST);
+        };
+        for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
+            const KeyItem k(g, cut, item);
+            if (k.n == 0) continue;
+            mbar_wait(kv_full, it & 1, wctx, kErrLoadWait);
+            scores();
+            grads(k.n == 1);
+            for (int i = 0; i < k.n; ++i, ++no) {
+                if (i == 0) mbar_wait(acc_free, (it & 1) ^ 1, wctx, kErrMmaWait);
+                mbar_wait(p_full, no & 1, wctx, kErrMmaWait);
+                tc_fence_after();
+                if (elect_one()) gather(tmem_base + C::TMEM_DV, tmem_base + C::TMEM_S, gm_lo0 + ro.at * (C::BYTES >> 4), i > 0);
+                __syncwarp();
+                if (i + 1 < k.n) scores();
+                mbar_wait(ds_full, no & 1, wctx, kErrMmaWait);
+                tc_fence_after();
+                if (elect_one()) {
+                    gather(tmem_base + C::TMEM_DK, tmem_base + C::TMEM_DP, qm_lo0 + ro.at * (C::BYTES >> 4), i > 0);
+                    umma_commit(qd_empty + ro.at);
+                    if (i + 1 == k.n) umma_commit(acc_full);
+                }
+                __syncwarp();
+                ro.next(NST);
+                if (i + 1 < k.n) grads(i + 2 == k.n);
+            }
+            ++it;
+        }
+    } else if (warp == 10) {
+        reg_dec<kDkvRegsCtl>();
+    } else if (warp >= 12) {
+        // ------------------------------------------------------------------ epilogue warps
+        reg_dec<kDkvRegsEpi>();
+        const int quarter = warp & 3;
+        const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        uint8_t* stage = sOut + quarter * 2 * OutStage<32>::BYTES;
+        uint32_t it = 0, seq = 0;
+        for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
+            const KeyItem k(g, cut, item);
+            const int first = k.k0 + quarter * 32, key = first + lane;
+            if (k.n > 0) {
+                mbar_wait(acc_full, it & 1, wctx, kErrMmaWait);
+                tc_fence_after();
+            }
+#pragma unroll
+            for (int j = 0; j < 2 * (D / 32); ++j) {
+                const int which = j / (D / 32), r = j % (D / 32);        // dV, then dK
+                const float scale = which ? g.scale : Weight<DT>::kUnit;
+                uint32_t v[32];
+                if (k.n > 0) {
+                    tmem_ld_32x32(tmem_lane + (which ? C::TMEM_DK : C::TMEM_DV) + 32 * r, v);
+                    tmem_ld_wait();
+                    if (j + 1 == 2 * (D / 32)) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acc_free);
+                    }
+                } else {                                                 // no query sees the tile
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = 0u;
+                }
+                if (32 * r >= g.C || first >= g.Tk) continue;
+                if (cut.splits == 1) {
+                    na2d_tc::stage_and_store<DT, 32, 2>(which ? &tm_dk : &tm_dv, stage, v, scale, 32 * r, first, k.m, k.b, 0, lane, &seq);
+                } else if (key < g.Tk) {
+                    float4* dst = reinterpret_cast<float4*>(
+                        (which ? cut.part_dk : cut.part_dv) +
+                        ((static_cast<size_t>(k.split) * g.units + static_cast<size_t>(k.b) * g.Nk + k.m) * g.Tk + key) * g.C + 32 * r);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (32 * r + 4 * e < g.C)
+                            dst[e] = make_float4(__uint_as_float(v[4 * e]) * scale, __uint_as_float(v[4 * e + 1]) * scale,
+                                                 __uint_as_float(v[4 * e + 2]) * scale, __uint_as_float(v[4 * e + 3]) * scale);
+                }
+            }
+            if (k.n > 0) ++it;
+        }
+        if (lane == 0) bulk_wait<0>();
+    } else {
+        // ------------------------------------------------------------------ softmax warps
+        reg_inc<kDkvRegsSoftmax>();
+        const int quarter = warp & 3, half = warp >> 2;
+        const int row = quarter * 32 + lane;                 // key of the tile = tensor-memory lane
+        const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t s_addr = tmem_lane + C::TMEM_S + 64 * half, dp_addr = tmem_lane + C::TMEM_DP + 64 * half;
+        const uint64_t scale2 = pair2(g.sl2, g.sl2), unit2 = pair2(Weight<DT>::kUnit, Weight<DT>::kUnit);
+        uint32_t m = 0;
+        Ring ring;
+        for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
+            const KeyItem k(g, cut, item);
+            const int key = k.k0 + row;
+            // the first token that sees this key
+            const int t_lo = key >= k.count ? 0x7fffffff : g.causal ? max(key + g.Tq - k.count, 0) : 0;
+            for (int i = 0; i < k.n; ++i, ++m) {
+                int h0, t0;
+                k.chunk(g, i, h0, t0);
+                const int closed = key >= k.count ? 64 : t_lo - t0 - 64 * half;     // columns of this half that do not see the key come first
+                const bool cover = __any_sync(0xffffffffu, closed > 0);
+                const float* x_lse = s_x + ring.at * 2 * kRows + 64 * half;
+                const float* x_delta = x_lse + kRows;
+                uint64_t pr[32];
+                mbar_wait(s_full, m & 1, wctx, kErrMmaWait);
+                tc_fence_after();
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    uint32_t s[32], w[16];
+                    tmem_ld_32x32(s_addr + 32 * a, s);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e4 = 0; e4 < 8; ++e4) {
+                        const ulonglong2 nl = *reinterpret_cast<const ulonglong2*>(x_lse + 32 * a + 4 * e4);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int e = 4 * e4 + 2 * h;
+                            const uint64_t y = fma2(pair2(s[e], s[e + 1]), scale2, h ? nl.y : nl.x);
+                            float p0 = fast_exp2(lo2(y)), p1 = fast_exp2(hi2(y));
+                            if (cover) {                     // by selection: what is not seen may hold anything
+                                if (32 * a + e < closed) p0 = 0.f;
+                                if (32 * a + e + 1 < closed) p1 = 0.f;
+                            }
+                            pr[16 * a + e / 2] = pair2(p0, p1);
+                            w[e / 2] = pack2<DT>(p0, p1);
+                        }
+                    }
+                    tmem_st_32x16(s_addr + 16 * a, w);       // over columns that this warp has read
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full);
+                mbar_wait(dp_full, m & 1, wctx, kErrMmaWait);
+                tc_fence_after();
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    uint32_t dp[32], w[16];
+                    tmem_ld_32x32(dp_addr + 32 * a, dp);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e4 = 0; e4 < 8; ++e4) {
+                        const ulonglong2 nd = *reinterpret_cast<const ulonglong2*>(x_delta + 32 * a + 4 * e4);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int e = 4 * e4 + 2 * h;
+                            const uint64_t ds = mul2(pr[16 * a + e / 2], fma2(pair2(dp[e], dp[e + 1]), unit2, h ? nd.y : nd.x));
+                            float d0 = lo2(ds), d1 = hi2(ds);
+                            if (cover) {
+                                if (32 * a + e < closed) d0 = 0.f;
+                                if (32 * a + e + 1 < closed) d1 = 0.f;
+                            }
+                            w[e / 2] = pack2<DT>(d0, d1);
+                        }
+                    }
+                    tmem_st_32x16(dp_addr + 16 * a, w);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ds_full);
+                ring.next(NST);
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// Adds the parts of dK and dV: `elements` of each part, 4 a thread.
+template <typename DT>
+__global__ void __launch_bounds__(256)
+attn_sum_kernel(const float* __restrict__ part_dk, const float* __restrict__ part_dv, DT* __restrict__ dk, DT* __restrict__ dv,
+                const long long elements, const int splits) {
+    after_previous_grid();
+    next_grid_may_start();
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= elements) return;
+    const float* src = (blockIdx.y ? part_dv : part_dk) + i;
+    float4 acc = *reinterpret_cast<const float4*>(src);
+#pragma unroll 4
+    for (int s = 1; s < splits; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(src + s * elements);
+        acc.x += v.x;
+        acc.y += v.y;
+        acc.z += v.z;
+        acc.w += v.w;
+    }
+    *reinterpret_cast<uint2*>((blockIdx.y ? dv : dk) + i) = make_uint2(pack2<DT>(acc.x, acc.y), pack2<DT>(acc.z, acc.w));
+}
+
+template <typename DT, int D>
+int launch_dkdv(const Place& at, const Geom& g, const KeyCut& cut, const Operand& q, const Operand& k, const Operand& v, const Operand& d_o,
+                const float* lse, const float* delta, const Operand& d_k, const Operand& d_v) {
+    using C = KeyCfg<D>;
+    CUtensorMap tq, tg, tk, tv, tdk, tdv;
+    int rc = operand_map(&tq, q, at.dtype, g.B, g.N, g.Tq, g.C, g.tt, g.hp, C::SLAB_C);
+    if (rc == NA2D_OK) rc = operand_map(&tg, d_o, at.dtype, g.B, g.N, g.Tq, g.C, g.tt, g.hp, C::SLAB_C);
+    if (rc == NA2D_OK) rc = operand_map(&tk, k, at.dtype, g.B, g.Nk, g.Tk, g.C, kRows, 1, C::SLAB_C);
+    if (rc == NA2D_OK) rc = operand_map(&tv, v, at.dtype, g.B, g.Nk, g.Tk, g.C, kRows, 1, C::SLAB_C);
+    if (rc == NA2D_OK) rc = operand_map(&tdk, d_k, at.dtype, g.B, g.Nk, g.Tk, g.C, 32, 1, 32);
+    if (rc == NA2D_OK) rc = operand_map(&tdv, d_v, at.dtype, g.B, g.Nk, g.Tk, g.C, 32, 1, 32);
+    if (rc != NA2D_OK) return rc;
+    auto kern = attn_dkdv_kernel<DT, D>;
+    static std::atomic<unsigned long long> opted{0};
+    if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted) != cudaSuccess) return NA2D_ERR_CUDA;
+    const int sms = na2d_tc::sm_count(at.device);
+    *at.launched += 1;
+    if (na2d_launch::launch(true, kern, cut.items < sms ? cut.items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdk, tdv, lse, delta, at.errors,
+                            g, cut) != cudaSuccess)
+        return NA2D_ERR_CUDA;
+    if (cut.splits == 1) return NA2D_OK;
+    const long long elements = (long long)g.units * g.Tk * g.C;
+    *at.launched += 1;
+    return na2d_launch::launch(true, attn_sum_kernel<DT>, dim3((unsigned)((elements / 4 + 255) / 256), 2), 256, 0, at.st,
+                               (const float*)cut.part_dk, (const float*)cut.part_dv, (DT*)d_k.ptr, (DT*)d_v.ptr, elements,
+                               cut.splits) == cudaSuccess
+               ? NA2D_OK
+               : NA2D_ERR_CUDA;
+}
+
+}  // namespace na2d_attn

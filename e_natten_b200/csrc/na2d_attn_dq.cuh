@@ -1,0 +1,430 @@
+// Attention over all keys, query half of the backward, on tcgen05 (bf16 / fp16, head dims up to 128).
+//
+//     S = Q K_c^T,  dP = dO V_c^T                          (tensor memory, fp32)
+//     P = exp(S - lse),  dS = P (dP - delta)               (softmax warps)
+//     dQ += dS K_c                                         (dS from tensor memory, 16 bit)
+// with delta = dO . o of the row, formed ahead by delta_kernel.  dS is rounded once to 16 bits for its product, as P is in the
+// forward: dQ is then about 1.4 times as far from its 64-bit value as its own rounding puts it.  (The softmax scale comes in the
+// epilogue: in fp16 dS keeps more of its bits without.)
+//
+// Persistent, one CTA per SM, one tile of 128 query rows at a time, keys in chunks of 128.  S has two buffers, so that the
+// exponentials of chunk n + 1 run while dQ and dP of chunks n and n + 1 are on the tensor pipe; dS goes over dP.
+//   warps 0-7   softmax: warps w and w + 4 share 32 rows and take 64 columns each;
+//   warp 8      producer (Q, dO, K, V);  warp 9  MMA issue;  warp 11  clears the rows of K beyond a batch entry's keys;
+//   warps 12-15 epilogue.
+#pragma once
+
+#include "na2d_attn_fwd.cuh"
+
+namespace na2d_attn {
+
+// delta = dO . o of each row, 8 channels a lane.  LPR lanes a row: C / 8, rounded up to a power of two.
+template <typename DT, int LPR>
+__global__ void __launch_bounds__(256)
+attn_delta_kernel(const DT* __restrict__ d_o, const Operand st_do, const DT* __restrict__ o, const Operand st_o, float* __restrict__ delta,
+                  const Geom g) {
+    after_previous_grid();
+    next_grid_may_start();
+    const long long rows = (long long)g.B * g.N * g.Tq;
+    const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    const int part = threadIdx.x % LPR;
+    float acc = 0.f;
+    if (row < rows && 8 * part < g.C) {
+        const int t = (int)(row % g.Tq);
+        const long long bn = row / g.Tq, b = bn / g.N, n = bn - b * g.N;
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(d_o + b * st_do.b + n * st_do.n + t * st_do.t) + part);
+        const uint4 y = __ldg(reinterpret_cast<const uint4*>(o + b * st_o.b + n * st_o.n + t * st_o.t) + part);
+        acc = na2d_delta::dot8<DT>(x, y, 0.f);
+    }
+#pragma unroll
+    for (int d = LPR / 2; d > 0; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
+    if (part == 0 && row < rows) delta[row] = acc;
+}
+
+template <int D>
+struct DqCfg : TileCfg<D> {
+    using T = TileCfg<D>;
+    static constexpr int NST = D == 128 ? 2 : 4;                         // chunks of K, and of V
+    static constexpr int OUT_BYTES = 4 * 2 * OutStage<32>::BYTES;
+    static constexpr int SMEM = 2 * T::BYTES + 2 * NST * T::BYTES + OUT_BYTES + 512 /*barriers*/ + 1024 /*alignment*/;
+    static constexpr int TMEM_S = 0, TMEM_DP = 256, TMEM_DQ = 384;       // S: two buffers of 128 columns
+    static_assert(SMEM <= kSmemLimit, "dQ kernel shared memory");
+};
+
+template <typename DT, int D>
+__global__ void __launch_bounds__(512, 1)
+attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+               const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+               const __grid_constant__ CUtensorMap tm_dq, DT* __restrict__ dq_rows, const Operand dq_st, const float* __restrict__ lse,
+               const float* __restrict__ delta, const ErrorState* __restrict__ errors, const Geom g, const int items) {
+    using C = DqCfg<D>;
+    constexpr int NST = C::NST;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sQ = smem;
+    uint8_t* sG = sQ + C::BYTES;                          // dO
+    uint8_t* sK = sG + C::BYTES;                          // NST x K chunk
+    uint8_t* sV = sK + NST * C::BYTES;                    // NST x V chunk
+    uint8_t* sOut = sV + NST * C::BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + C::OUT_BYTES);
+    uint64_t* q_full = bars;                 //     TMA -> MMA: Q and dO
+    uint64_t* q_empty = bars + 1;            //     MMA (commit) -> TMA
+    uint64_t* dq_full = bars + 2;            //     MMA (commit) -> epilogue
+    uint64_t* dq_free = bars + 3;            //     epilogue -> MMA
+    uint64_t* dp_full = bars + 4;            //     MMA (commit) -> softmax
+    uint64_t* ds_full = bars + 5;            //     softmax -> MMA
+    uint64_t* s_full = bars + 6;             // [2] MMA (commit) -> softmax
+    uint64_t* s_free = bars + 8;             // [2] softmax -> MMA: S is in registers
+    uint64_t* k_full = bars + 12;            // [4] TMA -> MMA: K and V chunk
+    uint64_t* k_empty = bars + 16;           // [4] MMA (commit) -> TMA
+    uint64_t* k_clear = bars + 20;           // [4] warp 11 -> MMA
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+    const WaitCtx wctx{reinterpret_cast<WaitState*>(bars + 25)};
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        wait_state_init(wctx.st, errors, kWaitLimitNs);
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        mbar_init(dq_full, 1);
+        mbar_init(dq_free, 4);
+        mbar_init(dp_full, 1);
+        mbar_init(ds_full, 8);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + i, 1);
+            mbar_init(s_free + i, 8);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(k_full + i, 1);
+            mbar_init(k_empty + i, 1);
+            mbar_init(k_clear + i, 1);
+        }
+        mbar_fence_init();
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_do);
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+        tma_prefetch_desc(&tm_dq);
+    }
+    after_previous_grid();
+    if (warp == 0) {
+        __syncwarp();
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    next_grid_may_start();
+    const uint32_t tmem_base = *tmem_slot;
+
+    // my items: with a causal mask the longer tiles first
+    auto tile_of = [&](int item) {
+        return g.causal ? RowTile(g, item % g.units, g.tiles - 1 - item / g.units) : RowTile(g, item / g.tiles, item % g.tiles);
+    };
+    auto chunks_of = [&](const RowTile& t) { return (t.keys(g) + kRows - 1) / kRows; };
+
+    if (warp == 8) {
+        // ------------------------------------------------------------------ producer
+        reg_dec<kDkvRegsCtl>();
+        if (lane == 0) {
+            LoadTracker lt(bars);
+            Ring ring;
+            uint32_t it = 0;
+            for (int item = blockIdx.x; item < items && lt.ok; item += gridDim.x) {
+                const RowTile t = tile_of(item);
+                const int n = chunks_of(t);
+                if (n == 0) continue;
+                if (!lt.acquire(q_empty, (it & 1) ^ 1, wctx)) break;
+                lt.arm(q_full, it & 1, 2 * C::load_bytes(g.hp * g.tt));
+#pragma unroll
+                for (int s = 0; s < C::NS; ++s) {
+                    tma_load_5d(sQ + s * C::SLAB, &tm_q, q_full, s * 64, t.t0, t.h0, t.b, 0);
+                    tma_load_5d(sG + s * C::SLAB, &tm_do, q_full, s * 64, t.t0, t.h0, t.b, 0);
+                }
+                ++it;
+                for (int c = 0; c < n; ++c) {
+                    if (!lt.acquire(k_empty + ring.at, ring.phase ^ 1, wctx)) break;
+                    lt.arm(k_full + ring.at, ring.phase, 2 * C::BYTES);
+#pragma unroll
+                    for (int s = 0; s < C::NS; ++s) {
+                        tma_load_5d(sK + ring.at * C::BYTES + s * C::SLAB, &tm_k, k_full + ring.at, s * 64, c * kRows, t.m, t.b, 0);
+                        tma_load_5d(sV + ring.at * C::BYTES + s * C::SLAB, &tm_v, k_full + ring.at, s * 64, c * kRows, t.m, t.b, 0);
+                    }
+                    ring.next(NST);
+                }
+            }
+            lt.drain(wctx);
+        }
+    } else if (warp == 11) {
+        // ------------------------------------------------------------------ zeros beyond the keys
+        reg_dec<kDkvRegsCtl>();
+        if (g.lengths) {
+            Ring ring;
+            for (int item = blockIdx.x; item < items; item += gridDim.x) {
+                const RowTile t = tile_of(item);
+                const int n = chunks_of(t), ragged = fwd_ragged_chunk(g, t.count, 0, n);
+                for (int c = 0; c < n; ++c) {
+                    if (c == ragged) {
+                        mbar_wait(k_full + ring.at, ring.phase, wctx, kErrLoadWait);
+                        __syncwarp();
+                        clear_rows<D>(sK + ring.at * C::BYTES, t.count % kRows, lane);
+                        if (lane == 0) mbar_arrive(k_clear + ring.at);
+                    } else if (lane == 0) {
+                        mbar_wait(k_full + ring.at, ring.phase, wctx, kErrLoadWait);
+                        mbar_arrive(k_clear + ring.at);
+                    }
+                    ring.next(NST);
+                }
+            }
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------------------ MMA issue
+        // Order on the tensor pipe: S(0) dP(0) S(1) | dQ(0) dP(1) S(2) | dQ(1) dP(2) S(3) | ...
+        reg_dec<kDkvRegsCtl>();
+        constexpr uint32_t idesc_s = umma_idesc(kRows, kRows, IsBf16<DT>::value, IsBf16<DT>::value, false, false);
+        constexpr uint32_t idesc_o = umma_idesc(kRows, D, IsBf16<DT>::value, IsBf16<DT>::value, false, true);
+        constexpr uint32_t hi = smem_desc_hi(C::ATOM, C::SWZ);
+        const uint32_t q_lo = smem_desc_lo(smem_u32(sQ), 16), g_lo = smem_desc_lo(smem_u32(sG), 16);
+        const uint32_t k_lo0 = smem_desc_lo(smem_u32(sK), 16), v_lo0 = smem_desc_lo(smem_u32(sV), 16);
+        const uint32_t km_lo0 = smem_desc_lo(smem_u32(sK), C::SLAB);
+        // D (128 columns) = A B^T of two K-major operands
+        auto product = [&](uint32_t t_d, uint32_t a_lo, uint32_t b_lo) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                constexpr int kPerSlab = C::SLAB_C / 16;
+                const int at = (((kk / kPerSlab) * C::SLAB) >> 4) + 2 * (kk % kPerSlab);
+                umma_ss(t_d, desc64(hi, a_lo + at), desc64(hi, b_lo + at), idesc_s, kk > 0);
+            }
+        };
+        Ring rs, rp, ro;                     // places of the chunks that S, dP and dQ are at
+        uint32_t ns = 0, no = 0, it = 0;     // chunks that S and dQ are at, tiles
+        auto scores = [&]() {
+            mbar_wait(k_full + rs.at, rs.phase, wctx, kErrLoadWait);
+            if (g.lengths) mbar_wait(k_clear + rs.at, rs.phase, wctx, kErrOther);
+            mbar_wait(s_free + (ns & 1), ((ns >> 1) & 1) ^ 1, wctx, kErrMmaWait);
+            tc_fence_after();
+            if (elect_one()) {
+                product(tmem_base + C::TMEM_S + (ns & 1) * kRows, q_lo, k_lo0 + rs.at * (C::BYTES >> 4));
+                umma_commit(s_full + (ns & 1));
+            }
+            __syncwarp();
+            ++ns;
+            rs.next(NST);
+        };
+        auto grads = [&](bool last) {        // (its chunk has landed: S came before)
+            if (elect_one()) {
+                product(tmem_base + C::TMEM_DP, g_lo, v_lo0 + rp.at * (C::BYTES >> 4));
+                umma_commit(dp_full);
+                if (last) umma_commit(q_empty);
+            }
+            __syncwarp();
+            rp.next(NST);
+        };
+        for (int item = blockIdx.x; item < items; item += gridDim.x) {
+            const int n = chunks_of(tile_of(item));
+            if (n == 0) continue;
+            mbar_wait(q_full, it & 1, wctx, kErrLoadWait);
+            scores();
+            grads(n == 1);                   // (dS of the chunk before has been read: dQ came before on the pipe)
+            for (int c = 0; c < n; ++c, ++no) {
+                if (c + 1 < n) scores();
+                if (c == 0) mbar_wait(dq_free, (it & 1) ^ 1, wctx, kErrMmaWait);
+                mbar_wait(ds_full, no & 1, wctx, kErrMmaWait);
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t km_lo = km_lo0 + ro.at * (C::BYTES >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < kRows / 16; ++kk)      // a warp's half of dS: 32 columns of pairs over its own half of dP
+                        umma_ts(tmem_base + C::TMEM_DQ, tmem_base + C::TMEM_DP + (kk / 4) * 64 + (kk % 4) * 8,
+                                desc64(hi, km_lo + ((kk * 16 * C::ROWB) >> 4)), idesc_o, (c > 0) || (kk > 0));
+                    umma_commit(k_empty + ro.at);
+                    if (c + 1 == n) umma_commit(dq_full);
+                }
+                __syncwarp();
+                ro.next(NST);
+                if (c + 1 < n) grads(c + 2 == n);
+            }
+            ++it;
+        }
+    } else if (warp == 10) {
+        reg_dec<kDkvRegsCtl>();
+    } else if (warp >= 12) {
+        // ------------------------------------------------------------------ epilogue warps
+        reg_dec<kDkvRegsEpi>();
+        const int quarter = warp & 3;
+        const int row = quarter * 32 + lane;
+        const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        uint8_t* stage = sOut + quarter * 2 * OutStage<32>::BYTES;
+        uint32_t it = 0, seq = 0;
+        for (int item = blockIdx.x; item < items; item += gridDim.x) {
+            const RowTile tile = tile_of(item);
+            const bool none = chunks_of(tile) == 0;
+            int n, t;
+            const bool ok = tile.row(g, row, n, t);
+            const int t_first = tile.t0 + quarter * 32;
+            if (!none) {
+                mbar_wait(dq_full, it & 1, wctx, kErrMmaWait);
+                tc_fence_after();
+            }
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                uint32_t v[32];
+                if (!none) {
+                    tmem_ld_32x32(tmem_lane + C::TMEM_DQ + 32 * j, v);
+                    tmem_ld_wait();
+                    if (j + 1 == D / 32) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(dq_free);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = 0u;
+                }
+                if (32 * j >= g.C) continue;
+                if (g.hp == 1) {
+                    if (t_first < g.Tq)
+                        na2d_tc::stage_and_store<DT, 32, 2>(&tm_dq, stage, v, g.scale, 32 * j, t_first, tile.h0, tile.b, 0, lane, &seq);
+                } else if (ok) {
+                    uint4* dst = reinterpret_cast<uint4*>(dq_rows + tile.b * dq_st.b + n * dq_st.n + t * dq_st.t + 32 * j);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (32 * j + 8 * e < g.C) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                w[i] = pack2<DT>(__uint_as_float(v[8 * e + 2 * i]) * g.scale, __uint_as_float(v[8 * e + 2 * i + 1]) * g.scale);
+                            dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                }
+            }
+            if (!none) ++it;
+        }
+        if (lane == 0) bulk_wait<0>();
+    } else {
+        // ------------------------------------------------------------------ softmax warps
+        reg_inc<kDkvRegsSoftmax>();
+        const int quarter = warp & 3, half = warp >> 2;
+        const int row = quarter * 32 + lane;
+        const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t dp_addr = tmem_lane + C::TMEM_DP + 64 * half;
+        const uint64_t scale2 = pair2(g.sl2, g.sl2);
+        uint32_t m = 0;                                      // chunks so far
+        for (int item = blockIdx.x; item < items; item += gridDim.x) {
+            const RowTile tile = tile_of(item);
+            const int chunks = chunks_of(tile);
+            if (chunks == 0) continue;
+            int n, t;
+            const bool ok = tile.row(g, row, n, t);
+            const bool idle = !__any_sync(0xffffffffu, ok);
+            float row_lse = -CUDART_INF_F, row_delta = 0.f;
+            if (ok) {
+                const size_t at = row_index(g, tile.b, n, t);
+                row_lse = __ldg(lse + at);
+                row_delta = __ldg(delta + at);
+            }
+            // a row that sees nothing has weights of zero: exp2(-infinity)
+            const float neg = row_lse == -CUDART_INF_F ? -CUDART_INF_F : -row_lse * kLog2e;
+            const uint64_t neg2 = pair2(neg, neg), delta2 = pair2(-row_delta, -row_delta);
+            const int seen = (ok ? keys_seen(g, tile.count, t) : 0) - 64 * half;
+            for (int c = 0; c < chunks; ++c, ++m) {
+                uint64_t pr[32];
+                mbar_wait(s_full + (m & 1), (m >> 1) & 1, wctx, kErrMmaWait);
+                tc_fence_after();
+                if (!idle) {
+                    uint32_t s[2][32];
+                    const uint32_t s_addr = tmem_lane + C::TMEM_S + (m & 1) * kRows + 64 * half;
+                    tmem_ld_32x32(s_addr, s[0]);
+                    tmem_ld_32x32(s_addr + 32, s[1]);
+                    tmem_ld_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_free + (m & 1));
+#pragma unroll
+                    for (int e2 = 0; e2 < 32; ++e2) {
+                        const uint64_t y = fma2(pair2(s[e2 / 16][2 * (e2 % 16)], s[e2 / 16][2 * (e2 % 16) + 1]), scale2, neg2);
+                        pr[e2] = pair2(fast_exp2(lo2(y)), fast_exp2(hi2(y)));
+                    }
+                } else if (lane == 0) {
+                    mbar_arrive(s_free + (m & 1));
+                }
+                mbar_wait(dp_full, m & 1, wctx, kErrMmaWait);
+                tc_fence_after();
+                if (!idle) {
+                    const int open = seen - c * kRows;       // columns of this half that the row sees
+                    const bool cover = __any_sync(0xffffffffu, open < 64);
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) {
+                        uint32_t dp[32], w[16];
+                        tmem_ld_32x32(dp_addr + 32 * a, dp);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e2 = 0; e2 < 16; ++e2) {
+                            const uint64_t ds = mul2(pr[16 * a + e2], add2(pair2(dp[2 * e2], dp[2 * e2 + 1]), delta2));
+                            float d0 = lo2(ds), d1 = hi2(ds);
+                            if (cover) {                     // by selection: columns that are not seen may hold anything
+                                if (32 * a + 2 * e2 >= open) d0 = 0.f;
+                                if (32 * a + 2 * e2 + 1 >= open) d1 = 0.f;
+                            }
+                            w[e2] = pack2<DT>(d0, d1);
+                        }
+                        // (over columns of dP that this warp has read: the first half of its own)
+                        tmem_st_32x16(dp_addr + 16 * a, w);
+                    }
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ds_full);
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+template <typename DT>
+int launch_delta(const Place& at, const Geom& g, const Operand& d_o, const Operand& o, float* delta) {
+    const long long rows = (long long)g.B * g.N * g.Tq;
+    const int lanes = g.C <= 32 ? 4 : g.C <= 64 ? 8 : 16;
+    const long long blocks = (rows * lanes + 255) / 256;
+    if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+    auto kern = lanes == 4 ? attn_delta_kernel<DT, 4> : lanes == 8 ? attn_delta_kernel<DT, 8> : attn_delta_kernel<DT, 16>;
+    *at.launched += 1;
+    return na2d_launch::launch(false, kern, (unsigned)blocks, 256, 0, at.st, (const DT*)d_o.ptr, d_o, (const DT*)o.ptr, o, delta, g) == cudaSuccess
+               ? NA2D_OK
+               : NA2D_ERR_CUDA;
+}
+
+template <typename DT, int D>
+int launch_dq(const Place& at, const Geom& g, const Operand& q, const Operand& k, const Operand& v, const Operand& d_o, const float* lse,
+              const float* delta, const Operand& d_q) {
+    using C = DqCfg<D>;
+    CUtensorMap tq, tg, tk, tv, tdq;
+    int rc = operand_map(&tq, q, at.dtype, g.B, g.N, g.Tq, g.C, g.tt, g.hp, C::SLAB_C);
+    if (rc == NA2D_OK) rc = operand_map(&tg, d_o, at.dtype, g.B, g.N, g.Tq, g.C, g.tt, g.hp, C::SLAB_C);
+    if (rc == NA2D_OK) rc = operand_map(&tk, k, at.dtype, g.B, g.Nk, g.Tk, g.C, kRows, 1, C::SLAB_C);
+    if (rc == NA2D_OK) rc = operand_map(&tv, v, at.dtype, g.B, g.Nk, g.Tk, g.C, kRows, 1, C::SLAB_C);
+    if (rc == NA2D_OK) rc = operand_map(&tdq, d_q, at.dtype, g.B, g.N, g.Tq, g.C, 32, 1, 32);
+    if (rc != NA2D_OK) return rc;
+    const long long items = (long long)g.units * g.tiles;
+    if (items > 0x3fffffffLL) return NA2D_ERR_TOO_LARGE;
+    auto kern = attn_dq_kernel<DT, D>;
+    static std::atomic<unsigned long long> opted{0};
+    if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted) != cudaSuccess) return NA2D_ERR_CUDA;
+    const int sms = na2d_tc::sm_count(at.device);
+    *at.launched += 1;
+    return na2d_launch::launch(true, kern, items < sms ? (int)items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdq, (DT*)d_q.ptr, d_q, lse,
+                               delta, at.errors, g, (int)items) == cudaSuccess
+               ? NA2D_OK
+               : NA2D_ERR_CUDA;
+}
+
+}  // namespace na2d_attn

@@ -18,12 +18,11 @@
 #include <optional>
 #include <tuple>
 
-#include "../../include/na2d.h"
+#include "na2d_torch.h"
 
 namespace {
 
-using at::Tensor;
-using MaybeTensor = std::optional<Tensor>;
+using namespace na2d_torch;
 
 // The library functions, as loaded by _lib.py (which may have been pointed at another build of them).
 struct Abi {
@@ -43,27 +42,6 @@ void bind_abi(uintptr_t forward, uintptr_t backward, uintptr_t backward_workspac
 int poll_device(int device) { return abi.poll(device, nullptr); }
 uintptr_t current_stream(int device) { return reinterpret_cast<uintptr_t>(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream()); }
 
-// Whether the kernels can read t in place: contiguous channels, no broadcast dimension, and for 16-bit types (the
-// tensor-core path's TMA tensor maps) a base and strides on 16-byte boundaries.
-bool kernel_ready(const Tensor& t) {
-    if (t.numel() == 0) return true;
-    if (t.dim() == 0) return false;
-    const auto sizes = t.sizes();
-    const auto strides = t.strides();
-    const int64_t last = t.dim() - 1;
-    if (strides[last] != 1 && sizes[last] != 1) return false;
-    const bool half = t.element_size() == 2;
-    if (half && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
-    for (int64_t i = 0; i < last; ++i) {
-        if (sizes[i] <= 1) continue;
-        if (strides[i] <= 0 || (half && strides[i] % 8)) return false;
-    }
-    return true;
-}
-Tensor in_place_or_copy(const Tensor& t) { return kernel_ready(t) ? t : t.contiguous(); }
-
-// A dimension of extent 1 may report any stride; the library ignores it, but all-zero means dense.
-int64_t at_least_one(int64_t stride) { return stride < 1 ? 1 : stride; }
 na2d_tensor describe(const Tensor& t) {
     TORCH_CHECK_VALUE(t.dim() == 5 || t.dim() == 4, "expected (B, heads, H, W, C) or (B, heads, T, C); got ", t.dim(), " dimensions");
     const auto s = t.strides();
@@ -161,13 +139,6 @@ std::tuple<int, MaybeTensor, MaybeTensor, MaybeTensor> backward(const Tensor& q_
 // a step of 1 x 2 x 16 x 16 x 32, window 5, fp32, whose kernels took 43 us (39 now), took 85 us instead of 114 (the poll without a copy is
 // part of that), one of 4 x 4 x 32 x 32 x 128, bf16, 81 instead of 113.  They save the same tensors in the same order and
 // return the same gradients.
-
-// Raises what _lib.check raises for a status.
-void check(int status) {
-    if (status == NA2D_OK) return;
-    pybind11::gil_scoped_acquire gil;
-    pybind11::module_::import("e_natten_b200._lib").attr("check")(status);
-}
 
 namespace ag = torch::autograd;
 
@@ -340,4 +311,5 @@ PYBIND11_MODULE(_na2d_torch, m) {
     m.def("attention_1d", &attention<true>);
     m.def("forward", &forward, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("backward", &backward, pybind11::call_guard<pybind11::gil_scoped_release>());
+    na2d_torch::add_block_operators(m);
 }

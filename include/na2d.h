@@ -275,6 +275,109 @@ int na2d_backward_static_scratch(const void* q, const void* k, const void* v, co
                                  int B, int N, int H, int W, int C, int kernel_size, int dtype,
                                  const na2d_rows* rows, int path, int device, void* stream);
 
+/* ---- What stands around the windows in a model ------------------------------------------------
+ *
+ * Group normalisation of channels-last maps, rotary positions on queries and keys, and attention over all keys (for the stages
+ * and the conditioning that want no window).  No reference counterparts.  Each call takes one struct, like the *_ex entry
+ * points: set struct_size, zero what a call does not use.  All launch on a->stream of a->device and return.
+ *
+ * na2d_heads: a (B, heads, T, C) operand, element strides of batch, head and token; channels contiguous; all three zero means
+ * dense.  A grid (B, heads, H, W, C) is one of T = H * W tokens where its rows follow one another. */
+typedef struct na2d_heads {
+    void* ptr;
+    int64_t stride_b, stride_n, stride_t;
+} na2d_heads;
+
+/* Attention over all keys.  s_ij = scale * q_i . k_j over the keys that row i sees, p_i = softmax(s_i), o_i = sum_j p_ij v_j.
+ *   N, Nk        query heads and key heads; Nk divides N, and N / Nk query heads share a key head.
+ *   key_lengths  int32 (B,) on the device, or NULL: batch entry b has the first key_lengths[b] of the Tk keys (clamped to
+ *                [0, Tk]).  What lies beyond them in k and v is never part of a result, whatever it holds; dK and dV are zero there.
+ *   causal       row i of Tq sees the first length - Tq + 1 + i keys of its entry: the queries are the last Tq of the sequence, and one
+ *                query is the newest token of a cache.
+ *   A row that sees no key has o = 0, lse = -infinity and no gradient.
+ *   path         AUTO: tensor cores for 16-bit types with C <= 128 a multiple of 8 and operands on 16-byte boundaries, else
+ *                CUDA cores (C <= 256, any strides).  SIMT and TENSOR ask for one of them.
+ *   o, d_q, d_k, d_v dense.  lse, delta: fp32 (B, N, Tq), dense; delta is scratch of the backward.
+ *   d_q, or d_k and d_v together, may be NULL: that half is left out.  No atomics: the same call gives the same bits.
+ *   workspace    scratch, 16-byte aligned, of na2d_attention_workspace bytes: few rows over many keys, and few keys under many
+ *                queries, are computed in parts that are joined there.  With less (or none) there are fewer parts: slower, and other
+ *                last bits. */
+typedef struct na2d_attention_args {
+    size_t struct_size;
+    int B, N, Nk, Tq, Tk, C, dtype, path, device, causal;
+    float scale;
+    void* stream;
+    na2d_heads q, k, v, o, d_o, d_q, d_k, d_v;
+    const int32_t* key_lengths;
+    float* lse;
+    float* delta;
+    void* workspace;
+    size_t workspace_bytes;
+} na2d_attention_args;
+int na2d_attention_forward(const na2d_attention_args* a);
+/* From q, k, v, o, lse and d_o; forms the probabilities again from lse. */
+int na2d_attention_backward(const na2d_attention_args* a);
+/* Bytes of workspace that the forward, or the backward, of this problem can use. */
+size_t na2d_attention_workspace(const na2d_attention_args* a, int backward);
+
+/* Group normalisation of a channels-last (B, P, C) map, P pixels, with affine parameters and an activation:
+ *   xhat = (x - mean) * rstd over the P x (C / groups) values of a batch entry's group,  y = act(xhat * weight + bias).
+ *   x, d_y       element strides of batch and pixel, channels contiguous; both zero means dense.  y, d_x dense.
+ *   weight, bias (C,), of param_dtype (NA2D_F32 or the map's dtype); NULL: ones, zeros.  d_weight, d_bias: the same type; NULL: not wanted.
+ *   activation   NA2D_ACT_NONE or NA2D_ACT_SILU (z * sigmoid(z)).
+ *   mean, rstd   fp32 (B, groups): written by the forward, read by the backward.
+ *   workspace    scratch, 16-byte aligned, at least na2d_group_norm_workspace bytes.
+ * Statistics and sums are in fp32, variances about the mean; no atomics. */
+typedef enum na2d_activation {
+    NA2D_ACT_NONE = 0,
+    NA2D_ACT_SILU = 1
+} na2d_activation;
+typedef struct na2d_pixels {
+    void* ptr;
+    int64_t stride_b, stride_p;
+} na2d_pixels;
+typedef struct na2d_norm_args {
+    size_t struct_size;
+    int B, C, groups, dtype, param_dtype, activation, device;
+    float eps;
+    int64_t P;
+    void* stream;
+    na2d_pixels x, d_y;
+    void *y, *d_x;
+    const void *weight, *bias;
+    void *d_weight, *d_bias;
+    float *mean, *rstd;
+    void* workspace;
+    size_t workspace_bytes;
+} na2d_norm_args;
+int na2d_group_norm_forward(const na2d_norm_args* a);
+int na2d_group_norm_backward(const na2d_norm_args* a);
+size_t na2d_group_norm_workspace(const na2d_norm_args* a, int backward);
+
+/* Rotary positions: turns pairs of the first `dims` channels of every query and key by the angles of their token's table row,
+ *   (a, b) -> (a cos - b sin, b cos + a sin),
+ * and copies the other channels.  Pair i is channels (2 i, 2 i + 1) where interleaved, else (i, dims / 2 + i).
+ *   table        fp32 (table_rows, dims / 2, 2), dense: cosine and sine of each pair (na2d_rotary_table writes one).
+ *   index        (B, T), dense, int32 or (index_64) int64: a token's table row; NULL: row t for token t.  A row outside
+ *                the table gives NaN in the turned channels.
+ *   inverse      turns back: the backward of the call, on gradients.
+ *   k.ptr may be NULL.  out_q, out_k dense; they may not overlap q and k. */
+typedef struct na2d_rotary_args {
+    size_t struct_size;
+    int B, N, Nk, T, C, dims, dtype, interleaved, inverse, index_64, device;
+    void* stream;
+    na2d_heads q, k;
+    void *out_q, *out_k;
+    const float* table;
+    int64_t table_rows;
+    const void* index;
+} na2d_rotary_args;
+int na2d_rotary(const na2d_rotary_args* a);
+/* table[p][a * pairs + i] = magnitude * (cos, sin)(positions[p][a] * frequencies[a][i]), angles and functions in 64 bits.
+ * positions (P, axes), frequencies (axes, pairs) on the device, in 64 bits, dense. */
+int na2d_rotary_table(const double* positions, const double* frequencies, int64_t P, int axes, int pairs, double magnitude,
+                      float* table, int device, void* stream);
+
 /* Reads and clears the error word that a kernel sets when a bounded wait
  * (mbarrier) ran out.  Synchronises the stream.  Returns NA2D_OK or NA2D_ERR_KERNEL_WAIT.
  * No reference counterpart. */
