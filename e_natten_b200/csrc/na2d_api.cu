@@ -698,6 +698,7 @@ int error_state(int device, const na2d_ptx::ErrorState** out) {
     return rc;
 }
 void count_launches(int n) { g_launches.fetch_add(n); }
+int sm_count(int device) { return na2d_tc::sm_count(device); }
 
 }  // namespace na2d_host
 

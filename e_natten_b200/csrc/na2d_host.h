@@ -37,6 +37,7 @@ int check_device(int device);
 // The device's error state for kernels with waits (the device must be current).
 int error_state(int device, const na2d_ptx::ErrorState** out);
 void count_launches(int n);
+int sm_count(int device);
 
 // Runs `step` with the device current and checked.
 template <typename F>

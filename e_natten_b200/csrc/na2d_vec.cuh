@@ -33,6 +33,7 @@ struct Vec {
     __device__ __forceinline__ Vec() {}
     __device__ __forceinline__ void load(const T* p) { bits = *reinterpret_cast<const raw*>(p); }
     __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<raw*>(p) = bits; }
+    __device__ __forceinline__ void store_streaming(T* p) const { __stcs(reinterpret_cast<raw*>(p), bits); }       // not read again soon
     __device__ __forceinline__ void widened(float (&f)[N]) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) f[i] = widen(at[i]);
