@@ -25,6 +25,7 @@ struct KeyCut {
     int key_tiles;
     int splits;
     int items;
+    Div by_splits, by_key_tiles;
     float* part_dk;         // (splits, B, Nk, Tk, C), where splits > 1
     float* part_dv;
 };
@@ -33,28 +34,39 @@ struct KeyCut {
 struct KeyItem {
     int b, m, k0, count, split;
     int lo, per_head;       // the tile's chunks: query tiles lo .. lo + per_head - 1 of each (group of) heads
-    int first, n;
+    int first, n, head, in_head;
     __device__ __forceinline__ KeyItem(const Geom& g, const KeyCut& cut, int item) {
-        split = item % cut.splits;
-        const int rest = item / cut.splits;
-        // (with a causal mask the first tiles are the longer ones)
-        const int tile = g.causal ? rest / g.units : rest % cut.key_tiles, unit = g.causal ? rest % g.units : rest / cut.key_tiles;
-        b = unit / g.Nk;
-        m = unit - b * g.Nk;
+        int tile, unit;
+        const int rest = cut.by_splits.split(item, split);
+        if (g.causal) {     // the first tiles are the longer ones
+            tile = g.by_units.split(rest, unit);
+        } else {
+            unit = cut.by_key_tiles.split(rest, tile);
+        }
+        b = g.by_nk.split(unit, m);
         k0 = tile * kRows;
         count = key_count(g, b);
         const int t_min = g.causal ? max(k0 + g.Tq - count, 0) : 0;        // the first token that sees the tile
         lo = t_min / kRows;
         per_head = k0 < count && t_min < g.Tq ? g.tiles_t - lo : 0;
-        const long long all = (long long)per_head * (g.tiles / g.tiles_t);
-        first = (int)(all * split / cut.splits);
-        n = (int)(all * (split + 1) / cut.splits) - first;
+        int end;
+        part_of(cut.by_splits, per_head * (g.G / g.hp), split, first, end);
+        n = end - first;
+        head = per_head > 0 ? first / per_head : 0;
+        in_head = first - head * per_head;
     }
-    // first head and token of the i-th chunk
-    __device__ __forceinline__ void chunk(const Geom& g, int i, int& h0, int& t0) const {
-        const int th = (first + i) / per_head;
-        h0 = m * g.G + th * g.hp;
-        t0 = (lo + first + i - th * per_head) * kRows;
+    // first head and token of the first chunk
+    __device__ __forceinline__ void start(const Geom& g, int& h0, int& t0) const {
+        h0 = m * g.G + head * g.hp;
+        t0 = (lo + in_head) * kRows;
+    }
+    // and of the one behind
+    __device__ __forceinline__ void step(const Geom& g, int& h0, int& t0) const {
+        t0 += kRows;
+        if (t0 == (lo + per_head) * kRows) {
+            t0 = lo * kRows;
+            h0 += g.hp;
+        }
     }
 };
 
@@ -62,9 +74,10 @@ template <int D>
 struct KeyCfg : TileCfg<D> {
     using T = TileCfg<D>;
     static constexpr int NST = D == 128 ? 2 : 4;                         // chunks of Q and dO
+    static constexpr int NKV = D == 128 ? 1 : 2;                         // tiles of K and V: the next one's while this one's are read
     static constexpr int OUT_BYTES = 4 * 2 * OutStage<32>::BYTES;
     static constexpr int X_BYTES = NST * 2 * kRows * 4;                  // [ring slot]{-lse * log2(e), -delta}[row]
-    static constexpr int SMEM = 2 * T::BYTES + 2 * NST * T::BYTES + OUT_BYTES + X_BYTES + 512 /*barriers*/ + 1024 /*alignment*/;
+    static constexpr int SMEM = 2 * NKV * T::BYTES + 2 * NST * T::BYTES + OUT_BYTES + X_BYTES + 512 /*barriers*/ + 1024 /*alignment*/;
     static constexpr int TMEM_S = 0, TMEM_DP = 128, TMEM_DV = 256, TMEM_DK = 384;
     static_assert(SMEM <= kSmemLimit, "dK/dV kernel shared memory");
 };
@@ -81,36 +94,38 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                  const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv, const float* __restrict__ lse,
                  const float* __restrict__ delta, const ErrorState* __restrict__ errors, const Geom g, const KeyCut cut) {
     using C = KeyCfg<D>;
-    constexpr int NST = C::NST;
+    constexpr int NST = C::NST, NKV = C::NKV;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sK = smem;
-    uint8_t* sV = sK + C::BYTES;
-    uint8_t* sQ = sV + C::BYTES;                          // NST x Q chunk
+    uint8_t* sV = sK + NKV * C::BYTES;
+    uint8_t* sQ = sV + NKV * C::BYTES;                    // NST x Q chunk
     uint8_t* sG = sQ + NST * C::BYTES;                    // NST x dO chunk
     uint8_t* sOut = sG + NST * C::BYTES;
     float* s_x = reinterpret_cast<float*>(sOut + C::OUT_BYTES);
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_x + C::X_BYTES / 4);
-    uint64_t* kv_full = bars;                //     TMA -> MMA
-    uint64_t* kv_empty = bars + 1;           //     MMA (commit) -> TMA
-    uint64_t* acc_full = bars + 2;           //     MMA (commit) -> epilogue
-    uint64_t* acc_free = bars + 3;           //     epilogue -> MMA
-    uint64_t* s_full = bars + 4;             //     MMA (commit) -> softmax
-    uint64_t* p_full = bars + 5;             //     softmax -> MMA
-    uint64_t* dp_full = bars + 6;            //     MMA (commit) -> softmax
-    uint64_t* ds_full = bars + 7;            //     softmax -> MMA
-    uint64_t* qd_full = bars + 8;            // [4] TMA -> MMA
-    uint64_t* qd_empty = bars + 12;          // [4] MMA (commit) -> TMA
-    uint64_t* x_full = bars + 16;            // [4] producer -> MMA (and through it softmax): lse and delta
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
-    const WaitCtx wctx{reinterpret_cast<WaitState*>(bars + 21)};
+    uint64_t* kv_full = bars;                // [2] TMA -> MMA
+    uint64_t* kv_empty = bars + 2;           // [2] MMA (commit) -> TMA
+    uint64_t* acc_full = bars + 4;           //     MMA (commit) -> epilogue
+    uint64_t* acc_free = bars + 5;           //     epilogue -> MMA
+    uint64_t* s_full = bars + 6;             //     MMA (commit) -> softmax
+    uint64_t* p_full = bars + 7;             //     softmax -> MMA
+    uint64_t* dp_full = bars + 8;            //     MMA (commit) -> softmax
+    uint64_t* ds_full = bars + 9;            //     softmax -> MMA
+    uint64_t* qd_full = bars + 12;           // [4] TMA -> MMA
+    uint64_t* qd_empty = bars + 16;          // [4] MMA (commit) -> TMA
+    uint64_t* x_full = bars + 20;            // [4] producer -> MMA (and through it softmax): lse and delta
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+    const WaitCtx wctx{reinterpret_cast<WaitState*>(bars + 25)};
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
         wait_state_init(wctx.st, errors, kWaitLimitNs);
-        mbar_init(kv_full, 1);
-        mbar_init(kv_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(kv_full + i, 1);
+            mbar_init(kv_empty + i, 1);
+        }
         mbar_init(acc_full, 1);
         mbar_init(acc_free, 4);
         mbar_init(s_full, 1);
@@ -154,13 +169,13 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         Ring ring;
         for (int item = blockIdx.x; item < cut.items && lt.ok; item += gridDim.x) {
             const KeyItem k(g, cut, item);
-            for (int i = 0; i < k.n; ++i) {
-                int h0, t0;
-                k.chunk(g, i, h0, t0);
+            int h0, t0;
+            k.start(g, h0, t0);
+            for (int i = 0; i < k.n; ++i, k.step(g, h0, t0)) {
                 float x_lse[4], x_delta[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {                // (read ahead of the wait for a free slot)
-                    const int r = lane + 32 * u, h = g.hp == 1 ? 0 : r / g.tt, t = t0 + r - h * g.tt;
+                    const int r = lane + 32 * u, h = g.hp == 1 ? 0 : g.by_tt.quotient(r), t = t0 + r - h * g.tt;
                     x_lse[u] = -CUDART_INF_F;
                     x_delta[u] = 0.f;
                     if (h < g.hp && t < g.Tq) {
@@ -200,12 +215,13 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
                 const KeyItem k(g, cut, item);
                 if (k.n == 0) continue;
-                if (!lt.acquire(kv_empty, (it & 1) ^ 1, wctx)) break;
-                lt.arm(kv_full, it & 1, 2 * C::BYTES);
+                const uint32_t to = it % NKV, phase = (it / NKV) & 1;
+                if (!lt.acquire(kv_empty + to, phase ^ 1, wctx)) break;
+                lt.arm(kv_full + to, phase, 2 * C::BYTES);
 #pragma unroll
                 for (int s = 0; s < C::NS; ++s) {
-                    tma_load_5d(sK + s * C::SLAB, &tm_k, kv_full, s * 64, k.k0, k.m, k.b, 0);
-                    tma_load_5d(sV + s * C::SLAB, &tm_v, kv_full, s * 64, k.k0, k.m, k.b, 0);
+                    tma_load_5d(sK + to * C::BYTES + s * C::SLAB, &tm_k, kv_full + to, s * 64, k.k0, k.m, k.b, 0);
+                    tma_load_5d(sV + to * C::BYTES + s * C::SLAB, &tm_v, kv_full + to, s * 64, k.k0, k.m, k.b, 0);
                 }
                 ++it;
             }
@@ -242,16 +258,16 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             mbar_wait(x_full + rs.at, rs.phase, wctx, kErrLoadWait);
             tc_fence_after();
             if (elect_one()) {
-                product(tmem_base + C::TMEM_S, k_lo, q_lo0 + rs.at * (C::BYTES >> 4));
+                product(tmem_base + C::TMEM_S, k_lo + it % NKV * (C::BYTES >> 4), q_lo0 + rs.at * (C::BYTES >> 4));
                 umma_commit(s_full);
             }
             __syncwarp();
         };
         auto grads = [&](bool last) {
             if (elect_one()) {
-                product(tmem_base + C::TMEM_DP, v_lo, g_lo0 + rs.at * (C::BYTES >> 4));
+                product(tmem_base + C::TMEM_DP, v_lo + it % NKV * (C::BYTES >> 4), g_lo0 + rs.at * (C::BYTES >> 4));
                 umma_commit(dp_full);
-                if (last) umma_commit(kv_empty);
+                if (last) umma_commit(kv_empty + it % NKV);
             }
             __syncwarp();
             rs.next(NST);
@@ -259,18 +275,23 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
             const KeyItem k(g, cut, item);
             if (k.n == 0) continue;
-            mbar_wait(kv_full, it & 1, wctx, kErrLoadWait);
+            mbar_wait(kv_full + it % NKV, (it / NKV) & 1, wctx, kErrLoadWait);
             scores();
             grads(k.n == 1);
             for (int i = 0; i < k.n; ++i, ++no) {
                 if (i == 0) mbar_wait(acc_free, (it & 1) ^ 1, wctx, kErrMmaWait);
+                if (lane == 0) NA2D_TR(2, 0, no);
                 mbar_wait(p_full, no & 1, wctx, kErrMmaWait);
                 tc_fence_after();
+                if (lane == 0) NA2D_TR(2, 1, no);
                 if (elect_one()) gather(tmem_base + C::TMEM_DV, tmem_base + C::TMEM_S, gm_lo0 + ro.at * (C::BYTES >> 4), i > 0);
                 __syncwarp();
+                if (lane == 0) NA2D_TR(2, 2, no);
                 if (i + 1 < k.n) scores();
+                if (lane == 0) NA2D_TR(2, 3, no);
                 mbar_wait(ds_full, no & 1, wctx, kErrMmaWait);
                 tc_fence_after();
+                if (lane == 0) NA2D_TR(2, 4, no);
                 if (elect_one()) {
                     gather(tmem_base + C::TMEM_DK, tmem_base + C::TMEM_DP, qm_lo0 + ro.at * (C::BYTES >> 4), i > 0);
                     umma_commit(qd_empty + ro.at);
@@ -278,7 +299,9 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 }
                 __syncwarp();
                 ro.next(NST);
+                if (lane == 0) NA2D_TR(2, 5, no);
                 if (i + 1 < k.n) grads(i + 2 == k.n);
+                if (lane == 0) NA2D_TR(2, 6, no);
             }
             ++it;
         }
@@ -347,71 +370,77 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const int key = k.k0 + row;
             // the first token that sees this key
             const int t_lo = key >= k.count ? 0x7fffffff : g.causal ? max(key + g.Tq - k.count, 0) : 0;
-            for (int i = 0; i < k.n; ++i, ++m) {
-                int h0, t0;
-                k.chunk(g, i, h0, t0);
+            int h0, t0;
+            k.start(g, h0, t0);
+            for (int i = 0; i < k.n; ++i, ++m, k.step(g, h0, t0)) {
                 const int closed = key >= k.count ? 64 : t_lo - t0 - 64 * half;     // columns of this half that do not see the key come first
                 const bool cover = __any_sync(0xffffffffu, closed > 0);
                 const float* x_lse = s_x + ring.at * 2 * kRows + 64 * half;
                 const float* x_delta = x_lse + kRows;
                 uint64_t pr[32];
+                if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 0, m);
                 mbar_wait(s_full, m & 1, wctx, kErrMmaWait);
                 tc_fence_after();
+                if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 1, m);
+                uint32_t s[2][32];
+                tmem_ld_32x32(s_addr, s[0]);
+                tmem_ld_32x32(s_addr + 32, s[1]);
+                tmem_ld_wait();
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    uint32_t s[32], w[16];
-                    tmem_ld_32x32(s_addr + 32 * a, s);
-                    tmem_ld_wait();
+                for (int e4 = 0; e4 < 16; ++e4) {
+                    const ulonglong2 nl = *reinterpret_cast<const ulonglong2*>(x_lse + 4 * e4);
 #pragma unroll
-                    for (int e4 = 0; e4 < 8; ++e4) {
-                        const ulonglong2 nl = *reinterpret_cast<const ulonglong2*>(x_lse + 32 * a + 4 * e4);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int e = 4 * e4 + 2 * h;
-                            const uint64_t y = fma2(pair2(s[e], s[e + 1]), scale2, h ? nl.y : nl.x);
-                            float p0 = fast_exp2(lo2(y)), p1 = fast_exp2(hi2(y));
-                            if (cover) {                     // by selection: what is not seen may hold anything
-                                if (32 * a + e < closed) p0 = 0.f;
-                                if (32 * a + e + 1 < closed) p1 = 0.f;
-                            }
-                            pr[16 * a + e / 2] = pair2(p0, p1);
-                            w[e / 2] = pack2<DT>(p0, p1);
-                        }
+                    for (int h = 0; h < 2; ++h) {
+                        const int e = 4 * e4 + 2 * h;
+                        const uint64_t y = fma2(pair2(s[e / 32][e % 32], s[e / 32][e % 32 + 1]), scale2, h ? nl.y : nl.x);
+                        pr[e / 2] = pair2(fast_exp2(lo2(y)), fast_exp2(hi2(y)));
                     }
-                    tmem_st_32x16(s_addr + 16 * a, w);       // over columns that this warp has read
                 }
+                if (cover) {                                 // by selection: what is not seen may hold anything
+#pragma unroll
+                    for (int e = 0; e < 64; e += 2)
+                        pr[e / 2] = pair2(e < closed ? 0.f : lo2(pr[e / 2]), e + 1 < closed ? 0.f : hi2(pr[e / 2]));
+                }
+                uint32_t w[2][16];
+#pragma unroll
+                for (int e2 = 0; e2 < 32; ++e2) w[e2 / 16][e2 % 16] = pack2<DT>(lo2(pr[e2]), hi2(pr[e2]));
+                tmem_st_32x16(s_addr, w[0]);                 // over columns that this warp has read
+                tmem_st_32x16(s_addr + 16, w[1]);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full);
+                if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 2, m);
                 mbar_wait(dp_full, m & 1, wctx, kErrMmaWait);
                 tc_fence_after();
+                if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 3, m);
+                tmem_ld_32x32(dp_addr, s[0]);
+                tmem_ld_32x32(dp_addr + 32, s[1]);
+                tmem_ld_wait();
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    uint32_t dp[32], w[16];
-                    tmem_ld_32x32(dp_addr + 32 * a, dp);
-                    tmem_ld_wait();
+                for (int e4 = 0; e4 < 16; ++e4) {
+                    const ulonglong2 nd = *reinterpret_cast<const ulonglong2*>(x_delta + 4 * e4);
 #pragma unroll
-                    for (int e4 = 0; e4 < 8; ++e4) {
-                        const ulonglong2 nd = *reinterpret_cast<const ulonglong2*>(x_delta + 32 * a + 4 * e4);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int e = 4 * e4 + 2 * h;
-                            const uint64_t ds = mul2(pr[16 * a + e / 2], fma2(pair2(dp[e], dp[e + 1]), unit2, h ? nd.y : nd.x));
-                            float d0 = lo2(ds), d1 = hi2(ds);
-                            if (cover) {
-                                if (32 * a + e < closed) d0 = 0.f;
-                                if (32 * a + e + 1 < closed) d1 = 0.f;
-                            }
-                            w[e / 2] = pack2<DT>(d0, d1);
-                        }
+                    for (int h = 0; h < 2; ++h) {
+                        const int e = 4 * e4 + 2 * h;
+                        const uint64_t dp = pair2(s[e / 32][e % 32], s[e / 32][e % 32 + 1]);
+                        pr[e / 2] = mul2(pr[e / 2], IsBf16<DT>::value ? add2(dp, h ? nd.y : nd.x) : fma2(dp, unit2, h ? nd.y : nd.x));
                     }
-                    tmem_st_32x16(dp_addr + 16 * a, w);
                 }
+                if (cover) {
+#pragma unroll
+                    for (int e = 0; e < 64; e += 2)
+                        pr[e / 2] = pair2(e < closed ? 0.f : lo2(pr[e / 2]), e + 1 < closed ? 0.f : hi2(pr[e / 2]));
+                }
+#pragma unroll
+                for (int e2 = 0; e2 < 32; ++e2) w[e2 / 16][e2 % 16] = pack2<DT>(lo2(pr[e2]), hi2(pr[e2]));
+                tmem_st_32x16(dp_addr, w[0]);
+                tmem_st_32x16(dp_addr + 16, w[1]);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ds_full);
+                if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 4, m);
                 ring.next(NST);
             }
         }

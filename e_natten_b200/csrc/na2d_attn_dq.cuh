@@ -45,8 +45,9 @@ template <int D>
 struct DqCfg : TileCfg<D> {
     using T = TileCfg<D>;
     static constexpr int NST = D == 128 ? 2 : 4;                         // chunks of K, and of V
+    static constexpr int NQ = D == 128 ? 1 : 2;                          // tiles of Q and dO: the next one's while this one's are read
     static constexpr int OUT_BYTES = 4 * 2 * OutStage<32>::BYTES;
-    static constexpr int SMEM = 2 * T::BYTES + 2 * NST * T::BYTES + OUT_BYTES + 512 /*barriers*/ + 1024 /*alignment*/;
+    static constexpr int SMEM = 2 * NQ * T::BYTES + 2 * NST * T::BYTES + OUT_BYTES + 512 /*barriers*/ + 1024 /*alignment*/;
     static constexpr int TMEM_S = 0, TMEM_DP = 256, TMEM_DQ = 384;       // S: two buffers of 128 columns
     static_assert(SMEM <= kSmemLimit, "dQ kernel shared memory");
 };
@@ -58,23 +59,23 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                const __grid_constant__ CUtensorMap tm_dq, DT* __restrict__ dq_rows, const Operand dq_st, const float* __restrict__ lse,
                const float* __restrict__ delta, const ErrorState* __restrict__ errors, const Geom g, const int items) {
     using C = DqCfg<D>;
-    constexpr int NST = C::NST;
+    constexpr int NST = C::NST, NQ = C::NQ;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sQ = smem;
-    uint8_t* sG = sQ + C::BYTES;                          // dO
-    uint8_t* sK = sG + C::BYTES;                          // NST x K chunk
+    uint8_t* sG = sQ + NQ * C::BYTES;                     // dO
+    uint8_t* sK = sG + NQ * C::BYTES;                     // NST x K chunk
     uint8_t* sV = sK + NST * C::BYTES;                    // NST x V chunk
     uint8_t* sOut = sV + NST * C::BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + C::OUT_BYTES);
-    uint64_t* q_full = bars;                 //     TMA -> MMA: Q and dO
-    uint64_t* q_empty = bars + 1;            //     MMA (commit) -> TMA
-    uint64_t* dq_full = bars + 2;            //     MMA (commit) -> epilogue
-    uint64_t* dq_free = bars + 3;            //     epilogue -> MMA
-    uint64_t* dp_full = bars + 4;            //     MMA (commit) -> softmax
-    uint64_t* ds_full = bars + 5;            //     softmax -> MMA
-    uint64_t* s_full = bars + 6;             // [2] MMA (commit) -> softmax
-    uint64_t* s_free = bars + 8;             // [2] softmax -> MMA: S is in registers
+    uint64_t* q_full = bars;                 // [2] TMA -> MMA: Q and dO
+    uint64_t* q_empty = bars + 2;            // [2] MMA (commit) -> TMA
+    uint64_t* s_full = bars + 4;             // [2] MMA (commit) -> softmax
+    uint64_t* s_free = bars + 6;             // [2] softmax -> MMA: S is in registers
+    uint64_t* dq_full = bars + 8;            //     MMA (commit) -> epilogue
+    uint64_t* dq_free = bars + 9;            //     epilogue -> MMA
+    uint64_t* dp_full = bars + 10;           //     MMA (commit) -> softmax
+    uint64_t* ds_full = bars + 11;           //     softmax -> MMA
     uint64_t* k_full = bars + 12;            // [4] TMA -> MMA: K and V chunk
     uint64_t* k_empty = bars + 16;           // [4] MMA (commit) -> TMA
     uint64_t* k_clear = bars + 20;           // [4] warp 11 -> MMA
@@ -85,13 +86,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 
     if (tid == 0) {
         wait_state_init(wctx.st, errors, kWaitLimitNs);
-        mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
         mbar_init(dq_full, 1);
         mbar_init(dq_free, 4);
         mbar_init(dp_full, 1);
         mbar_init(ds_full, 8);
         for (int i = 0; i < 2; ++i) {
+            mbar_init(q_full + i, 1);
+            mbar_init(q_empty + i, 1);
             mbar_init(s_full + i, 1);
             mbar_init(s_free + i, 8);
         }
@@ -121,7 +122,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 
     // my items: with a causal mask the longer tiles first
     auto tile_of = [&](int item) {
-        return g.causal ? RowTile(g, item % g.units, g.tiles - 1 - item / g.units) : RowTile(g, item / g.tiles, item % g.tiles);
+        int unit, tile;
+        if (g.causal) {
+            tile = g.tiles - 1 - g.by_units.split(item, unit);
+        } else {
+            unit = g.by_tiles.split(item, tile);
+        }
+        return RowTile(g, unit, tile);
     };
     auto chunks_of = [&](const RowTile& t) { return (t.keys(g) + kRows - 1) / kRows; };
 
@@ -136,12 +143,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 const RowTile t = tile_of(item);
                 const int n = chunks_of(t);
                 if (n == 0) continue;
-                if (!lt.acquire(q_empty, (it & 1) ^ 1, wctx)) break;
-                lt.arm(q_full, it & 1, 2 * C::load_bytes(g.hp * g.tt));
+                const uint32_t to = it % NQ, phase = (it / NQ) & 1;
+                if (!lt.acquire(q_empty + to, phase ^ 1, wctx)) break;
+                lt.arm(q_full + to, phase, 2 * C::load_bytes(g.hp * g.tt));
 #pragma unroll
                 for (int s = 0; s < C::NS; ++s) {
-                    tma_load_5d(sQ + s * C::SLAB, &tm_q, q_full, s * 64, t.t0, t.h0, t.b, 0);
-                    tma_load_5d(sG + s * C::SLAB, &tm_do, q_full, s * 64, t.t0, t.h0, t.b, 0);
+                    tma_load_5d(sQ + to * C::BYTES + s * C::SLAB, &tm_q, q_full + to, s * 64, t.t0, t.h0, t.b, 0);
+                    tma_load_5d(sG + to * C::BYTES + s * C::SLAB, &tm_do, q_full + to, s * 64, t.t0, t.h0, t.b, 0);
                 }
                 ++it;
                 for (int c = 0; c < n; ++c) {
@@ -206,7 +214,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             mbar_wait(s_free + (ns & 1), ((ns >> 1) & 1) ^ 1, wctx, kErrMmaWait);
             tc_fence_after();
             if (elect_one()) {
-                product(tmem_base + C::TMEM_S + (ns & 1) * kRows, q_lo, k_lo0 + rs.at * (C::BYTES >> 4));
+                product(tmem_base + C::TMEM_S + (ns & 1) * kRows, q_lo + it % NQ * (C::BYTES >> 4), k_lo0 + rs.at * (C::BYTES >> 4));
                 umma_commit(s_full + (ns & 1));
             }
             __syncwarp();
@@ -215,24 +223,29 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         };
         auto grads = [&](bool last) {        // (its chunk has landed: S came before)
             if (elect_one()) {
-                product(tmem_base + C::TMEM_DP, g_lo, v_lo0 + rp.at * (C::BYTES >> 4));
+                product(tmem_base + C::TMEM_DP, g_lo + it % NQ * (C::BYTES >> 4), v_lo0 + rp.at * (C::BYTES >> 4));
                 umma_commit(dp_full);
-                if (last) umma_commit(q_empty);
+                if (last) umma_commit(q_empty + it % NQ);
             }
             __syncwarp();
             rp.next(NST);
         };
+        int next = (int)blockIdx.x < items ? chunks_of(tile_of(blockIdx.x)) : 0;
         for (int item = blockIdx.x; item < items; item += gridDim.x) {
-            const int n = chunks_of(tile_of(item));
+            const int n = next;
+            next = item + (int)gridDim.x < items ? chunks_of(tile_of(item + gridDim.x)) : 0;      // (ahead: a length is a load from memory)
             if (n == 0) continue;
-            mbar_wait(q_full, it & 1, wctx, kErrLoadWait);
+            mbar_wait(q_full + it % NQ, (it / NQ) & 1, wctx, kErrLoadWait);
             scores();
             grads(n == 1);                   // (dS of the chunk before has been read: dQ came before on the pipe)
             for (int c = 0; c < n; ++c, ++no) {
+                if (lane == 0) NA2D_TR(2, 0, no);
                 if (c + 1 < n) scores();
+                if (lane == 0) NA2D_TR(2, 1, no);
                 if (c == 0) mbar_wait(dq_free, (it & 1) ^ 1, wctx, kErrMmaWait);
                 mbar_wait(ds_full, no & 1, wctx, kErrMmaWait);
                 tc_fence_after();
+                if (lane == 0) NA2D_TR(2, 2, no);
                 if (elect_one()) {
                     const uint32_t km_lo = km_lo0 + ro.at * (C::BYTES >> 4);
 #pragma unroll
@@ -244,6 +257,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 }
                 __syncwarp();
                 ro.next(NST);
+                if (lane == 0) NA2D_TR(2, 3, no);
                 if (c + 1 < n) grads(c + 2 == n);
             }
             ++it;
@@ -331,8 +345,10 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             const int seen = (ok ? keys_seen(g, tile.count, t) : 0) - 64 * half;
             for (int c = 0; c < chunks; ++c, ++m) {
                 uint64_t pr[32];
+                if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 0, m);
                 mbar_wait(s_full + (m & 1), (m >> 1) & 1, wctx, kErrMmaWait);
                 tc_fence_after();
+                if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 1, m);
                 if (!idle) {
                     uint32_t s[2][32];
                     const uint32_t s_addr = tmem_lane + C::TMEM_S + (m & 1) * kRows + 64 * half;
@@ -350,34 +366,36 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 } else if (lane == 0) {
                     mbar_arrive(s_free + (m & 1));
                 }
+                if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 2, m);
                 mbar_wait(dp_full, m & 1, wctx, kErrMmaWait);
                 tc_fence_after();
+                if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 3, m);
                 if (!idle) {
+                    uint32_t dp[2][32], w[2][16];
+                    tmem_ld_32x32(dp_addr, dp[0]);
+                    tmem_ld_32x32(dp_addr + 32, dp[1]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e2 = 0; e2 < 32; ++e2)
+                        pr[e2] = mul2(pr[e2], add2(pair2(dp[e2 / 16][2 * (e2 % 16)], dp[e2 / 16][2 * (e2 % 16) + 1]), delta2));
                     const int open = seen - c * kRows;       // columns of this half that the row sees
-                    const bool cover = __any_sync(0xffffffffu, open < 64);
+                    if (__any_sync(0xffffffffu, open < 64)) {
+                        // by selection: columns that are not seen may hold anything
 #pragma unroll
-                    for (int a = 0; a < 2; ++a) {
-                        uint32_t dp[32], w[16];
-                        tmem_ld_32x32(dp_addr + 32 * a, dp);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e2 = 0; e2 < 16; ++e2) {
-                            const uint64_t ds = mul2(pr[16 * a + e2], add2(pair2(dp[2 * e2], dp[2 * e2 + 1]), delta2));
-                            float d0 = lo2(ds), d1 = hi2(ds);
-                            if (cover) {                     // by selection: columns that are not seen may hold anything
-                                if (32 * a + 2 * e2 >= open) d0 = 0.f;
-                                if (32 * a + 2 * e2 + 1 >= open) d1 = 0.f;
-                            }
-                            w[e2] = pack2<DT>(d0, d1);
-                        }
-                        // (over columns of dP that this warp has read: the first half of its own)
-                        tmem_st_32x16(dp_addr + 16 * a, w);
+                        for (int e = 0; e < 64; e += 2)
+                            pr[e / 2] = pair2(e >= open ? 0.f : lo2(pr[e / 2]), e + 1 >= open ? 0.f : hi2(pr[e / 2]));
                     }
+#pragma unroll
+                    for (int e2 = 0; e2 < 32; ++e2) w[e2 / 16][e2 % 16] = pack2<DT>(lo2(pr[e2]), hi2(pr[e2]));
+                    // (over columns of dP that this warp has read: the first half of its own)
+                    tmem_st_32x16(dp_addr, w[0]);
+                    tmem_st_32x16(dp_addr + 16, w[1]);
                     tmem_st_wait();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ds_full);
+                if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 4, m);
             }
         }
     }

@@ -32,7 +32,7 @@ int by_head_dim(int C, F&& f) {
 
 int NA2D_TC_NAME(forward)(const Place& at, const Geom& g, const Parts& parts, const Operand& q, const Operand& k, const Operand& v,
                           const Operand& o, float* lse) {
-    FwdCut cut{parts.count, (g.tiles + 1) / 2, 0, parts.a, parts.b};
+    FwdCut cut{parts.count, (g.tiles + 1) / 2, 0, Div(parts.count), Div((g.tiles + 1) / 2), parts.a, parts.b};
     const long long items = g.tiles > 1 ? (long long)g.units * cut.pairs * cut.splits : ((long long)g.units * cut.splits + 1) / 2;
     if (items > 0x3fffffffLL) return NA2D_ERR_TOO_LARGE;
     cut.items = (int)items;
@@ -49,7 +49,8 @@ int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Parts& parts, c
         if (rc != NA2D_OK || !x.d_k.ptr) return rc;
         Geom gk = g;
         if (g.causal) cut_rows(gk, false);               // a chunk's masks go by the column alone
-        KeyCut cut{(g.Tk + kRows - 1) / kRows, parts.count, 0, parts.a, parts.b};
+        const int key_tiles = (g.Tk + kRows - 1) / kRows;
+        KeyCut cut{key_tiles, parts.count, 0, Div(parts.count), Div(key_tiles), parts.a, parts.b};
         const long long items = (long long)gk.units * cut.key_tiles * cut.splits;
         if (items > 0x3fffffffLL) return (int)NA2D_ERR_TOO_LARGE;
         cut.items = (int)items;
@@ -58,23 +59,30 @@ int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Parts& parts, c
 }
 
 #if NA2D_TC_DT == 1
-// Parts of the keys in the forward: where the tiles are fewer than the SMs (two tiles a CTA), so many that every CTA has two parts
-// to its two groups twice over, each of at least 4 chunks.
+// Parts of the keys in the forward: where the tiles are fewer than the groups that the SMs have (two a CTA), so many that each group has
+// about eight, since lengths that differ make parts that differ; of at least 4 chunks each.
 int forward_parts(const Geom& g, int sms) {
     const long long tiles = (long long)g.units * g.tiles;
     const int chunks = (g.Tk + kRows - 1) / kRows;
     if (tiles >= 2 * sms) return 1;
-    const long long want = (4LL * sms + tiles - 1) / tiles;
+    const long long want = (16LL * sms + tiles - 1) / tiles;
     return (int)std::max(1LL, std::min<long long>(want, chunks / 4));
 }
 
-// Parts of the queries in the key half, by the same rule with one tile a CTA.
+// Parts of the queries in the key half, by the same rule with one tile a CTA, and fewer: a part costs its sums' way through memory.
 int key_parts(const Geom& g, int sms) {
     const long long tiles = (long long)g.units * ((g.Tk + kRows - 1) / kRows);
     if (tiles >= sms) return 1;
-    const long long want = (2LL * sms + tiles - 1) / tiles;
+    const long long want = (4LL * sms + tiles - 1) / tiles;
     return (int)std::max(1LL, std::min<long long>(want, g.tiles / 4));
 }
 #endif
 
 }  // namespace na2d_attn
+
+#ifdef NA2D_TRACE
+// Development aid: the trace that CTA 0 of this unit's kernels recorded (see na2d_tc.cuh).
+extern "C" int NA2D_TC_NAME(na2d_debug_trace_attn)(unsigned long long* out, int max_entries) {
+    return na2d_tc::copy_trace(out, max_entries);
+}
+#endif
