@@ -40,7 +40,7 @@ struct Geom {
     int B, N, Nk, G, Tq, Tk, C;
     int units;                              // B * Nk
     int hp, tt;                             // heads and tokens of a query tile
-    int tiles_t, tiles;                     // query tiles along the tokens, and in all, of a unit
+    int tiles_t, groups, tiles;             // query tiles of a unit: along the tokens, (groups of) heads, in all
     int causal;
     const int* lengths;                     // (B,) on the device, or null
     float scale, sl2;                       // the softmax scale, and times log2(e)
@@ -54,9 +54,10 @@ inline void cut_rows(Geom& g, bool pack = true) {
     g.hp = 1;
     for (int h = 2; pack && h <= g.G && (long long)h * g.Tq <= kRows; ++h)
         if (g.G % h == 0) g.hp = h;
-    g.tt = g.hp > 1 ? g.Tq : kRows;
+    g.tt = g.Tq < kRows ? g.Tq : kRows;
     g.tiles_t = g.hp > 1 ? 1 : (g.Tq + kRows - 1) / kRows;
-    g.tiles = g.tiles_t * (g.G / g.hp);
+    g.groups = g.G / g.hp;
+    g.tiles = g.tiles_t * g.groups;
     g.by_nk = Div(g.Nk);
     g.by_tt = Div(g.tt);
     g.by_tiles_t = Div(g.tiles_t);

@@ -67,20 +67,8 @@ int make_problem(const na2d_attention_args* a, Problem* p) {
     return NA2D_OK;
 }
 
-// Floats of one part's results: o and lse, or dK and dV.
-size_t part_floats(const Geom& g, bool backward) {
-    return backward ? 2 * (size_t)g.units * g.Tk * g.C : (size_t)g.B * g.N * g.Tq * (g.C + 1);
-}
-
-// As many parts as the call is best cut into and the workspace holds.
-na2d_attn::Parts parts_for(const na2d_attention_args* a, const Geom& g, bool backward) {
-    const int sms = na2d_tc::sm_count(a->device);
-    const int want = backward ? na2d_attn::key_parts(g, sms) : na2d_attn::forward_parts(g, sms);
-    const size_t floats = part_floats(g, backward), room = a->workspace ? a->workspace_bytes / sizeof(float) / floats : 0;
-    const int count = (size_t)want <= room ? want : (int)room;
-    if (count <= 1) return na2d_attn::Parts{1, nullptr, nullptr};
-    float* at = static_cast<float*>(a->workspace);
-    return na2d_attn::Parts{count, at, at + (size_t)count * (backward ? floats / 2 : (size_t)g.B * g.N * g.Tq * g.C)};
+na2d_attn::Scratch scratch_of(const na2d_attention_args* a) {
+    return na2d_attn::Scratch{static_cast<float*>(a->workspace), a->workspace ? a->workspace_bytes / sizeof(float) : 0};
 }
 
 int place(const na2d_attention_args* a, int* launched, na2d_attn::Place* at) {
@@ -109,9 +97,9 @@ int na2d_attention_forward(const na2d_attention_args* a) {
         if (!p.tensor) {
             rc = na2d_attn::simt_forward(at, p.g, p.q, p.k, p.v, p.o, a->lse);
         } else {
-            const na2d_attn::Parts parts = parts_for(a, p.g, false);
-            rc = a->dtype == NA2D_BF16 ? na2d_attn::forward_bf16(at, p.g, parts, p.q, p.k, p.v, p.o, a->lse)
-                                       : na2d_attn::forward_f16(at, p.g, parts, p.q, p.k, p.v, p.o, a->lse);
+            const na2d_attn::Scratch scratch = scratch_of(a);
+            rc = a->dtype == NA2D_BF16 ? na2d_attn::forward_bf16(at, p.g, scratch, p.q, p.k, p.v, p.o, a->lse)
+                                       : na2d_attn::forward_f16(at, p.g, scratch, p.q, p.k, p.v, p.o, a->lse);
         }
         return finish(rc, launched, "attention forward launch");
     });
@@ -131,8 +119,8 @@ int na2d_attention_backward(const na2d_attention_args* a) {
         if (!p.tensor) {
             rc = na2d_attn::simt_backward(at, p.g, x);
         } else {
-            const na2d_attn::Parts parts = parts_for(a, p.g, true);
-            rc = a->dtype == NA2D_BF16 ? na2d_attn::backward_bf16(at, p.g, parts, x) : na2d_attn::backward_f16(at, p.g, parts, x);
+            const na2d_attn::Scratch scratch = scratch_of(a);
+            rc = a->dtype == NA2D_BF16 ? na2d_attn::backward_bf16(at, p.g, scratch, x) : na2d_attn::backward_f16(at, p.g, scratch, x);
         }
         return finish(rc, launched, "attention backward launch");
     });
@@ -142,8 +130,7 @@ size_t na2d_attention_workspace(const na2d_attention_args* a, int backward) {
     Problem p;
     if (make_problem(a, &p) != NA2D_OK || !p.tensor || (backward && !a->d_k.ptr)) return 0;
     const int sms = na2d_tc::sm_count(a->device);
-    const int parts = backward ? na2d_attn::key_parts(p.g, sms) : na2d_attn::forward_parts(p.g, sms);
-    return parts > 1 ? parts * part_floats(p.g, backward != 0) * sizeof(float) : 0;
+    return (backward ? na2d_attn::key_floats(p.g, sms) : na2d_attn::forward_floats(p.g, sms)) * sizeof(float);
 }
 
 }  // extern "C"

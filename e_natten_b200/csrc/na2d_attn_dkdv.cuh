@@ -25,6 +25,7 @@ struct KeyCut {
     int key_tiles;
     int splits;
     int items;
+    int each;               // chunks of a part
     Div by_splits, by_key_tiles;
     float* part_dk;         // (splits, B, Nk, Tk, C), where splits > 1
     float* part_dv;
@@ -49,9 +50,9 @@ struct KeyItem {
         const int t_min = g.causal ? max(k0 + g.Tq - count, 0) : 0;        // the first token that sees the tile
         lo = t_min / kRows;
         per_head = k0 < count && t_min < g.Tq ? g.tiles_t - lo : 0;
-        int end;
-        part_of(cut.by_splits, per_head * (g.G / g.hp), split, first, end);
-        n = end - first;
+        const int all = per_head * g.groups;
+        first = min(split * cut.each, all);
+        n = min(cut.each, all - first);
         head = per_head > 0 ? first / per_head : 0;
         in_head = first - head * per_head;
     }

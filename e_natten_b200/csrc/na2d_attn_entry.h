@@ -6,15 +6,17 @@
 
 namespace na2d_attn {
 
-// Rows of o, or of dK and dV, computed in parts: how many, and where the parts go (fp32; null with one part).
-struct Parts {
-    int count;
-    float *a, *b;           // forward: o and lse; key half: dK and dV
+// Scratch for results that are computed in parts (fp32): with less than *_floats() of it there are fewer parts.
+struct Scratch {
+    float* at;
+    size_t floats;
 };
+size_t forward_floats(const Geom& g, int sms);
+size_t key_floats(const Geom& g, int sms);
 
 // 16 bits, C a multiple of 8 up to 128, every operand on 16-byte boundaries; o, d_q, d_k and d_v dense.
-int forward_bf16(const Place& at, const Geom& g, const Parts& parts, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);
-int forward_f16(const Place& at, const Geom& g, const Parts& parts, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);
+int forward_bf16(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);
+int forward_f16(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);
 
 // d_q.ptr or d_k.ptr (with d_v.ptr) may be null: that half is left out.  Writes delta.
 struct Backward {
@@ -22,12 +24,8 @@ struct Backward {
     const float* lse;
     float* delta;
 };
-int backward_bf16(const Place& at, const Geom& g, const Parts& parts, const Backward& x);
-int backward_f16(const Place& at, const Geom& g, const Parts& parts, const Backward& x);
-
-// Parts that a call is best cut into.
-int forward_parts(const Geom& g, int sms);
-int key_parts(const Geom& g, int sms);
+int backward_bf16(const Place& at, const Geom& g, const Scratch& scratch, const Backward& x);
+int backward_f16(const Place& at, const Geom& g, const Scratch& scratch, const Backward& x);
 
 // CUDA cores: any strides, C up to kSimtMaxC, fp32 and 16 bits.
 constexpr int kSimtMaxC = 256;

@@ -5,8 +5,10 @@
 // 128; on the tensor pipe a group's P V(c) S(c + 1) run under the other group's exponentials.  PAIR: the two tiles are neighbours of
 // one unit and share every chunk of K and V in shared memory; else (units of a single tile) each has its own.
 //
-// Few rows and many keys: the keys of a tile are cut into `splits` parts, each an item of its own, whose o (fp32) and lse go to a
-// workspace and are joined by combine_kernel.
+// Few rows and many keys: the keys of a row are taken in parts, whose o (fp32) and lse go to a workspace and are joined by
+// attn_combine_kernel.  Units of several tiles: `splits` parts of each, every one an item.  Units of one tile (single tokens on caches): all
+// units' chunks lie on one line, of which every group takes the same length, wherever units begin and end; with parts of a unit for
+// items, caches of different lengths left some CTAs 1.4 times the mean's work (16 x 4 caches of up to 32768 keys: 141 us).
 //
 //   warps 0-7   softmax: a thread owns a row, reads its 128 scores, writes P over S as packed 16-bit pairs;
 //   warp 8      producer of Q, K and V;    warps 9, 11  MMA issue, one a group: a warp that served both in turn had 3000 cycles of
@@ -41,69 +43,144 @@ struct FwdCut {
     int splits;
     int pairs;              // PAIR: items of a unit and split
     int items;
+    int each;               // chunks of a part
+    int line;               // not PAIR: the chunks of all units on one line, that many groups take; 0: not
     Div by_splits, by_pairs;
-    float* part_o;          // (splits, B, N, Tq, C), where splits > 1
-    float* part_lse;        // (splits, B, N, Tq)
+    float* part_o;          // (splits, B, N, Tq, C), where splits > 1; line: (groups + units, rows of a unit, C)
+    float* part_lse;        // (splits, B, N, Tq); line: (groups + units, rows of a unit)
 };
 
 // One group's half of an item: chunks [c0, c0 + n) of a tile.
 struct FwdPart {
     RowTile tile;
     bool any;               // there is a tile
-    int split, c0, n;
+    int slot, c0, n;        // slot: the part's place in the workspace
 };
 
-// Chunks [c0, c1) of part `split` of `chunks`: as many for each part, fewer for the last ones.
-__device__ __forceinline__ void part_of(const Div& by_splits, int chunks, int split, int& c0, int& c1) {
-    if (by_splits.d == 1) {
-        c0 = 0;
-        c1 = chunks;
-        return;
+// Batch entries on the line, at most (units are fewer than the groups where it is used).
+constexpr int kLineEntries = 1024;
+// before[b]: chunks of one key head of the entries before b; of all of them at before[B].  Written by one warp.
+__device__ __forceinline__ void line_table(const Geom& g, int* before, int lane) {
+    int sum = 0;
+    for (int b0 = 0; b0 < g.B; b0 += 32) {
+        int n = b0 + lane < g.B ? (key_count(g, b0 + lane) + kRows - 1) / kRows : 0;
+        const int own = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, n, d);
+            if (lane >= d) n += up;
+        }
+        if (b0 + lane < g.B) before[b0 + lane] = sum + n - own;
+        sum += __shfl_sync(0xffffffffu, n, 31);
     }
-    const int each = by_splits.quotient(chunks + (int)by_splits.d - 1);
-    c0 = min(split * each, chunks);
-    c1 = min(c0 + each, chunks);
+    if (lane == 0) before[g.B] = sum;
 }
+// A group's stretch [at, end) of the line, and the unit that `at` lies in.
+struct Stretch {
+    int at, end, b, m;
+    __device__ __forceinline__ void start(const Geom& g, const int* before, int group, int groups) {
+        const int all = before[g.B] * g.Nk, each = (all + groups - 1) / max(groups, 1);
+        at = min(group * each, all);
+        end = min(at + each, all);
+        if (at >= end) return;
+        int lo = 0, hi = g.B;                            // before[lo] <= at's < before[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (before[mid] * g.Nk <= at) lo = mid;
+            else hi = mid;
+        }
+        b = lo;
+        m = (at - before[b] * g.Nk) / (before[b + 1] - before[b]);
+    }
+    __device__ __forceinline__ bool any() const { return at < end; }
+    __device__ __forceinline__ int length(const int* before) const { return before[b + 1] - before[b]; }       // of the unit
+    __device__ __forceinline__ int first(const Geom& g, const int* before) const { return before[b] * g.Nk + m * length(before); }
+    // to the next unit
+    __device__ __forceinline__ void next(const Geom& g, const int* before) {
+        at = min(end, first(g, before) + length(before));
+        if (at < end && ++m == g.Nk) {
+            m = 0;
+            do ++b;
+            while (length(before) == 0);                 // (at < end: there is one)
+        }
+    }
+};
 
+// The items of a CTA, which every role walks by itself.
 template <bool PAIR>
-__device__ __forceinline__ void fwd_parts(const Geom& g, const FwdCut& cut, int item, FwdPart (&p)[2]) {
-    if constexpr (PAIR) {
-        int split, pair, unit;
-        const int rest = cut.by_splits.split(item, split);
-        if (g.causal) {     // the later tiles are the longer ones: they go first, so that no CTA is left with one at the end
-            pair = cut.pairs - 1 - g.by_units.split(rest, unit);
-        } else {
-            unit = cut.by_pairs.split(rest, pair);
-        }
-        int chunks[2], most = 0;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            p[x].any = 2 * pair + x < g.tiles;
-            p[x].tile = RowTile(g, unit, p[x].any ? 2 * pair + x : 2 * pair);
-            chunks[x] = p[x].any ? (p[x].tile.keys(g) + kRows - 1) / kRows : 0;
-            most = max(most, chunks[x]);
-        }
-        int c0, c1;
-        part_of(cut.by_splits, most, split, c0, c1);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            p[x].split = split;
-            p[x].c0 = c0;
-            p[x].n = max(min(chunks[x], c1) - c0, 0);
-        }
-    } else {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int f = 2 * item + x;
-            int unit, c1;
-            p[x].any = f < g.units * cut.splits;
-            p[x].split = g.by_units.split(p[x].any ? f : 0, unit);
-            p[x].tile = RowTile(g, unit, 0);
-            part_of(cut.by_splits, (p[x].tile.keys(g) + kRows - 1) / kRows, p[x].split, p[x].c0, c1);
-            p[x].n = p[x].any ? c1 - p[x].c0 : 0;
+struct FwdWalk {
+    int item;
+    Stretch s[2];
+    __device__ __forceinline__ FwdWalk(const Geom& g, const FwdCut& cut, const int* before) : item(blockIdx.x) {
+        if constexpr (!PAIR) {
+            if (cut.line) {
+                s[0].start(g, before, 2 * blockIdx.x, 2 * gridDim.x);
+                s[1].start(g, before, 2 * blockIdx.x + 1, 2 * gridDim.x);
+            }
         }
     }
-}
+    __device__ __forceinline__ bool more(const FwdCut& cut) const {
+        if constexpr (!PAIR)
+            if (cut.line) return s[0].any() || s[1].any();
+        return item < cut.items;
+    }
+    __device__ __forceinline__ void next(const Geom& g, const FwdCut& cut, const int* before) {
+        item += gridDim.x;
+        if constexpr (!PAIR) {
+            if (cut.line) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    if (s[x].any()) s[x].next(g, before);
+            }
+        }
+    }
+    __device__ __forceinline__ void parts(const Geom& g, const FwdCut& cut, const int* before, FwdPart (&p)[2]) const {
+        if constexpr (PAIR) {
+            int split, pair, unit;
+            const int rest = cut.by_splits.split(item, split);
+            if (g.causal) {     // the later tiles are the longer ones: they go first, so that no CTA is left with one at the end
+                pair = cut.pairs - 1 - g.by_units.split(rest, unit);
+            } else {
+                unit = cut.by_pairs.split(rest, pair);
+            }
+            int chunks[2], most = 0;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                p[x].any = 2 * pair + x < g.tiles;
+                p[x].tile = RowTile(g, unit, p[x].any ? 2 * pair + x : 2 * pair);
+                chunks[x] = p[x].any ? (p[x].tile.keys(g) + kRows - 1) / kRows : 0;
+                most = max(most, chunks[x]);
+            }
+            const int c0 = min(split * cut.each, most), c1 = min(c0 + cut.each, most);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                p[x].slot = split;
+                p[x].c0 = c0;
+                p[x].n = max(min(chunks[x], c1) - c0, 0);
+            }
+        } else if (cut.line) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                p[x].any = s[x].any();
+                const int unit = p[x].any ? s[x].b * g.Nk + s[x].m : 0;
+                p[x].tile = RowTile(g, unit, 0);
+                p[x].slot = 2 * blockIdx.x + x + unit;   // from part to part either the group or the unit is one more
+                const int first = p[x].any ? s[x].first(g, before) : 0;
+                p[x].c0 = p[x].any ? s[x].at - first : 0;
+                p[x].n = p[x].any ? min(s[x].end, first + s[x].length(before)) - s[x].at : 0;
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int unit = 2 * item + x;
+                p[x].any = unit < g.units;
+                p[x].tile = RowTile(g, p[x].any ? unit : 0, 0);
+                p[x].slot = p[x].c0 = 0;
+                p[x].n = p[x].any ? (p[x].tile.keys(g) + kRows - 1) / kRows : 0;
+            }
+        }
+    }
+};
 
 // The part's chunk that holds keys beyond its batch entry's (and not beyond Tk, where TMA fills with zeros), or -1.
 __device__ __forceinline__ int fwd_ragged_chunk(const Geom& g, int count, int c0, int n) {
@@ -118,9 +195,10 @@ struct FwdCfg : TileCfg<D> {
     static constexpr int NQ = D == 128 ? 1 : 2;                          // Q tiles of a group
     static constexpr int OUT_BYTES = 4 * 2 * OutStage<32>::BYTES;        // two staging buffers for each epilogue warp
     static constexpr int X_BYTES = 2 * 2 * 2 * kRows * 4;                // row sum, final maximum [group][tile parity][row]
-    static constexpr int SMEM = 2 * NQ * T::BYTES + 2 * NST * T::BYTES + OUT_BYTES + X_BYTES + 512 /*barriers*/ + 1024 /*alignment*/;
+    static constexpr int LINE_BYTES = (kLineEntries + 1) * 4;
+    static constexpr int SMEM = 2 * NQ * T::BYTES + 2 * NST * T::BYTES + OUT_BYTES + X_BYTES + 512 /*barriers*/ + LINE_BYTES + 1024 /*alignment*/;
     static constexpr int TMEM_S = 0, TMEM_O = 256;                       // of group x: S + 128 x, O + D x
-    static_assert(SMEM <= kSmemLimit, "forward kernel shared memory");
+    static_assert(SMEM <= kSmemLimit && NST <= 8, "forward kernel shared memory");
 };
 
 // Logarithm (base 2) by which a row's maximum may grow before its sums are rescaled: the weights stay below 2^8, within fp16 by far,
@@ -137,7 +215,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sQ = smem;                                   // [group][NQ] Q tiles
-    uint8_t* sK = sQ + 2 * NQ * C::BYTES;                 // NST x K chunk
+    uint8_t* sK = sQ + 2 * NQ * C::BYTES;               // NST x K chunk
     uint8_t* sV = sK + NST * C::BYTES;                    // NST x V chunk
     uint8_t* sOut = sV + NST * C::BYTES;                  // output staging
     float* x_sum = reinterpret_cast<float*>(sOut + C::OUT_BYTES);     // [group][tile parity][row]
@@ -147,16 +225,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     uint64_t* q_empty = bars + 4;            // [2][2] MMA (commit) -> TMA
     uint64_t* o_full = bars + 8;             // [2] MMA (commit) -> epilogue
     uint64_t* o_free = bars + 10;            // [2] epilogue -> MMA
-    uint64_t* s_full = bars + 32;            // [2] MMA (commit) -> softmax
-    uint64_t* p_full = bars + 34;            // [2] softmax -> MMA
-    uint64_t* p_half = bars + 36;            // [2] softmax -> MMA: the first 64 columns of P
-    uint64_t* k_full = bars + 12;            // [4] TMA -> MMA
-    uint64_t* k_empty = bars + 16;           // [4] MMA (commit) -> TMA
-    uint64_t* v_full = bars + 20;            // [4] TMA -> MMA
-    uint64_t* v_empty = bars + 24;           // [4] MMA (commit) -> TMA
-    uint64_t* v_clear = bars + 28;           // [4] warp 10 -> MMA: rows beyond the keys are zeros
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 38);
-    const WaitCtx wctx{reinterpret_cast<WaitState*>(bars + 39)};
+    uint64_t* s_full = bars + 52;            // [2] MMA (commit) -> softmax
+    uint64_t* p_full = bars + 54;            // [2] softmax -> MMA
+    uint64_t* p_half = bars + 56;            // [2] softmax -> MMA: the first 64 columns of P
+    uint64_t* k_full = bars + 12;            // [8] TMA -> MMA
+    uint64_t* v_full = bars + 20;            // [8] TMA -> MMA
+    uint64_t* k_empty = bars + 28;           // [8] MMA (commit) -> TMA
+    uint64_t* v_empty = bars + 36;           // [8] MMA (commit) -> TMA
+    uint64_t* v_clear = bars + 44;           // [8] warp 10 -> MMA: rows beyond the keys are zeros
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 58);
+    const WaitCtx wctx{reinterpret_cast<WaitState*>(bars + 59)};
+    int* before = reinterpret_cast<int*>(bars + 64);      // the line's table
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -172,6 +251,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         for (int i = 0; i < 4; ++i) {
             mbar_init(q_full + i, 1);
             mbar_init(q_empty + i, 1);
+        }
+        for (int i = 0; i < NST; ++i) {
             mbar_init(k_full + i, 1);
             mbar_init(k_empty + i, PAIR ? 2 : 1);        // a pair's chunks are read by both groups
             mbar_init(v_full + i, 1);
@@ -190,6 +271,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
+    if (!PAIR && warp == 1 && cut.line) line_table(g, before, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -224,9 +306,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     rv.next(NST);
                 }
             };
-            for (int item = blockIdx.x; item < cut.items && lt.ok; item += gridDim.x) {
+            for (FwdWalk<PAIR> walk(g, cut, before); walk.more(cut) && lt.ok; walk.next(g, cut, before)) {
                 FwdPart p[2];
-                fwd_parts<PAIR>(g, cut, item, p);
+                walk.parts(g, cut, before, p);
                 const int most = max(p[0].n, p[1].n);
                 for (int c = 0; c <= most && lt.ok; ++c) {
 #pragma unroll
@@ -255,9 +337,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         reg_dec<kDkvRegsCtl>();
         if (g.lengths) {
             Ring ring;
-            for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
+            for (FwdWalk<PAIR> walk(g, cut, before); walk.more(cut); walk.next(g, cut, before)) {
                 FwdPart p[2];
-                fwd_parts<PAIR>(g, cut, item, p);
+                walk.parts(g, cut, before, p);
                 const int most = max(p[0].n, p[1].n);
                 const int at[2] = {fwd_ragged_chunk(g, p[0].tile.count, p[0].c0, PAIR ? most : p[0].n),
                                    PAIR ? -1 : fwd_ragged_chunk(g, p[1].tile.count, p[1].c0, p[1].n)};
@@ -288,20 +370,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         // Loads of the item that come before the group's chunk c.
         struct Item {
             int n, other;                    // chunks of the group, and of the other one
-            __device__ __forceinline__ Item(const Geom& g, const FwdCut& cut, int item, int x) {
+            __device__ __forceinline__ Item(const Geom& g, const FwdCut& cut, const int* before, const FwdWalk<PAIR>& walk, int x) {
                 n = other = 0;
-                if (item >= cut.items) return;
+                if (!walk.more(cut)) return;
                 FwdPart p[2];
-                fwd_parts<PAIR>(g, cut, item, p);
+                walk.parts(g, cut, before, p);
                 n = x ? p[1].n : p[0].n;
                 other = x ? p[0].n : p[1].n;
             }
             __device__ __forceinline__ uint32_t loads() const { return PAIR ? max(n, other) : n + other; }
-            __device__ __forceinline__ uint32_t before(int c, int x) const { return PAIR ? c : c + min(c + x, other); }
+            __device__ __forceinline__ uint32_t ahead(int c, int x) const { return PAIR ? c : c + min(c + x, other); }
         };
         uint32_t base = 0, chunks = 0, tiles = 0;        // loads, this group's chunks and tiles so far
         auto scores = [&](const Item& t, int c) {
-            const uint32_t at = (base + t.before(c, x)) % NST, phase = ((base + t.before(c, x)) / NST) & 1;
+            const uint32_t at = (base + t.ahead(c, x)) % NST, phase = ((base + t.ahead(c, x)) / NST) & 1;
             if (lane == 0) NA2D_TR(1 + x, 3, chunks + (c > 0));
             mbar_wait(k_full + at, phase, wctx, kErrLoadWait);
             if (lane == 0) NA2D_TR(1 + x, 4, chunks + (c > 0));
@@ -311,8 +393,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     constexpr int kPerSlab = C::SLAB_C / 16;
-                    const int in = (((kk / kPerSlab) * C::SLAB) >> 4) + 2 * (kk % kPerSlab);
-                    umma_ss(t_s, desc64(hi, q_lo + in), desc64(hi, k_lo + in), idesc_s, kk > 0);
+                    const int slab = kk / kPerSlab, in = 2 * (kk % kPerSlab);
+                    umma_ss(t_s, desc64(hi, q_lo + ((slab * C::SLAB) >> 4) + in), desc64(hi, k_lo + ((slab * C::SLAB) >> 4) + in), idesc_s, kk > 0);
                 }
                 umma_commit(s_full + x);                                      // and P V of the group's chunk before
                 umma_commit(k_empty + at);
@@ -321,15 +403,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             }
             __syncwarp();
         };
-        Item t(g, cut, blockIdx.x, x);
-        for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
+        FwdWalk<PAIR> walk(g, cut, before);
+        Item t(g, cut, before, walk, x);
+        while (walk.more(cut)) {
             if (t.n > 0) {
                 mbar_wait(q_full + 2 * x + tiles % NQ, (tiles / NQ) & 1, wctx, kErrLoadWait);
                 scores(t, 0);
             }
-            const Item next(g, cut, item + gridDim.x, x);
+            walk.next(g, cut, before);
+            const Item next(g, cut, before, walk, x);
             for (int c = 0; c < t.n; ++c, ++chunks) {
-                const uint32_t at = (base + t.before(c, x)) % NST, phase = ((base + t.before(c, x)) / NST) & 1;
+                const uint32_t at = (base + t.ahead(c, x)) % NST, phase = ((base + t.ahead(c, x)) / NST) & 1;
                 if (c == 0) mbar_wait(o_free + x, (tiles & 1) ^ 1, wctx, kErrMmaWait);      // the tile before has been read out
                 mbar_wait(v_full + at, phase, wctx, kErrLoadWait);
                 if (g.lengths) mbar_wait(v_clear + at, phase, wctx, kErrOther);
@@ -375,17 +459,19 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const int row = quarter * 32 + lane;                 // row of the tile = tensor-memory lane
         const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         uint8_t* stage = sOut + quarter * 2 * OutStage<32>::BYTES;
-        const bool by_tma = g.hp == 1 && cut.splits == 1;
+        const bool in_parts = cut.splits > 1 || cut.line, by_tma = g.hp == 1 && !in_parts;
+        const size_t part_rows = cut.line ? (size_t)g.G * g.Tq : static_cast<size_t>(g.B) * g.N * g.Tq;     // of the workspace
         uint32_t it[2] = {0, 0}, seq = 0;
-        for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
+        for (FwdWalk<PAIR> walk(g, cut, before); walk.more(cut); walk.next(g, cut, before)) {
             FwdPart p[2];
-            fwd_parts<PAIR>(g, cut, item, p);
+            walk.parts(g, cut, before, p);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 if (!p[x].any) continue;
                 int n, t;
                 const bool ok = p[x].tile.row(g, row, n, t);
                 const size_t at = row_index(g, p[x].tile.b, n, t);
+                const size_t part_at = p[x].slot * part_rows + (cut.line ? (size_t)(n - p[x].tile.m * g.G) * g.Tq + t : at);
                 const bool none = p[x].n == 0;               // no key: zeros
                 float total = 0.f, fin = 0.f;
                 if (!none) {
@@ -419,7 +505,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     if (by_tma) {
                         if (t_first < g.Tq)
                             na2d_tc::stage_and_store<DT, 32, 2>(&tm_o, stage, v, inv, 32 * j, t_first, h_first, p[x].tile.b, 0, lane, &seq);
-                    } else if (ok && cut.splits == 1) {
+                    } else if (ok && !in_parts) {
                         uint4* dst = reinterpret_cast<uint4*>(o_rows + p[x].tile.b * o_st.b + n * o_st.n + t * o_st.t + 32 * j);
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
@@ -431,7 +517,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                                 dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
                             }
                     } else if (ok && !none) {
-                        float4* dst = reinterpret_cast<float4*>(cut.part_o + (p[x].split * (static_cast<size_t>(g.B) * g.N * g.Tq) + at) * g.C + 32 * j);
+                        float4* dst = reinterpret_cast<float4*>(cut.part_o + part_at * g.C + 32 * j);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             if (32 * j + 4 * e < g.C)
@@ -440,7 +526,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     }
                 }
                 if (ok) {
-                    float* to = cut.splits == 1 ? lse + at : cut.part_lse + p[x].split * (static_cast<size_t>(g.B) * g.N * g.Tq) + at;
+                    float* to = in_parts ? cut.part_lse + part_at : lse + at;
                     *to = total == 0.f ? -CUDART_INF_F : (fin + log2f(total)) * kLn2;
                 }
                 if (!none) ++it[x];
@@ -460,9 +546,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         // waiting for their MMAs (4 x 4 x 4096 x 128: 4640 cycles a chunk of either).  Both go through the turns of an item's longer half.
         const uint32_t my_turn = 1 + group, other_turn = 2 - group;
         if (group) bar_arrive(other_turn, 256);              // a goes first
-        for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
+        for (FwdWalk<PAIR> walk(g, cut, before); walk.more(cut); walk.next(g, cut, before)) {
             FwdPart both[2];
-            fwd_parts<PAIR>(g, cut, item, both);
+            walk.parts(g, cut, before, both);
             const FwdPart p = group ? both[1] : both[0];
             const int turns = max(both[0].n, both[1].n);
             int n, t;
@@ -591,33 +677,55 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 template <typename DT>
 __global__ void __launch_bounds__(128)
 attn_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse, DT* __restrict__ o, const Operand o_st,
-                    float* __restrict__ lse, const Geom g, const int splits) {
+                    float* __restrict__ lse, const Geom g, const int splits, const int line_groups) {
     __shared__ float4 sums[3][32];
     after_previous_grid();
     next_grid_may_start();
-    const size_t rows = static_cast<size_t>(g.B) * g.N * g.Tq, row = blockIdx.x;
+    const size_t row = blockIdx.x, bn = row / g.Tq;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int t = (int)(row % g.Tq), c = 4 * lane, b = (int)(bn / g.N), n = (int)(bn - (size_t)b * g.N);
+    // the row's parts: places first, first + stride, ... of the workspace
+    size_t first = row, stride = static_cast<size_t>(g.B) * g.N * g.Tq;
+    int parts = splits;
+    if (line_groups > 0) {
+        int before = 0, all = 0;                         // chunks of one key head of the entries before b, and of all
+        for (int i = lane; i < g.B; i += 32) {
+            const int chunks = (key_count(g, i) + kRows - 1) / kRows;
+            all += chunks;
+            if (i < b) before += chunks;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            all += __shfl_xor_sync(0xffffffffu, all, d);
+            before += __shfl_xor_sync(0xffffffffu, before, d);
+        }
+        all *= g.Nk;
+        const int m = n / g.G, each = max(1, (all + line_groups - 1) / line_groups);
+        const int chunks = (key_count(g, b) + kRows - 1) / kRows, at = before * g.Nk + m * chunks;
+        const int lo = at / each, hi = (at + chunks - 1) / each;         // groups that have some of them
+        parts = chunks > 0 ? hi - lo + 1 : 0;
+        stride = static_cast<size_t>(g.G) * g.Tq;
+        first = (lo + b * g.Nk + m) * stride + static_cast<size_t>(n - m * g.G) * g.Tq + t;
+    }
     float top = -CUDART_INF_F;
-    for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[s * rows + row]);
+    for (int s = lane; s < parts; s += 32) top = fmaxf(top, part_lse[first + s * stride]);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     // (a NaN of a part stays one: the maximum skips it, its weight does not)
     const float base = top == -CUDART_INF_F ? 0.f : top;
     float total = 0.f;
-    for (int s = lane; s < splits; s += 32) total += expf(part_lse[s * rows + row] - base);
+    for (int s = lane; s < parts; s += 32) total += expf(part_lse[first + s * stride] - base);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    const int t = (int)(row % g.Tq), c = 4 * lane;
-    const size_t bn = row / g.Tq;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (c < g.C) {
 #pragma unroll 4
-        for (int s = warp; s < splits; s += 4) {
-            const float part = part_lse[s * rows + row];
+        for (int s = warp; s < parts; s += 4) {
+            const float part = part_lse[first + s * stride];
             if (part == -CUDART_INF_F) continue;             // nothing was written for it
             const float w = expf(part - base) * inv;
-            const float4 v = *reinterpret_cast<const float4*>(part_o + (s * rows + row) * g.C + c);
+            const float4 v = *reinterpret_cast<const float4*>(part_o + (first + s * stride) * g.C + c);
             acc.x = fmaf(w, v.x, acc.x);
             acc.y = fmaf(w, v.y, acc.y);
             acc.z = fmaf(w, v.z, acc.z);
@@ -633,9 +741,19 @@ attn_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ 
         acc.z += sums[w][lane].z;
         acc.w += sums[w][lane].w;
     }
-    DT* dst = o + (bn / g.N) * o_st.b + (bn % g.N) * o_st.n + t * o_st.t;
+    DT* dst = o + b * o_st.b + n * o_st.n + t * o_st.t;
     *reinterpret_cast<uint2*>(dst + c) = make_uint2(pack2<DT>(acc.x, acc.y), pack2<DT>(acc.z, acc.w));
     if (lane == 0) lse[row] = total == 0.f ? -CUDART_INF_F : base + logf(total);
+}
+
+template <typename DT>
+int launch_combine(const Place& at, const Geom& g, const FwdCut& cut, const Operand& o, float* lse) {
+    const long long rows = (long long)g.B * g.N * g.Tq;
+    *at.launched += 1;
+    return na2d_launch::launch(true, attn_combine_kernel<DT>, (unsigned)rows, 128, 0, at.st, (const float*)cut.part_o,
+                               (const float*)cut.part_lse, (DT*)o.ptr, o, lse, g, cut.splits, cut.line) == cudaSuccess
+               ? NA2D_OK
+               : NA2D_ERR_CUDA;
 }
 
 template <typename DT, int D, bool PAIR>
@@ -653,22 +771,18 @@ int launch_fwd_as(const Place& at, const Geom& g, const FwdCut& cut, const Opera
     if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted) != cudaSuccess) return NA2D_ERR_CUDA;
     const int sms = na2d_tc::sm_count(at.device);
     *at.launched += 1;
-    if (na2d_launch::launch(false, kern, cut.items < sms ? cut.items : sms, 512, C::SMEM, at.st, tq, tk, tv, to, (DT*)o.ptr, o, lse,
+    const int grid = cut.line ? cut.line / 2 : cut.items < sms ? cut.items : sms;
+    if (na2d_launch::launch(false, kern, grid, 512, C::SMEM, at.st, tq, tk, tv, to, (DT*)o.ptr, o, lse,
                             at.errors, g, cut) != cudaSuccess)
         return NA2D_ERR_CUDA;
-    if (cut.splits == 1) return NA2D_OK;
-    const long long rows = (long long)g.B * g.N * g.Tq;
-    *at.launched += 1;
-    return na2d_launch::launch(true, attn_combine_kernel<DT>, (unsigned)rows, 128, 0, at.st, (const float*)cut.part_o,
-                               (const float*)cut.part_lse, (DT*)o.ptr, o, lse, g, cut.splits) == cudaSuccess
-               ? NA2D_OK
-               : NA2D_ERR_CUDA;
+    return cut.splits == 1 && !cut.line ? NA2D_OK : launch_combine<DT>(at, g, cut, o, lse);
 }
 
 template <typename DT, int D>
 int launch_fwd(const Place& at, const Geom& g, const FwdCut& cut, const Operand& q, const Operand& k, const Operand& v,
                const Operand& o, float* lse) {
-    return g.tiles > 1 ? launch_fwd_as<DT, D, true>(at, g, cut, q, k, v, o, lse) : launch_fwd_as<DT, D, false>(at, g, cut, q, k, v, o, lse);
+    if (g.tiles > 1) return launch_fwd_as<DT, D, true>(at, g, cut, q, k, v, o, lse);
+    return launch_fwd_as<DT, D, false>(at, g, cut, q, k, v, o, lse);
 }
 
 }  // namespace na2d_attn

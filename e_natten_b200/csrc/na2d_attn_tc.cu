@@ -3,6 +3,7 @@
 #include "na2d_attn_entry.h"
 #include "na2d_delta.cuh"
 #include "na2d_attn_fwd.cuh"
+#include "na2d_attn_few.cuh"
 #include "na2d_attn_dq.cuh"
 #include "na2d_attn_dkdv.cuh"
 
@@ -28,18 +29,70 @@ int by_head_dim(int C, F&& f) {
     return f(std::integral_constant<int, 128>{});
 }
 
-}  // namespace
+// Whether the chunks of all units go on one line: units of one tile, fewer than the groups of the SMs (two a CTA).
+bool on_line(const Geom& g, int sms) { return g.tiles == 1 && g.units < 2 * sms && g.B <= kLineEntries && g.Tk > kRows; }
 
-int NA2D_TC_NAME(forward)(const Place& at, const Geom& g, const Parts& parts, const Operand& q, const Operand& k, const Operand& v,
-                          const Operand& o, float* lse) {
-    FwdCut cut{parts.count, (g.tiles + 1) / 2, 0, Div(parts.count), Div((g.tiles + 1) / 2), parts.a, parts.b};
-    const long long items = g.tiles > 1 ? (long long)g.units * cut.pairs * cut.splits : ((long long)g.units * cut.splits + 1) / 2;
-    if (items > 0x3fffffffLL) return NA2D_ERR_TOO_LARGE;
-    cut.items = (int)items;
-    return by_head_dim(g.C, [&](auto d) { return launch_fwd<NA2D_TC_TYPE, decltype(d)::value>(at, g, cut, q, k, v, o, lse); });
+// Whether the kernel for few rows takes them.
+bool few_rows(const Geom& g) { return g.G * g.Tq <= kFewRows; }
+
+// Takers of the line: CTAs, or their groups (two a CTA); fewer where that would leave them less than 2 chunks each.
+int line_groups(const Geom& g, int sms) {
+    const long long chunks = (long long)g.units * ((g.Tk + kRows - 1) / kRows);
+    if (few_rows(g)) return (int)std::max(1LL, std::min((long long)sms, (chunks + 1) / 2));
+    return 2 * (int)std::max(1LL, std::min((long long)sms, (chunks + 3) / 4));
 }
 
-int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Parts& parts, const Backward& x) {
+// Parts of the keys in the forward of units of several tiles: where the tiles are fewer than the groups, so many that each group has about
+// four, since where lengths differ many of them are empty; of at least 4 chunks each.
+int forward_parts(const Geom& g, int sms) {
+    const long long tiles = (long long)g.units * g.tiles;
+    const int chunks = (g.Tk + kRows - 1) / kRows;
+    if (g.tiles == 1 || tiles >= 2 * sms) return 1;
+    return (int)std::max(1LL, std::min<long long>((8LL * sms + tiles - 1) / tiles, chunks / 4));
+}
+
+// Parts of the queries in the key half, by the same rule with one tile a CTA: a part costs its sums' way through memory.
+int key_parts(const Geom& g, int sms) {
+    const long long tiles = (long long)g.units * ((g.Tk + kRows - 1) / kRows);
+    if (tiles >= sms) return 1;
+    return (int)std::max(1LL, std::min<long long>((4LL * sms + tiles - 1) / tiles, g.tiles / 4));
+}
+
+size_t line_rows(const Geom& g, int sms) { return (size_t)(line_groups(g, sms) + g.units) * g.G * g.Tq; }
+size_t all_rows(const Geom& g) { return (size_t)g.B * g.N * g.Tq; }
+size_t key_part(const Geom& g) { return (size_t)g.units * g.Tk * g.C; }
+
+}  // namespace
+
+int NA2D_TC_NAME(forward)(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v,
+                          const Operand& o, float* lse) {
+    const int sms = na2d_tc::sm_count(at.device);
+    FwdCut cut{};
+    cut.pairs = (g.tiles + 1) / 2;
+    if (on_line(g, sms) && scratch.floats >= line_rows(g, sms) * (g.C + 1)) {
+        cut.line = line_groups(g, sms);
+        cut.part_o = scratch.at;
+        cut.part_lse = scratch.at + line_rows(g, sms) * g.C;
+    }
+    cut.splits = (int)std::min<size_t>(forward_parts(g, sms), std::max<size_t>(1, scratch.floats / (all_rows(g) * (g.C + 1))));
+    if (cut.splits > 1) {
+        cut.part_o = scratch.at;
+        cut.part_lse = scratch.at + cut.splits * all_rows(g) * g.C;
+    }
+    const int chunks = (g.Tk + kRows - 1) / kRows;
+    cut.each = (chunks + cut.splits - 1) / cut.splits;
+    cut.by_splits = Div(cut.splits);
+    cut.by_pairs = Div(cut.pairs);
+    const long long items = g.tiles > 1 ? (long long)g.units * cut.pairs * cut.splits : ((long long)g.units + 1) / 2;
+    if (items > 0x3fffffffLL) return NA2D_ERR_TOO_LARGE;
+    cut.items = (int)items;
+    return by_head_dim(g.C, [&](auto d) {
+        return cut.line && few_rows(g) ? launch_few<NA2D_TC_TYPE, decltype(d)::value>(at, g, cut, q, k, v, o, lse)
+                                       : launch_fwd<NA2D_TC_TYPE, decltype(d)::value>(at, g, cut, q, k, v, o, lse);
+    });
+}
+
+int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Scratch& scratch, const Backward& x) {
     int rc = launch_delta<NA2D_TC_TYPE>(at, g, x.d_o, x.o, x.delta);
     if (rc != NA2D_OK) return rc;
     return by_head_dim(g.C, [&](auto d) {
@@ -49,8 +102,16 @@ int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Parts& parts, c
         if (rc != NA2D_OK || !x.d_k.ptr) return rc;
         Geom gk = g;
         if (g.causal) cut_rows(gk, false);               // a chunk's masks go by the column alone
-        const int key_tiles = (g.Tk + kRows - 1) / kRows;
-        KeyCut cut{key_tiles, parts.count, 0, Div(parts.count), Div(key_tiles), parts.a, parts.b};
+        KeyCut cut{};
+        cut.key_tiles = (g.Tk + kRows - 1) / kRows;
+        cut.splits = (int)std::min<size_t>(key_parts(g, na2d_tc::sm_count(at.device)), std::max<size_t>(1, scratch.floats / (2 * key_part(g))));
+        cut.each = (gk.tiles + cut.splits - 1) / cut.splits;
+        cut.by_splits = Div(cut.splits);
+        cut.by_key_tiles = Div(cut.key_tiles);
+        if (cut.splits > 1) {
+            cut.part_dk = scratch.at;
+            cut.part_dv = scratch.at + cut.splits * key_part(g);
+        }
         const long long items = (long long)gk.units * cut.key_tiles * cut.splits;
         if (items > 0x3fffffffLL) return (int)NA2D_ERR_TOO_LARGE;
         cut.items = (int)items;
@@ -59,22 +120,14 @@ int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Parts& parts, c
 }
 
 #if NA2D_TC_DT == 1
-// Parts of the keys in the forward: where the tiles are fewer than the groups that the SMs have (two a CTA), so many that each group has
-// about eight, since lengths that differ make parts that differ; of at least 4 chunks each.
-int forward_parts(const Geom& g, int sms) {
-    const long long tiles = (long long)g.units * g.tiles;
-    const int chunks = (g.Tk + kRows - 1) / kRows;
-    if (tiles >= 2 * sms) return 1;
-    const long long want = (16LL * sms + tiles - 1) / tiles;
-    return (int)std::max(1LL, std::min<long long>(want, chunks / 4));
+size_t forward_floats(const Geom& g, int sms) {
+    if (on_line(g, sms)) return line_rows(g, sms) * (g.C + 1);
+    const int parts = forward_parts(g, sms);
+    return parts > 1 ? parts * all_rows(g) * (g.C + 1) : 0;
 }
-
-// Parts of the queries in the key half, by the same rule with one tile a CTA, and fewer: a part costs its sums' way through memory.
-int key_parts(const Geom& g, int sms) {
-    const long long tiles = (long long)g.units * ((g.Tk + kRows - 1) / kRows);
-    if (tiles >= sms) return 1;
-    const long long want = (4LL * sms + tiles - 1) / tiles;
-    return (int)std::max(1LL, std::min<long long>(want, g.tiles / 4));
+size_t key_floats(const Geom& g, int sms) {
+    const int parts = key_parts(g, sms);
+    return parts > 1 ? 2 * parts * key_part(g) : 0;
 }
 #endif
 
