@@ -1,9 +1,12 @@
 // Attention over all keys on CUDA cores: fp32, head dims that are no multiple of 8 or beyond 128, and any strides.
 //
-// A block has BT query rows (or keys) and walks the other side in tiles of BT, in fp32.  256 threads as 16 x 16; a thread has a
-// (BT / 16)^2 piece of a score tile and (BT / 16) x (CP / 16) sums of an output tile, all in registers.  Tiles lie in shared memory as
-// rows of CP + 4 floats, so that the 16-byte loads of a column of threads fall into different banks.
-// What bounds it: the multiply-adds, and beside them shared memory (12 wavefronts for 64 multiply-adds a thread).
+// A block has 128 or 64 query rows (or 64 keys) and walks the other side in tiles, in fp32; the next tile is on its way to registers
+// meanwhile.  256 threads as 16 x 16; a thread has 8 x 4 (4 x 4) of a score tile and its rows' part of an output tile, all in registers, and
+// multiplies and adds two channels at a time.  Tiles lie in shared memory as rows of CP + 4 floats, so that the 16-byte loads of a column
+// of threads fall into different banks; neighbouring lanes are two rows of one column, because a warp's 16-byte loads are shared between
+// neighbours only (with 16 columns side by side each load took its full four turns: 1305 us against 1209).
+// What bounds it: the multiply-adds, and beside them the loads from shared memory.  Batch 4, 4 heads of 128, 1024 tokens, fp32, forward and
+// backward: 1130 us, 34 TFLOP/s over the nine products that are done (the seven that have to be: 406 us at the measured rate).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -23,55 +26,89 @@ template <> __device__ __forceinline__ float narrow<float>(float x) { return x; 
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
 
-template <int CP>
+// BM rows of one side stay, tiles of BT of the other pass by.
+template <int CP, int BM>
 struct SimtCfg {
-    static constexpr int BT = CP <= 128 ? 64 : 32;       // rows of a tile
-    static constexpr int R = BT / 16;                    // rows and columns of a thread's piece of a score tile
+    static constexpr int BT = CP <= 128 ? 64 : 32;
+    static constexpr int RM = BM / 16, R = BT / 16;      // rows and columns of a thread's piece of a score tile
     static constexpr int NC = CP / 16;                   // columns of a thread's output row: 4 at 4 tx + 64 j (2 at 2 tx for CP 32)
     static constexpr int LD = CP + 4, LS = BT + 4;
-    static constexpr int TILE = BT * LD, SCORES = BT * LS;       // floats
+    static constexpr int HELD = BM * LD, TILE = BT * LD, SCORES = BM * LS;       // floats
 };
 
-// Rows [row0, row0 + BT) of a (T, C) operand as a tile; zeros beyond `rows` and beyond C.
-template <typename DT, int CP>
-__device__ __forceinline__ void load_tile(float* dst, const DT* src, long long stride, int row0, int rows, int C, bool vec) {
-    using S = SimtCfg<CP>;
-    if (vec) {                                           // fp32 on 16-byte boundaries, C a multiple of 4
-        for (int i = threadIdx.x; i < S::BT * (CP / 4); i += kThreads) {
-            const int r = i / (CP / 4), c = 4 * (i % (CP / 4));
+// Rows [row0, row0 + BT) of a (T, C) operand on their way to a tile, in registers (`fetch`, well ahead) and then in shared memory (`put`);
+// zeros beyond `rows` and beyond C.
+template <typename DT, int CP, int ROWS>
+struct Tile {
+    static constexpr int LD = CP + 4, K = ROWS * CP / 4 / kThreads;              // pieces of 4 channels a thread
+    float4 piece[K];
+    __device__ __forceinline__ void fetch(const DT* src, long long stride, int row0, int rows, int C, bool vec) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = threadIdx.x + k * kThreads, r = i / (CP / 4), c = 4 * (i % (CP / 4));
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row0 + r < rows && c < C) v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(src) + (row0 + r) * stride + c);
-            *reinterpret_cast<float4*>(dst + r * S::LD + c) = v;
-        }
-    } else {
-        for (int i = threadIdx.x; i < S::BT * CP; i += kThreads) {
-            const int r = i / CP, c = i % CP;
-            dst[r * S::LD + c] = row0 + r < rows && c < C ? widen(src[(row0 + r) * stride + c]) : 0.f;
+            if (row0 + r < rows) {
+                const DT* at = src + (row0 + r) * stride + c;
+                if (vec) {                                           // fp32 on 16-byte boundaries, C a multiple of 4
+                    if (c < C) v = __ldg(reinterpret_cast<const float4*>(at));
+                } else {
+                    if (c < C) v.x = widen(at[0]);
+                    if (c + 1 < C) v.y = widen(at[1]);
+                    if (c + 2 < C) v.z = widen(at[2]);
+                    if (c + 3 < C) v.w = widen(at[3]);
+                }
+            }
+            piece[k] = v;
         }
     }
-}
+    // One after the other, for rows that stay.
+    static __device__ __forceinline__ void bring(float* dst, const DT* src, long long stride, int row0, int rows, int C, bool vec) {
+        Tile<DT, CP, ROWS / 2> half;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+            half.fetch(src, stride, row0 + h * (ROWS / 2), rows, C, vec);
+            half.put(dst + h * (ROWS / 2) * LD);
+        }
+    }
+    __device__ __forceinline__ void put(float* dst) const {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = threadIdx.x + k * kThreads;
+            *reinterpret_cast<float4*>(dst + (i / (CP / 4)) * LD + 4 * (i % (CP / 4))) = piece[k];
+        }
+    }
+};
 
-// s[i][j] = a row (ty + 16 i) . b row (tx + 16 j)
-template <int CP>
-__device__ __forceinline__ void dot_tile(const float* a, const float* b, float (&s)[SimtCfg<CP>::R][SimtCfg<CP>::R], int tx, int ty) {
-    using S = SimtCfg<CP>;
+// s[i][j] = a row (ty + 16 i) . b row (tx + 16 j).  Two channels' sums side by side: a packed multiply-add leaves every other issue slot to
+// the loads.
+template <int CP, int BM>
+__device__ __forceinline__ void dot_tile(const float* a, const float* b, float (&s)[BM / 16][SimtCfg<CP, BM>::R], int tx, int ty) {
+    using S = SimtCfg<CP, BM>;
+    uint64_t sum[S::RM][S::R];
 #pragma unroll
-    for (int i = 0; i < S::R; ++i)
+    for (int i = 0; i < S::RM; ++i)
 #pragma unroll
-        for (int j = 0; j < S::R; ++j) s[i][j] = 0.f;
+        for (int j = 0; j < S::R; ++j) sum[i][j] = 0;
 #pragma unroll 4
     for (int c = 0; c < CP; c += 4) {
-        float4 x[S::R], y[S::R];
+        ulonglong2 x[S::RM], y[S::R];
 #pragma unroll
-        for (int i = 0; i < S::R; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * S::LD + c);
+        for (int i = 0; i < S::RM; ++i) x[i] = *reinterpret_cast<const ulonglong2*>(a + (ty + 16 * i) * S::LD + c);
 #pragma unroll
-        for (int j = 0; j < S::R; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * S::LD + c);
+        for (int j = 0; j < S::R; ++j) y[j] = *reinterpret_cast<const ulonglong2*>(b + (tx + 16 * j) * S::LD + c);
 #pragma unroll
-        for (int i = 0; i < S::R; ++i)
+        for (int i = 0; i < S::RM; ++i)
 #pragma unroll
-            for (int j = 0; j < S::R; ++j)
-                s[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, s[i][j]))));
+            for (int j = 0; j < S::R; ++j) sum[i][j] = na2d_ptx::fma2(x[i].x, y[j].x, sum[i][j]);
+#pragma unroll
+        for (int i = 0; i < S::RM; ++i)
+#pragma unroll
+            for (int j = 0; j < S::R; ++j) sum[i][j] = na2d_ptx::fma2(x[i].y, y[j].y, sum[i][j]);
     }
+#pragma unroll
+    for (int i = 0; i < S::RM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::R; ++j) s[i][j] = na2d_ptx::lo2(sum[i][j]) + na2d_ptx::hi2(sum[i][j]);
 }
 
 // First channel of the k-th pair of a thread's output columns.
@@ -80,43 +117,55 @@ __device__ __forceinline__ int out_col(int tx, int k) {
     return CP == 32 ? 2 * tx + 32 * k : 4 * tx + 64 * (k / 2) + 2 * (k % 2);
 }
 
-// acc[i][] += sum_k w[row ty + 16 i][k] b[k][], w in rows of LS floats
-template <int CP>
-__device__ __forceinline__ void apply_tile(const float* w, const float* b, float (&acc)[SimtCfg<CP>::R][SimtCfg<CP>::NC], int tx, int ty) {
-    using S = SimtCfg<CP>;
+// A thread's part of an output tile, in pairs of columns.
+template <int CP, int BM>
+struct Sums {
+    using S = SimtCfg<CP, BM>;
+    uint64_t at[S::RM][S::NC / 2];
+    __device__ __forceinline__ Sums() {
+#pragma unroll
+        for (int i = 0; i < S::RM; ++i)
+#pragma unroll
+            for (int c = 0; c < S::NC / 2; ++c) at[i][c] = 0;
+    }
+    // += sum_k w[row ty + 16 i][k] b[k][], w in rows of LS floats
+    __device__ __forceinline__ void add(const float* w, const float* b, int tx, int ty) {
 #pragma unroll 2
-    for (int k = 0; k < S::BT; k += 4) {
-        float4 x[S::R];
+        for (int k = 0; k < S::BT; k += 4) {
+            float4 x[S::RM];
 #pragma unroll
-        for (int i = 0; i < S::R; ++i) x[i] = *reinterpret_cast<const float4*>(w + (ty + 16 * i) * S::LS + k);
+            for (int i = 0; i < S::RM; ++i) x[i] = *reinterpret_cast<const float4*>(w + (ty + 16 * i) * S::LS + k);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            float y[S::NC];
-            if constexpr (CP == 32) {
-                const float2 v = *reinterpret_cast<const float2*>(b + (k + kk) * S::LD + 2 * tx);
-                y[0] = v.x;
-                y[1] = v.y;
-            } else {
+            for (int kk = 0; kk < 4; ++kk) {
+                uint64_t y[S::NC / 2];
+                if constexpr (CP == 32) {
+                    y[0] = *reinterpret_cast<const uint64_t*>(b + (k + kk) * S::LD + 2 * tx);
+                } else {
 #pragma unroll
-                for (int j = 0; j < S::NC / 4; ++j)
-                    *reinterpret_cast<float4*>(y + 4 * j) = *reinterpret_cast<const float4*>(b + (k + kk) * S::LD + 4 * tx + 64 * j);
-            }
+                    for (int j = 0; j < S::NC / 4; ++j) {
+                        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(b + (k + kk) * S::LD + 4 * tx + 64 * j);
+                        y[2 * j] = v.x;
+                        y[2 * j + 1] = v.y;
+                    }
+                }
 #pragma unroll
-            for (int i = 0; i < S::R; ++i) {
-                const float xi = kk == 0 ? x[i].x : kk == 1 ? x[i].y : kk == 2 ? x[i].z : x[i].w;
+                for (int i = 0; i < S::RM; ++i) {
+                    const float xi = kk == 0 ? x[i].x : kk == 1 ? x[i].y : kk == 2 ? x[i].z : x[i].w;
+                    const uint64_t xx = na2d_ptx::pair2(xi, xi);
 #pragma unroll
-                for (int c = 0; c < S::NC; ++c) acc[i][c] = fmaf(xi, y[c], acc[i][c]);
+                    for (int c = 0; c < S::NC / 2; ++c) at[i][c] = na2d_ptx::fma2(xx, y[c], at[i][c]);
+                }
             }
         }
     }
-}
+};
 
-template <typename DT, int CP>
+template <typename DT, int CP, int BM>
 __device__ __forceinline__ void store_rows(DT* dst, long long stride, int row0, int rows, int C,
-                                           const float (&acc)[SimtCfg<CP>::R][SimtCfg<CP>::NC], const float (&scale)[SimtCfg<CP>::R], int tx, int ty) {
-    using S = SimtCfg<CP>;
+                                           const Sums<CP, BM>& acc, const float (&scale)[BM / 16], int tx, int ty) {
+    using S = SimtCfg<CP, BM>;
 #pragma unroll
-    for (int i = 0; i < S::R; ++i) {
+    for (int i = 0; i < S::RM; ++i) {
         const int r = row0 + ty + 16 * i;
         if (r >= rows) continue;
 #pragma unroll
@@ -124,20 +173,20 @@ __device__ __forceinline__ void store_rows(DT* dst, long long stride, int row0, 
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int c = out_col<CP>(tx, k) + e;
-                if (c < C) dst[r * stride + c] = narrow<DT>(acc[i][2 * k + e] * scale[i]);
+                if (c < C) dst[r * stride + c] = narrow<DT>((e ? na2d_ptx::hi2(acc.at[i][k]) : na2d_ptx::lo2(acc.at[i][k])) * scale[i]);
             }
     }
 }
 
-// Sum (or maximum) over the 16 threads of a row: half a warp.
+// Sum (or maximum) over the 16 threads of a row: every other lane of a warp.
 __device__ __forceinline__ float row_sum(float x) {
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    for (int d = 16; d > 1; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
     return x;
 }
 __device__ __forceinline__ float row_max(float x) {
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    for (int d = 16; d > 1; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
     return x;
 }
 
@@ -145,33 +194,35 @@ template <typename DT>
 __device__ __forceinline__ DT* rows_of(const Operand& x, int b, int n) { return static_cast<DT*>(x.ptr) + b * x.b + n * x.n; }
 
 // ---- forward: a block has BT queries of one head ------------------------------------------------------------------
-template <typename DT, int CP>
+template <typename DT, int CP, int BM>
 __global__ void __launch_bounds__(kThreads)
 simt_fwd_kernel(const Operand q, const Operand k, const Operand v, const Operand o, float* __restrict__ lse, const Geom g, const int tiles, const int vec) {
-    using S = SimtCfg<CP>;
+    using S = SimtCfg<CP, BM>;
     extern __shared__ __align__(16) float smem[];
-    float *sQ = smem, *sKV = sQ + S::TILE, *sP = sKV + S::TILE;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    float *sQ = smem, *sKV = sQ + S::HELD, *sP = sKV + S::TILE;
+    const int tx = threadIdx.x % 32 / 2, ty = threadIdx.x / 32 * 2 + threadIdx.x % 2;
     const int bn = blockIdx.x / tiles, b = bn / g.N, n = bn - b * g.N, m = n / g.G;
-    const int t0 = (g.causal ? tiles - 1 - (int)(blockIdx.x % tiles) : (int)(blockIdx.x % tiles)) * S::BT;
-    const int count = key_count(g, b), keys = keys_seen(g, count, min(t0 + S::BT, g.Tq) - 1);
-    load_tile<DT, CP>(sQ, rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
-    float acc[S::R][S::NC], top[S::R], total[S::R];
+    const int t0 = (g.causal ? tiles - 1 - (int)(blockIdx.x % tiles) : (int)(blockIdx.x % tiles)) * BM;
+    const int count = key_count(g, b), keys = keys_seen(g, count, min(t0 + BM, g.Tq) - 1);
+    Tile<DT, CP, BM>::bring(sQ, rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
+    Tile<DT, CP, S::BT> tile;
+    if (keys > 0) tile.fetch(rows_of<DT>(k, b, m), k.t, 0, count, g.C, vec);
+    Sums<CP, BM> acc;
+    float top[S::RM], total[S::RM];
 #pragma unroll
-    for (int i = 0; i < S::R; ++i) {
+    for (int i = 0; i < S::RM; ++i) {
         top[i] = -CUDART_INF_F;
         total[i] = 0.f;
-#pragma unroll
-        for (int c = 0; c < S::NC; ++c) acc[i][c] = 0.f;
     }
     for (int k0 = 0; k0 < keys; k0 += S::BT) {
         __syncthreads();
-        load_tile<DT, CP>(sKV, rows_of<DT>(k, b, m), k.t, k0, count, g.C, vec);
+        tile.put(sKV);
+        tile.fetch(rows_of<DT>(v, b, m), v.t, k0, count, g.C, vec);
         __syncthreads();
-        float s[S::R][S::R];
-        dot_tile<CP>(sQ, sKV, s, tx, ty);
+        float s[S::RM][S::R];
+        dot_tile<CP, BM>(sQ, sKV, s, tx, ty);
 #pragma unroll
-        for (int i = 0; i < S::R; ++i) {
+        for (int i = 0; i < S::RM; ++i) {
             const int t = t0 + ty + 16 * i, seen = t < g.Tq ? keys_seen(g, count, t) : 0;
             float high = top[i];
 #pragma unroll
@@ -190,24 +241,26 @@ simt_fwd_kernel(const Operand q, const Operand k, const Operand v, const Operand
             }
             total[i] = fmaf(total[i], old, sum);
             top[i] = high;
+            const uint64_t old2 = na2d_ptx::pair2(old, old);
 #pragma unroll
-            for (int c = 0; c < S::NC; ++c) acc[i][c] *= old;
+            for (int c = 0; c < S::NC / 2; ++c) acc.at[i][c] = na2d_ptx::mul2(acc.at[i][c], old2);
         }
         __syncthreads();
-        load_tile<DT, CP>(sKV, rows_of<DT>(v, b, m), v.t, k0, count, g.C, vec);
+        tile.put(sKV);
+        if (k0 + S::BT < keys) tile.fetch(rows_of<DT>(k, b, m), k.t, k0 + S::BT, count, g.C, vec);
         __syncthreads();
-        apply_tile<CP>(sP, sKV, acc, tx, ty);
+        acc.add(sP, sKV, tx, ty);
     }
-    float inv[S::R];
+    float inv[S::RM];
 #pragma unroll
-    for (int i = 0; i < S::R; ++i) {
+    for (int i = 0; i < S::RM; ++i) {
         const float sum = row_sum(total[i]);
         inv[i] = sum == 0.f ? 0.f : 1.f / sum;
         const int t = t0 + ty + 16 * i;
         if (tx == 0 && t < g.Tq)
             lse[row_index(g, b, n, t)] = sum == 0.f ? -CUDART_INF_F : (top[i] + log2f(sum)) * na2d_tc::kLn2;
     }
-    store_rows<DT, CP>(rows_of<DT>(o, b, n), o.t, t0, g.Tq, g.C, acc, inv, tx, ty);
+    store_rows<DT, CP, BM>(rows_of<DT>(o, b, n), o.t, t0, g.Tq, g.C, acc, inv, tx, ty);
 }
 
 // ---- delta = dO . o, a warp a row -------------------------------------------------------------------------------------
@@ -226,51 +279,60 @@ __global__ void __launch_bounds__(kThreads) simt_delta_kernel(const Operand d_o,
 }
 
 // ---- query half of the backward -----------------------------------------------------------------------------------------
-template <typename DT, int CP>
+template <typename DT, int CP, int BM>
 __global__ void __launch_bounds__(kThreads)
 simt_dq_kernel(const Operand q, const Operand k, const Operand v, const Operand d_o, const Operand d_q, const float* __restrict__ lse,
                const float* __restrict__ delta, const Geom g, const int tiles, const int vec) {
-    using S = SimtCfg<CP>;
+    using S = SimtCfg<CP, BM>;
     extern __shared__ __align__(16) float smem[];
-    float *sQ = smem, *sG = sQ + S::TILE, *sKV = sG + S::TILE, *sP = sKV + S::TILE;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    float *sQ = smem, *sG = sQ + S::HELD, *sKV = sG + S::HELD, *sP = sKV + S::TILE;
+    const int tx = threadIdx.x % 32 / 2, ty = threadIdx.x / 32 * 2 + threadIdx.x % 2;
     const int bn = blockIdx.x / tiles, b = bn / g.N, n = bn - b * g.N, m = n / g.G;
-    const int t0 = (g.causal ? tiles - 1 - (int)(blockIdx.x % tiles) : (int)(blockIdx.x % tiles)) * S::BT;
-    const int count = key_count(g, b), keys = keys_seen(g, count, min(t0 + S::BT, g.Tq) - 1);
-    load_tile<DT, CP>(sQ, rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
-    load_tile<DT, CP>(sG, rows_of<DT>(d_o, b, n), d_o.t, t0, g.Tq, g.C, vec);
-    float acc[S::R][S::NC], neg[S::R], del[S::R], scale[S::R];
-    int seen[S::R];
+    const int t0 = (g.causal ? tiles - 1 - (int)(blockIdx.x % tiles) : (int)(blockIdx.x % tiles)) * BM;
+    const int count = key_count(g, b), keys = keys_seen(g, count, min(t0 + BM, g.Tq) - 1);
+    Tile<DT, CP, BM>::bring(sQ, rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
+    Tile<DT, CP, BM>::bring(sG, rows_of<DT>(d_o, b, n), d_o.t, t0, g.Tq, g.C, vec);
+    Tile<DT, CP, S::BT> tile;
+    if (keys > 0) tile.fetch(rows_of<DT>(v, b, m), v.t, 0, count, g.C, vec);
+    Sums<CP, BM> acc;
+    float neg[S::RM], del[S::RM], scale[S::RM];
 #pragma unroll
-    for (int i = 0; i < S::R; ++i) {
+    for (int i = 0; i < S::RM; ++i) {
         const int t = t0 + ty + 16 * i;
-        seen[i] = t < g.Tq ? keys_seen(g, count, t) : 0;
-        neg[i] = seen[i] ? -lse[row_index(g, b, n, t)] * na2d_tc::kLog2e : 0.f;
-        del[i] = seen[i] ? delta[row_index(g, b, n, t)] : 0.f;
+        const bool row = t < g.Tq && keys_seen(g, count, t) > 0;
+        neg[i] = row ? -lse[row_index(g, b, n, t)] * na2d_tc::kLog2e : 0.f;
+        del[i] = row ? delta[row_index(g, b, n, t)] : 0.f;
         scale[i] = g.scale;
-#pragma unroll
-        for (int c = 0; c < S::NC; ++c) acc[i][c] = 0.f;
     }
     for (int k0 = 0; k0 < keys; k0 += S::BT) {
         __syncthreads();
-        load_tile<DT, CP>(sKV, rows_of<DT>(v, b, m), v.t, k0, count, g.C, vec);
+        tile.put(sKV);
+        tile.fetch(rows_of<DT>(k, b, m), k.t, k0, count, g.C, vec);
         __syncthreads();
-        float dp[S::R][S::R], s[S::R][S::R];
-        dot_tile<CP>(sG, sKV, dp, tx, ty);
-        __syncthreads();
-        load_tile<DT, CP>(sKV, rows_of<DT>(k, b, m), k.t, k0, count, g.C, vec);
-        __syncthreads();
-        dot_tile<CP>(sQ, sKV, s, tx, ty);
+        float s[S::RM][S::R];
+        dot_tile<CP, BM>(sG, sKV, s, tx, ty);
 #pragma unroll
-        for (int i = 0; i < S::R; ++i)
+        for (int i = 0; i < S::RM; ++i)
 #pragma unroll
-            for (int j = 0; j < S::R; ++j)
-                sP[(ty + 16 * i) * S::LS + tx + 16 * j] =
-                    k0 + tx + 16 * j < seen[i] ? exp2f(fmaf(s[i][j], g.sl2, neg[i])) * (dp[i][j] - del[i]) : 0.f;
+            for (int j = 0; j < S::R; ++j) sP[(ty + 16 * i) * S::LS + tx + 16 * j] = s[i][j] - del[i];
         __syncthreads();
-        apply_tile<CP>(sP, sKV, acc, tx, ty);
+        tile.put(sKV);
+        if (k0 + S::BT < keys) tile.fetch(rows_of<DT>(v, b, m), v.t, k0 + S::BT, count, g.C, vec);
+        __syncthreads();
+        dot_tile<CP, BM>(sQ, sKV, s, tx, ty);
+#pragma unroll
+        for (int i = 0; i < S::RM; ++i) {
+            const int t = t0 + ty + 16 * i, seen = t < g.Tq ? keys_seen(g, count, t) : 0;
+#pragma unroll
+            for (int j = 0; j < S::R; ++j) {
+                float* at = sP + (ty + 16 * i) * S::LS + tx + 16 * j;        // holds dP - delta, of this very thread
+                *at = k0 + tx + 16 * j < seen ? exp2f(fmaf(s[i][j], g.sl2, neg[i])) * *at : 0.f;
+            }
+        }
+        __syncwarp();
+        acc.add(sP, sKV, tx, ty);
     }
-    store_rows<DT, CP>(rows_of<DT>(d_q, b, n), d_q.t, t0, g.Tq, g.C, acc, scale, tx, ty);
+    store_rows<DT, CP, BM>(rows_of<DT>(d_q, b, n), d_q.t, t0, g.Tq, g.C, acc, scale, tx, ty);
 }
 
 // ---- key half: a block has BT keys of one key head and walks the queries of every head that shares it ------------------------
@@ -278,32 +340,39 @@ template <typename DT, int CP>
 __global__ void __launch_bounds__(kThreads)
 simt_dkdv_kernel(const Operand q, const Operand k, const Operand v, const Operand d_o, const Operand d_k, const Operand d_v,
                  const float* __restrict__ lse, const float* __restrict__ delta, const Geom g, const int tiles, const int vec) {
-    using S = SimtCfg<CP>;
+    constexpr int BM = CP <= 128 ? 64 : 32;
+    using S = SimtCfg<CP, BM>;
     extern __shared__ __align__(16) float smem[];
-    float *sK = smem, *sV = sK + S::TILE, *sX = sV + S::TILE, *sP = sX + S::TILE;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    float *sK = smem, *sV = sK + S::TILE, *sX = sV + S::TILE, *sY = sX + S::TILE, *sP = sY + S::TILE;
+    const int tx = threadIdx.x % 32 / 2, ty = threadIdx.x / 32 * 2 + threadIdx.x % 2;
     const int unit = blockIdx.x / tiles, b = unit / g.Nk, m = unit - b * g.Nk;
     const int k0 = (blockIdx.x % tiles) * S::BT;
     const int count = key_count(g, b);
     const int t_min = g.causal ? max(k0 + g.Tq - count, 0) : 0;      // the first token that sees the tile
-    load_tile<DT, CP>(sK, rows_of<DT>(k, b, m), k.t, k0, count, g.C, vec);
-    load_tile<DT, CP>(sV, rows_of<DT>(v, b, m), v.t, k0, count, g.C, vec);
-    float acc_k[S::R][S::NC], acc_v[S::R][S::NC], scale_k[S::R], scale_v[S::R];
+    Tile<DT, CP, BM> tile;
+    tile.fetch(rows_of<DT>(k, b, m), k.t, k0, count, g.C, vec);
+    tile.put(sK);
+    tile.fetch(rows_of<DT>(v, b, m), v.t, k0, count, g.C, vec);
+    tile.put(sV);
+    Sums<CP, BM> acc_k, acc_v;
+    float scale_k[S::R], scale_v[S::R];
 #pragma unroll
     for (int i = 0; i < S::R; ++i) {
         scale_k[i] = g.scale;
         scale_v[i] = 1.f;
-#pragma unroll
-        for (int c = 0; c < S::NC; ++c) acc_k[i][c] = acc_v[i][c] = 0.f;
     }
-    for (int n = m * g.G; k0 < count && n < (m + 1) * g.G; ++n) {
-        for (int t0 = t_min / S::BT * S::BT; t0 < g.Tq; t0 += S::BT) {
-            // rows of a piece are keys (ty), columns queries (tx)
+    const int first = t_min / S::BT * S::BT;
+    const bool any = k0 < count && first < g.Tq;
+    if (any) tile.fetch(rows_of<DT>(q, b, m * g.G), q.t, first, g.Tq, g.C, vec);
+    for (int n = m * g.G; any && n < (m + 1) * g.G; ++n) {
+        for (int t0 = first; t0 < g.Tq; t0 += S::BT) {
+            // rows of a piece are keys (ty), columns queries (tx).  Q stays in sX, dO goes to sY.
             __syncthreads();
-            load_tile<DT, CP>(sX, rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
+            tile.put(sX);
+            tile.fetch(rows_of<DT>(d_o, b, n), d_o.t, t0, g.Tq, g.C, vec);
             __syncthreads();
             float p[S::R][S::R], dp[S::R][S::R];
-            dot_tile<CP>(sK, sX, p, tx, ty);
+            dot_tile<CP, BM>(sK, sX, p, tx, ty);
             float del[S::R];
 #pragma unroll
             for (int j = 0; j < S::R; ++j) {
@@ -313,28 +382,29 @@ simt_dkdv_kernel(const Operand q, const Operand k, const Operand v, const Operan
 #pragma unroll
                 for (int i = 0; i < S::R; ++i) p[i][j] = k0 + ty + 16 * i < seen ? exp2f(fmaf(p[i][j], g.sl2, neg)) : 0.f;
             }
-            __syncthreads();
-            load_tile<DT, CP>(sX, rows_of<DT>(d_o, b, n), d_o.t, t0, g.Tq, g.C, vec);
+            tile.put(sY);                                // (last read before the first barrier of this round)
+            const bool more = t0 + S::BT < g.Tq;
+            if (more || n + 1 < (m + 1) * g.G)
+                tile.fetch(rows_of<DT>(q, b, more ? n : n + 1), q.t, more ? t0 + S::BT : first, g.Tq, g.C, vec);
 #pragma unroll
             for (int i = 0; i < S::R; ++i)
 #pragma unroll
                 for (int j = 0; j < S::R; ++j) sP[(ty + 16 * i) * S::LS + tx + 16 * j] = p[i][j];
             __syncthreads();
-            dot_tile<CP>(sV, sX, dp, tx, ty);
-            apply_tile<CP>(sP, sX, acc_v, tx, ty);
+            dot_tile<CP, BM>(sV, sY, dp, tx, ty);
+            acc_v.add(sP, sY, tx, ty);
             __syncthreads();
-            load_tile<DT, CP>(sX, rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
 #pragma unroll
             for (int i = 0; i < S::R; ++i)
 #pragma unroll
                 for (int j = 0; j < S::R; ++j)       // (by selection: what is not seen may hold anything)
                     sP[(ty + 16 * i) * S::LS + tx + 16 * j] = p[i][j] == 0.f ? 0.f : p[i][j] * (dp[i][j] - del[j]);
             __syncthreads();
-            apply_tile<CP>(sP, sX, acc_k, tx, ty);
+            acc_k.add(sP, sX, tx, ty);
         }
     }
-    store_rows<DT, CP>(rows_of<DT>(d_k, b, m), d_k.t, k0, g.Tk, g.C, acc_k, scale_k, tx, ty);
-    store_rows<DT, CP>(rows_of<DT>(d_v, b, m), d_v.t, k0, g.Tk, g.C, acc_v, scale_v, tx, ty);
+    store_rows<DT, CP, BM>(rows_of<DT>(d_k, b, m), d_k.t, k0, g.Tk, g.C, acc_k, scale_k, tx, ty);
+    store_rows<DT, CP, BM>(rows_of<DT>(d_v, b, m), d_v.t, k0, g.Tk, g.C, acc_v, scale_v, tx, ty);
 }
 
 // ---- launchers ---------------------------------------------------------------------------------------------------------
@@ -366,21 +436,46 @@ int start(const Place& at, K kernel, unsigned blocks, int floats, std::atomic<un
     return cudaGetLastError() == cudaSuccess ? NA2D_OK : NA2D_ERR_CUDA;
 }
 
-template <typename DT, int CP>
+// 128 query rows a block where blocks of 64 would take the SMs more than one round: a piece of 8 x 4 scores reads 12 operands from shared
+// memory for its 32 products, one of 4 x 4 reads 8 for 16.  Forward and query half with 256 blocks of 64: 277 and 417 us; with 128 of 128:
+// 244 and 365 us.
+template <int CP, typename F>
+int by_rows(const Place& at, const Geom& g, F&& f) {
+    if constexpr (CP <= 128) {
+        if ((long long)g.B * g.N * ((g.Tq + 63) / 64) > na2d_tc::sm_count(at.device)) return f(std::integral_constant<int, 128>{});
+        return f(std::integral_constant<int, 64>{});
+    } else {
+        return f(std::integral_constant<int, 32>{});
+    }
+}
+
+template <typename DT, int CP, int BM>
 int forward_as(const Place& at, const Geom& g, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse) {
-    using S = SimtCfg<CP>;
+    using S = SimtCfg<CP, BM>;
     static std::atomic<unsigned long long> opted{0};
     const int vec = vectors(q, at.dtype, g.C) && vectors(k, at.dtype, g.C) && vectors(v, at.dtype, g.C);
     int tiles = 0;
     unsigned blocks = 0;
-    if (int rc = blocks_of((long long)g.B * g.N, g.Tq, S::BT, &tiles, &blocks)) return rc;
-    return start(at, simt_fwd_kernel<DT, CP>, blocks, 2 * S::TILE + S::SCORES, opted, q, k, v, o, lse, g, tiles, vec);
+    if (int rc = blocks_of((long long)g.B * g.N, g.Tq, BM, &tiles, &blocks)) return rc;
+    return start(at, simt_fwd_kernel<DT, CP, BM>, blocks, S::HELD + S::TILE + S::SCORES, opted, q, k, v, o, lse, g, tiles, vec);
+}
+
+template <typename DT, int CP, int BM>
+int queries_as(const Place& at, const Geom& g, const Backward& x, int vec) {
+    using S = SimtCfg<CP, BM>;
+    static std::atomic<unsigned long long> opted{0};
+    int tiles = 0;
+    unsigned blocks = 0;
+    if (int rc = blocks_of((long long)g.B * g.N, g.Tq, BM, &tiles, &blocks)) return rc;
+    return start(at, simt_dq_kernel<DT, CP, BM>, blocks, 2 * S::HELD + S::TILE + S::SCORES, opted, x.q, x.k, x.v, x.d_o, x.d_q, x.lse,
+                 (const float*)x.delta, g, tiles, vec);
 }
 
 template <typename DT, int CP>
 int backward_as(const Place& at, const Geom& g, const Backward& x) {
-    using S = SimtCfg<CP>;
-    static std::atomic<unsigned long long> opted_q{0}, opted_k{0};
+    constexpr int BM = CP <= 128 ? 64 : 32;
+    using S = SimtCfg<CP, BM>;
+    static std::atomic<unsigned long long> opted{0};
     int vec = 1, tiles = 0;
     for (const Operand* t : {&x.q, &x.k, &x.v, &x.d_o}) vec = vec && vectors(*t, at.dtype, g.C);
     const long long rows = (long long)g.B * g.N * g.Tq;
@@ -388,16 +483,13 @@ int backward_as(const Place& at, const Geom& g, const Backward& x) {
     simt_delta_kernel<DT><<<(unsigned)((rows + 7) / 8), kThreads, 0, at.st>>>(x.d_o, x.o, x.delta, g);
     *at.launched += 1;
     if (cudaGetLastError() != cudaSuccess) return NA2D_ERR_CUDA;
-    unsigned blocks = 0;
     if (x.d_q.ptr) {
-        if (int rc = blocks_of((long long)g.B * g.N, g.Tq, S::BT, &tiles, &blocks)) return rc;
-        if (int rc = start(at, simt_dq_kernel<DT, CP>, blocks, 3 * S::TILE + S::SCORES, opted_q, x.q, x.k, x.v, x.d_o, x.d_q, x.lse,
-                           (const float*)x.delta, g, tiles, vec))
-            return rc;
+        if (int rc = by_rows<CP>(at, g, [&](auto bm) { return queries_as<DT, CP, decltype(bm)::value>(at, g, x, vec); })) return rc;
     }
     if (!x.d_k.ptr) return NA2D_OK;
-    if (int rc = blocks_of(g.units, g.Tk, S::BT, &tiles, &blocks)) return rc;
-    return start(at, simt_dkdv_kernel<DT, CP>, blocks, 3 * S::TILE + S::SCORES, opted_k, x.q, x.k, x.v, x.d_o, x.d_k, x.d_v, x.lse,
+    unsigned blocks = 0;
+    if (int rc = blocks_of(g.units, g.Tk, BM, &tiles, &blocks)) return rc;
+    return start(at, simt_dkdv_kernel<DT, CP>, blocks, 4 * S::TILE + S::SCORES, opted, x.q, x.k, x.v, x.d_o, x.d_k, x.d_v, x.lse,
                  (const float*)x.delta, g, tiles, vec);
 }
 
@@ -406,7 +498,10 @@ int backward_as(const Place& at, const Geom& g, const Backward& x) {
 int simt_forward(const Place& at, const Geom& g, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse) {
     auto run = [&](auto type) {
         using DT = decltype(type);
-        return by_channels<DT>(g.C, [&](auto cp) { return forward_as<DT, decltype(cp)::value>(at, g, q, k, v, o, lse); });
+        return by_channels<DT>(g.C, [&](auto cp) {
+            constexpr int CP = decltype(cp)::value;
+            return by_rows<CP>(at, g, [&](auto bm) { return forward_as<DT, CP, decltype(bm)::value>(at, g, q, k, v, o, lse); });
+        });
     };
     return at.dtype == NA2D_F32 ? run(float{}) : at.dtype == NA2D_BF16 ? run(__nv_bfloat16{}) : run(__half{});
 }
