@@ -10,14 +10,17 @@
 // tensor memory are in use, S^T and dP^T having one buffer each; the two halves of a chunk's arithmetic take turns with the MMAs:
 //     softmax   P(n)         | dS(n)        | P(n+1)        | dS(n+1)
 //     tensor          dP(n)  | dV(n) S(n+1) | dK(n) dP(n+1) | dV(n+1) ...
-// Few keys and many queries: the chunks of a tile are cut into `splits` parts, whose fp32 sums go to a workspace and are added by
-// attn_sum_kernel.
+// Where tiles and CTAs do not go into one another, or batch entries have lengths of their own, the chunks of all tiles that hold a key lie on
+// one line, of which every CTA takes the same stretch (causal calls, whose tiles see different numbers of chunks, cut a tile's chunks into
+// `splits` parts where the tiles are few).  What a CTA has of a tile that it does not see all chunks of goes to a workspace as fp32 sums,
+// which attn_join_kernel (attn_sum_kernel) adds in their order.
 //   warps 0-7   softmax: warps w and w + 4 share 32 keys and take 64 queries each;
 //   warp 8      producer of the Q / dO chunks and of the chunks' lse and delta;  warp 11  producer of the K, V tile;
 //   warp 9      MMA issue;  warps 12-15 epilogue.
 #pragma once
 
 #include "na2d_attn_dq.cuh"
+#include "na2d_attn_fwd.cuh"
 
 namespace na2d_attn {
 
@@ -26,14 +29,33 @@ struct KeyCut {
     int splits;
     int items;
     int each;               // chunks of a part
+    int line;               // the chunks of all tiles that hold keys on one line, that many CTAs take; 0: not
     Div by_splits, by_key_tiles;
-    float* part_dk;         // (splits, B, Nk, Tk, C), where splits > 1
+    float* part_dk;         // (splits, B, Nk, Tk, C), where splits > 1; line: (2 a CTA, keys of a tile, C)
     float* part_dv;
+};
+
+// A tile of keys by its number on the line; `before` as line_table writes it.
+struct LineTile {
+    int b, m, k0;
+    __device__ __forceinline__ LineTile(const Geom& g, const int* before, int tile) {
+        int lo = 0, hi = g.B;                            // before[lo] Nk <= tile < before[hi] Nk
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (before[mid] * g.Nk <= tile) lo = mid;
+            else hi = mid;
+        }
+        const int own = tile - before[lo] * g.Nk, len = before[lo + 1] - before[lo];
+        b = lo;
+        m = own / len;
+        k0 = (own - m * len) * kRows;
+    }
 };
 
 // One item: chunks [first, first + n) of those that see a key tile.
 struct KeyItem {
-    int b, m, k0, count, split;
+    int b, m, k0, count;
+    int split;              // line: the part's place in the workspace, -1 for a whole tile
     int lo, per_head;       // the tile's chunks: query tiles lo .. lo + per_head - 1 of each (group of) heads
     int first, n, head, in_head;
     __device__ __forceinline__ KeyItem(const Geom& g, const KeyCut& cut, int item) {
@@ -56,6 +78,21 @@ struct KeyItem {
         head = per_head > 0 ? first / per_head : 0;
         in_head = first - head * per_head;
     }
+    // chunks from `at` on of a line that ends at `end`
+    __device__ __forceinline__ KeyItem(const Geom& g, const int* before, int at, int end) {
+        const int tile = g.by_tiles.split(at, first);
+        const LineTile x(g, before, tile);
+        b = x.b;
+        m = x.m;
+        k0 = x.k0;
+        count = key_count(g, b);
+        lo = 0;
+        per_head = g.tiles_t;
+        n = min(g.tiles - first, end - at);
+        head = first / per_head;
+        in_head = first - head * per_head;
+        split = n == g.tiles ? -1 : 2 * (int)blockIdx.x + (first == 0);
+    }
     // first head and token of the first chunk
     __device__ __forceinline__ void start(const Geom& g, int& h0, int& t0) const {
         h0 = m * g.G + head * g.hp;
@@ -68,6 +105,25 @@ struct KeyItem {
             t0 = lo * kRows;
             h0 += g.hp;
         }
+    }
+};
+
+// The items of a CTA, which every role walks by itself.
+struct KeyWalk {
+    int item, at, end;
+    __device__ __forceinline__ KeyWalk(const Geom& g, const KeyCut& cut, const int* before) : item(blockIdx.x), at(0), end(0) {
+        if (!cut.line) return;
+        const int all = before[g.B] * g.Nk * g.tiles, each = (all + cut.line - 1) / cut.line;
+        at = min((int)blockIdx.x * each, all);
+        end = min(at + each, all);
+    }
+    __device__ __forceinline__ bool more(const KeyCut& cut) const { return cut.line ? at < end : item < cut.items; }
+    __device__ __forceinline__ KeyItem get(const Geom& g, const KeyCut& cut, const int* before) const {
+        return cut.line ? KeyItem(g, before, at, end) : KeyItem(g, cut, item);
+    }
+    __device__ __forceinline__ void next(const KeyItem& k) {
+        item += gridDim.x;
+        at += k.n;
     }
 };
 
@@ -97,6 +153,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     using C = KeyCfg<D>;
     constexpr int NST = C::NST, NKV = C::NKV;
     extern __shared__ uint8_t smem_raw[];
+    __shared__ int before[kLineEntries + 1];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sK = smem;
     uint8_t* sV = sK + NKV * C::BYTES;
@@ -157,6 +214,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
+    if (warp == 1 && cut.line) line_table(g, before, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -168,8 +226,9 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         reg_dec<kDkvRegsCtl>();
         LoadTracker lt(bars);
         Ring ring;
-        for (int item = blockIdx.x; item < cut.items && lt.ok; item += gridDim.x) {
-            const KeyItem k(g, cut, item);
+        for (KeyWalk walk(g, cut, before); walk.more(cut) && lt.ok;) {
+            const KeyItem k = walk.get(g, cut, before);
+            walk.next(k);
             int h0, t0;
             k.start(g, h0, t0);
             for (int i = 0; i < k.n; ++i, k.step(g, h0, t0)) {
@@ -213,8 +272,9 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (lane == 0) {
             LoadTracker lt(bars);
             uint32_t it = 0;
-            for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
-                const KeyItem k(g, cut, item);
+            for (KeyWalk walk(g, cut, before); walk.more(cut);) {
+                const KeyItem k = walk.get(g, cut, before);
+                walk.next(k);
                 if (k.n == 0) continue;
                 const uint32_t to = it % NKV, phase = (it / NKV) & 1;
                 if (!lt.acquire(kv_empty + to, phase ^ 1, wctx)) break;
@@ -273,8 +333,9 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             __syncwarp();
             rs.next(NST);
         };
-        for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
-            const KeyItem k(g, cut, item);
+        for (KeyWalk walk(g, cut, before); walk.more(cut);) {
+            const KeyItem k = walk.get(g, cut, before);
+            walk.next(k);
             if (k.n == 0) continue;
             mbar_wait(kv_full + it % NKV, (it / NKV) & 1, wctx, kErrLoadWait);
             scores();
@@ -315,8 +376,9 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         uint8_t* stage = sOut + quarter * 2 * OutStage<32>::BYTES;
         uint32_t it = 0, seq = 0;
-        for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
-            const KeyItem k(g, cut, item);
+        for (KeyWalk walk(g, cut, before); walk.more(cut);) {
+            const KeyItem k = walk.get(g, cut, before);
+            walk.next(k);
             const int first = k.k0 + quarter * 32, key = first + lane;
             if (k.n > 0) {
                 mbar_wait(acc_full, it & 1, wctx, kErrMmaWait);
@@ -340,12 +402,12 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                     for (int e = 0; e < 32; ++e) v[e] = 0u;
                 }
                 if (32 * r >= g.C || first >= g.Tk) continue;
-                if (cut.splits == 1) {
+                if (cut.line ? k.split < 0 : cut.splits == 1) {
                     na2d_tc::stage_and_store<DT, 32, 2>(which ? &tm_dk : &tm_dv, stage, v, scale, 32 * r, first, k.m, k.b, 0, lane, &seq);
                 } else if (key < g.Tk) {
-                    float4* dst = reinterpret_cast<float4*>(
-                        (which ? cut.part_dk : cut.part_dv) +
-                        ((static_cast<size_t>(k.split) * g.units + static_cast<size_t>(k.b) * g.Nk + k.m) * g.Tk + key) * g.C + 32 * r);
+                    const size_t at = cut.line ? static_cast<size_t>(k.split) * kRows + quarter * 32 + lane
+                                               : (static_cast<size_t>(k.split) * g.units + static_cast<size_t>(k.b) * g.Nk + k.m) * g.Tk + key;
+                    float4* dst = reinterpret_cast<float4*>((which ? cut.part_dk : cut.part_dv) + at * g.C + 32 * r);
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         if (32 * r + 4 * e < g.C)
@@ -366,8 +428,9 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         const uint64_t scale2 = pair2(g.sl2, g.sl2), unit2 = pair2(Weight<DT>::kUnit, Weight<DT>::kUnit);
         uint32_t m = 0;
         Ring ring;
-        for (int item = blockIdx.x; item < cut.items; item += gridDim.x) {
-            const KeyItem k(g, cut, item);
+        for (KeyWalk walk(g, cut, before); walk.more(cut);) {
+            const KeyItem k = walk.get(g, cut, before);
+            walk.next(k);
             const int key = k.k0 + row;
             // the first token that sees this key
             const int t_lo = key >= k.count ? 0x7fffffff : g.causal ? max(key + g.Tq - k.count, 0) : 0;
@@ -477,6 +540,48 @@ attn_sum_kernel(const float* __restrict__ part_dk, const float* __restrict__ par
     *reinterpret_cast<uint2*>((blockIdx.y ? dv : dk) + i) = make_uint2(pack2<DT>(acc.x, acc.y), pack2<DT>(acc.z, acc.w));
 }
 
+// Line: a block joins the parts of one tile of keys, or writes zeros where the tile holds none.
+template <typename DT>
+__global__ void __launch_bounds__(256)
+attn_join_kernel(const float* __restrict__ part_dk, const float* __restrict__ part_dv, DT* __restrict__ dk, DT* __restrict__ dv,
+                 const Geom g, const KeyCut cut) {
+    after_previous_grid();
+    next_grid_may_start();
+    int tile, m, before = 0, all = 0;                    // tiles of one key head of the entries before b, and of all
+    const int unit = cut.by_key_tiles.split(blockIdx.x, tile), b = g.by_nk.split(unit, m), lane = threadIdx.x & 31;
+    for (int i = lane; i < g.B; i += 32) {
+        const int tiles = (key_count(g, i) + kRows - 1) / kRows;
+        all += tiles;
+        if (i < b) before += tiles;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, d);
+        before += __shfl_xor_sync(0xffffffffu, before, d);
+    }
+    const int tiles = (key_count(g, b) + kRows - 1) / kRows, each = (all * g.Nk * g.tiles + cut.line - 1) / cut.line;
+    const int at = (before * g.Nk + m * tiles + tile) * g.tiles;
+    const int lo = tile < tiles ? at / each : 0, hi = tile < tiles ? (at + g.tiles - 1) / each : 0;      // CTAs that have some of it
+    if (tile < tiles && lo == hi) return;                // one had them all
+    const int vectors = g.C / 4, rows = min(kRows, g.Tk - tile * kRows);
+    const float* part = blockIdx.y ? part_dv : part_dk;
+    DT* dst = (blockIdx.y ? dv : dk) + (static_cast<size_t>(unit) * g.Tk + static_cast<size_t>(tile) * kRows) * g.C;
+    for (int i = threadIdx.x; i < rows * vectors; i += 256) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (tile < tiles) {
+#pragma unroll 4
+            for (int s = lo; s <= hi; ++s) {             // lo has the tile's first chunk
+                const float4 v = *reinterpret_cast<const float4*>(part + (2 * s + (s == lo)) * static_cast<size_t>(kRows) * g.C + 4 * i);
+                acc.x += v.x;
+                acc.y += v.y;
+                acc.z += v.z;
+                acc.w += v.w;
+            }
+        }
+        *reinterpret_cast<uint2*>(dst + 4 * i) = make_uint2(pack2<DT>(acc.x, acc.y), pack2<DT>(acc.z, acc.w));
+    }
+}
+
 template <typename DT, int D>
 int launch_dkdv(const Place& at, const Geom& g, const KeyCut& cut, const Operand& q, const Operand& k, const Operand& v, const Operand& d_o,
                 const float* lse, const float* delta, const Operand& d_k, const Operand& d_v) {
@@ -494,9 +599,16 @@ int launch_dkdv(const Place& at, const Geom& g, const KeyCut& cut, const Operand
     if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted) != cudaSuccess) return NA2D_ERR_CUDA;
     const int sms = na2d_tc::sm_count(at.device);
     *at.launched += 1;
-    if (na2d_launch::launch(true, kern, cut.items < sms ? cut.items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdk, tdv, lse, delta, at.errors,
+    if (na2d_launch::launch(true, kern, cut.line ? cut.line : cut.items < sms ? cut.items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdk, tdv, lse, delta, at.errors,
                             g, cut) != cudaSuccess)
         return NA2D_ERR_CUDA;
+    if (cut.line) {
+        *at.launched += 1;
+        return na2d_launch::launch(true, attn_join_kernel<DT>, dim3((unsigned)(g.units * cut.key_tiles), 2), 256, 0, at.st,
+                                   (const float*)cut.part_dk, (const float*)cut.part_dv, (DT*)d_k.ptr, (DT*)d_v.ptr, g, cut) == cudaSuccess
+                   ? NA2D_OK
+                   : NA2D_ERR_CUDA;
+    }
     if (cut.splits == 1) return NA2D_OK;
     const long long elements = (long long)g.units * g.Tk * g.C;
     *at.launched += 1;

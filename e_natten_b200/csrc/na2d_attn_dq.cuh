@@ -18,27 +18,38 @@
 
 namespace na2d_attn {
 
-// delta = dO . o of each row, 8 channels a lane.  LPR lanes a row: C / 8, rounded up to a power of two.
+// delta = dO . o of each row, 8 channels a lane.  LPR lanes a row: C / 8, rounded up to a power of two.  A lane has kDeltaRows rows of one
+// head, 256 / LPR apart, all under way at once.
+constexpr int kDeltaRows = 4;
 template <typename DT, int LPR>
 __global__ void __launch_bounds__(256)
 attn_delta_kernel(const DT* __restrict__ d_o, const Operand st_do, const DT* __restrict__ o, const Operand st_o, float* __restrict__ delta,
-                  const Geom g) {
+                  const Geom g, const Div by_tiles, const Div by_heads) {
     after_previous_grid();
     next_grid_may_start();
-    const long long rows = (long long)g.B * g.N * g.Tq;
-    const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-    const int part = threadIdx.x % LPR;
-    float acc = 0.f;
-    if (row < rows && 8 * part < g.C) {
-        const int t = (int)(row % g.Tq);
-        const long long bn = row / g.Tq, b = bn / g.N, n = bn - b * g.N;
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(d_o + b * st_do.b + n * st_do.n + t * st_do.t) + part);
-        const uint4 y = __ldg(reinterpret_cast<const uint4*>(o + b * st_o.b + n * st_o.n + t * st_o.t) + part);
-        acc = na2d_delta::dot8<DT>(x, y, 0.f);
+    constexpr int kStep = 256 / LPR;
+    int tile, n;
+    const int bn = by_tiles.split(blockIdx.x, tile), b = by_heads.split(bn, n);
+    const int part = threadIdx.x % LPR, t0 = tile * kDeltaRows * kStep + threadIdx.x / LPR;
+    const DT *x = d_o + b * st_do.b + n * st_do.n + 8 * part, *y = o + b * st_o.b + n * st_o.n + 8 * part;
+    uint4 vx[kDeltaRows], vy[kDeltaRows];
+#pragma unroll
+    for (int i = 0; i < kDeltaRows; ++i) {
+        const int t = t0 + i * kStep;
+        vx[i] = vy[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (t < g.Tq && 8 * part < g.C) {
+            vx[i] = __ldg(reinterpret_cast<const uint4*>(x + t * st_do.t));
+            vy[i] = __ldg(reinterpret_cast<const uint4*>(y + t * st_o.t));
+        }
     }
 #pragma unroll
-    for (int d = LPR / 2; d > 0; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
-    if (part == 0 && row < rows) delta[row] = acc;
+    for (int i = 0; i < kDeltaRows; ++i) {
+        float acc = na2d_delta::dot8<DT>(vx[i], vy[i], 0.f);
+#pragma unroll
+        for (int d = LPR / 2; d > 0; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
+        const int t = t0 + i * kStep;
+        if (part == 0 && t < g.Tq) delta[static_cast<size_t>(bn) * g.Tq + t] = acc;
+    }
 }
 
 template <int D>
@@ -326,19 +337,29 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const uint32_t dp_addr = tmem_lane + C::TMEM_DP + 64 * half;
         const uint64_t scale2 = pair2(g.sl2, g.sl2);
         uint32_t m = 0;                                      // chunks so far
+        // lse and delta of a row: read an item ahead, since few chunks to an item would not cover the way to memory
+        auto fetch = [&](int item, float& of_lse, float& of_delta) {
+            of_lse = -CUDART_INF_F;
+            of_delta = 0.f;
+            if (item >= items) return;
+            const RowTile tile = tile_of(item);
+            int n, t;
+            if (!tile.row(g, row, n, t)) return;
+            const size_t at = row_index(g, tile.b, n, t);
+            of_lse = __ldg(lse + at);
+            of_delta = __ldg(delta + at);
+        };
+        float next_lse, next_delta;
+        fetch(blockIdx.x, next_lse, next_delta);
         for (int item = blockIdx.x; item < items; item += gridDim.x) {
+            const float row_lse = next_lse, row_delta = next_delta;
+            fetch(item + gridDim.x, next_lse, next_delta);
             const RowTile tile = tile_of(item);
             const int chunks = chunks_of(tile);
             if (chunks == 0) continue;
             int n, t;
             const bool ok = tile.row(g, row, n, t);
             const bool idle = !__any_sync(0xffffffffu, ok);
-            float row_lse = -CUDART_INF_F, row_delta = 0.f;
-            if (ok) {
-                const size_t at = row_index(g, tile.b, n, t);
-                row_lse = __ldg(lse + at);
-                row_delta = __ldg(delta + at);
-            }
             // a row that sees nothing has weights of zero: exp2(-infinity)
             const float neg = row_lse == -CUDART_INF_F ? -CUDART_INF_F : -row_lse * kLog2e;
             const uint64_t neg2 = pair2(neg, neg), delta2 = pair2(-row_delta, -row_delta);
@@ -410,13 +431,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 
 template <typename DT>
 int launch_delta(const Place& at, const Geom& g, const Operand& d_o, const Operand& o, float* delta) {
-    const long long rows = (long long)g.B * g.N * g.Tq;
-    const int lanes = g.C <= 32 ? 4 : g.C <= 64 ? 8 : 16;
-    const long long blocks = (rows * lanes + 255) / 256;
+    const int lanes = g.C <= 32 ? 4 : g.C <= 64 ? 8 : 16, rows = kDeltaRows * 256 / lanes, tiles = (g.Tq + rows - 1) / rows;
+    const long long blocks = (long long)g.B * g.N * tiles;
     if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
     auto kern = lanes == 4 ? attn_delta_kernel<DT, 4> : lanes == 8 ? attn_delta_kernel<DT, 8> : attn_delta_kernel<DT, 16>;
     *at.launched += 1;
-    return na2d_launch::launch(false, kern, (unsigned)blocks, 256, 0, at.st, (const DT*)d_o.ptr, d_o, (const DT*)o.ptr, o, delta, g) == cudaSuccess
+    return na2d_launch::launch(false, kern, (unsigned)blocks, 256, 0, at.st, (const DT*)d_o.ptr, d_o, (const DT*)o.ptr, o, delta, g, Div(tiles),
+                               Div(g.N)) == cudaSuccess
                ? NA2D_OK
                : NA2D_ERR_CUDA;
 }

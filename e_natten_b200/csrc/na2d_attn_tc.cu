@@ -51,16 +51,26 @@ int forward_parts(const Geom& g, int sms) {
     return (int)std::max(1LL, std::min<long long>((8LL * sms + tiles - 1) / tiles, chunks / 4));
 }
 
-// Parts of the queries in the key half, by the same rule with one tile a CTA: a part costs its sums' way through memory.
+// CTAs that share the line of the key half's chunks, at least 4 chunks each; 0 where every tile is a CTA's item.  By items a CTA has a
+// whole number of tiles, and with lengths some of them are empty; the line costs its parts' way through memory, about 4 chunks' time.
+int key_line(const Geom& g, int sms) {
+    const long long tiles = (long long)g.units * ((g.Tk + kRows - 1) / kRows), chunks = tiles * g.tiles;
+    if (g.causal || g.B > kLineEntries || chunks + sms > 0x7fffffffLL) return 0;
+    const bool pays = g.lengths ? g.tiles >= 8 : (tiles + sms - 1) / sms * g.tiles > (chunks + sms - 1) / sms + 4;
+    return pays ? (int)std::max(1LL, std::min<long long>(sms, chunks / 4)) : 0;
+}
+
+// Parts of the queries in the key half of causal calls, where tiles are fewer than CTAs: a part costs its sums' way through memory.
 int key_parts(const Geom& g, int sms) {
     const long long tiles = (long long)g.units * ((g.Tk + kRows - 1) / kRows);
-    if (tiles >= sms) return 1;
+    if (!g.causal || tiles >= sms) return 1;
     return (int)std::max(1LL, std::min<long long>((4LL * sms + tiles - 1) / tiles, g.tiles / 4));
 }
 
 size_t line_rows(const Geom& g, int sms) { return (size_t)(line_groups(g, sms) + g.units) * g.G * g.Tq; }
 size_t all_rows(const Geom& g) { return (size_t)g.B * g.N * g.Tq; }
 size_t key_part(const Geom& g) { return (size_t)g.units * g.Tk * g.C; }
+size_t line_part(const Geom& g, int line) { return (size_t)line * 2 * 2 * kRows * g.C; }        // of dK and dV, 2 a CTA
 
 }  // namespace
 
@@ -104,13 +114,15 @@ int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Scratch& scratc
         if (g.causal) cut_rows(gk, false);               // a chunk's masks go by the column alone
         KeyCut cut{};
         cut.key_tiles = (g.Tk + kRows - 1) / kRows;
-        cut.splits = (int)std::min<size_t>(key_parts(g, na2d_tc::sm_count(at.device)), std::max<size_t>(1, scratch.floats / (2 * key_part(g))));
+        const int sms = na2d_tc::sm_count(at.device), line = key_line(g, sms);
+        if (line && scratch.floats >= line_part(g, line)) cut.line = line;
+        cut.splits = (int)std::min<size_t>(key_parts(g, sms), std::max<size_t>(1, scratch.floats / (2 * key_part(g))));
         cut.each = (gk.tiles + cut.splits - 1) / cut.splits;
         cut.by_splits = Div(cut.splits);
         cut.by_key_tiles = Div(cut.key_tiles);
-        if (cut.splits > 1) {
+        if (cut.line || cut.splits > 1) {
             cut.part_dk = scratch.at;
-            cut.part_dv = scratch.at + cut.splits * key_part(g);
+            cut.part_dv = scratch.at + (cut.line ? line_part(g, cut.line) / 2 : cut.splits * key_part(g));
         }
         const long long items = (long long)gk.units * cut.key_tiles * cut.splits;
         if (items > 0x3fffffffLL) return (int)NA2D_ERR_TOO_LARGE;
@@ -126,6 +138,7 @@ size_t forward_floats(const Geom& g, int sms) {
     return parts > 1 ? parts * all_rows(g) * (g.C + 1) : 0;
 }
 size_t key_floats(const Geom& g, int sms) {
+    if (const int line = key_line(g, sms)) return line_part(g, line);
     const int parts = key_parts(g, sms);
     return parts > 1 ? 2 * parts * key_part(g) : 0;
 }

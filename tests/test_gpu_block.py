@@ -181,6 +181,20 @@ def test_attention_of_few_keys_in_parts(dtype):
     check_attention(q, k, v, rand(2, 8, 1500, 64, dtype=dtype, seed=3), 0.125, lengths=torch.tensor([100, 37], device=DEV))
 
 
+@pytest.mark.parametrize("dtype,C", [(BF16, 64), (F16, 128), (BF16, 32)])
+@pytest.mark.parametrize("B,N,Nk,Tq,Tk,lengths", [
+    (10, 5, 5, 1024, 384, None),                                      # 150 tiles of keys: a second round for two of them
+    (7, 4, 2, 700, 300, [300, 0, 129, 1, 128, 299, 0]),               # some tiles hold no key
+    (3, 2, 1, 1100, 900, [0, 0, 0]),
+    (3, 2, 2, 1030, 140, [0, 140, 0]),
+])
+def test_attention_shares_the_queries_out(B, N, Nk, Tq, Tk, lengths, dtype, C):
+    """The key half, where its CTAs take equal stretches of all tiles' queries."""
+    q, d_o = rand(B, N, Tq, C, dtype=dtype), rand(B, N, Tq, C, dtype=dtype, seed=3)
+    k, v = rand(B, Nk, Tk, C, dtype=dtype, seed=1), rand(B, Nk, Tk, C, dtype=dtype, seed=2)
+    check_attention(q, k, v, d_o, C ** -0.5, lengths=None if lengths is None else torch.tensor(lengths, device=DEV))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_attention_on_grids_and_views(dtype):
     """(B, heads, H, W, C) views of a packed projection, a gradient with heads last, an image whose rows do not follow one another."""
