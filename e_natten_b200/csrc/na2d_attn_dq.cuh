@@ -219,13 +219,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         };
         Ring rs, rp, ro;                     // places of the chunks that S, dP and dQ are at
         uint32_t ns = 0, no = 0, it = 0;     // chunks that S and dQ are at, tiles
-        auto scores = [&]() {
+        auto scores = [&](uint32_t tile) {
             mbar_wait(k_full + rs.at, rs.phase, wctx, kErrLoadWait);
             if (g.lengths) mbar_wait(k_clear + rs.at, rs.phase, wctx, kErrOther);
             mbar_wait(s_free + (ns & 1), ((ns >> 1) & 1) ^ 1, wctx, kErrMmaWait);
             tc_fence_after();
             if (elect_one()) {
-                product(tmem_base + C::TMEM_S + (ns & 1) * kRows, q_lo + it % NQ * (C::BYTES >> 4), k_lo0 + rs.at * (C::BYTES >> 4));
+                product(tmem_base + C::TMEM_S + (ns & 1) * kRows, q_lo + tile % NQ * (C::BYTES >> 4), k_lo0 + rs.at * (C::BYTES >> 4));
                 umma_commit(s_full + (ns & 1));
             }
             __syncwarp();
@@ -241,17 +241,28 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             __syncwarp();
             rp.next(NST);
         };
+        bool ahead = false;                  // the tile's first scores have been issued
         int next = (int)blockIdx.x < items ? chunks_of(tile_of(blockIdx.x)) : 0;
         for (int item = blockIdx.x; item < items; item += gridDim.x) {
             const int n = next;
             next = item + (int)gridDim.x < items ? chunks_of(tile_of(item + gridDim.x)) : 0;      // (ahead: a length is a load from memory)
             if (n == 0) continue;
-            mbar_wait(q_full + it % NQ, (it / NQ) & 1, wctx, kErrLoadWait);
-            scores();
+            if (!ahead) {
+                mbar_wait(q_full + it % NQ, (it / NQ) & 1, wctx, kErrLoadWait);
+                scores(it);
+            }
             grads(n == 1);                   // (dS of the chunk before has been read: dQ came before on the pipe)
             for (int c = 0; c < n; ++c, ++no) {
                 if (lane == 0) NA2D_TR(2, 0, no);
-                if (c + 1 < n) scores();
+                if (c + 1 < n) {
+                    scores(it);
+                } else {                     // with room for its Q: the next tile's first scores, under this one's last chunk
+                    ahead = NQ > 1 && next > 0;
+                    if (ahead) {
+                        mbar_wait(q_full + (it + 1) % NQ, ((it + 1) / NQ) & 1, wctx, kErrLoadWait);
+                        scores(it + 1);
+                    }
+                }
                 if (lane == 0) NA2D_TR(2, 1, no);
                 if (c == 0) mbar_wait(dq_free, (it & 1) ^ 1, wctx, kErrMmaWait);
                 mbar_wait(ds_full, no & 1, wctx, kErrMmaWait);
