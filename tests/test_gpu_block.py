@@ -353,6 +353,15 @@ def test_group_norm(shape, groups, dtype, activation):
     check_norm(x, groups, rand(C, seed=1, scale=0.3, shift=1.0), rand(C, seed=2), rand(*shape, dtype=dtype, seed=3), activation)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape,groups", [((2, 9, 7, 301), 1), ((1, 5, 1542), 3), ((3, 60, 61, 301), 1), ((1, 1, 2055), 5)], ids=str)
+def test_group_norm_of_wide_groups(shape, groups, dtype):
+    """More channels a group than a block has threads, and no whole vectors."""
+    C = shape[-1]
+    x = (rand(*shape, scale=1.5) + rand(C, seed=5)).to(dtype)
+    check_norm(x, groups, rand(C, seed=1, scale=0.3, shift=1.0), rand(C, seed=2), rand(*shape, dtype=dtype, seed=3))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_group_norm_parameters(dtype):
     """Of the map's dtype, or one of them, or none."""
