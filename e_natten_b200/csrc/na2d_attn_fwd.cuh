@@ -205,6 +205,9 @@ struct FwdCfg : TileCfg<D> {
 // and most chunks after the first rescale nothing.
 constexpr float kGrow = 8.f;
 
+// Columns of P whose product starts ahead of the others.
+constexpr int kMost = 96;
+
 template <typename DT, int D, bool PAIR>
 __global__ void __launch_bounds__(512, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -227,7 +230,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     uint64_t* o_free = bars + 10;            // [2] epilogue -> MMA
     uint64_t* s_full = bars + 52;            // [2] MMA (commit) -> softmax
     uint64_t* p_full = bars + 54;            // [2] softmax -> MMA
-    uint64_t* p_half = bars + 56;            // [2] softmax -> MMA: the first 64 columns of P
+    uint64_t* p_most = bars + 56;            // [2] softmax -> MMA: the first kMost columns of P
     uint64_t* k_full = bars + 12;            // [8] TMA -> MMA
     uint64_t* v_full = bars + 20;            // [8] TMA -> MMA
     uint64_t* k_empty = bars + 28;           // [8] MMA (commit) -> TMA
@@ -246,7 +249,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             mbar_init(o_free + i, 4);
             mbar_init(s_full + i, 1);
             mbar_init(p_full + i, 4);
-            mbar_init(p_half + i, 4);
+            mbar_init(p_most + i, 4);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(q_full + i, 1);
@@ -382,33 +385,31 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             __device__ __forceinline__ uint32_t ahead(int c, int x) const { return PAIR ? c : c + min(c + x, other); }
         };
         uint32_t base = 0, chunks = 0, tiles = 0;        // loads, this group's chunks and tiles so far
+        // (by the elected lane, K there)
         auto scores = [&](const Item& t, int c) {
-            const uint32_t at = (base + t.ahead(c, x)) % NST, phase = ((base + t.ahead(c, x)) / NST) & 1;
-            if (lane == 0) NA2D_TR(1 + x, 3, chunks + (c > 0));
-            mbar_wait(k_full + at, phase, wctx, kErrLoadWait);
-            if (lane == 0) NA2D_TR(1 + x, 4, chunks + (c > 0));
-            tc_fence_after();
-            const uint32_t q_lo = q_lo0 + tiles % NQ * (C::BYTES >> 4), k_lo = k_lo0 + at * (C::BYTES >> 4);
-            if (elect_one()) {
+            const uint32_t at = (base + t.ahead(c, x)) % NST, q_lo = q_lo0 + tiles % NQ * (C::BYTES >> 4), k_lo = k_lo0 + at * (C::BYTES >> 4);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    constexpr int kPerSlab = C::SLAB_C / 16;
-                    const int slab = kk / kPerSlab, in = 2 * (kk % kPerSlab);
-                    umma_ss(t_s, desc64(hi, q_lo + ((slab * C::SLAB) >> 4) + in), desc64(hi, k_lo + ((slab * C::SLAB) >> 4) + in), idesc_s, kk > 0);
-                }
-                umma_commit(s_full + x);                                      // and P V of the group's chunk before
-                umma_commit(k_empty + at);
-                if (c + 1 == t.n) umma_commit(q_empty + 2 * x + tiles % NQ);
-                NA2D_TR(1 + x, 5, chunks + (c > 0));
+            for (int kk = 0; kk < D / 16; ++kk) {
+                constexpr int kPerSlab = C::SLAB_C / 16;
+                const int slab = kk / kPerSlab, in = 2 * (kk % kPerSlab);
+                umma_ss(t_s, desc64(hi, q_lo + ((slab * C::SLAB) >> 4) + in), desc64(hi, k_lo + ((slab * C::SLAB) >> 4) + in), idesc_s, kk > 0);
             }
-            __syncwarp();
+            umma_commit(s_full + x);                                          // and P V of the group's chunk before
+            umma_commit(k_empty + at);
+            if (c + 1 == t.n) umma_commit(q_empty + 2 * x + tiles % NQ);
+        };
+        auto key_wait = [&](const Item& t, int c) {
+            mbar_wait(k_full + (base + t.ahead(c, x)) % NST, ((base + t.ahead(c, x)) / NST) & 1, wctx, kErrLoadWait);
         };
         FwdWalk<PAIR> walk(g, cut, before);
         Item t(g, cut, before, walk, x);
         while (walk.more(cut)) {
             if (t.n > 0) {
                 mbar_wait(q_full + 2 * x + tiles % NQ, (tiles / NQ) & 1, wctx, kErrLoadWait);
-                scores(t, 0);
+                key_wait(t, 0);
+                tc_fence_after();
+                if (elect_one()) scores(t, 0);
+                __syncwarp();
             }
             walk.next(g, cut, before);
             const Item next(g, cut, before, walk, x);
@@ -417,27 +418,30 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 if (c == 0) mbar_wait(o_free + x, (tiles & 1) ^ 1, wctx, kErrMmaWait);      // the tile before has been read out
                 mbar_wait(v_full + at, phase, wctx, kErrLoadWait);
                 if (g.lengths) mbar_wait(v_clear + at, phase, wctx, kErrOther);
+                const bool more = c + 1 < t.n;
+                if (more) key_wait(t, c + 1);            // (its load does not wait for this chunk's P V)
                 if (lane == 0) NA2D_TR(1 + x, 0, chunks);
                 const uint32_t v_lo = v_lo0 + at * (C::BYTES >> 4);
+                auto product = [&](int from, int to) {
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    mbar_wait((half ? p_full : p_half) + x, chunks & 1, wctx, kErrMmaWait);
-                    tc_fence_after();
-                    if (elect_one()) {
-#pragma unroll
-                        for (int kk = half * kRows / 32; kk < (half + 1) * kRows / 32; ++kk)
-                            umma_ts(t_o, t_s + 8 * kk, desc64(hi, v_lo + ((kk * 16 * C::ROWB) >> 4)), idesc_o, (c > 0) || (kk > 0));
-                    }
-                    __syncwarp();
-                }
+                    for (int kk = from; kk < to; ++kk)
+                        umma_ts(t_o, t_s + 8 * kk, desc64(hi, v_lo + ((kk * 16 * C::ROWB) >> 4)), idesc_o, (c > 0) || (kk > 0));
+                };
+                mbar_wait(p_most + x, chunks & 1, wctx, kErrMmaWait);
+                tc_fence_after();
+                if (elect_one()) product(0, kMost / 16);
+                __syncwarp();
+                mbar_wait(p_full + x, chunks & 1, wctx, kErrMmaWait);
+                tc_fence_after();
                 if (lane == 0) NA2D_TR(1 + x, 1, chunks);
                 if (elect_one()) {
+                    product(kMost / 16, kRows / 16);
                     umma_commit(v_empty + at);
-                    if (c + 1 == t.n) umma_commit(o_full + x);
+                    if (!more) umma_commit(o_full + x);
+                    else scores(t, c + 1);               // into the buffer that P V has just read: a thread's MMAs run in their order
                     NA2D_TR(1 + x, 2, chunks);
                 }
                 __syncwarp();
-                if (c + 1 < t.n) scores(t, c + 1);       // into the buffer that P V has just read: a thread's MMAs run in their order
             }
             // chunks that only the pair's other tile has: their buffers wait for both groups
             for (int c = t.n; PAIR && c < t.other; ++c) {
@@ -568,7 +572,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
-                            mbar_arrive(p_half + group);
+                            mbar_arrive(p_most + group);
                             mbar_arrive(p_full + group);
                         }
                         ++m;
@@ -638,11 +642,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                         w[e2] = pack2<DT>(p0, p1);
                     }
                     tmem_st_32x16(s_addr + 16 * a, w);
-                    if (a == 1) {                            // the first half of P V goes under the other half's exponentials
+                    if (32 * (a + 1) == kMost) {             // most of P V goes under the last exponentials
                         tmem_st_wait();
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(p_half + group);
+                        if (lane == 0) mbar_arrive(p_most + group);
                     }
                 }
                 bar_arrive(other_turn, 256);
