@@ -314,42 +314,46 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         };
         Ring rs, ro;                          // places of the chunks that S and the outputs are at
         uint32_t no = 0, it = 0;
+        // what the elected lane issues
         auto scores = [&]() {
-            mbar_wait(qd_full + rs.at, rs.phase, wctx, kErrLoadWait);
-            mbar_wait(x_full + rs.at, rs.phase, wctx, kErrLoadWait);
-            tc_fence_after();
-            if (elect_one()) {
-                product(tmem_base + C::TMEM_S, k_lo + it % NKV * (C::BYTES >> 4), q_lo0 + rs.at * (C::BYTES >> 4));
-                umma_commit(s_full);
-            }
-            __syncwarp();
+            product(tmem_base + C::TMEM_S, k_lo + it % NKV * (C::BYTES >> 4), q_lo0 + rs.at * (C::BYTES >> 4));
+            umma_commit(s_full);
         };
         auto grads = [&](bool last) {
-            if (elect_one()) {
-                product(tmem_base + C::TMEM_DP, v_lo + it % NKV * (C::BYTES >> 4), g_lo0 + rs.at * (C::BYTES >> 4));
-                umma_commit(dp_full);
-                if (last) umma_commit(kv_empty + it % NKV);
-            }
-            __syncwarp();
-            rs.next(NST);
+            product(tmem_base + C::TMEM_DP, v_lo + it % NKV * (C::BYTES >> 4), g_lo0 + rs.at * (C::BYTES >> 4));
+            umma_commit(dp_full);
+            if (last) umma_commit(kv_empty + it % NKV);
+        };
+        auto chunk_wait = [&]() {
+            mbar_wait(qd_full + rs.at, rs.phase, wctx, kErrLoadWait);
+            mbar_wait(x_full + rs.at, rs.phase, wctx, kErrLoadWait);
         };
         for (KeyWalk walk(g, cut, before); walk.more(cut);) {
             const KeyItem k = walk.get(g, cut, before);
             walk.next(k);
             if (k.n == 0) continue;
             mbar_wait(kv_full + it % NKV, (it / NKV) & 1, wctx, kErrLoadWait);
-            scores();
-            grads(k.n == 1);
+            chunk_wait();
+            tc_fence_after();
+            if (elect_one()) {
+                scores();
+                grads(k.n == 1);
+            }
+            __syncwarp();
+            rs.next(NST);
             for (int i = 0; i < k.n; ++i, ++no) {
+                const bool more = i + 1 < k.n;
                 if (i == 0) mbar_wait(acc_free, (it & 1) ^ 1, wctx, kErrMmaWait);
+                if (more) chunk_wait();      // (of the next one, ahead of what holds this one up)
                 if (lane == 0) NA2D_TR(2, 0, no);
                 mbar_wait(p_full, no & 1, wctx, kErrMmaWait);
                 tc_fence_after();
                 if (lane == 0) NA2D_TR(2, 1, no);
-                if (elect_one()) gather(tmem_base + C::TMEM_DV, tmem_base + C::TMEM_S, gm_lo0 + ro.at * (C::BYTES >> 4), i > 0);
+                if (elect_one()) {
+                    gather(tmem_base + C::TMEM_DV, tmem_base + C::TMEM_S, gm_lo0 + ro.at * (C::BYTES >> 4), i > 0);
+                    if (more) scores();
+                }
                 __syncwarp();
-                if (lane == 0) NA2D_TR(2, 2, no);
-                if (i + 1 < k.n) scores();
                 if (lane == 0) NA2D_TR(2, 3, no);
                 mbar_wait(ds_full, no & 1, wctx, kErrMmaWait);
                 tc_fence_after();
@@ -357,13 +361,13 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 if (elect_one()) {
                     gather(tmem_base + C::TMEM_DK, tmem_base + C::TMEM_DP, qm_lo0 + ro.at * (C::BYTES >> 4), i > 0);
                     umma_commit(qd_empty + ro.at);
-                    if (i + 1 == k.n) umma_commit(acc_full);
+                    if (more) grads(i + 2 == k.n);
+                    else umma_commit(acc_full);
                 }
                 __syncwarp();
+                if (more) rs.next(NST);
                 ro.next(NST);
                 if (lane == 0) NA2D_TR(2, 5, no);
-                if (i + 1 < k.n) grads(i + 2 == k.n);
-                if (lane == 0) NA2D_TR(2, 6, no);
             }
             ++it;
         }

@@ -232,14 +232,10 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             ++ns;
             rs.next(NST);
         };
-        auto grads = [&](bool last) {        // (its chunk has landed: S came before)
-            if (elect_one()) {
-                product(tmem_base + C::TMEM_DP, g_lo + it % NQ * (C::BYTES >> 4), v_lo0 + rp.at * (C::BYTES >> 4));
-                umma_commit(dp_full);
-                if (last) umma_commit(q_empty + it % NQ);
-            }
-            __syncwarp();
-            rp.next(NST);
+        auto grads = [&](bool last) {        // (by the elected lane; its chunk has landed: S came before)
+            product(tmem_base + C::TMEM_DP, g_lo + it % NQ * (C::BYTES >> 4), v_lo0 + rp.at * (C::BYTES >> 4));
+            umma_commit(dp_full);
+            if (last) umma_commit(q_empty + it % NQ);
         };
         bool ahead = false;                  // the tile's first scores have been issued
         int next = (int)blockIdx.x < items ? chunks_of(tile_of(blockIdx.x)) : 0;
@@ -251,7 +247,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 mbar_wait(q_full + it % NQ, (it / NQ) & 1, wctx, kErrLoadWait);
                 scores(it);
             }
-            grads(n == 1);                   // (dS of the chunk before has been read: dQ came before on the pipe)
+            if (elect_one()) grads(n == 1);  // (dS of the chunk before has been read: dQ came before on the pipe)
+            __syncwarp();
+            rp.next(NST);
             for (int c = 0; c < n; ++c, ++no) {
                 if (lane == 0) NA2D_TR(2, 0, no);
                 if (c + 1 < n) {
@@ -275,12 +273,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                         umma_ts(tmem_base + C::TMEM_DQ, tmem_base + C::TMEM_DP + (kk / 4) * 64 + (kk % 4) * 8,
                                 desc64(hi, km_lo + ((kk * 16 * C::ROWB) >> 4)), idesc_o, (c > 0) || (kk > 0));
                     umma_commit(k_empty + ro.at);
-                    if (c + 1 == n) umma_commit(dq_full);
+                    if (c + 1 < n) grads(c + 2 == n);
+                    else umma_commit(dq_full);
                 }
                 __syncwarp();
+                if (c + 1 < n) rp.next(NST);
                 ro.next(NST);
                 if (lane == 0) NA2D_TR(2, 3, no);
-                if (c + 1 < n) grads(c + 2 == n);
             }
             ++it;
         }
