@@ -395,6 +395,28 @@ __device__ __forceinline__ void wait_for(const Role& role, const Pass& s, const 
     role.sync();
 }
 
+// A warp's groups one after the other, `use(g, v)` with lane's values of group g's runs, lane, lane + 32, ...: the next group's come while one
+// is used (each on its own was a chain of reads from L2, 8 us a set).
+constexpr int kRunsLane = 8, kMostRuns = 32 * kRunsLane;
+template <typename F>
+__device__ __forceinline__ void each_group(const Role& role, const Pass& s, const float2* part, F&& use) {
+    float2 v[kRunsLane], next[kRunsLane];
+    auto fetch = [&](int g) {
+#pragma unroll
+        for (int j = 0; j < kRunsLane; ++j) {
+            const int r = role.lane + 32 * j;
+            next[j] = r < s.runs && g < s.groups ? __ldcg(part + (long long)g * s.runs + r) : make_float2(0.f, 0.f);
+        }
+    };
+    fetch(role.warp);
+    for (int g = role.warp; g < s.groups; g += kHalf / 32) {
+#pragma unroll
+        for (int j = 0; j < kRunsLane; ++j) v[j] = next[j];
+        fetch(g + kHalf / 32);
+        use(g, v);
+    }
+}
+
 constexpr int kStage = 4;                       // pixels of a thread that are copied, and summed, together
 
 // What a thread reads of a run passes through shared memory that is its own, copied there several stages ahead: enough bytes are under
@@ -717,13 +739,17 @@ __global__ void __launch_bounds__(2 * kHalf, 1) norm_fwd_kernel(const Norm n, co
         wait_for(role, s, s.summed + i);
         if (mine) {
             const float inv_m = 1.f / ((float)n.P * n.cg);
-            for (int g = warp; g < s.groups; g += kHalf / 32) {
-                const float2* part = set.part + ((long long)at.unit * s.groups + g) * s.runs;
-                auto values = [&](int run) { return (float)(min(n.P, (run + 1) * s.run) - run * s.run) * n.cg; };
-                float sum = 0.f, square = 0.f;
-                for (int r = lane; r < s.runs; r += 32) sum = fmaf(values(r), part[r].x, sum);
+            each_group(role, s, set.part + (long long)at.unit * s.groups * s.runs, [&](int g, const float2 (&part)[kRunsLane]) {
+                float values[kRunsLane], sum = 0.f, square = 0.f;
+#pragma unroll
+                for (int j = 0; j < kRunsLane; ++j) {
+                    const long long first = (lane + 32 * j) * s.run;
+                    values[j] = (float)max(min(n.P, first + s.run) - first, 0ll) * n.cg;
+                    sum = fmaf(values[j], part[j].x, sum);
+                }
                 const float mean = warp_sum(sum) * inv_m;
-                for (int r = lane; r < s.runs; r += 32) square += fmaf(values(r) * (part[r].x - mean), part[r].x - mean, part[r].y);
+#pragma unroll
+                for (int j = 0; j < kRunsLane; ++j) square += fmaf(values[j] * (part[j].x - mean), part[j].x - mean, part[j].y);
                 const float rstd = rsqrtf(fmaf(warp_sum(square), inv_m, n.eps));
                 if (lane == 0) {
                     stats[g] = make_float2(mean, rstd);
@@ -732,7 +758,7 @@ __global__ void __launch_bounds__(2 * kHalf, 1) norm_fwd_kernel(const Norm n, co
                         n.rstd[at.b * n.G + at.c0 / n.cg + g] = rstd;
                     }
                 }
-            }
+            });
             role.sync();
             if (at.pixels > 0) {
                 Affine<N> k;
@@ -845,19 +871,19 @@ __global__ void __launch_bounds__(2 * kHalf, 1) norm_bwd_kernel(const Norm n, co
         wait_for(role, s, s.summed + i);
         if (mine) {
             const float inv_m = 1.f / ((float)n.P * n.cg);
-            for (int g = warp; g < s.groups; g += kHalf / 32) {
-                const float2* part = set.part + ((long long)at.unit * s.groups + g) * s.runs;
+            each_group(role, s, set.part + (long long)at.unit * s.groups * s.runs, [&](int g, const float2 (&part)[kRunsLane]) {
+                const int at_g = at.b * n.G + at.c0 / n.cg + g;
+                const float rstd = n.rstd[at_g], mean = n.mean[at_g];
                 float s1 = 0.f, s2 = 0.f;
-                for (int r = lane; r < s.runs; r += 32) {
-                    s1 += part[r].x;
-                    s2 += part[r].y;
+#pragma unroll
+                for (int j = 0; j < kRunsLane; ++j) {
+                    s1 += part[j].x;
+                    s2 += part[j].y;
                 }
                 s1 = warp_sum(s1) * inv_m;
                 s2 = warp_sum(s2) * inv_m;
-                const int at_g = at.b * n.G + at.c0 / n.cg + g;
-                const float rstd = n.rstd[at_g];
-                if (lane == 0) group[g] = make_float4(n.mean[at_g], rstd, -rstd * s1, -rstd * rstd * s2);
-            }
+                if (lane == 0) group[g] = make_float4(mean, rstd, -rstd * s1, -rstd * rstd * s2);
+            });
             role.sync();
             if (at.pixels > 0) {
                 Affine<N> k;
@@ -1006,7 +1032,7 @@ __global__ void __launch_bounds__(kThreads) norm_params_kernel(const float2* __r
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 constexpr int kChipBytes = 112 << 10;           // shared memory of a block on the chip: two blocks an SM
-constexpr long long kL2Bytes = 72ll << 20;      // what a set of the two passes reads: it is in L2 still when it is written (4 x 256^2 x 512, step: 12 MB 451 us, 36 MB 429, 72 MB 405)
+constexpr long long kL2Bytes = 72ll << 20;      // what a set of the two passes reads: it is in L2 still when it is written (4 x 256^2 x 512, step: 12 MB 451 us, 36 MB 415, 72 MB 401; 150 MB: 380, but 3 x 300^2 x 384 172 for 139 us forward, its sets being uneven)
 
 int power_of_two(int n) {
     int p = 1;
@@ -1090,7 +1116,7 @@ bool pass_plan(const Norm& n, int esize, int vec, bool backward, int sms, Pass* 
     s->at_once = (int)std::max(1LL, std::min({(long long)s->units, kL2Bytes / std::max(1LL, (long long)bytes(s->channels)), (long long)sms}));
     s->sets = (s->units + s->at_once - 1) / s->at_once;
     const int rows = kHalf / s->cols_p2;
-    const long long runs = std::max(1LL, std::min((long long)sms / s->at_once, n.P / (kStage * rows)));
+    const long long runs = std::max(1LL, std::min({(long long)sms / s->at_once, (long long)kMostRuns, (long long)(n.P / (kStage * rows))}));
     s->run = (n.P + runs - 1) / runs;
     s->runs = (int)((n.P + s->run - 1) / s->run);
     return true;
