@@ -6,6 +6,9 @@
 // over the query chunks of every head that shares the key head, accumulated in tensor memory: no atomics, and the order of the sums is
 // the same in every call.  P and dS are rounded once to 16 bits for their products.
 //
+// Bound by the chain from a chunk's scores to its dS: the tensor pipe works about half of the time (8 heads x 16384 x 128, causal: 1115 us,
+// 990 TFLOP/s over the four products; 4 x 4 heads x 4096 x 128: 298 us; 8 x 16 heads on 4 key heads, 3136 rows on up to 333 keys of 64: 95 us).
+//
 // Persistent, one CTA per SM, one tile of 128 keys (row r of every MMA) at a time, queries in chunks of 128.  All 512 columns of
 // tensor memory are in use, S^T and dP^T having one buffer each; the two halves of a chunk's arithmetic take turns with the MMAs:
 //     softmax   P(n)         | dS(n)        | P(n+1)        | dS(n+1)

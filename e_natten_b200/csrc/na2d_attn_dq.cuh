@@ -7,6 +7,12 @@
 // forward: dQ is then about 1.4 times as far from its 64-bit value as its own rounding puts it.  (The softmax scale comes in the
 // epilogue: in fp16 dS keeps more of its bits without.)
 //
+// Bound as the key half is: 8 heads x 16384 x 128, causal, bf16: 782 us, 1050 TFLOP/s over the three products.
+//
+// Where tiles and CTAs do not go into one another (few rows and many keys, one tile more than a round), the chunks of all tiles lie on one
+// line, of which every CTA takes the same stretch; what it has of a tile that it does not see all keys of goes to a workspace as fp32 sums,
+// which attn_join_rows_kernel adds in their order.
+//
 // Persistent, one CTA per SM, one tile of 128 query rows at a time, keys in chunks of 128.  S has two buffers, so that the
 // exponentials of chunk n + 1 run while dQ and dP of chunks n and n + 1 are on the tensor pipe; dS goes over dP.
 //   warps 0-7   softmax: warps w and w + 4 share 32 rows and take 64 columns each;
@@ -19,7 +25,7 @@
 namespace na2d_attn {
 
 // delta = dO . o of each row, 8 channels a lane.  LPR lanes a row: C / 8, rounded up to a power of two.  A lane has kDeltaRows rows of one
-// head, 256 / LPR apart, all under way at once.
+// head, 256 / LPR apart, all under way at once (8 x 16 heads x 3136 x 64: 16.5 us, 6.2 TB/s; with one row a lane 24).
 constexpr int kDeltaRows = 4;
 template <typename DT, int LPR>
 __global__ void __launch_bounds__(256)
@@ -52,6 +58,66 @@ attn_delta_kernel(const DT* __restrict__ d_o, const Operand st_do, const DT* __r
     }
 }
 
+struct RowCut {
+    int items;              // tiles
+    int line;               // the chunks of all tiles on one line, that many CTAs take; 0: an item is a tile
+    float* part;            // line: (2 a CTA, rows of a tile, C)
+};
+
+// One item: chunks [c0, c0 + n) of a tile of rows.
+struct RowItem {
+    RowTile tile;
+    int c0, n;
+    int part;               // its place in the workspace, -1 where it has all of the tile's chunks
+};
+// The items of a CTA, which every role walks by itself.  (LINE when compiled: the other form's code in every role of a kernel whose items are
+// short costs it 15 %.)
+template <bool LINE>
+struct RowWalk {
+    int item, at, end;
+    __device__ __forceinline__ RowWalk(const Geom& g, const RowCut& cut, const int* before) : item(blockIdx.x), at(0), end(0) {
+        if constexpr (!LINE) return;
+        const int all = before[g.B] * g.Nk * g.tiles, each = (all + cut.line - 1) / cut.line;
+        at = min((int)blockIdx.x * each, all);
+        end = min(at + each, all);
+    }
+    __device__ __forceinline__ bool more(const RowCut& cut) const { return LINE ? at < end : item < cut.items; }
+    __device__ __forceinline__ RowItem get(const Geom& g, const RowCut& cut, const int* before) const {
+        RowItem x;
+        int unit, tile;
+        if constexpr (LINE) {
+            const int per_entry = g.Nk * g.tiles;
+            int lo = 0, hi = g.B;                        // before[lo] per_entry <= at < before[hi] per_entry
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (before[mid] * per_entry <= at) lo = mid;
+                else hi = mid;
+            }
+            const int own = at - before[lo] * per_entry, len = before[lo + 1] - before[lo], which = own / len;
+            x.c0 = own - which * len;
+            x.n = min(len - x.c0, end - at);
+            x.part = x.n == len ? -1 : 2 * (int)blockIdx.x + (x.c0 == 0);
+            unit = lo * g.Nk + g.by_tiles.split(which, tile);
+            x.tile = RowTile(g, unit, tile);
+        } else {
+            if (g.causal) {                              // the longer tiles first
+                tile = g.tiles - 1 - g.by_units.split(item, unit);
+            } else {
+                unit = g.by_tiles.split(item, tile);
+            }
+            x.tile = RowTile(g, unit, tile);
+            x.c0 = 0;
+            x.n = (x.tile.keys(g) + kRows - 1) / kRows;
+            x.part = -1;
+        }
+        return x;
+    }
+    __device__ __forceinline__ void next(const RowItem& x) {
+        if constexpr (LINE) at += x.n;
+        else item += gridDim.x;
+    }
+};
+
 template <int D>
 struct DqCfg : TileCfg<D> {
     using T = TileCfg<D>;
@@ -63,15 +129,16 @@ struct DqCfg : TileCfg<D> {
     static_assert(SMEM <= kSmemLimit, "dQ kernel shared memory");
 };
 
-template <typename DT, int D>
+template <typename DT, int D, bool LINE>
 __global__ void __launch_bounds__(512, 1)
 attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                const __grid_constant__ CUtensorMap tm_dq, DT* __restrict__ dq_rows, const Operand dq_st, const float* __restrict__ lse,
-               const float* __restrict__ delta, const ErrorState* __restrict__ errors, const Geom g, const int items) {
+               const float* __restrict__ delta, const ErrorState* __restrict__ errors, const Geom g, const RowCut cut) {
     using C = DqCfg<D>;
     constexpr int NST = C::NST, NQ = C::NQ;
     extern __shared__ uint8_t smem_raw[];
+    __shared__ int before[LINE ? kLineEntries + 1 : 1];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sQ = smem;
     uint8_t* sG = sQ + NQ * C::BYTES;                     // dO
@@ -125,23 +192,12 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
+    if (LINE && warp == 1) line_table(g, before, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     next_grid_may_start();
     const uint32_t tmem_base = *tmem_slot;
-
-    // my items: with a causal mask the longer tiles first
-    auto tile_of = [&](int item) {
-        int unit, tile;
-        if (g.causal) {
-            tile = g.tiles - 1 - g.by_units.split(item, unit);
-        } else {
-            unit = g.by_tiles.split(item, tile);
-        }
-        return RowTile(g, unit, tile);
-    };
-    auto chunks_of = [&](const RowTile& t) { return (t.keys(g) + kRows - 1) / kRows; };
 
     if (warp == 8) {
         // ------------------------------------------------------------------ producer
@@ -150,9 +206,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             LoadTracker lt(bars);
             Ring ring;
             uint32_t it = 0;
-            for (int item = blockIdx.x; item < items && lt.ok; item += gridDim.x) {
-                const RowTile t = tile_of(item);
-                const int n = chunks_of(t);
+            for (RowWalk<LINE> walk(g, cut, before); walk.more(cut) && lt.ok;) {
+                const RowItem x = walk.get(g, cut, before);
+                const RowTile& t = x.tile;
+                const int n = x.n;
+                walk.next(x);
                 if (n == 0) continue;
                 const uint32_t to = it % NQ, phase = (it / NQ) & 1;
                 if (!lt.acquire(q_empty + to, phase ^ 1, wctx)) break;
@@ -168,8 +226,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                     lt.arm(k_full + ring.at, ring.phase, 2 * C::BYTES);
 #pragma unroll
                     for (int s = 0; s < C::NS; ++s) {
-                        tma_load_5d(sK + ring.at * C::BYTES + s * C::SLAB, &tm_k, k_full + ring.at, s * 64, c * kRows, t.m, t.b, 0);
-                        tma_load_5d(sV + ring.at * C::BYTES + s * C::SLAB, &tm_v, k_full + ring.at, s * 64, c * kRows, t.m, t.b, 0);
+                        tma_load_5d(sK + ring.at * C::BYTES + s * C::SLAB, &tm_k, k_full + ring.at, s * 64, (x.c0 + c) * kRows, t.m, t.b, 0);
+                        tma_load_5d(sV + ring.at * C::BYTES + s * C::SLAB, &tm_v, k_full + ring.at, s * 64, (x.c0 + c) * kRows, t.m, t.b, 0);
                     }
                     ring.next(NST);
                 }
@@ -181,9 +239,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         reg_dec<kDkvRegsCtl>();
         if (g.lengths) {
             Ring ring;
-            for (int item = blockIdx.x; item < items; item += gridDim.x) {
-                const RowTile t = tile_of(item);
-                const int n = chunks_of(t), ragged = fwd_ragged_chunk(g, t.count, 0, n);
+            for (RowWalk<LINE> walk(g, cut, before); walk.more(cut);) {
+                const RowItem x = walk.get(g, cut, before);
+                const RowTile& t = x.tile;
+                const int n = x.n, ragged = fwd_ragged_chunk(g, t.count, x.c0, n);
+                walk.next(x);
                 for (int c = 0; c < n; ++c) {
                     if (c == ragged) {
                         mbar_wait(k_full + ring.at, ring.phase, wctx, kErrLoadWait);
@@ -238,10 +298,18 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             if (last) umma_commit(q_empty + it % NQ);
         };
         bool ahead = false;                  // the tile's first scores have been issued
-        int next = (int)blockIdx.x < items ? chunks_of(tile_of(blockIdx.x)) : 0;
-        for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        RowWalk<LINE> walk(g, cut, before);
+        // chunks of the walk's item (asked for ahead: a length is a load from memory)
+        auto take = [&]() {
+            if (!walk.more(cut)) return -1;
+            const RowItem x = walk.get(g, cut, before);
+            walk.next(x);
+            return x.n;
+        };
+        int next = take();
+        while (next >= 0) {
             const int n = next;
-            next = item + (int)gridDim.x < items ? chunks_of(tile_of(item + gridDim.x)) : 0;      // (ahead: a length is a load from memory)
+            next = take();
             if (n == 0) continue;
             if (!ahead) {
                 mbar_wait(q_full + it % NQ, (it / NQ) & 1, wctx, kErrLoadWait);
@@ -293,9 +361,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         uint8_t* stage = sOut + quarter * 2 * OutStage<32>::BYTES;
         uint32_t it = 0, seq = 0;
-        for (int item = blockIdx.x; item < items; item += gridDim.x) {
-            const RowTile tile = tile_of(item);
-            const bool none = chunks_of(tile) == 0;
+        for (RowWalk<LINE> walk(g, cut, before); walk.more(cut);) {
+            const RowItem x = walk.get(g, cut, before);
+            const RowTile& tile = x.tile;
+            const bool none = x.n == 0;
+            walk.next(x);
             int n, t;
             const bool ok = tile.row(g, row, n, t);
             const int t_first = tile.t0 + quarter * 32;
@@ -319,7 +389,14 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                     for (int e = 0; e < 32; ++e) v[e] = 0u;
                 }
                 if (32 * j >= g.C) continue;
-                if (g.hp == 1) {
+                if (LINE && x.part >= 0) {
+                    float4* dst = reinterpret_cast<float4*>(cut.part + (static_cast<size_t>(x.part) * kRows + row) * g.C + 32 * j);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (ok && 32 * j + 4 * e < g.C)
+                            dst[e] = make_float4(__uint_as_float(v[4 * e]) * g.scale, __uint_as_float(v[4 * e + 1]) * g.scale,
+                                                 __uint_as_float(v[4 * e + 2]) * g.scale, __uint_as_float(v[4 * e + 3]) * g.scale);
+                } else if (g.hp == 1) {
                     if (t_first < g.Tq)
                         na2d_tc::stage_and_store<DT, 32, 2>(&tm_dq, stage, v, g.scale, 32 * j, t_first, tile.h0, tile.b, 0, lane, &seq);
                 } else if (ok) {
@@ -348,24 +425,28 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const uint64_t scale2 = pair2(g.sl2, g.sl2);
         uint32_t m = 0;                                      // chunks so far
         // lse and delta of a row: read an item ahead, since few chunks to an item would not cover the way to memory
-        auto fetch = [&](int item, float& of_lse, float& of_delta) {
-            of_lse = -CUDART_INF_F;
-            of_delta = 0.f;
-            if (item >= items) return;
-            const RowTile tile = tile_of(item);
-            int n, t;
-            if (!tile.row(g, row, n, t)) return;
-            const size_t at = row_index(g, tile.b, n, t);
-            of_lse = __ldg(lse + at);
-            of_delta = __ldg(delta + at);
-        };
+        RowItem next;
         float next_lse, next_delta;
-        fetch(blockIdx.x, next_lse, next_delta);
-        for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        RowWalk<LINE> walk(g, cut, before);
+        auto fetch = [&]() {
+            next.n = -1;
+            next_lse = -CUDART_INF_F;
+            next_delta = 0.f;
+            if (!walk.more(cut)) return;
+            next = walk.get(g, cut, before);
+            walk.next(next);
+            int n, t;
+            if (!next.tile.row(g, row, n, t)) return;
+            const size_t at = row_index(g, next.tile.b, n, t);
+            next_lse = __ldg(lse + at);
+            next_delta = __ldg(delta + at);
+        };
+        fetch();
+        while (next.n >= 0) {
+            const RowTile tile = next.tile;
+            const int chunks = next.n, c0 = next.c0;
             const float row_lse = next_lse, row_delta = next_delta;
-            fetch(item + gridDim.x, next_lse, next_delta);
-            const RowTile tile = tile_of(item);
-            const int chunks = chunks_of(tile);
+            fetch();
             if (chunks == 0) continue;
             int n, t;
             const bool ok = tile.row(g, row, n, t);
@@ -373,7 +454,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             // a row that sees nothing has weights of zero: exp2(-infinity)
             const float neg = row_lse == -CUDART_INF_F ? -CUDART_INF_F : -row_lse * kLog2e;
             const uint64_t neg2 = pair2(neg, neg), delta2 = pair2(-row_delta, -row_delta);
-            const int seen = (ok ? keys_seen(g, tile.count, t) : 0) - 64 * half;
+            const int seen = (ok ? keys_seen(g, tile.count, t) : 0) - 64 * half - c0 * kRows;      // from the item's first chunk on
             for (int c = 0; c < chunks; ++c, ++m) {
                 uint64_t pr[32];
                 if ((tid & 127) == 0) NA2D_TR(half ? 0 : 3, 0, m);
@@ -452,8 +533,51 @@ int launch_delta(const Place& at, const Geom& g, const Operand& d_o, const Opera
                : NA2D_ERR_CUDA;
 }
 
+// Line: a block joins the parts of one tile of rows, or writes zeros where the batch entry has no keys.
+template <typename DT>
+__global__ void __launch_bounds__(256)
+attn_join_rows_kernel(const float* __restrict__ part, DT* __restrict__ dq, const Operand st, const Geom g, const RowCut cut) {
+    after_previous_grid();
+    next_grid_may_start();
+    int which, m, before = 0, all = 0;                   // chunks of a tile of the entries before b, and of all
+    const int unit = g.by_tiles.split(blockIdx.x, which), b = g.by_nk.split(unit, m), lane = threadIdx.x & 31;
+    for (int i = lane; i < g.B; i += 32) {
+        const int chunks = (key_count(g, i) + kRows - 1) / kRows;
+        all += chunks;
+        if (i < b) before += chunks;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, d);
+        before += __shfl_xor_sync(0xffffffffu, before, d);
+    }
+    const RowTile tile(g, unit, which);
+    const int chunks = (tile.count + kRows - 1) / kRows, each = (all * g.Nk * g.tiles + cut.line - 1) / cut.line;
+    const int at = (before * g.Nk + m * chunks) * g.tiles + which * chunks;
+    const int lo = chunks ? at / each : 0, hi = chunks ? (at + chunks - 1) / each : 0;       // CTAs that have some of it
+    if (chunks && lo == hi) return;                      // one had them all
+    const int vectors = g.C / 4;
+    for (int i = threadIdx.x; i < kRows * vectors; i += 256) {
+        const int r = i / vectors, c = 4 * (i - r * vectors);
+        int n, t;
+        if (!tile.row(g, r, n, t)) continue;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (chunks) {
+#pragma unroll 4
+            for (int s = lo; s <= hi; ++s) {             // lo has the tile's first chunk
+                const float4 v = *reinterpret_cast<const float4*>(part + ((2 * s + (s == lo)) * static_cast<size_t>(kRows) + r) * g.C + c);
+                acc.x += v.x;
+                acc.y += v.y;
+                acc.z += v.z;
+                acc.w += v.w;
+            }
+        }
+        *reinterpret_cast<uint2*>(dq + tile.b * st.b + n * st.n + t * st.t + c) = make_uint2(pack2<DT>(acc.x, acc.y), pack2<DT>(acc.z, acc.w));
+    }
+}
+
 template <typename DT, int D>
-int launch_dq(const Place& at, const Geom& g, const Operand& q, const Operand& k, const Operand& v, const Operand& d_o, const float* lse,
+int launch_dq(const Place& at, const Geom& g, RowCut cut, const Operand& q, const Operand& k, const Operand& v, const Operand& d_o, const float* lse,
               const float* delta, const Operand& d_q) {
     using C = DqCfg<D>;
     CUtensorMap tq, tg, tk, tv, tdq;
@@ -465,13 +589,19 @@ int launch_dq(const Place& at, const Geom& g, const Operand& q, const Operand& k
     if (rc != NA2D_OK) return rc;
     const long long items = (long long)g.units * g.tiles;
     if (items > 0x3fffffffLL) return NA2D_ERR_TOO_LARGE;
-    auto kern = attn_dq_kernel<DT, D>;
-    static std::atomic<unsigned long long> opted{0};
-    if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted) != cudaSuccess) return NA2D_ERR_CUDA;
+    cut.items = (int)items;
+    auto kern = cut.line ? attn_dq_kernel<DT, D, true> : attn_dq_kernel<DT, D, false>;
+    static std::atomic<unsigned long long> opted[2]{};
+    if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted[cut.line > 0]) != cudaSuccess) return NA2D_ERR_CUDA;
     const int sms = na2d_tc::sm_count(at.device);
     *at.launched += 1;
-    return na2d_launch::launch(true, kern, items < sms ? (int)items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdq, (DT*)d_q.ptr, d_q, lse,
-                               delta, at.errors, g, (int)items) == cudaSuccess
+    if (na2d_launch::launch(true, kern, cut.line ? cut.line : items < sms ? (int)items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdq, (DT*)d_q.ptr,
+                            d_q, lse, delta, at.errors, g, cut) != cudaSuccess)
+        return NA2D_ERR_CUDA;
+    if (!cut.line) return NA2D_OK;
+    *at.launched += 1;
+    return na2d_launch::launch(true, attn_join_rows_kernel<DT>, (unsigned)items, 256, 0, at.st, (const float*)cut.part, (DT*)d_q.ptr, d_q, g,
+                               cut) == cudaSuccess
                ? NA2D_OK
                : NA2D_ERR_CUDA;
 }

@@ -12,7 +12,7 @@ struct Scratch {
     size_t floats;
 };
 size_t forward_floats(const Geom& g, int sms);
-size_t key_floats(const Geom& g, int sms);
+size_t backward_floats(const Geom& g, int sms, bool d_q, bool d_k);
 
 // 16 bits, C a multiple of 8 up to 128, every operand on 16-byte boundaries; o, d_q, d_k and d_v dense.
 int forward_bf16(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);

@@ -60,6 +60,14 @@ int key_line(const Geom& g, int sms) {
     return pays ? (int)std::max(1LL, std::min<long long>(sms, chunks / 4)) : 0;
 }
 
+// The same for the query half, whose tiles are of rows and whose chunks of keys.
+int row_line(const Geom& g, int sms) {
+    const long long tiles = (long long)g.units * g.tiles, each = (g.Tk + kRows - 1) / kRows, chunks = tiles * each;
+    if (g.causal || g.B > kLineEntries || chunks + sms > 0x7fffffffLL) return 0;
+    const bool pays = (tiles + sms - 1) / sms * each > (chunks + sms - 1) / sms + 4;
+    return pays ? (int)std::max(1LL, std::min<long long>(sms, chunks / 4)) : 0;
+}
+
 // Parts of the queries in the key half of causal calls, where tiles are fewer than CTAs: a part costs its sums' way through memory.
 int key_parts(const Geom& g, int sms) {
     const long long tiles = (long long)g.units * ((g.Tk + kRows - 1) / kRows);
@@ -70,6 +78,7 @@ int key_parts(const Geom& g, int sms) {
 size_t line_rows(const Geom& g, int sms) { return (size_t)(line_groups(g, sms) + g.units) * g.G * g.Tq; }
 size_t all_rows(const Geom& g) { return (size_t)g.B * g.N * g.Tq; }
 size_t key_part(const Geom& g) { return (size_t)g.units * g.Tk * g.C; }
+size_t row_part(const Geom& g, int line) { return (size_t)line * 2 * kRows * g.C; }             // 2 a CTA
 size_t line_part(const Geom& g, int line) { return (size_t)line * 2 * 2 * kRows * g.C; }        // of dK and dV, 2 a CTA
 
 }  // namespace
@@ -108,13 +117,19 @@ int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Scratch& scratc
     return by_head_dim(g.C, [&](auto d) {
         constexpr int D = decltype(d)::value;
         int rc = NA2D_OK;
-        if (x.d_q.ptr) rc = launch_dq<NA2D_TC_TYPE, D>(at, g, x.q, x.k, x.v, x.d_o, x.lse, x.delta, x.d_q);
+        const int sms = na2d_tc::sm_count(at.device), rows = row_line(g, sms);
+        RowCut row_cut{};
+        if (rows && scratch.floats >= row_part(g, rows)) {
+            row_cut.line = rows;
+            row_cut.part = scratch.at;
+        }
+        if (x.d_q.ptr) rc = launch_dq<NA2D_TC_TYPE, D>(at, g, row_cut, x.q, x.k, x.v, x.d_o, x.lse, x.delta, x.d_q);
         if (rc != NA2D_OK || !x.d_k.ptr) return rc;
         Geom gk = g;
         if (g.causal) cut_rows(gk, false);               // a chunk's masks go by the column alone
         KeyCut cut{};
         cut.key_tiles = (g.Tk + kRows - 1) / kRows;
-        const int sms = na2d_tc::sm_count(at.device), line = key_line(g, sms);
+        const int line = key_line(g, sms);
         if (line && scratch.floats >= line_part(g, line)) cut.line = line;
         cut.splits = (int)std::min<size_t>(key_parts(g, sms), std::max<size_t>(1, scratch.floats / (2 * key_part(g))));
         cut.each = (gk.tiles + cut.splits - 1) / cut.splits;
@@ -137,10 +152,12 @@ size_t forward_floats(const Geom& g, int sms) {
     const int parts = forward_parts(g, sms);
     return parts > 1 ? parts * all_rows(g) * (g.C + 1) : 0;
 }
-size_t key_floats(const Geom& g, int sms) {
-    if (const int line = key_line(g, sms)) return line_part(g, line);
+size_t backward_floats(const Geom& g, int sms, bool d_q, bool d_k) {         // the halves' one after the other
+    size_t floats = d_q ? row_part(g, row_line(g, sms)) : 0;
+    if (!d_k) return floats;
+    if (const int line = key_line(g, sms)) return std::max(floats, line_part(g, line));
     const int parts = key_parts(g, sms);
-    return parts > 1 ? 2 * parts * key_part(g) : 0;
+    return std::max(floats, parts > 1 ? 2 * parts * key_part(g) : 0);
 }
 #endif
 

@@ -299,9 +299,9 @@ typedef struct na2d_heads {
  *                CUDA cores (C <= 256, any strides).  SIMT and TENSOR ask for one of them.
  *   o, d_q, d_k, d_v dense.  lse, delta: fp32 (B, N, Tq), dense; delta is scratch of the backward.
  *   d_q, or d_k and d_v together, may be NULL: that half is left out.  No atomics: the same call gives the same bits.
- *   workspace    scratch, 16-byte aligned, of na2d_attention_workspace bytes: few rows over many keys, and few keys under many
- *                queries, are computed in parts that are joined there.  With less (or none) there are fewer parts: slower, and other
- *                last bits. */
+ *   workspace    scratch, 16-byte aligned, of na2d_attention_workspace bytes: where the tiles of rows, or of keys, do not share out evenly
+ *                over the SMs (few of either, entries of different lengths), some are computed in parts that are joined there.  With
+ *                less, or none, there are fewer parts: slower, and other last bits. */
 typedef struct na2d_attention_args {
     size_t struct_size;
     int B, N, Nk, Tq, Tk, C, dtype, path, device, causal;

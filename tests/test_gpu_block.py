@@ -195,6 +195,20 @@ def test_attention_shares_the_queries_out(B, N, Nk, Tq, Tk, lengths, dtype, C):
     check_attention(q, k, v, d_o, C ** -0.5, lengths=None if lengths is None else torch.tensor(lengths, device=DEV))
 
 
+@pytest.mark.parametrize("dtype,C", [(BF16, 64), (F16, 128), (F16, 32)])
+@pytest.mark.parametrize("B,N,Nk,Tq,Tk,lengths", [
+    (10, 5, 5, 384, 1024, None),                                      # 150 tiles of rows: a second round for two of them
+    (3, 4, 2, 100, 3000, [3000, 0, 1537]),                            # few rows, many keys
+    (2, 6, 1, 33, 2500, [0, 0]),
+    (5, 15, 15, 300, 1100, [1100, 130, 0, 1, 1099]),
+])
+def test_attention_shares_the_keys_out(B, N, Nk, Tq, Tk, lengths, dtype, C):
+    """The query half, where its CTAs take equal stretches of all tiles' keys."""
+    q, d_o = rand(B, N, Tq, C, dtype=dtype), rand(B, N, Tq, C, dtype=dtype, seed=3)
+    k, v = rand(B, Nk, Tk, C, dtype=dtype, seed=1), rand(B, Nk, Tk, C, dtype=dtype, seed=2)
+    check_attention(q, k, v, d_o, C ** -0.5, lengths=None if lengths is None else torch.tensor(lengths, device=DEV))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_attention_on_grids_and_views(dtype):
     """(B, heads, H, W, C) views of a packed projection, a gradient with heads last, an image whose rows do not follow one another."""
