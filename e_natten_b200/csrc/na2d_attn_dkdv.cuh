@@ -7,7 +7,8 @@
 // the same in every call.  P and dS are rounded once to 16 bits for their products.
 //
 // Bound by the chain from a chunk's scores to its dS: the tensor pipe works about half of the time (8 heads x 16384 x 128, causal: 1115 us,
-// 990 TFLOP/s over the four products; 4 x 4 heads x 4096 x 128: 298 us; 8 x 16 heads on 4 key heads, 3136 rows on up to 333 keys of 64: 95 us).
+// 990 TFLOP/s over the four products; 4 x 4 heads x 4096 x 128: 256 us; 8 x 16 heads on 4 key heads, 3136 rows on up to 333 keys of 64: 90 us,
+// and 129 with items in place of the line).
 //
 // Persistent, one CTA per SM, one tile of 128 keys (row r of every MMA) at a time, queries in chunks of 128.  All 512 columns of
 // tensor memory are in use, S^T and dP^T having one buffer each; the two halves of a chunk's arithmetic take turns with the MMAs:
@@ -112,21 +113,23 @@ struct KeyItem {
 };
 
 // The items of a CTA, which every role walks by itself.
+template <bool LINE>
 struct KeyWalk {
     int item, at, end;
     __device__ __forceinline__ KeyWalk(const Geom& g, const KeyCut& cut, const int* before) : item(blockIdx.x), at(0), end(0) {
-        if (!cut.line) return;
+        if constexpr (!LINE) return;
         const int all = before[g.B] * g.Nk * g.tiles, each = (all + cut.line - 1) / cut.line;
         at = min((int)blockIdx.x * each, all);
         end = min(at + each, all);
     }
-    __device__ __forceinline__ bool more(const KeyCut& cut) const { return cut.line ? at < end : item < cut.items; }
+    __device__ __forceinline__ bool more(const KeyCut& cut) const { return LINE ? at < end : item < cut.items; }
     __device__ __forceinline__ KeyItem get(const Geom& g, const KeyCut& cut, const int* before) const {
-        return cut.line ? KeyItem(g, before, at, end) : KeyItem(g, cut, item);
+        if constexpr (LINE) return KeyItem(g, before, at, end);
+        else return KeyItem(g, cut, item);
     }
     __device__ __forceinline__ void next(const KeyItem& k) {
-        item += gridDim.x;
-        at += k.n;
+        if constexpr (LINE) at += k.n;
+        else item += gridDim.x;
     }
 };
 
@@ -147,7 +150,7 @@ template <typename DT> struct Weight {
     static constexpr float kShift = IsBf16<DT>::value ? 0.f : 6.f, kUnit = IsBf16<DT>::value ? 1.f : 1.f / 64.f;
 };
 
-template <typename DT, int D>
+template <typename DT, int D, bool LINE>
 __global__ void __launch_bounds__(512, 1)
 attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -156,7 +159,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     using C = KeyCfg<D>;
     constexpr int NST = C::NST, NKV = C::NKV;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int before[kLineEntries + 1];
+    __shared__ int before[LINE ? kLineEntries + 1 : 1];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sK = smem;
     uint8_t* sV = sK + NKV * C::BYTES;
@@ -217,7 +220,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
-    if (warp == 1 && cut.line) line_table(g, before, lane);
+    if (LINE && warp == 1) line_table(g, before, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -229,7 +232,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         reg_dec<kDkvRegsCtl>();
         LoadTracker lt(bars);
         Ring ring;
-        for (KeyWalk walk(g, cut, before); walk.more(cut) && lt.ok;) {
+        for (KeyWalk<LINE> walk(g, cut, before); walk.more(cut) && lt.ok;) {
             const KeyItem k = walk.get(g, cut, before);
             walk.next(k);
             int h0, t0;
@@ -275,7 +278,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (lane == 0) {
             LoadTracker lt(bars);
             uint32_t it = 0;
-            for (KeyWalk walk(g, cut, before); walk.more(cut);) {
+            for (KeyWalk<LINE> walk(g, cut, before); walk.more(cut);) {
                 const KeyItem k = walk.get(g, cut, before);
                 walk.next(k);
                 if (k.n == 0) continue;
@@ -331,7 +334,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             mbar_wait(qd_full + rs.at, rs.phase, wctx, kErrLoadWait);
             mbar_wait(x_full + rs.at, rs.phase, wctx, kErrLoadWait);
         };
-        for (KeyWalk walk(g, cut, before); walk.more(cut);) {
+        for (KeyWalk<LINE> walk(g, cut, before); walk.more(cut);) {
             const KeyItem k = walk.get(g, cut, before);
             walk.next(k);
             if (k.n == 0) continue;
@@ -383,7 +386,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         uint8_t* stage = sOut + quarter * 2 * OutStage<32>::BYTES;
         uint32_t it = 0, seq = 0;
-        for (KeyWalk walk(g, cut, before); walk.more(cut);) {
+        for (KeyWalk<LINE> walk(g, cut, before); walk.more(cut);) {
             const KeyItem k = walk.get(g, cut, before);
             walk.next(k);
             const int first = k.k0 + quarter * 32, key = first + lane;
@@ -409,10 +412,10 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                     for (int e = 0; e < 32; ++e) v[e] = 0u;
                 }
                 if (32 * r >= g.C || first >= g.Tk) continue;
-                if (cut.line ? k.split < 0 : cut.splits == 1) {
+                if (LINE ? k.split < 0 : cut.splits == 1) {
                     na2d_tc::stage_and_store<DT, 32, 2>(which ? &tm_dk : &tm_dv, stage, v, scale, 32 * r, first, k.m, k.b, 0, lane, &seq);
                 } else if (key < g.Tk) {
-                    const size_t at = cut.line ? static_cast<size_t>(k.split) * kRows + quarter * 32 + lane
+                    const size_t at = LINE ? static_cast<size_t>(k.split) * kRows + quarter * 32 + lane
                                                : (static_cast<size_t>(k.split) * g.units + static_cast<size_t>(k.b) * g.Nk + k.m) * g.Tk + key;
                     float4* dst = reinterpret_cast<float4*>((which ? cut.part_dk : cut.part_dv) + at * g.C + 32 * r);
 #pragma unroll
@@ -435,7 +438,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         const uint64_t scale2 = pair2(g.sl2, g.sl2), unit2 = pair2(Weight<DT>::kUnit, Weight<DT>::kUnit);
         uint32_t m = 0;
         Ring ring;
-        for (KeyWalk walk(g, cut, before); walk.more(cut);) {
+        for (KeyWalk<LINE> walk(g, cut, before); walk.more(cut);) {
             const KeyItem k = walk.get(g, cut, before);
             walk.next(k);
             const int key = k.k0 + row;
@@ -601,9 +604,9 @@ int launch_dkdv(const Place& at, const Geom& g, const KeyCut& cut, const Operand
     if (rc == NA2D_OK) rc = operand_map(&tdk, d_k, at.dtype, g.B, g.Nk, g.Tk, g.C, 32, 1, 32);
     if (rc == NA2D_OK) rc = operand_map(&tdv, d_v, at.dtype, g.B, g.Nk, g.Tk, g.C, 32, 1, 32);
     if (rc != NA2D_OK) return rc;
-    auto kern = attn_dkdv_kernel<DT, D>;
-    static std::atomic<unsigned long long> opted{0};
-    if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted) != cudaSuccess) return NA2D_ERR_CUDA;
+    auto kern = cut.line ? attn_dkdv_kernel<DT, D, true> : attn_dkdv_kernel<DT, D, false>;
+    static std::atomic<unsigned long long> opted[2]{};
+    if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted[cut.line > 0]) != cudaSuccess) return NA2D_ERR_CUDA;
     const int sms = na2d_tc::sm_count(at.device);
     *at.launched += 1;
     if (na2d_launch::launch(true, kern, cut.line ? cut.line : cut.items < sms ? cut.items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdk, tdv, lse, delta, at.errors,
