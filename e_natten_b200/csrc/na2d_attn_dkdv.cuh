@@ -4,7 +4,8 @@
 //     P^T = exp(S^T - lse),  dS^T = P^T (dP^T - delta)     (softmax warps)
 //     dV += P^T dO_c,  dK += dS^T Q_c                      (P^T, dS^T from tensor memory, 16 bit)
 // over the query chunks of every head that shares the key head, accumulated in tensor memory: no atomics, and the order of the sums is
-// the same in every call.  P and dS are rounded once to 16 bits for their products.
+// the same in every call.  P is rounded once to 16 bits for its product; dS goes into its own as what it rounds to and the rest, as in the
+// query half.
 //
 // Bound by the chain from a chunk's scores to its dS: the tensor pipe works about half of the time (8 heads x 16384 x 128, causal: 1115 us,
 // 990 TFLOP/s over the four products; 4 x 4 heads x 4096 x 128: 256 us; 8 x 16 heads on 4 key heads, 3136 rows on up to 333 keys of 64: 90 us,
@@ -366,6 +367,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 if (lane == 0) NA2D_TR(2, 4, no);
                 if (elect_one()) {
                     gather(tmem_base + C::TMEM_DK, tmem_base + C::TMEM_DP, qm_lo0 + ro.at * (C::BYTES >> 4), i > 0);
+                    gather(tmem_base + C::TMEM_DK, tmem_base + C::TMEM_DP + 32, qm_lo0 + ro.at * (C::BYTES >> 4), 1);
                     umma_commit(qd_empty + ro.at);
                     if (more) grads(i + 2 == k.n);
                     else umma_commit(acc_full);
@@ -510,6 +512,10 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 for (int e2 = 0; e2 < 32; ++e2) w[e2 / 16][e2 % 16] = pack2<DT>(lo2(pr[e2]), hi2(pr[e2]));
                 tmem_st_32x16(dp_addr, w[0]);
                 tmem_st_32x16(dp_addr + 16, w[1]);
+#pragma unroll
+                for (int e2 = 0; e2 < 32; ++e2) w[e2 / 16][e2 % 16] = pack_rest<DT>(pr[e2], w[e2 / 16][e2 % 16]);
+                tmem_st_32x16(dp_addr + 32, w[0]);           // (dP's other columns, read, too)
+                tmem_st_32x16(dp_addr + 48, w[1]);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();

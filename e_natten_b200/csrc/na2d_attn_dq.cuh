@@ -3,9 +3,10 @@
 //     S = Q K_c^T,  dP = dO V_c^T                          (tensor memory, fp32)
 //     P = exp(S - lse),  dS = P (dP - delta)               (softmax warps)
 //     dQ += dS K_c                                         (dS from tensor memory, 16 bit)
-// with delta = dO . o of the row, formed ahead by delta_kernel.  dS is rounded once to 16 bits for its product, as P is in the
-// forward: dQ is then about 1.4 times as far from its 64-bit value as its own rounding puts it.  (The softmax scale comes in the
-// epilogue: in fp16 dS keeps more of its bits without.)
+// with delta = dO . o of the row, formed ahead by delta_kernel.  dS goes into its product as two numbers of 16 bits, what it rounds to and
+// the rest: rounded to one, it put dQ 1.4 to 1.5 times as far from its 64-bit value as dQ's own rounding does, and together with the rounding of
+// o in delta up to 1.7 times; now that is up to 1.3 times.  (The softmax scale comes in the epilogue: in fp16 dS keeps more of
+// its bits without.)
 //
 // Bound as the key half is: 8 heads x 16384 x 128, causal, bf16: 782 us, 1050 TFLOP/s over the three products.
 //
@@ -337,9 +338,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 if (elect_one()) {
                     const uint32_t km_lo = km_lo0 + ro.at * (C::BYTES >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < kRows / 16; ++kk)      // a warp's half of dS: 32 columns of pairs over its own half of dP
-                        umma_ts(tmem_base + C::TMEM_DQ, tmem_base + C::TMEM_DP + (kk / 4) * 64 + (kk % 4) * 8,
-                                desc64(hi, km_lo + ((kk * 16 * C::ROWB) >> 4)), idesc_o, (c > 0) || (kk > 0));
+                    for (int kk = 0; kk < kRows / 8; ++kk)       // a warp's half of dS: 32 columns of pairs over its own half of dP, then the rests
+                        umma_ts(tmem_base + C::TMEM_DQ, tmem_base + C::TMEM_DP + (kk % 8 / 4) * 64 + kk / 8 * 32 + (kk % 4) * 8,
+                                desc64(hi, km_lo + ((kk % 8 * 16 * C::ROWB) >> 4)), idesc_o, (c > 0) || (kk > 0));
                     umma_commit(k_empty + ro.at);
                     if (c + 1 < n) grads(c + 2 == n);
                     else umma_commit(dq_full);
@@ -499,9 +500,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                     }
 #pragma unroll
                     for (int e2 = 0; e2 < 32; ++e2) w[e2 / 16][e2 % 16] = pack2<DT>(lo2(pr[e2]), hi2(pr[e2]));
-                    // (over columns of dP that this warp has read: the first half of its own)
+                    // (over columns of dP that this warp has read: dS in the first half of its own, its rests in the second)
                     tmem_st_32x16(dp_addr, w[0]);
                     tmem_st_32x16(dp_addr + 16, w[1]);
+#pragma unroll
+                    for (int e2 = 0; e2 < 32; ++e2) w[e2 / 16][e2 % 16] = pack_rest<DT>(pr[e2], w[e2 / 16][e2 % 16]);
+                    tmem_st_32x16(dp_addr + 32, w[0]);
+                    tmem_st_32x16(dp_addr + 48, w[1]);
                     tmem_st_wait();
                 }
                 tc_fence_before();

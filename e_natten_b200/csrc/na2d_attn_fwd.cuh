@@ -209,6 +209,20 @@ struct FwdCfg : TileCfg<D> {
 // and most chunks after the first rescale nothing.
 constexpr float kGrow = 8.f;
 
+// What rounding a pair to `w` left of it, rounded itself: the two together have 16 (22) bits.
+template <typename DT>
+__device__ __forceinline__ uint32_t pack_rest(uint64_t pair, uint32_t w) {
+    uint64_t had;
+    if constexpr (IsBf16<DT>::value) {
+        had = na2d_ptx::pair2(w << 16, w & 0xffff0000u);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        had = na2d_ptx::pair2(f.x, f.y);
+    }
+    const uint64_t rest = na2d_ptx::fma2(had, na2d_ptx::pair2(-1.f, -1.f), pair);
+    return pack2<DT>(na2d_ptx::lo2(rest), na2d_ptx::hi2(rest));
+}
+
 // Columns of P whose product starts ahead of the others (64: 166 us for 156).
 constexpr int kMost = 96;
 

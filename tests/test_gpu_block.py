@@ -11,12 +11,14 @@ Tolerances, from what is rounded (u: the unit roundoff, 2^-8 bf16, 2^-11 fp16):
  * 32-bit results: 2^-24 for each step of sums that are taken over threads and tiles (a few hundred terms one after another at
    most, errors of either sign) and exponentials whose argument of up to 2^5 is off by 2^-24 of itself: 1e-5 for gradients.
 """
+import ctypes
 import math
 
 import pytest
 import torch
 
 import e_natten_b200 as na
+from e_natten_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -207,6 +209,44 @@ def test_attention_shares_the_keys_out(B, N, Nk, Tq, Tk, lengths, dtype, C):
     q, d_o = rand(B, N, Tq, C, dtype=dtype), rand(B, N, Tq, C, dtype=dtype, seed=3)
     k, v = rand(B, Nk, Tk, C, dtype=dtype, seed=1), rand(B, Nk, Tk, C, dtype=dtype, seed=2)
     check_attention(q, k, v, d_o, C ** -0.5, lengths=None if lengths is None else torch.tensor(lengths, device=DEV))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,C", [(BF16, 64), (F16, 128), (F16, 32)])
+@pytest.mark.parametrize("B,N,Nk,Tq,Tk,lengths", [(1, 2, 2, 1500, 1500, None), (2, 4, 2, 1100, 1300, [1300, 700]), (1, 2, 1, 2100, 130, [130])])
+def test_attention_gradients_in_parts_and_whole(B, N, Nk, Tq, Tk, lengths, dtype, C, causal):
+    """With its workspace a backward cuts tiles into parts, without it does not: the same fp32 sums in another order (2e-5 of values of
+    order one), rounded once to the type (a flip of its last bit)."""
+    q, d_o = rand(B, N, Tq, C, dtype=dtype), rand(B, N, Tq, C, dtype=dtype, seed=3)
+    k, v = rand(B, Nk, Tk, C, dtype=dtype, seed=1), rand(B, Nk, Tk, C, dtype=dtype, seed=2)
+    lengths = None if lengths is None else torch.tensor(lengths, device=DEV, dtype=torch.int32)
+    o, lse = na.attention_with_lse(q, k, v, C ** -0.5, causal, lengths)
+    a = _lib.AttentionArgs()
+    a.struct_size = ctypes.sizeof(_lib.AttentionArgs)
+    a.B, a.N, a.Nk, a.Tq, a.Tk, a.C, a.dtype, a.causal, a.scale = B, N, Nk, Tq, Tk, C, 1 if dtype == BF16 else 2, causal, C ** -0.5
+    a.stream = torch.cuda.current_stream(DEV).cuda_stream
+    delta = torch.empty_like(lse)
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("d_o", d_o)):
+        setattr(a, name, _lib.Heads(t.data_ptr(), 0, 0, 0))
+    a.lse, a.delta = lse.data_ptr(), delta.data_ptr()
+    if lengths is not None:
+        a.key_lengths = lengths.data_ptr()
+    results = []
+    for whole in (False, True):
+        out = [torch.full_like(t, float("nan")) for t in (q, k, v)]
+        for name, t in zip(("d_q", "d_k", "d_v"), out):
+            setattr(a, name, _lib.Heads(t.data_ptr(), 0, 0, 0))
+        room = _lib.lib.na2d_attention_workspace(ctypes.byref(a), 1)
+        assert room > 0
+        workspace = torch.empty(room, dtype=torch.uint8, device=DEV)
+        a.workspace, a.workspace_bytes = (None, 0) if whole else (workspace.data_ptr(), room)
+        _lib.check(_lib.lib.na2d_attention_backward(ctypes.byref(a)))
+        na.check_kernels(DEV)
+        results.append(out)
+    for name, got, want in zip("qkv", *results):
+        got, want = got.double(), want.double()
+        assert torch.isfinite(want).all() and torch.isfinite(got).all(), name
+        assert ((got - want).abs() <= 2 * U[dtype] * want.abs() + 2e-5).all(), name
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
