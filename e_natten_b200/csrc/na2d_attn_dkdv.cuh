@@ -7,9 +7,9 @@
 // the same in every call.  P is rounded once to 16 bits for its product; dS goes into its own as what it rounds to and the rest, as in the
 // query half.
 //
-// Bound by the chain from a chunk's scores to its dS: the tensor pipe works about half of the time (8 heads x 16384 x 128, causal: 1115 us,
-// 990 TFLOP/s over the four products; 4 x 4 heads x 4096 x 128: 256 us; 8 x 16 heads on 4 key heads, 3136 rows on up to 333 keys of 64: 90 us,
-// and 129 with items in place of the line).
+// Bound by the chain from a chunk's scores to its dS: the tensor pipe works about half of the time (8 heads x 16384 x 128, causal: 1340 us,
+// 820 TFLOP/s over four products; 4 x 4 heads x 4096 x 128: 284 us; 8 x 16 heads on 4 key heads, 3136 rows on up to 333 keys of 64: 102 us.
+// With dS in one number 1115, 256 and 90 us; with items in place of the line the last one took 129).
 //
 // Persistent, one CTA per SM, one tile of 128 keys (row r of every MMA) at a time, queries in chunks of 128.  All 512 columns of
 // tensor memory are in use, S^T and dP^T having one buffer each; the two halves of a chunk's arithmetic take turns with the MMAs:

@@ -8,11 +8,12 @@
 // o in delta up to 1.7 times; now that is up to 1.3 times.  (The softmax scale comes in the epilogue: in fp16 dS keeps more of
 // its bits without.)
 //
-// Bound as the key half is: 8 heads x 16384 x 128, causal, bf16: 782 us, 1050 TFLOP/s over the three products.
+// Bound as the key half is: 8 heads x 16384 x 128, causal, bf16: 1024 us, 805 TFLOP/s over three products (with dS in one number: 782 us).
 //
 // Where tiles and CTAs do not go into one another (few rows and many keys, one tile more than a round), the chunks of all tiles lie on one
 // line, of which every CTA takes the same stretch; what it has of a tile that it does not see all keys of goes to a workspace as fp32 sums,
-// which attn_join_rows_kernel adds in their order (4 x 4 heads x 4096 x 128, 512 tiles: 178 us for 228).
+// which attn_join_rows_kernel adds in their order (4 x 4 heads x 4096 x 128, 512 tiles, dS
+// in one number: 178 us for 228; in two: 223).
 //
 // Persistent, one CTA per SM, one tile of 128 query rows at a time, keys in chunks of 128.  S has two buffers, so that the
 // exponentials of chunk n + 1 run while dQ and dP of chunks n and n + 1 are on the tensor pipe; dS goes over dP.

@@ -1036,7 +1036,9 @@ __global__ void __launch_bounds__(kThreads) norm_params_kernel(const float2* __r
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 constexpr int kChipBytes = 112 << 10;           // shared memory of a block on the chip: two blocks an SM
-constexpr long long kL2Bytes = 72ll << 20;      // what a set of the two passes reads (4 x 256^2 x 512, step: 12 MB 451 us, 36 MB 415, 72 MB 401; 150 MB: 380, but 3 x 300^2 x 384 172 for 139 us forward, its sets being uneven)
+// What a set of the two passes reads.  4 x 256^2 x 512, forward and backward: 12 MB 451 us, 36 MB 415, 72 MB 385 to 407, 150 MB 380; but there
+// 3 x 300^2 x 384 takes 172 us forward for 139, its sets being uneven.
+constexpr long long kL2Bytes = 72ll << 20;
 
 int power_of_two(int n) {
     int p = 1;
