@@ -556,7 +556,7 @@ attn_sum_kernel(const float* __restrict__ part_dk, const float* __restrict__ par
     *reinterpret_cast<uint2*>((blockIdx.y ? dv : dk) + i) = make_uint2(pack2<DT>(acc.x, acc.y), pack2<DT>(acc.z, acc.w));
 }
 
-// Line: a block joins the parts of one tile of keys, or writes zeros where the tile holds none.
+// Line: a block joins the parts of an eighth of one tile of keys, or writes zeros where the tile holds none.
 template <typename DT>
 __global__ void __launch_bounds__(256)
 attn_join_kernel(const float* __restrict__ part_dk, const float* __restrict__ part_dv, DT* __restrict__ dk, DT* __restrict__ dv,
@@ -579,10 +579,10 @@ attn_join_kernel(const float* __restrict__ part_dk, const float* __restrict__ pa
     const int at = (before * g.Nk + m * tiles + tile) * g.tiles;
     const int lo = tile < tiles ? at / each : 0, hi = tile < tiles ? (at + g.tiles - 1) / each : 0;      // CTAs that have some of it
     if (tile < tiles && lo == hi) return;                // one had them all
-    const int vectors = g.C / 4, rows = min(kRows, g.Tk - tile * kRows);
+    const int vectors = g.C / 4, first = blockIdx.z * kJoinRows, rows = min(first + kJoinRows, min(kRows, g.Tk - tile * kRows));
     const float* part = blockIdx.y ? part_dv : part_dk;
     DT* dst = (blockIdx.y ? dv : dk) + (static_cast<size_t>(unit) * g.Tk + static_cast<size_t>(tile) * kRows) * g.C;
-    for (int i = threadIdx.x; i < rows * vectors; i += 256) {
+    for (int i = first * vectors + threadIdx.x; i < rows * vectors; i += 256) {
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         if (tile < tiles) {
 #pragma unroll 4
@@ -620,7 +620,7 @@ int launch_dkdv(const Place& at, const Geom& g, const KeyCut& cut, const Operand
         return NA2D_ERR_CUDA;
     if (cut.line) {
         *at.launched += 1;
-        return na2d_launch::launch(true, attn_join_kernel<DT>, dim3((unsigned)(g.units * cut.key_tiles), 2), 256, 0, at.st,
+        return na2d_launch::launch(true, attn_join_kernel<DT>, dim3((unsigned)(g.units * cut.key_tiles), 2, kJoinBlocks), 256, 0, at.st,
                                    (const float*)cut.part_dk, (const float*)cut.part_dv, (DT*)d_k.ptr, (DT*)d_v.ptr, g, cut) == cudaSuccess
                    ? NA2D_OK
                    : NA2D_ERR_CUDA;
