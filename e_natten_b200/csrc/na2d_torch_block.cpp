@@ -361,6 +361,23 @@ Tensor group_norm(const Tensor& x, int64_t groups, const MaybeTensor& weight_in,
 }
 
 // ---- rotary positions ----------------------------------------------------------------------------------------------------------
+// What turns x (B, heads, T, C): a table and, or not, the tokens' rows of it.
+void check_turn(const Tensor& x, const Tensor& table, const Tensor& index) {
+    TORCH_CHECK_VALUE(table.dim() == 3 && table.size(2) == 2 && table.scalar_type() == at::kFloat && table.device() == x.device(),
+                      "table must be a float32 tensor of (rows, pairs, 2) on q's device (rotary_table makes one)");
+    TORCH_CHECK_VALUE(table.size(1) > 0 && 2 * table.size(1) <= x.size(3), "table turns ", 2 * table.size(1), " channels of a head dim of ",
+                      x.size(3));
+    if (!index.defined()) {
+        TORCH_CHECK_VALUE(table.size(0) >= x.size(2), "table has ", table.size(0), " rows for ", x.size(2), " tokens");
+        return;
+    }
+    const int64_t rows = x.size(0) * x.size(2);
+    TORCH_CHECK_VALUE((index.scalar_type() == at::kInt || index.scalar_type() == at::kLong) && index.device() == x.device() && index.dim() >= 2 &&
+                          index.size(0) == x.size(0) && index.numel() == rows,
+                      "index must be an int32 or int64 tensor with a table row for each token of each batch entry, on q's device");
+    TORCH_CHECK_VALUE(table.size(0) > 0 || rows == 0, "table has no rows");
+}
+
 // The rows (B, heads, T, C) of q and k turned; either may be undefined.
 std::tuple<Tensor, Tensor> turn(const Tensor& q_in, const Tensor& k_in, const Tensor& table, const Tensor& index, bool interleaved, bool inverse) {
     const Tensor &first_in = q_in.defined() ? q_in : k_in, second_in = q_in.defined() ? k_in : Tensor();
@@ -418,7 +435,12 @@ struct Rotary : ag::Function<Rotary> {
         const Tensor g_q = ctx->needs_input_grad(0) ? grads[0] : Tensor();
         const Tensor g_k = grads.size() > 1 && ctx->needs_input_grad(1) ? grads[1] : Tensor();
         Tensor d_q, d_k;
-        if (g_q.defined() || g_k.defined()) std::tie(d_q, d_k) = turn(g_q, g_k, s[0], s[1], ctx->saved_data["interleaved"].toBool(), true);
+        if (g_q.defined() || g_k.defined()) {
+            // (hooks on saved tensors may hand back other ones than were saved)
+            check_turn(g_q.defined() ? g_q : g_k, s[0], s[1]);
+            const Tensor table = s[0].contiguous(), index = s[1].defined() ? s[1].contiguous() : s[1];
+            std::tie(d_q, d_k) = turn(g_q, g_k, table, index, ctx->saved_data["interleaved"].toBool(), true);
+        }
         return {d_q, d_k, Tensor(), Tensor(), Tensor()};
     }
 };
@@ -432,23 +454,10 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q_in, const MaybeTensor& k_
         TORCH_CHECK_VALUE(k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3),
                           "q and k may differ in their number of heads only; got ", q.sizes(), " and ", k.sizes());
     }
-    TORCH_CHECK_VALUE(table_in.dim() == 3 && table_in.size(2) == 2 && table_in.scalar_type() == at::kFloat && table_in.device() == q.device(),
-                      "table must be a float32 tensor of (rows, pairs, 2) on q's device (rotary_table makes one)");
-    TORCH_CHECK_VALUE(table_in.size(1) > 0 && 2 * table_in.size(1) <= q.size(3), "table turns ", 2 * table_in.size(1), " channels of a head dim of ",
-                      q.size(3));
     TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && table_in.requires_grad()), "rotary has no gradient for its table");
-    const Tensor table = table_in.contiguous();
-    Tensor index;
-    if (index_in) {
-        const int64_t rows = q.size(0) * q.size(2);
-        TORCH_CHECK_VALUE((index_in->scalar_type() == at::kInt || index_in->scalar_type() == at::kLong) && index_in->device() == q.device() &&
-                              index_in->dim() >= 2 && index_in->size(0) == q.size(0) && index_in->numel() == rows,
-                          "index must be an int32 or int64 tensor with a table row for each token of each batch entry, on q's device");
-        TORCH_CHECK_VALUE(table.size(0) > 0 || rows == 0, "table has no rows");
-        index = index_in->contiguous();
-    } else {
-        TORCH_CHECK_VALUE(table.size(0) >= q.size(2), "table has ", table.size(0), " rows for ", q.size(2), " tokens");
-    }
+    const Tensor index_of = index_in.value_or(Tensor());
+    check_turn(q, table_in, index_of);
+    const Tensor table = table_in.contiguous(), index = index_of.defined() ? index_of.contiguous() : index_of;
     Tensor out_q, out_k;
     if (wants_grad({q, k})) {
         const auto out = Rotary::apply(q, maybe(k), table, maybe(index), interleaved);
