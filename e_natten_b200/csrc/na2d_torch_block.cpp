@@ -97,6 +97,7 @@ void check_attention(const Tensor& q, const Tensor& k, const Tensor& v) {
     check_map(q, "q");
     check_like(k, q, "k", "q");
     check_like(v, q, "v", "q");
+    TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4, "q, k and v must be (B, heads, T, C); got ", q.sizes(), " and ", k.sizes());
     TORCH_CHECK_VALUE(k.sizes().equals(v.sizes()), "k and v must have the same shape; got ", k.sizes(), " and ", v.sizes());
     TORCH_CHECK_VALUE(q.size(0) == k.size(0) && q.size(3) == k.size(3), "q and k must have the same batch size and head dim; got ", q.sizes(),
                       " and ", k.sizes());
@@ -151,9 +152,11 @@ std::tuple<Tensor, Tensor> attention_forward(const Tensor& q_in, const Tensor& k
 }
 
 std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& o_in,
-                                                      const Tensor& lse_in, const Tensor& d_o_in, const Tensor& lengths,
+                                                      const Tensor& lse_in, const Tensor& d_o_in, const Tensor& lengths_in,
                                                       const AttentionCall& call, bool need_dq, bool need_dkdv) {
+    // (hooks on saved tensors may hand back other ones than were saved)
     check_attention(q_in, k_in, v_in);
+    const Tensor lengths = lengths_of(lengths_in, q_in, k_in);
     check_like(o_in, q_in, "o", "q");
     check_like(d_o_in, q_in, "the gradient of o", "q");
     TORCH_CHECK_VALUE(o_in.sizes().equals(q_in.sizes()) && d_o_in.sizes().equals(q_in.sizes()), "o and its gradient must have q's shape");

@@ -50,3 +50,10 @@ def test_rotary_without_index_refuses_a_saved_table_of_too_few_rows():
     table = na.rotary_table(torch.arange(4, device=DEV), na.rotary_frequencies(32))
     q = rand(2, 3, 4, 32).requires_grad_()
     refused_in_backward(lambda: na.rotary(q, None, table), (q,), CHANGES["row"], lambda t: True)
+
+
+@pytest.mark.parametrize("change", CHANGES)
+def test_attention_refuses_saved_lengths_of_another_form(change):
+    lengths = torch.tensor([5, 7], device=DEV, dtype=torch.int32)
+    q, k, v = (rand(2, 2, 7, 32, dtype=BF16, seed=i).requires_grad_() for i in range(3))
+    refused_in_backward(lambda: na.attention(q, k, v, key_lengths=lengths), (q, k, v), CHANGES[change], lambda t: not t.is_floating_point())
