@@ -108,8 +108,8 @@ def rotary_table(positions: torch.Tensor, frequencies: torch.Tensor, magnitude: 
     if frequencies.shape[0] != axes:
         raise ValueError(f"frequencies for {frequencies.shape[0]} axes, positions on {axes}")
     pairs = frequencies.shape[1]
-    at = positions.to(torch.float64).contiguous()
-    by = frequencies.to(positions.device, torch.float64).contiguous()
+    at = positions.to(torch.float64).resolve_neg().contiguous()
+    by = frequencies.to(positions.device, torch.float64).resolve_neg().contiguous()
     table = torch.empty((positions.shape[0], axes * pairs, 2), dtype=torch.float32, device=positions.device)
     if table.numel():
         device = positions.device.index

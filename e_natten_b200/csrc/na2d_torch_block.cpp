@@ -43,11 +43,15 @@ void bind_block_abi(uintptr_t attention_forward, uintptr_t attention_backward, u
 int dtype_of(const Tensor& t) {
     return t.scalar_type() == at::kFloat ? NA2D_F32 : t.scalar_type() == at::kBFloat16 ? NA2D_BF16 : NA2D_F16;
 }
+// What t says of itself is in its memory.
+void check_plain(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), name, ": a lazily negated or zero tensor is not supported");
+}
 void check_map(const Tensor& t, const char* name) {
     TORCH_CHECK_VALUE(t.is_cuda() && t.layout() == at::kStrided, name, ": e_natten_b200 runs on CUDA tensors only (there is no CPU path)");
     TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, name, ": dtype ",
                       t.scalar_type(), " not supported (float32, bfloat16, float16)");
-    TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), name, ": a lazily negated or zero tensor is not supported");
+    check_plain(t, name);
 }
 void check_like(const Tensor& t, const Tensor& first, const char* name, const char* first_name) {
     check_map(t, name);
@@ -110,6 +114,7 @@ Tensor lengths_of(const Tensor& lengths, const Tensor& q, const Tensor& k) {
     TORCH_CHECK_VALUE(lengths.dim() == 1 && lengths.size(0) == q.size(0) && lengths.device() == q.device() &&
                           (lengths.scalar_type() == at::kInt || lengths.scalar_type() == at::kLong),
                       "key_lengths must be an int32 or int64 tensor of (B,) on q's device");
+    check_plain(lengths, "key_lengths");
     if (lengths.scalar_type() == at::kLong) return lengths.clamp(0, k.size(2)).to(at::kInt);
     return lengths.contiguous();
 }
@@ -265,6 +270,7 @@ void check_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, const
                               (p->scalar_type() == at::kFloat || p->scalar_type() == x.scalar_type()),
                           "weight and bias must be (C,), on x's device, float32 or of x's dtype");
         TORCH_CHECK_VALUE(!first || p->scalar_type() == first->scalar_type(), "weight and bias must have one dtype");
+        check_plain(*p, "weight and bias");
         first = p;
     }
 }
@@ -368,6 +374,7 @@ Tensor group_norm(const Tensor& x, int64_t groups, const MaybeTensor& weight_in,
 void check_turn(const Tensor& x, const Tensor& table, const Tensor& index) {
     TORCH_CHECK_VALUE(table.dim() == 3 && table.size(2) == 2 && table.scalar_type() == at::kFloat && table.device() == x.device(),
                       "table must be a float32 tensor of (rows, pairs, 2) on q's device (rotary_table makes one)");
+    check_plain(table, "table");
     TORCH_CHECK_VALUE(table.size(1) > 0 && 2 * table.size(1) <= x.size(3), "table turns ", 2 * table.size(1), " channels of a head dim of ",
                       x.size(3));
     if (!index.defined()) {
@@ -378,6 +385,7 @@ void check_turn(const Tensor& x, const Tensor& table, const Tensor& index) {
     TORCH_CHECK_VALUE((index.scalar_type() == at::kInt || index.scalar_type() == at::kLong) && index.device() == x.device() && index.dim() >= 2 &&
                           index.size(0) == x.size(0) && index.numel() == rows,
                       "index must be an int32 or int64 tensor with a table row for each token of each batch entry, on q's device");
+    check_plain(index, "index");
     TORCH_CHECK_VALUE(table.size(0) > 0 || rows == 0, "table has no rows");
 }
 
@@ -439,8 +447,9 @@ struct Rotary : ag::Function<Rotary> {
         const Tensor g_k = grads.size() > 1 && ctx->needs_input_grad(1) ? grads[1] : Tensor();
         Tensor d_q, d_k;
         if (g_q.defined() || g_k.defined()) {
-            // (hooks on saved tensors may hand back other ones than were saved)
-            check_turn(g_q.defined() ? g_q : g_k, s[0], s[1]);
+            if (g_q.defined()) check_map(g_q, "the gradient of q");
+            if (g_k.defined()) check_map(g_k, "the gradient of k");
+            check_turn(g_q.defined() ? g_q : g_k, s[0], s[1]);              // (hooks may hand back other tensors than were saved)
             const Tensor table = s[0].contiguous(), index = s[1].defined() ? s[1].contiguous() : s[1];
             std::tie(d_q, d_k) = turn(g_q, g_k, table, index, ctx->saved_data["interleaved"].toBool(), true);
         }

@@ -57,3 +57,31 @@ def test_attention_refuses_saved_lengths_of_another_form(change):
     lengths = torch.tensor([5, 7], device=DEV, dtype=torch.int32)
     q, k, v = (rand(2, 2, 7, 32, dtype=BF16, seed=i).requires_grad_() for i in range(3))
     refused_in_backward(lambda: na.attention(q, k, v, key_lengths=lengths), (q, k, v), CHANGES[change], lambda t: not t.is_floating_point())
+
+
+def test_a_lazily_negated_gradient_is_refused():
+    """Its memory has the other sign."""
+    x = rand(1, 2, 8, 32).requires_grad_()
+    table = na.rotary_table(torch.arange(8, device=DEV), na.rotary_frequencies(32))
+    for call in (lambda: na.rotary(x, None, table)[0], lambda: na.rotary(x, x, table)[1], lambda: na.attention(x, x, x), lambda: na.group_norm(x, 4)):
+        y = call()
+        with pytest.raises(ValueError, match="lazily negated"):
+            torch.autograd.grad(y, x, torch._neg_view(torch.ones_like(y)))
+
+
+def test_lazily_negated_tables_lengths_and_parameters_are_refused():
+    x, negated = rand(2, 2, 8, 32), torch._neg_view
+    table, index = na.rotary_table(torch.arange(8, device=DEV), na.rotary_frequencies(32)), torch.arange(16, device=DEV).view(2, 8) % 8
+    lengths, w = torch.tensor([3, 5], device=DEV), rand(32)
+    for call in (lambda: na.rotary(x, None, negated(table)), lambda: na.rotary(x, None, table, negated(index)),
+                 lambda: na.attention(x, x, x, key_lengths=negated(lengths)), lambda: na.attention(x, x, x, key_lengths=negated(lengths.int())),
+                 lambda: na.group_norm(x, 4, negated(w)), lambda: na.group_norm(x, 4, None, negated(w)),
+                 lambda: na.rotary(negated(x), None, table), lambda: na.attention(x, negated(x), x), lambda: na.group_norm(negated(x), 4)):
+        with pytest.raises(ValueError, match="lazily negated"):
+            call()
+
+
+def test_a_rotary_table_of_lazily_negated_positions():
+    positions, frequencies = torch.arange(5, device=DEV, dtype=torch.float64), na.rotary_frequencies(8)
+    want = na.rotary_table(-positions, -frequencies)
+    assert torch.equal(na.rotary_table(torch._neg_view(positions), torch._neg_view(frequencies)), want)
