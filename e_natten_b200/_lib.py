@@ -157,7 +157,7 @@ def _load_torch_ext():
                            for fn in (lib.na2d_forward_ex, lib.na2d_backward_ex, lib.na2d_backward_workspace, lib.na2d_poll)))
     _na2d_torch.bind_block_abi(*(C.cast(fn, C.c_void_p).value for fn in (
         lib.na2d_attention_forward, lib.na2d_attention_backward, lib.na2d_attention_workspace, lib.na2d_group_norm_forward,
-        lib.na2d_group_norm_backward, lib.na2d_group_norm_workspace, lib.na2d_rotary, lib.na2d_poll)))
+        lib.na2d_group_norm_backward, lib.na2d_group_norm_workspace, lib.na2d_rotary, lib.na2d_rotary_table, lib.na2d_poll)))
     return _na2d_torch
 
 

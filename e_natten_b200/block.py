@@ -107,15 +107,9 @@ def rotary_table(positions: torch.Tensor, frequencies: torch.Tensor, magnitude: 
         frequencies = frequencies.expand(axes, -1)
     if frequencies.shape[0] != axes:
         raise ValueError(f"frequencies for {frequencies.shape[0]} axes, positions on {axes}")
-    pairs = frequencies.shape[1]
-    at = positions.to(torch.float64).resolve_neg().contiguous()
-    by = frequencies.to(positions.device, torch.float64).resolve_neg().contiguous()
-    table = torch.empty((positions.shape[0], axes * pairs, 2), dtype=torch.float32, device=positions.device)
-    if table.numel():
-        device = positions.device.index
-        _lib.check(_lib.lib.na2d_rotary_table(at.data_ptr(), by.data_ptr(), positions.shape[0], axes, pairs, float(magnitude),
-                                              table.data_ptr(), device, torch_ext.stream(device)))
-    return table
+    at = positions.to(torch.float64).resolve_neg()
+    at = at if at.dim() == 2 else at.unsqueeze(-1)
+    return torch_ext.rotary_table(at, frequencies.to(positions.device, torch.float64).resolve_neg(), float(magnitude))
 
 
 def rotary(q, k, table: torch.Tensor, index: Optional[torch.Tensor] = None,

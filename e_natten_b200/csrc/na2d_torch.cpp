@@ -8,10 +8,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_cpp_function.h>
 #include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/ATen.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cstring>
@@ -253,21 +250,6 @@ struct AttentionNode {
         ag::registerCppFunction(typeid(ag::CppNode<Attention<ONE_D>>), ag::_initFunctionPyTypeObject(type, kName, properties, methods));
     }
 };
-
-// Whether anything looks into the call that the functions of functional.py serve and the native ones do not: a functional
-// transform, forward-mode gradients, a trace, a function or dispatch mode.
-bool looked_into() {
-    const auto tls = c10::impl::tls_local_dispatch_key_set();
-    return tls.included_.has(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) || tls.included_.has(c10::DispatchKey::Functionalize) ||
-           tls.included_.has(c10::DispatchKey::Python) || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
-           at::impl::torch_function_mode_enabled() || torch::jit::tracer::isTracing();
-}
-bool ordinary(const Tensor& t) {
-    return t.is_cuda() && t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.is_neg() && !t.is_conj() &&
-           !t._is_zerotensor() && !t.key_set().has(c10::DispatchKey::FuncTorchBatched) &&
-           !t.key_set().has(c10::DispatchKey::FuncTorchGradWrapper) && !t.key_set().has(c10::DispatchKey::Functionalize) &&
-           !t._fw_grad(0).defined();
-}
 
 // The operator on (q, k, v, kernel_size, scale) as the caller passed them; None where the call is not an ordinary one or an
 // argument is not what the operator takes: functional.py serves it, or says what is wrong.

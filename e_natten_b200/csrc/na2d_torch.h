@@ -1,8 +1,11 @@
-// What the files of the extension module share: layout tests and the exception of a status.
+// What the files of the extension module share: layout tests, the exception of a status, whether a call is an ordinary one.
 #pragma once
 
 #include <torch/csrc/utils/pybind.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/ATen.h>
+#include <ATen/PythonTorchFunctionTLS.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <optional>
 
@@ -39,6 +42,22 @@ inline void check(int status) {
     if (status == NA2D_OK) return;
     pybind11::gil_scoped_acquire gil;
     pybind11::module_::import("e_natten_b200._lib").attr("check")(status);
+}
+
+// Whether anything looks into the calls of this thread: a functional transform, forward-mode gradients, a trace, a function or dispatch
+// mode.
+inline bool looked_into() {
+    const auto tls = c10::impl::tls_local_dispatch_key_set();
+    return tls.included_.has(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) || tls.included_.has(c10::DispatchKey::Functionalize) ||
+           tls.included_.has(c10::DispatchKey::Python) || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+           at::impl::torch_function_mode_enabled() || torch::jit::tracer::isTracing();
+}
+// Whether t is a tensor whose memory is all there is to it.
+inline bool ordinary(const Tensor& t) {
+    return t.is_cuda() && t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.is_neg() && !t.is_conj() &&
+           !t._is_zerotensor() && !t.key_set().has(c10::DispatchKey::FuncTorchBatched) &&
+           !t.key_set().has(c10::DispatchKey::FuncTorchGradWrapper) && !t.key_set().has(c10::DispatchKey::Functionalize) &&
+           !t._fw_grad(0).defined();
 }
 
 // group_norm, rotary and attention (na2d_torch_block.cpp).

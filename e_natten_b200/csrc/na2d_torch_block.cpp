@@ -1,12 +1,20 @@
 // group_norm, rotary and attention on PyTorch tensors: argument checks, layouts, allocation, the calls of the C ABI and the autograd
 // functions.  A call that needs no gradient goes straight to the library.
+//
+// A call that something looks into (a trace, a dispatch mode) goes through PyTorch's dispatcher as an operator of the library e_natten_b200:
+// whoever records calls sees one, with its arguments, and can make it again.  What the functions here do for themselves is not seen; a
+// trace of them would be the allocation of their results and nothing else.  Ordinary calls do without the dispatcher.
 #include <torch/csrc/autograd/custom_function.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/library.h>
 
 #include <cstring>
 #include <limits>
 #include <tuple>
+#include <vector>
 
 #include "na2d_torch.h"
 
@@ -24,11 +32,12 @@ struct Abi {
     int (*norm_backward)(const na2d_norm_args*) = nullptr;
     size_t (*norm_workspace)(const na2d_norm_args*, int) = nullptr;
     int (*rotary)(const na2d_rotary_args*) = nullptr;
+    int (*rotary_table)(const double*, const double*, int64_t, int, int, double, float*, int, void*) = nullptr;
     int (*poll)(int, void*) = nullptr;
 } abi;
 
 void bind_block_abi(uintptr_t attention_forward, uintptr_t attention_backward, uintptr_t attention_workspace, uintptr_t norm_forward,
-                    uintptr_t norm_backward, uintptr_t norm_workspace, uintptr_t rotary, uintptr_t poll) {
+                    uintptr_t norm_backward, uintptr_t norm_workspace, uintptr_t rotary, uintptr_t rotary_table, uintptr_t poll) {
     abi.attention_forward = reinterpret_cast<decltype(abi.attention_forward)>(attention_forward);
     abi.attention_backward = reinterpret_cast<decltype(abi.attention_backward)>(attention_backward);
     abi.attention_workspace = reinterpret_cast<decltype(abi.attention_workspace)>(attention_workspace);
@@ -36,6 +45,7 @@ void bind_block_abi(uintptr_t attention_forward, uintptr_t attention_backward, u
     abi.norm_backward = reinterpret_cast<decltype(abi.norm_backward)>(norm_backward);
     abi.norm_workspace = reinterpret_cast<decltype(abi.norm_workspace)>(norm_workspace);
     abi.rotary = reinterpret_cast<decltype(abi.rotary)>(rotary);
+    abi.rotary_table = reinterpret_cast<decltype(abi.rotary_table)>(rotary_table);
     abi.poll = reinterpret_cast<decltype(abi.poll)>(poll);
 }
 
@@ -77,6 +87,29 @@ bool wants_grad(std::initializer_list<Tensor> tensors) {
 Tensor scratch(size_t bytes, const Tensor& like) {
     return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
+
+// ---- operators of the dispatcher ------------------------------------------------------------------------------------
+// Whether a call on these tensors goes through the dispatcher.
+bool goes_through(std::initializer_list<Tensor> tensors) {
+    if (looked_into()) return true;
+    for (const Tensor& t : tensors)
+        if (t.defined() && !ordinary(t) && !t.is_neg() && !t._is_zerotensor()) return true;      // (those two are refused)
+    return false;
+}
+// The operator of that name, on arguments of F.
+template <typename F>
+c10::TypedOperatorHandle<F> operator_of(const char* name) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+using AttentionForward = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const MaybeTensor&, double, bool, int64_t);
+using AttentionBackward = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const MaybeTensor&,
+                                              double, bool, int64_t, bool, bool);
+using Norm = Tensor(const Tensor&, const MaybeTensor&, const MaybeTensor&, int64_t, double, int64_t);
+using NormForward = std::tuple<Tensor, Tensor>(const Tensor&, const MaybeTensor&, const MaybeTensor&, int64_t, double, int64_t);
+using NormBackward = std::vector<Tensor>(const Tensor&, const MaybeTensor&, const MaybeTensor&, const Tensor&, const Tensor&, int64_t, double, int64_t, bool,
+                                         bool, bool);
+using Turn = std::vector<Tensor>(const Tensor&, const MaybeTensor&, const Tensor&, const MaybeTensor&, bool, bool);
+using Table = Tensor(const Tensor&, const Tensor&, double);
 
 // (B, heads, T, C), of (B, heads, H, W, C) too: a view where the grid's rows follow one another.
 Tensor tokens(const Tensor& t, const char* name) {
@@ -199,11 +232,29 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& q_in, const 
     return {d_q, d_k, d_v};
 }
 
+// The operators' kernels: arguments as whoever calls them has them.
+std::tuple<Tensor, Tensor> attention_forward_op(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, double scale,
+                                                bool causal, int64_t path) {
+    check_attention(q, k, v);
+    return attention_forward(q, k, v, lengths_of(lengths.value_or(Tensor()), q, k), {scale, causal, (int)path});
+}
+std::vector<Tensor> attention_backward_op(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& d_o,
+                                          const MaybeTensor& lengths, double scale, bool causal, int64_t path, bool need_dq, bool need_dkdv) {
+    auto [d_q, d_k, d_v] = attention_backward(q, k, v, o, lse, d_o, lengths.value_or(Tensor()), {scale, causal, (int)path}, need_dq, need_dkdv);
+    return !need_dkdv ? std::vector<Tensor>{d_q} : need_dq ? std::vector<Tensor>{d_q, d_k, d_v} : std::vector<Tensor>{d_k, d_v};
+}
+
 struct Attention : ag::Function<Attention> {
     static ag::variable_list forward(ag::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                                      const MaybeTensor& lengths_in, double scale, bool causal, int64_t path) {
         const Tensor lengths = lengths_in.value_or(Tensor());
-        auto [o, lse] = attention_forward(q, k, v, lengths, {scale, causal, (int)path});
+        Tensor o, lse;
+        if (goes_through({q, k, v, lengths})) {
+            at::AutoDispatchBelowADInplaceOrView below;
+            std::tie(o, lse) = operator_of<AttentionForward>("e_natten_b200::attention").call(q, k, v, lengths_in, scale, causal, path);
+        } else {
+            std::tie(o, lse) = attention_forward(q, k, v, lengths, {scale, causal, (int)path});
+        }
         ctx->save_for_backward({q, k, v, o, lse, lengths});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["causal"] = causal;
@@ -216,14 +267,31 @@ struct Attention : ag::Function<Attention> {
         check_once("attention");
         const auto s = ctx->get_saved_variables();
         const Tensor d_o = grads[0].defined() ? grads[0] : at::zeros(s[0].sizes(), s[0].options());
-        const bool need_dk = ctx->needs_input_grad(1), need_dv = ctx->needs_input_grad(2);
-        auto [d_q, d_k, d_v] = attention_backward(
-            s[0], s[1], s[2], s[3], s[4], d_o, s[5],
-            {ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool(), (int)ctx->saved_data["path"].toInt()},
-            ctx->needs_input_grad(0), need_dk || need_dv);
+        const bool need_dq = ctx->needs_input_grad(0), need_dk = ctx->needs_input_grad(1), need_dv = ctx->needs_input_grad(2);
+        const AttentionCall call{ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool(), (int)ctx->saved_data["path"].toInt()};
+        Tensor d_q, d_k, d_v;
+        if (goes_through({s[0], s[1], s[2], s[3], s[4], d_o, s[5]})) {
+            const auto found = operator_of<AttentionBackward>("e_natten_b200::attention_backward")
+                                   .call(s[0], s[1], s[2], s[3], s[4], d_o, maybe(s[5]), call.scale, call.causal, call.path, need_dq, need_dk || need_dv);
+            if (need_dq) d_q = found.front();
+            if (need_dk || need_dv) std::tie(d_k, d_v) = std::make_tuple(found[found.size() - 2], found.back());
+        } else {
+            std::tie(d_q, d_k, d_v) = attention_backward(s[0], s[1], s[2], s[3], s[4], d_o, s[5], call, need_dq, need_dk || need_dv);
+        }
         return {d_q, need_dk ? d_k : Tensor(), need_dv ? d_v : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
+
+std::tuple<Tensor, Tensor> attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& lengths, double scale, bool causal,
+                                              int64_t path) {
+    if (wants_grad({q, k, v})) {
+        check_attention(q, k, v);
+        const auto out = Attention::apply(q, k, v, maybe(lengths_of(lengths.value_or(Tensor()), q, k)), scale, causal, path);
+        return {out[0], out[1]};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    return operator_of<AttentionForward>("e_natten_b200::attention").call(q, k, v, lengths, scale, causal, path);
+}
 
 std::tuple<Tensor, Tensor> attention(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, double scale, bool causal,
                                      const MaybeTensor& lengths_in, int64_t path) {
@@ -232,7 +300,9 @@ std::tuple<Tensor, Tensor> attention(const Tensor& q_in, const Tensor& k_in, con
     check_attention(q, k, v);
     const Tensor lengths = lengths_of(lengths_in.value_or(Tensor()), q, k);
     Tensor o, lse;
-    if (wants_grad({q, k, v})) {
+    if (goes_through({q, k, v, lengths})) {
+        std::tie(o, lse) = operator_of<AttentionForward>("e_natten_b200::attention").call(q, k, v, maybe(lengths), scale, causal, path);
+    } else if (wants_grad({q, k, v})) {
         const auto out = Attention::apply(q, k, v, maybe(lengths), scale, causal, path);
         o = out[0];
         lse = out[1];
@@ -314,11 +384,71 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor& x_in, const Tensor& weight
     return {y, stats};
 }
 
+// d_x, d_weight, d_bias, those that are wanted.
+std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& x_in, const Tensor& weight_in, const Tensor& bias_in, const Tensor& stats,
+                                                 const Tensor& d_y_in, const NormCall& call, bool need_x, bool need_w, bool need_b) {
+    const Tensor weight = dense_param(weight_in), bias = dense_param(bias_in);
+    check_norm(x_in, weight, bias, call);
+    check_like(d_y_in, x_in, "the gradient of y", "x");
+    TORCH_CHECK_VALUE(d_y_in.sizes().equals(x_in.sizes()), "the gradient of y must have x's shape");
+    TORCH_CHECK_VALUE(stats.is_contiguous() && stats.scalar_type() == at::kFloat && stats.device() == x_in.device() &&
+                          stats.numel() == 2 * x_in.size(0) * call.groups,
+                      "the saved statistics must be what the forward saved");
+    Tensor d_x, d_w, d_b;
+    need_w = need_w && weight.defined();
+    need_b = need_b && bias.defined();
+    if (need_x) d_x = at::empty(x_in.sizes(), x_in.options());
+    if (x_in.numel() == 0) {
+        if (need_w) d_w = at::zeros_like(weight);
+        if (need_b) d_b = at::zeros_like(bias);
+        return {d_x, d_w, d_b};
+    }
+    if (need_w) d_w = at::empty(weight.sizes(), weight.options());
+    if (need_b) d_b = at::empty(bias.sizes(), bias.options());
+    const Tensor x = pixels(x_in), d_y = pixels(d_y_in);
+    na2d_norm_args a = norm_args(x, weight, bias, stats, call);
+    a.d_y = pixels_of(d_y);
+    a.d_x = d_x.defined() ? d_x.data_ptr() : nullptr;
+    a.d_weight = need_w ? d_w.data_ptr() : nullptr;
+    a.d_bias = need_b ? d_b.data_ptr() : nullptr;
+    const Tensor workspace = scratch(abi.norm_workspace(&a, 1), x);
+    a.workspace = workspace.data_ptr();
+    a.workspace_bytes = workspace.numel();
+    check(abi.norm_backward(&a));
+    return {d_x, d_w, d_b};
+}
+
+// The operators' kernels.
+std::tuple<Tensor, Tensor> norm_forward_op(const Tensor& x, const MaybeTensor& weight_in, const MaybeTensor& bias_in, int64_t groups, double eps,
+                                           int64_t activation) {
+    const Tensor weight = weight_in.value_or(Tensor()), bias = bias_in.value_or(Tensor());
+    check_norm(x, weight, bias, {groups, eps, activation});
+    return norm_forward(x, weight, bias, {groups, eps, activation});
+}
+Tensor norm_op(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, int64_t groups, double eps, int64_t activation) {
+    return std::get<0>(norm_forward_op(x, weight, bias, groups, eps, activation));
+}
+std::vector<Tensor> norm_backward_op(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, const Tensor& stats, const Tensor& d_y,
+                                     int64_t groups, double eps, int64_t activation, bool need_x, bool need_w, bool need_b) {
+    const auto [d_x, d_w, d_b] = norm_backward(x, weight.value_or(Tensor()), bias.value_or(Tensor()), stats, d_y, {groups, eps, activation}, need_x,
+                                               need_w, need_b);
+    std::vector<Tensor> found;
+    for (const Tensor& t : {d_x, d_w, d_b})
+        if (t.defined()) found.push_back(t);
+    return found;
+}
+
 struct GroupNorm : ag::Function<GroupNorm> {
     static Tensor forward(ag::AutogradContext* ctx, const Tensor& x, const MaybeTensor& weight_in, const MaybeTensor& bias_in, int64_t groups,
                           double eps, int64_t activation) {
         const Tensor weight = weight_in.value_or(Tensor()), bias = bias_in.value_or(Tensor());
-        auto [y, stats] = norm_forward(x, weight, bias, {groups, eps, activation});
+        Tensor y, stats;
+        if (goes_through({x, weight, bias})) {
+            at::AutoDispatchBelowADInplaceOrView below;
+            std::tie(y, stats) = operator_of<NormForward>("e_natten_b200::group_norm_forward").call(x, weight_in, bias_in, groups, eps, activation);
+        } else {
+            std::tie(y, stats) = norm_forward(x, weight, bias, {groups, eps, activation});
+        }
         ctx->save_for_backward({x, weight, bias, stats});
         ctx->saved_data["groups"] = groups;
         ctx->saved_data["eps"] = eps;
@@ -328,43 +458,39 @@ struct GroupNorm : ag::Function<GroupNorm> {
     static ag::variable_list backward(ag::AutogradContext* ctx, const ag::variable_list& grads) {
         check_once("group_norm");
         const auto s = ctx->get_saved_variables();
-        const Tensor &x_in = s[0], weight = dense_param(s[1]), bias = dense_param(s[2]), &stats = s[3];
         const NormCall call{ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["activation"].toInt()};
-        check_norm(x_in, weight, bias, call);
-        const Tensor& d_y_in = grads[0];
-        check_like(d_y_in, x_in, "the gradient of y", "x");
-        TORCH_CHECK_VALUE(d_y_in.sizes().equals(x_in.sizes()), "the gradient of y must have x's shape");
-        TORCH_CHECK_VALUE(stats.is_contiguous() && stats.scalar_type() == at::kFloat && stats.device() == x_in.device() &&
-                              stats.numel() == 2 * x_in.size(0) * call.groups,
-                          "the saved statistics must be what the forward saved");
+        const bool need_x = ctx->needs_input_grad(0), need_w = s[1].defined() && ctx->needs_input_grad(1),
+                   need_b = s[2].defined() && ctx->needs_input_grad(s[1].defined() ? 2 : 1);
         Tensor d_x, d_w, d_b;
-        const bool need_w = weight.defined() && ctx->needs_input_grad(1), need_b = bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1);
-        if (ctx->needs_input_grad(0)) d_x = at::empty(x_in.sizes(), x_in.options());
-        if (x_in.numel() == 0) {
-            if (need_w) d_w = at::zeros_like(weight);
-            if (need_b) d_b = at::zeros_like(bias);
-            return {d_x, d_w, d_b, Tensor(), Tensor(), Tensor()};
+        if (goes_through({s[0], s[1], s[2], s[3], grads[0]})) {
+            const auto found = operator_of<NormBackward>("e_natten_b200::group_norm_backward")
+                                   .call(s[0], maybe(s[1]), maybe(s[2]), s[3], grads[0], call.groups, call.eps, call.activation, need_x, need_w, need_b);
+            auto next = found.begin();
+            if (need_x) d_x = *next++;
+            if (need_w) d_w = *next++;
+            if (need_b) d_b = *next++;
+        } else {
+            std::tie(d_x, d_w, d_b) = norm_backward(s[0], s[1], s[2], s[3], grads[0], call, need_x, need_w, need_b);
         }
-        if (need_w) d_w = at::empty(weight.sizes(), weight.options());
-        if (need_b) d_b = at::empty(bias.sizes(), bias.options());
-        const Tensor x = pixels(x_in), d_y = pixels(d_y_in);
-        na2d_norm_args a = norm_args(x, weight, bias, stats, call);
-        a.d_y = pixels_of(d_y);
-        a.d_x = d_x.defined() ? d_x.data_ptr() : nullptr;
-        a.d_weight = need_w ? d_w.data_ptr() : nullptr;
-        a.d_bias = need_b ? d_b.data_ptr() : nullptr;
-        const Tensor workspace = scratch(abi.norm_workspace(&a, 1), x);
-        a.workspace = workspace.data_ptr();
-        a.workspace_bytes = workspace.numel();
-        check(abi.norm_backward(&a));
         return {d_x, d_w, d_b, Tensor(), Tensor(), Tensor()};
     }
 };
+
+Tensor norm_autograd(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, int64_t groups, double eps, int64_t activation) {
+    if (wants_grad({x, weight.value_or(Tensor()), bias.value_or(Tensor())})) {
+        check_norm(x, weight.value_or(Tensor()), bias.value_or(Tensor()), {groups, eps, activation});
+        return GroupNorm::apply(x, weight, bias, groups, eps, activation);
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    return operator_of<Norm>("e_natten_b200::group_norm").call(x, weight, bias, groups, eps, activation);
+}
 
 Tensor group_norm(const Tensor& x, int64_t groups, const MaybeTensor& weight_in, const MaybeTensor& bias_in, double eps, int64_t activation) {
     const Tensor weight = weight_in.value_or(Tensor()), bias = bias_in.value_or(Tensor());
     const NormCall call{groups, eps, activation};
     check_norm(x, weight, bias, call);
+    if (goes_through({x, weight, bias}))
+        return operator_of<Norm>("e_natten_b200::group_norm").call(x, maybe(weight), maybe(bias), groups, eps, activation);
     if (wants_grad({x, weight, bias})) return GroupNorm::apply(x, maybe(weight), maybe(bias), groups, eps, activation);
     return std::get<0>(norm_forward(x, weight, bias, call));
 }
@@ -429,13 +555,41 @@ std::tuple<Tensor, Tensor> turn(const Tensor& q_in, const Tensor& k_in, const Te
     return q_in.defined() ? std::make_tuple(out_first, out_second) : std::make_tuple(Tensor(), out_first);
 }
 
+// q and k of one call, or their gradients.
+void check_turned(const Tensor& q, const Tensor& k) {
+    check_map(q, "q");
+    TORCH_CHECK_VALUE(q.dim() == 4, "q must be (B, heads, T, C); got ", q.sizes());
+    if (!k.defined()) return;
+    check_like(k, q, "k", "q");
+    TORCH_CHECK_VALUE(k.dim() == 4 && k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3),
+                      "q and k may differ in their number of heads only; got ", q.sizes(), " and ", k.sizes());
+}
+// The operator's kernel.
+std::vector<Tensor> turn_op(const Tensor& q, const MaybeTensor& k_in, const Tensor& table, const MaybeTensor& index_in, bool interleaved, bool inverse) {
+    const Tensor k = k_in.value_or(Tensor()), index = index_in.value_or(Tensor());
+    check_turned(q, k);
+    check_turn(q, table, index);
+    const auto [out_q, out_k] = turn(q, k, table.contiguous(), index.defined() ? index.contiguous() : index, interleaved, inverse);
+    return k.defined() ? std::vector<Tensor>{out_q, out_k} : std::vector<Tensor>{out_q};
+}
+// The same for whoever may look into the call; either of q and k may be undefined.
+std::tuple<Tensor, Tensor> turn_through(const Tensor& q, const Tensor& k, const Tensor& table, const Tensor& index, bool interleaved, bool inverse) {
+    if (!goes_through({q, k, table, index})) return turn(q, k, table, index, interleaved, inverse);
+    const bool two = q.defined() && k.defined();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto out = operator_of<Turn>("e_natten_b200::rotary")
+                         .call(q.defined() ? q : k, two ? MaybeTensor(k) : MaybeTensor(), table, maybe(index), interleaved, inverse);
+    return two ? std::make_tuple(out[0], out[1]) : q.defined() ? std::make_tuple(out[0], Tensor()) : std::make_tuple(Tensor(), out[0]);
+}
+
 struct Rotary : ag::Function<Rotary> {
     static ag::variable_list forward(ag::AutogradContext* ctx, const Tensor& q, const MaybeTensor& k_in, const Tensor& table,
-                                     const MaybeTensor& index_in, bool interleaved) {
+                                     const MaybeTensor& index_in, bool interleaved, bool inverse) {
         const Tensor k = k_in.value_or(Tensor()), index = index_in.value_or(Tensor());
-        auto [out_q, out_k] = turn(q, k, table, index, interleaved, false);
+        auto [out_q, out_k] = turn_through(q, k, table, index, interleaved, inverse);
         ctx->save_for_backward({table, index});
         ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["inverse"] = inverse;
         ctx->set_materialize_grads(false);
         if (!k.defined()) return {out_q};
         return {out_q, out_k};
@@ -451,28 +605,38 @@ struct Rotary : ag::Function<Rotary> {
             if (g_k.defined()) check_map(g_k, "the gradient of k");
             check_turn(g_q.defined() ? g_q : g_k, s[0], s[1]);              // (hooks may hand back other tensors than were saved)
             const Tensor table = s[0].contiguous(), index = s[1].defined() ? s[1].contiguous() : s[1];
-            std::tie(d_q, d_k) = turn(g_q, g_k, table, index, ctx->saved_data["interleaved"].toBool(), true);
+            std::tie(d_q, d_k) = turn_through(g_q, g_k, table, index, ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool());
         }
-        return {d_q, d_k, Tensor(), Tensor(), Tensor()};
+        return {d_q, d_k, Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
+
+std::vector<Tensor> turn_autograd(const Tensor& q, const MaybeTensor& k, const Tensor& table, const MaybeTensor& index, bool interleaved, bool inverse) {
+    if (wants_grad({q, k.value_or(Tensor())})) {
+        check_turned(q, k.value_or(Tensor()));
+        check_turn(q, table, index.value_or(Tensor()));
+        return Rotary::apply(q, k, table.contiguous(), index ? MaybeTensor(index->contiguous()) : index, interleaved, inverse);
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    return operator_of<Turn>("e_natten_b200::rotary").call(q, k, table, index, interleaved, inverse);
+}
 
 std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q_in, const MaybeTensor& k_in, const Tensor& table_in, const MaybeTensor& index_in,
                                        bool interleaved) {
     check_map(q_in, "q");
     const Tensor q = tokens(q_in, "q"), k = k_in ? tokens(*k_in, "k") : Tensor();
-    if (k.defined()) {
-        check_like(k, q, "k", "q");
-        TORCH_CHECK_VALUE(k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3),
-                          "q and k may differ in their number of heads only; got ", q.sizes(), " and ", k.sizes());
-    }
+    check_turned(q, k);
     TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && table_in.requires_grad()), "rotary has no gradient for its table");
     const Tensor index_of = index_in.value_or(Tensor());
     check_turn(q, table_in, index_of);
     const Tensor table = table_in.contiguous(), index = index_of.defined() ? index_of.contiguous() : index_of;
     Tensor out_q, out_k;
-    if (wants_grad({q, k})) {
-        const auto out = Rotary::apply(q, maybe(k), table, maybe(index), interleaved);
+    if (goes_through({q, k, table, index})) {
+        const auto out = operator_of<Turn>("e_natten_b200::rotary").call(q, maybe(k), table, maybe(index), interleaved, false);
+        out_q = out[0];
+        if (k.defined()) out_k = out[1];
+    } else if (wants_grad({q, k})) {
+        const auto out = Rotary::apply(q, maybe(k), table, maybe(index), interleaved, false);
         out_q = out[0];
         if (k.defined()) out_k = out[1];
     } else {
@@ -480,6 +644,56 @@ std::tuple<Tensor, MaybeTensor> rotary(const Tensor& q_in, const MaybeTensor& k_
     }
     auto shaped = [](const Tensor& t, const Tensor& like) { return like.dim() == 5 ? t.unflatten(2, {like.size(2), like.size(3)}) : t; };
     return {shaped(out_q, q_in), k_in ? MaybeTensor(shaped(out_k, *k_in)) : MaybeTensor()};
+}
+
+// positions (P, axes), frequencies (axes, pairs), float64 -> (P, axes * pairs, 2)
+Tensor table_op(const Tensor& positions_in, const Tensor& frequencies_in, double magnitude) {
+    const Tensor positions = positions_in.contiguous(), frequencies = frequencies_in.contiguous();
+    for (const Tensor* t : {&positions, &frequencies}) check_plain(*t, "positions and frequencies");
+    TORCH_CHECK_VALUE(positions.is_cuda() && frequencies.device() == positions.device() && positions.scalar_type() == at::kDouble &&
+                          frequencies.scalar_type() == at::kDouble && positions.dim() == 2 && frequencies.dim() == 2 &&
+                          positions.size(1) == frequencies.size(0),
+                      "positions must be (P, axes), frequencies (axes, pairs), both float64 on one CUDA device");
+    Tensor table = at::empty({positions.size(0), frequencies.numel(), 2}, positions.options().dtype(at::kFloat));
+    if (table.numel() != 0)
+        check(abi.rotary_table(positions.data_ptr<double>(), frequencies.data_ptr<double>(), positions.size(0), extent(positions.size(1), "axes"),
+                               extent(frequencies.size(1), "pairs"), magnitude, table.data_ptr<float>(), positions.device().index(),
+                               stream_of(positions)));
+    return table;
+}
+Tensor rotary_table(const Tensor& positions, const Tensor& frequencies, double magnitude) {
+    if (goes_through({positions, frequencies})) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return operator_of<Table>("e_natten_b200::rotary_table").call(positions, frequencies, magnitude);
+    }
+    return table_op(positions, frequencies, magnitude);
+}
+
+// The operators.  `*_forward` and `*_backward` are what the others are made of, for whoever looks in below autograd; they have no gradient.
+TORCH_LIBRARY(e_natten_b200, m) {
+    m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? key_lengths, float scale, bool causal, int path) -> (Tensor, Tensor)");
+    m.def("attention_backward(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor d_o, Tensor? key_lengths, float scale, bool causal, "
+          "int path, bool need_dq, bool need_dkdv) -> Tensor[]");
+    m.def("group_norm(Tensor x, Tensor? weight, Tensor? bias, int groups, float eps, int activation) -> Tensor");
+    m.def("group_norm_forward(Tensor x, Tensor? weight, Tensor? bias, int groups, float eps, int activation) -> (Tensor, Tensor)");
+    m.def("group_norm_backward(Tensor x, Tensor? weight, Tensor? bias, Tensor stats, Tensor d_y, int groups, float eps, int activation, "
+          "bool need_dx, bool need_dweight, bool need_dbias) -> Tensor[]");
+    m.def("rotary(Tensor q, Tensor? k, Tensor table, Tensor? index, bool interleaved, bool inverse) -> Tensor[]");
+    m.def("rotary_table(Tensor positions, Tensor frequencies, float magnitude) -> Tensor");
+}
+TORCH_LIBRARY_IMPL(e_natten_b200, CUDA, m) {
+    m.impl("attention", &attention_forward_op);
+    m.impl("attention_backward", &attention_backward_op);
+    m.impl("group_norm", &norm_op);
+    m.impl("group_norm_forward", &norm_forward_op);
+    m.impl("group_norm_backward", &norm_backward_op);
+    m.impl("rotary", &turn_op);
+    m.impl("rotary_table", &table_op);
+}
+TORCH_LIBRARY_IMPL(e_natten_b200, Autograd, m) {
+    m.impl("attention", &attention_autograd);
+    m.impl("group_norm", &norm_autograd);
+    m.impl("rotary", &turn_autograd);
 }
 
 }  // namespace
@@ -490,6 +704,7 @@ void add_block_operators(pybind11::module_& m) {
     m.def("attention", &attention, release());
     m.def("group_norm", &group_norm, release());
     m.def("rotary", &rotary, release());
+    m.def("rotary_table", &rotary_table, release());
 }
 
 }  // namespace na2d_torch
