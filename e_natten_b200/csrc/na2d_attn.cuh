@@ -131,6 +131,25 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int first, int lane) {
 
 #endif
 
+// fp16: what bounds |dO . V|, from which the backward takes the power of two that its dS go into their products with (ds_shift).
+struct Bounds {
+    float* unit;            // (units, 2): the largest squared norms of the dO rows that see keys and of V's rows
+    float* row;             // (B, N, Tq): the squared norm of a dO row
+};
+
+#ifdef __CUDACC__
+// s so that |dS| 2^s stays below 2^15, given the squared norms of dO and V: |dP| and |delta| are at most the norms' product.  dS and
+// the rest that rounding leaves of it are then within fp16's 2^-24 of a largest value near its end, whatever the size of gradients
+// (unshifted, weights of 2^-14 times gradients of 1e-2 were half lost, and dS beyond 65504 infinite).
+__device__ __forceinline__ int ds_shift(float d_o_square, float v_square) {
+    const float square = d_o_square * v_square;              // 2^-96 to 2^78 for numbers of fp16
+    if (!(square > 0.f) || square == CUDART_INF_F) return 0;
+    const int e = (__float_as_int(square) >> 23) - 127;      // square < 2^(e + 1)
+    return 14 - ((e + 2) >> 1);
+}
+__device__ __forceinline__ float exp2i(int s) { return __int_as_float((s + 127) << 23); }      // |s| < 127
+#endif
+
 // What a launcher gets: geometry, element type, place, error state, launch counter.
 struct Place {
     int dtype, device;

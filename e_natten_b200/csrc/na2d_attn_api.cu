@@ -130,7 +130,9 @@ size_t na2d_attention_workspace(const na2d_attention_args* a, int backward) {
     Problem p;
     if (make_problem(a, &p) != NA2D_OK || !p.tensor) return 0;
     const int sms = na2d_tc::sm_count(a->device);
-    return (backward ? na2d_attn::backward_floats(p.g, sms, a->d_q.ptr != nullptr, a->d_k.ptr != nullptr) : na2d_attn::forward_floats(p.g, sms)) * sizeof(float);
+    return (backward ? na2d_attn::backward_floats(p.g, sms, a->dtype == NA2D_F16, a->d_q.ptr != nullptr, a->d_k.ptr != nullptr)
+                     : na2d_attn::forward_floats(p.g, sms)) *
+           sizeof(float);
 }
 
 }  // extern "C"

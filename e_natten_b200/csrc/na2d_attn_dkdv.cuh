@@ -5,7 +5,7 @@
 //     dV += P^T dO_c,  dK += dS^T Q_c                      (P^T, dS^T from tensor memory, 16 bit)
 // over the query chunks of every head that shares the key head, accumulated in tensor memory: no atomics, and the order of the sums is
 // the same in every call.  P is rounded once to 16 bits for its product; dS goes into its own as what it rounds to and the rest, as in the
-// query half.
+// query half, in fp16 times a power of two (ds_shift, one for all rows of a unit, since they are summed).
 //
 // Bound by the chain from a chunk's scores to its dS: the tensor pipe works about half of the time (8 heads x 16384 x 128, causal: 1340 us,
 // 820 TFLOP/s over four products; 4 x 4 heads x 4096 x 128: 284 us; 8 x 16 heads on 4 key heads, 3136 rows on up to 333 keys of 64: 102 us.
@@ -148,15 +148,23 @@ struct KeyCfg : TileCfg<D> {
 
 // P for its product, times 2^kShift: in fp16 the weights of long sequences would fall among the subnormal numbers.
 template <typename DT> struct Weight {
-    static constexpr float kShift = IsBf16<DT>::value ? 0.f : 6.f, kUnit = IsBf16<DT>::value ? 1.f : 1.f / 64.f;
+    static constexpr int kBits = IsBf16<DT>::value ? 0 : 6;
+    static constexpr float kShift = kBits, kUnit = IsBf16<DT>::value ? 1.f : 1.f / 64.f;
 };
+// The power of two that dS of a unit goes into its product with.
+template <typename DT>
+__device__ __forceinline__ int unit_shift(const Geom& g, const Bounds& bounds, const KeyItem& k) {
+    if constexpr (IsBf16<DT>::value) return 0;
+    const float2 squares = __ldg(reinterpret_cast<const float2*>(bounds.unit) + k.b * g.Nk + k.m);
+    return ds_shift(squares.x, squares.y);
+}
 
 template <typename DT, int D, bool LINE>
 __global__ void __launch_bounds__(512, 1)
 attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                  const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv, const float* __restrict__ lse,
-                 const float* __restrict__ delta, const ErrorState* __restrict__ errors, const Geom g, const KeyCut cut) {
+                 const float* __restrict__ delta, const Bounds bounds, const ErrorState* __restrict__ errors, const Geom g, const KeyCut cut) {
     using C = KeyCfg<D>;
     constexpr int NST = C::NST, NKV = C::NKV;
     extern __shared__ uint8_t smem_raw[];
@@ -238,6 +246,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             walk.next(k);
             int h0, t0;
             k.start(g, h0, t0);
+            const float unit = exp2i(unit_shift<DT>(g, bounds, k) - Weight<DT>::kBits);      // dS over P as it is here, and dP
             for (int i = 0; i < k.n; ++i, k.step(g, h0, t0)) {
                 float x_lse[4], x_delta[4];
 #pragma unroll
@@ -265,7 +274,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 for (int u = 0; u < 4; ++u) {
                     // rows that see nothing, or are none: weights of exp2(-infinity)
                     x[lane + 32 * u] = x_lse[u] == -CUDART_INF_F ? -CUDART_INF_F : Weight<DT>::kShift - x_lse[u] * kLog2e;
-                    x[kRows + lane + 32 * u] = -x_delta[u] * Weight<DT>::kUnit;
+                    x[kRows + lane + 32 * u] = -x_delta[u] * unit;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(x_full + ring.at);
@@ -392,6 +401,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const KeyItem k = walk.get(g, cut, before);
             walk.next(k);
             const int first = k.k0 + quarter * 32, key = first + lane;
+            const float scale_dk = g.scale * exp2i(-unit_shift<DT>(g, bounds, k));
             if (k.n > 0) {
                 mbar_wait(acc_full, it & 1, wctx, kErrMmaWait);
                 tc_fence_after();
@@ -399,7 +409,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll
             for (int j = 0; j < 2 * (D / 32); ++j) {
                 const int which = j / (D / 32), r = j % (D / 32);        // dV, then dK
-                const float scale = which ? g.scale : Weight<DT>::kUnit;
+                const float scale = which ? scale_dk : Weight<DT>::kUnit;
                 uint32_t v[32];
                 if (k.n > 0) {
                     tmem_ld_32x32(tmem_lane + (which ? C::TMEM_DK : C::TMEM_DV) + 32 * r, v);
@@ -437,7 +447,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         const int row = quarter * 32 + lane;                 // key of the tile = tensor-memory lane
         const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         const uint32_t s_addr = tmem_lane + C::TMEM_S + 64 * half, dp_addr = tmem_lane + C::TMEM_DP + 64 * half;
-        const uint64_t scale2 = pair2(g.sl2, g.sl2), unit2 = pair2(Weight<DT>::kUnit, Weight<DT>::kUnit);
+        const uint64_t scale2 = pair2(g.sl2, g.sl2);
         uint32_t m = 0;
         Ring ring;
         for (KeyWalk<LINE> walk(g, cut, before); walk.more(cut);) {
@@ -446,6 +456,8 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const int key = k.k0 + row;
             // the first token that sees this key
             const int t_lo = key >= k.count ? 0x7fffffff : g.causal ? max(key + g.Tq - k.count, 0) : 0;
+            const float unit = exp2i(unit_shift<DT>(g, bounds, k) - Weight<DT>::kBits);
+            const uint64_t unit2 = pair2(unit, unit);
             int h0, t0;
             k.start(g, h0, t0);
             for (int i = 0; i < k.n; ++i, ++m, k.step(g, h0, t0)) {
@@ -600,7 +612,7 @@ attn_join_kernel(const float* __restrict__ part_dk, const float* __restrict__ pa
 
 template <typename DT, int D>
 int launch_dkdv(const Place& at, const Geom& g, const KeyCut& cut, const Operand& q, const Operand& k, const Operand& v, const Operand& d_o,
-                const float* lse, const float* delta, const Operand& d_k, const Operand& d_v) {
+                const float* lse, const float* delta, const Bounds& bounds, const Operand& d_k, const Operand& d_v) {
     using C = KeyCfg<D>;
     CUtensorMap tq, tg, tk, tv, tdk, tdv;
     int rc = operand_map(&tq, q, at.dtype, g.B, g.N, g.Tq, g.C, g.tt, g.hp, C::SLAB_C);
@@ -615,8 +627,8 @@ int launch_dkdv(const Place& at, const Geom& g, const KeyCut& cut, const Operand
     if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted[cut.line > 0]) != cudaSuccess) return NA2D_ERR_CUDA;
     const int sms = na2d_tc::sm_count(at.device);
     *at.launched += 1;
-    if (na2d_launch::launch(true, kern, cut.line ? cut.line : cut.items < sms ? cut.items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdk, tdv, lse, delta, at.errors,
-                            g, cut) != cudaSuccess)
+    if (na2d_launch::launch(true, kern, cut.line ? cut.line : cut.items < sms ? cut.items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdk, tdv, lse, delta, bounds,
+                            at.errors, g, cut) != cudaSuccess)
         return NA2D_ERR_CUDA;
     if (cut.line) {
         *at.launched += 1;

@@ -5,8 +5,8 @@
 //     dQ += dS K_c                                         (dS from tensor memory, 16 bit)
 // with delta = dO . o of the row, formed ahead by delta_kernel.  dS goes into its product as two numbers of 16 bits, what it rounds to and
 // the rest: rounded to one, it put dQ 1.4 to 1.5 times as far from its 64-bit value as dQ's own rounding does, and together with the rounding of
-// o in delta up to 1.7 times; now that is up to 1.3 times.  (The softmax scale comes in the epilogue: in fp16 dS keeps more of
-// its bits without.)
+// o in delta up to 1.7 times; now that is up to 1.3 times.  The softmax scale comes in the epilogue, and in fp16, whose numbers end at 2^-24 and
+// 2^16, so does the power of two that each row's dS carries (ds_shift; P has it as a summand of its exponent).
 //
 // Bound as the key half is: 8 heads x 16384 x 128, causal, bf16: 1024 us, 805 TFLOP/s over three products (with dS in one number: 782 us).
 //
@@ -26,16 +26,40 @@
 
 namespace na2d_attn {
 
-// delta = dO . o of each row, 8 channels a lane.  LPR lanes a row: C / 8, rounded up to a power of two.  A lane has kDeltaRows rows of one
+// delta = dO . o of each row, 8 channels a lane; fp16: the norms of dO and, by the blocks behind row_blocks, of V, too.  LPR lanes a row: C / 8, rounded up to a power of two.  A lane has kDeltaRows rows of one
 // head, 256 / LPR apart, all under way at once (8 x 16 heads x 3136 x 64: 16.5 us, 6.2 TB/s; with one row a lane 24).
 constexpr int kDeltaRows = 4;
 template <typename DT, int LPR>
 __global__ void __launch_bounds__(256)
 attn_delta_kernel(const DT* __restrict__ d_o, const Operand st_do, const DT* __restrict__ o, const Operand st_o, float* __restrict__ delta,
-                  const Geom g, const Div by_tiles, const Div by_heads) {
+                  const Geom g, const Div by_tiles, const Div by_heads, const Operand v, const Bounds bounds, const Div by_key_tiles,
+                  const unsigned row_blocks) {
     after_previous_grid();
     next_grid_may_start();
     constexpr int kStep = 256 / LPR;
+    // the largest of the warp's finite squares -> `to` (of which there are no two orders)
+    auto largest = [](float x, float* to) {
+        const unsigned top = __reduce_max_sync(0xffffffffu, x < CUDART_INF_F ? __float_as_uint(x) : 0u);
+        if (threadIdx.x % 32 == 0 && top) atomicMax(reinterpret_cast<unsigned*>(to), top);
+    };
+    if (!IsBf16<DT>::value && blockIdx.x >= row_blocks) {
+        int tile, m;
+        const int unit = by_key_tiles.split(blockIdx.x - row_blocks, tile), b = g.by_nk.split(unit, m), part = threadIdx.x % LPR;
+        const int k0 = tile * kDeltaRows * kStep + threadIdx.x / LPR, count = key_count(g, b);
+        const DT* x = static_cast<const DT*>(v.ptr) + b * v.b + m * v.n + 8 * part;
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < kDeltaRows; ++i) {
+            const int key = k0 + i * kStep;
+            const uint4 vx = key < count && 8 * part < g.C ? __ldg(reinterpret_cast<const uint4*>(x + key * v.t)) : make_uint4(0u, 0u, 0u, 0u);
+            float square = na2d_delta::dot8<DT>(vx, vx, 0.f);
+#pragma unroll
+            for (int d = LPR / 2; d > 0; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
+            if (square < CUDART_INF_F) top = fmaxf(top, square);
+        }
+        largest(top, bounds.unit + 2 * unit + 1);
+        return;
+    }
     int tile, n;
     const int bn = by_tiles.split(blockIdx.x, tile), b = by_heads.split(bn, n);
     const int part = threadIdx.x % LPR, t0 = tile * kDeltaRows * kStep + threadIdx.x / LPR;
@@ -50,6 +74,8 @@ attn_delta_kernel(const DT* __restrict__ d_o, const Operand st_do, const DT* __r
             vy[i] = __ldg(reinterpret_cast<const uint4*>(y + t * st_o.t));
         }
     }
+    const int count = IsBf16<DT>::value ? 0 : key_count(g, b);
+    float top = 0.f;
 #pragma unroll
     for (int i = 0; i < kDeltaRows; ++i) {
         float acc = na2d_delta::dot8<DT>(vx[i], vy[i], 0.f);
@@ -57,7 +83,15 @@ attn_delta_kernel(const DT* __restrict__ d_o, const Operand st_do, const DT* __r
         for (int d = LPR / 2; d > 0; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
         const int t = t0 + i * kStep;
         if (part == 0 && t < g.Tq) delta[static_cast<size_t>(bn) * g.Tq + t] = acc;
+        if constexpr (!IsBf16<DT>::value) {
+            float square = na2d_delta::dot8<DT>(vx[i], vx[i], 0.f);
+#pragma unroll
+            for (int d = LPR / 2; d > 0; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
+            if (part == 0 && t < g.Tq) bounds.row[static_cast<size_t>(bn) * g.Tq + t] = square;
+            if (t < g.Tq && keys_seen(g, count, t) > 0 && square < CUDART_INF_F) top = fmaxf(top, square);
+        }
     }
+    if constexpr (!IsBf16<DT>::value) largest(top, bounds.unit + 2 * (b * g.Nk + n / g.G));
 }
 
 struct RowCut {
@@ -136,7 +170,7 @@ __global__ void __launch_bounds__(512, 1)
 attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                const __grid_constant__ CUtensorMap tm_dq, DT* __restrict__ dq_rows, const Operand dq_st, const float* __restrict__ lse,
-               const float* __restrict__ delta, const ErrorState* __restrict__ errors, const Geom g, const RowCut cut) {
+               const float* __restrict__ delta, const Bounds bounds, const ErrorState* __restrict__ errors, const Geom g, const RowCut cut) {
     using C = DqCfg<D>;
     constexpr int NST = C::NST, NQ = C::NQ;
     extern __shared__ uint8_t smem_raw[];
@@ -371,6 +405,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             int n, t;
             const bool ok = tile.row(g, row, n, t);
             const int t_first = tile.t0 + quarter * 32;
+            float scale = g.scale;
+            if constexpr (!IsBf16<DT>::value) {
+                if (ok && !none)
+                    scale *= exp2i(-ds_shift(__ldg(bounds.row + row_index(g, tile.b, n, t)), __ldg(bounds.unit + 2 * (tile.b * g.Nk + tile.m) + 1)));
+            }
             if (!none) {
                 mbar_wait(dq_full, it & 1, wctx, kErrMmaWait);
                 tc_fence_after();
@@ -396,11 +435,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         if (ok && 32 * j + 4 * e < g.C)
-                            dst[e] = make_float4(__uint_as_float(v[4 * e]) * g.scale, __uint_as_float(v[4 * e + 1]) * g.scale,
-                                                 __uint_as_float(v[4 * e + 2]) * g.scale, __uint_as_float(v[4 * e + 3]) * g.scale);
+                            dst[e] = make_float4(__uint_as_float(v[4 * e]) * scale, __uint_as_float(v[4 * e + 1]) * scale,
+                                                 __uint_as_float(v[4 * e + 2]) * scale, __uint_as_float(v[4 * e + 3]) * scale);
                 } else if (g.hp == 1) {
                     if (t_first < g.Tq)
-                        na2d_tc::stage_and_store<DT, 32, 2>(&tm_dq, stage, v, g.scale, 32 * j, t_first, tile.h0, tile.b, 0, lane, &seq);
+                        na2d_tc::stage_and_store<DT, 32, 2>(&tm_dq, stage, v, scale, 32 * j, t_first, tile.h0, tile.b, 0, lane, &seq);
                 } else if (ok) {
                     uint4* dst = reinterpret_cast<uint4*>(dq_rows + tile.b * dq_st.b + n * dq_st.n + t * dq_st.t + 32 * j);
 #pragma unroll
@@ -409,7 +448,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                             uint32_t w[4];
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                w[i] = pack2<DT>(__uint_as_float(v[8 * e + 2 * i]) * g.scale, __uint_as_float(v[8 * e + 2 * i + 1]) * g.scale);
+                                w[i] = pack2<DT>(__uint_as_float(v[8 * e + 2 * i]) * scale, __uint_as_float(v[8 * e + 2 * i + 1]) * scale);
                             dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                 }
@@ -426,9 +465,10 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const uint32_t dp_addr = tmem_lane + C::TMEM_DP + 64 * half;
         const uint64_t scale2 = pair2(g.sl2, g.sl2);
         uint32_t m = 0;                                      // chunks so far
-        // lse and delta of a row: read an item ahead, since few chunks to an item would not cover the way to memory
+        // lse and delta of a row (fp16: and the squares that its dS are bounded by): read an item ahead, since few chunks to an item would
+        // not cover the way to memory
         RowItem next;
-        float next_lse, next_delta;
+        float next_lse, next_delta, next_row = 0.f, next_unit = 0.f;
         RowWalk<LINE> walk(g, cut, before);
         auto fetch = [&]() {
             next.n = -1;
@@ -442,19 +482,23 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             const size_t at = row_index(g, next.tile.b, n, t);
             next_lse = __ldg(lse + at);
             next_delta = __ldg(delta + at);
+            if constexpr (!IsBf16<DT>::value) {
+                next_row = __ldg(bounds.row + at);
+                next_unit = __ldg(bounds.unit + 2 * (next.tile.b * g.Nk + next.tile.m) + 1);
+            }
         };
         fetch();
         while (next.n >= 0) {
             const RowTile tile = next.tile;
             const int chunks = next.n, c0 = next.c0;
-            const float row_lse = next_lse, row_delta = next_delta;
+            const float row_lse = next_lse, row_delta = next_delta, shift = IsBf16<DT>::value ? 0.f : (float)ds_shift(next_row, next_unit);
             fetch();
             if (chunks == 0) continue;
             int n, t;
             const bool ok = tile.row(g, row, n, t);
             const bool idle = !__any_sync(0xffffffffu, ok);
             // a row that sees nothing has weights of zero: exp2(-infinity)
-            const float neg = row_lse == -CUDART_INF_F ? -CUDART_INF_F : -row_lse * kLog2e;
+            const float neg = row_lse == -CUDART_INF_F ? -CUDART_INF_F : IsBf16<DT>::value ? -row_lse * kLog2e : shift - row_lse * kLog2e;
             const uint64_t neg2 = pair2(neg, neg), delta2 = pair2(-row_delta, -row_delta);
             const int seen = (ok ? keys_seen(g, tile.count, t) : 0) - 64 * half - c0 * kRows;      // from the item's first chunk on
             for (int c = 0; c < chunks; ++c, ++m) {
@@ -527,14 +571,16 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 }
 
 template <typename DT>
-int launch_delta(const Place& at, const Geom& g, const Operand& d_o, const Operand& o, float* delta) {
+int launch_delta(const Place& at, const Geom& g, const Operand& d_o, const Operand& o, const Operand& v, float* delta, const Bounds& bounds) {
     const int lanes = g.C <= 32 ? 4 : g.C <= 64 ? 8 : 16, rows = kDeltaRows * 256 / lanes, tiles = (g.Tq + rows - 1) / rows;
-    const long long blocks = (long long)g.B * g.N * tiles;
+    const int key_tiles = (g.Tk + rows - 1) / rows;
+    const long long row_blocks = (long long)g.B * g.N * tiles, blocks = row_blocks + (IsBf16<DT>::value ? 0 : (long long)g.units * key_tiles);
     if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+    if (!IsBf16<DT>::value && cudaMemsetAsync(bounds.unit, 0, (size_t)g.units * 2 * sizeof(float), at.st) != cudaSuccess) return NA2D_ERR_CUDA;
     auto kern = lanes == 4 ? attn_delta_kernel<DT, 4> : lanes == 8 ? attn_delta_kernel<DT, 8> : attn_delta_kernel<DT, 16>;
     *at.launched += 1;
     return na2d_launch::launch(false, kern, (unsigned)blocks, 256, 0, at.st, (const DT*)d_o.ptr, d_o, (const DT*)o.ptr, o, delta, g, Div(tiles),
-                               Div(g.N)) == cudaSuccess
+                               Div(g.N), v, bounds, Div(key_tiles), (unsigned)row_blocks) == cudaSuccess
                ? NA2D_OK
                : NA2D_ERR_CUDA;
 }
@@ -586,7 +632,7 @@ attn_join_rows_kernel(const float* __restrict__ part, DT* __restrict__ dq, const
 
 template <typename DT, int D>
 int launch_dq(const Place& at, const Geom& g, RowCut cut, const Operand& q, const Operand& k, const Operand& v, const Operand& d_o, const float* lse,
-              const float* delta, const Operand& d_q) {
+              const float* delta, const Bounds& bounds, const Operand& d_q) {
     using C = DqCfg<D>;
     CUtensorMap tq, tg, tk, tv, tdq;
     int rc = operand_map(&tq, q, at.dtype, g.B, g.N, g.Tq, g.C, g.tt, g.hp, C::SLAB_C);
@@ -604,7 +650,7 @@ int launch_dq(const Place& at, const Geom& g, RowCut cut, const Operand& q, cons
     const int sms = na2d_tc::sm_count(at.device);
     *at.launched += 1;
     if (na2d_launch::launch(true, kern, cut.line ? cut.line : items < sms ? (int)items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdq, (DT*)d_q.ptr,
-                            d_q, lse, delta, at.errors, g, cut) != cudaSuccess)
+                            d_q, lse, delta, bounds, at.errors, g, cut) != cudaSuccess)
         return NA2D_ERR_CUDA;
     if (!cut.line) return NA2D_OK;
     *at.launched += 1;

@@ -6,13 +6,14 @@
 
 namespace na2d_attn {
 
-// Scratch for results that are computed in parts (fp32): with less than *_floats() of it there are fewer parts.
+// Scratch (fp32) for results that are computed in parts, of which there are fewer with less than *_floats() of it, and for the bounds of
+// fp16's backward.
 struct Scratch {
     float* at;
     size_t floats;
 };
 size_t forward_floats(const Geom& g, int sms);
-size_t backward_floats(const Geom& g, int sms, bool d_q, bool d_k);
+size_t backward_floats(const Geom& g, int sms, bool f16, bool d_q, bool d_k);
 
 // 16 bits, C a multiple of 8 up to 128, every operand on 16-byte boundaries; o, d_q, d_k and d_v dense.
 int forward_bf16(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);

@@ -79,6 +79,8 @@ size_t line_rows(const Geom& g, int sms) { return (size_t)(line_groups(g, sms) +
 size_t all_rows(const Geom& g) { return (size_t)g.B * g.N * g.Tq; }
 size_t key_part(const Geom& g) { return (size_t)g.units * g.Tk * g.C; }
 size_t row_part(const Geom& g, int line) { return (size_t)line * 2 * kRows * g.C; }             // 2 a CTA
+size_t bound_units(const Geom& g) { return ((size_t)g.units * 2 + 3) / 4 * 4; }                 // floats, in whole 16 bytes
+size_t bound_floats(const Geom& g) { return bound_units(g) + (all_rows(g) + 3) / 4 * 4; }
 size_t line_part(const Geom& g, int line) { return (size_t)line * 2 * 2 * kRows * g.C; }        // of dK and dV, 2 a CTA
 
 }  // namespace
@@ -111,8 +113,29 @@ int NA2D_TC_NAME(forward)(const Place& at, const Geom& g, const Scratch& scratch
     });
 }
 
-int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Scratch& scratch, const Backward& x) {
-    int rc = launch_delta<NA2D_TC_TYPE>(at, g, x.d_o, x.o, x.delta);
+int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Scratch& given, const Backward& x) {
+    // fp16's bounds come first in the workspace; without one they lie in the stream's memory pool for the time of the call
+    struct Own {
+        float* at = nullptr;
+        cudaStream_t st;
+        ~Own() {
+            if (at) cudaFreeAsync(at, st);
+        }
+    } own;
+    own.st = at.st;
+    Bounds bounds{};
+    Scratch scratch = given;
+    if (!IsBf16<NA2D_TC_TYPE>::value) {
+        if (given.floats >= bound_floats(g)) {
+            bounds.unit = given.at;
+            scratch = Scratch{given.at + bound_floats(g), given.floats - bound_floats(g)};
+        } else {
+            if (cudaMallocAsync(reinterpret_cast<void**>(&own.at), bound_floats(g) * sizeof(float), at.st) != cudaSuccess) return NA2D_ERR_CUDA;
+            bounds.unit = own.at;
+        }
+        bounds.row = bounds.unit + bound_units(g);
+    }
+    int rc = launch_delta<NA2D_TC_TYPE>(at, g, x.d_o, x.o, x.v, x.delta, bounds);
     if (rc != NA2D_OK) return rc;
     return by_head_dim(g.C, [&](auto d) {
         constexpr int D = decltype(d)::value;
@@ -123,7 +146,7 @@ int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Scratch& scratc
             row_cut.line = rows;
             row_cut.part = scratch.at;
         }
-        if (x.d_q.ptr) rc = launch_dq<NA2D_TC_TYPE, D>(at, g, row_cut, x.q, x.k, x.v, x.d_o, x.lse, x.delta, x.d_q);
+        if (x.d_q.ptr) rc = launch_dq<NA2D_TC_TYPE, D>(at, g, row_cut, x.q, x.k, x.v, x.d_o, x.lse, x.delta, bounds, x.d_q);
         if (rc != NA2D_OK || !x.d_k.ptr) return rc;
         Geom gk = g;
         if (g.causal) cut_rows(gk, false);               // a chunk's masks go by the column alone
@@ -142,7 +165,7 @@ int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Scratch& scratc
         const long long items = (long long)gk.units * cut.key_tiles * cut.splits;
         if (items > 0x3fffffffLL) return (int)NA2D_ERR_TOO_LARGE;
         cut.items = (int)items;
-        return launch_dkdv<NA2D_TC_TYPE, D>(at, gk, cut, x.q, x.k, x.v, x.d_o, x.lse, x.delta, x.d_k, x.d_v);
+        return launch_dkdv<NA2D_TC_TYPE, D>(at, gk, cut, x.q, x.k, x.v, x.d_o, x.lse, x.delta, bounds, x.d_k, x.d_v);
     });
 }
 
@@ -152,12 +175,13 @@ size_t forward_floats(const Geom& g, int sms) {
     const int parts = forward_parts(g, sms);
     return parts > 1 ? parts * all_rows(g) * (g.C + 1) : 0;
 }
-size_t backward_floats(const Geom& g, int sms, bool d_q, bool d_k) {         // the halves' one after the other
+size_t backward_floats(const Geom& g, int sms, bool f16, bool d_q, bool d_k) {       // the halves' one after the other
+    const size_t bounds = f16 ? bound_floats(g) : 0;
     size_t floats = d_q ? row_part(g, row_line(g, sms)) : 0;
-    if (!d_k) return floats;
-    if (const int line = key_line(g, sms)) return std::max(floats, line_part(g, line));
+    if (!d_k) return bounds + floats;
+    if (const int line = key_line(g, sms)) return bounds + std::max(floats, line_part(g, line));
     const int parts = key_parts(g, sms);
-    return std::max(floats, parts > 1 ? 2 * parts * key_part(g) : 0);
+    return bounds + std::max(floats, parts > 1 ? 2 * parts * key_part(g) : 0);
 }
 #endif
 

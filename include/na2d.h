@@ -301,7 +301,9 @@ typedef struct na2d_heads {
  *   d_q, or d_k and d_v together, may be NULL: that half is left out.  No atomics: the same call gives the same bits.
  *   workspace    scratch, 16-byte aligned, of na2d_attention_workspace bytes: where the tiles of rows, or of keys, do not share out evenly
  *                over the SMs (few of either, entries of different lengths), some are computed in parts that are joined there.  With
- *                less, or none, there are fewer parts: slower, and other last bits. */
+ *                less, or none, there are fewer parts: slower, and other last bits.  The backward of NA2D_F16 on tensor cores also
+ *                keeps the rows' gradient norms there; with less than those take it allocates them on the stream for the call.
+ *   NA2D_F16     gradients may be of any size that the type holds: dS carries a power of two through its 16-bit products. */
 typedef struct na2d_attention_args {
     size_t struct_size;
     int B, N, Nk, Tq, Tk, C, dtype, path, device, causal;

@@ -146,3 +146,98 @@ def test_a_call_recorded_by_a_dispatch_mode_runs_again(which):
     for grad in (False, True)[:1 if which == "rotary_table" else 2]:
         graph = make_fx(lambda *args: results(f, args, grad))(*make(0))
         same(graph(*make(1)), results(f, make(1), grad))
+
+
+# ---- fp16 gradients far from one ------------------------------------------------------------------------------------------
+def gradients(q, k, v, d_o, scale, causal=False, lengths=None):
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    got = torch.autograd.grad(na.attention(q, k, v, scale, causal, lengths), (q, k, v), d_o)
+    na.check_kernels(DEV)
+    return got
+
+
+def near(got, want, terms, units, what):
+    """`units` roundings of fp16 in the norm, of the gradient or, where its terms cancel, of these; and half a step of the
+    numbers below 2^-14, which are 2^-24 apart."""
+    got, want = got.double(), want.double()
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    err = (got - want).square().mean().sqrt()
+    bound = units * U[F16] * want.square().mean().sqrt().clamp_min(terms) + 2.0 ** -25
+    assert err <= bound, f"{what}: {err:.2e} of {bound:.2e}"
+
+
+@pytest.mark.parametrize("size", [1e-4, 1e-3, 1e-2, 1.0, 100.0])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("C,Tq,Tk", [(128, 600, 8192), (64, 130, 16384), (128, 4096, 4096)])
+def test_fp16_gradients_of_any_size_on_long_rows(C, Tq, Tk, causal, size):
+    """Weights of 2^-14 times gradients of 1e-4 are below every number of fp16.  K is large for dq and Q for dk, so that the results
+    themselves are not."""
+    for name, kq in (("dq", (1 / 64, 64.0)), ("dk", (64.0, 1 / 64))):
+        q, k = rand(1, 2, Tq, C, dtype=F16, scale=kq[0]), rand(1, 1, Tk, C, dtype=F16, seed=1, scale=kq[1])
+        v, d_o = rand(1, 1, Tk, C, dtype=F16, seed=2), rand(1, 2, Tq, C, dtype=F16, seed=3, scale=size)
+        got = gradients(q, k, v, d_o, C ** -0.5, causal)
+        want = plain_attention(q, k, v, d_o, C ** -0.5, causal, None)
+        if name == "dq":
+            near(got[0], want[2], want[5][0], 1.5, name)
+        else:
+            near(got[1], want[3], want[6][0], 1.5, name)
+        near(got[2], want[4], 0.0, 1.5, "dv")
+
+
+@pytest.mark.parametrize("N,Nk,Tq,Tk,C", [(2, 2, 200, 40, 64), (4, 2, 30, 150, 128), (2, 1, 1000, 100, 32)])
+def test_fp16_gradients_that_are_large_on_the_way(N, Nk, Tq, Tk, C):
+    """dO . V reaches 1e7, dq and dk do not."""
+    q, k = rand(1, N, Tq, C, dtype=F16, scale=0.01), rand(1, Nk, Tk, C, dtype=F16, seed=1, scale=0.01)
+    v, d_o = rand(1, Nk, Tk, C, dtype=F16, seed=2, scale=30.0), rand(1, N, Tq, C, dtype=F16, seed=3, scale=1e4)
+    got = gradients(q, k, v, d_o, C ** -0.5)
+    want = plain_attention(q, k, v, d_o, C ** -0.5, False, None)
+    assert max(t.abs().max() for t in want[2:5]) < 65504
+    near(got[0], want[2], want[5][0], 1.5, "dq")
+    near(got[1], want[3], want[6][0], 1.5, "dk")
+    near(got[2], want[4], 0.0, 1.5, "dv")
+
+
+@pytest.mark.parametrize("C,Tq,Tk", [(128, 512, 8192), (64, 2000, 2000)])
+def test_fp16_rows_of_different_sizes(C, Tq, Tk):
+    """Every row's dq is as near as its own gradient allows, whatever the other rows' are."""
+    size = torch.logspace(-5, 0, 8, device=DEV).repeat_interleave(Tq // 8)[:, None]
+    q, k, v = rand(1, 1, Tq, C, dtype=F16, scale=1 / 64), rand(1, 1, Tk, C, dtype=F16, seed=1, scale=64.0), rand(1, 1, Tk, C, dtype=F16, seed=2)
+    d_o = (rand(1, 1, Tq, C, seed=3) * size).to(F16)
+    got = gradients(q, k, v, d_o, C ** -0.5)
+    want = plain_attention(q, k, v, d_o, C ** -0.5, False, None)
+    for i in range(8):
+        rows = slice(i * (Tq // 8), (i + 1) * (Tq // 8))
+        part = plain_attention(q[:, :, rows], k, v, d_o[:, :, rows], C ** -0.5, False, None)
+        near(got[0][:, :, rows], part[2], part[5][0], 1.5, f"rows {i}")
+    near(got[1], want[3], want[6][0], 1.5, "dk")
+
+
+def test_fp16_gradients_without_a_workspace():
+    """The C entry keeps its bounds elsewhere then; the gradients are the same sums (parts are joined in another order, then one rounding)."""
+    B, N, Nk, Tq, Tk, C = 2, 4, 2, 300, 2100, 64
+    q, k, v = rand(B, N, Tq, C, dtype=F16), rand(B, Nk, Tk, C, dtype=F16, seed=1), rand(B, Nk, Tk, C, dtype=F16, seed=2)
+    d_o, lengths = rand(B, N, Tq, C, dtype=F16, seed=3, scale=1e-3), torch.tensor([2100, 77], device=DEV, dtype=torch.int32)
+    o, lse = na.attention_with_lse(q, k, v, 0.125, False, lengths)
+    want = plain_attention(q, k, v, d_o, 0.125, False, lengths)
+    a, delta = _lib.AttentionArgs(), torch.empty_like(lse)
+    a.struct_size = ctypes.sizeof(a)
+    a.B, a.N, a.Nk, a.Tq, a.Tk, a.C, a.dtype, a.scale = B, N, Nk, Tq, Tk, C, _lib.DTYPE_F16, 0.125
+    a.stream, a.lse, a.delta, a.key_lengths = torch.cuda.current_stream().cuda_stream, lse.data_ptr(), delta.data_ptr(), lengths.data_ptr()
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("d_o", d_o)):
+        setattr(a, name, _lib.Heads(t.data_ptr(), 0, 0, 0))
+    for halves in ("qkv", "q", "kv"):
+        out = {name: torch.full_like(t, math.nan) for name, t in (("q", q), ("k", k), ("v", v))}
+        for name, t in out.items():
+            setattr(a, "d_" + name, _lib.Heads(t.data_ptr() if name in halves else None, 0, 0, 0))
+        room = _lib.lib.na2d_attention_workspace(ctypes.byref(a), 1)
+        bounds = 4 * (B * N * Tq + 2 * B * Nk)
+        assert room >= bounds
+        workspace = torch.full((room,), 255, dtype=torch.uint8, device=DEV)
+        for size in (0, bounds - 4, bounds + 64, room):
+            a.workspace, a.workspace_bytes = (workspace.data_ptr(), size) if size else (None, 0)
+            _lib.check(_lib.lib.na2d_attention_backward(ctypes.byref(a)))
+            na.check_kernels(DEV)
+            for b in range(B):
+                for name, ref, terms in (("q", want[2], want[5]), ("k", want[3], want[6]), ("v", want[4], torch.zeros(B))):
+                    if name in halves:
+                        near(out[name][b], ref[b], float(terms[b]), 1.5, f"d{name} {b} {size}")
