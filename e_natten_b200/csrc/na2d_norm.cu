@@ -20,7 +20,8 @@
 // (206), memory at 4.4 TB/s; 16 x 14^2 x 1024, fp16, on the chip: 20 + 26 us with a cold L2 (5).  Forward, 2 x 97 x 131 x 384, fp16: 21 us (6).
 //
 // Variances are sums of squares about a mean at every step (of a slab; of four pixels, merged with those before), so that maps
-// whose mean is far above their spread lose nothing.  All sums are in fp32 and in an order that the sizes alone fix.
+// whose mean is far above their spread lose nothing.  All sums are in fp32 and in an order that the sizes alone fix; a thread of the two
+// forms has some thousand values on maps of 2^20 pixels, one of the kernels for wide groups any number, which it sums with what rounding loses.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -925,6 +926,17 @@ __global__ void __launch_bounds__(2 * kHalf, 1) norm_bwd_kernel(const Norm n, co
 }
 
 // ---- groups wider than a block of vectors: a block a group, a thread a channel at a time ---------------------------------
+// A sum of any number of values, with what its roundings lost (a thread has all pixels of its channels, hundreds of thousands of values:
+// without, the variance of 2^20 came out 5e-4 too small).
+struct LongSum {
+    float sum = 0.f, lost = 0.f;
+    __device__ __forceinline__ void add(float x) {
+        const float next = sum + x, part = next - sum;
+        lost += (sum - (next - part)) + (x - part);
+        sum = next;
+    }
+    __device__ __forceinline__ float value() const { return sum + lost; }
+};
 __device__ __forceinline__ float block_sum(float x, float* red) {
     x = warp_sum(x);
     __syncthreads();
@@ -944,16 +956,16 @@ __global__ void __launch_bounds__(kThreads) norm_wide_fwd_kernel(const Norm n) {
     const int b = blockIdx.x / n.G, g = blockIdx.x - b * n.G;
     const T* x = static_cast<const T*>(n.x.ptr) + b * n.x.b + g * n.cg;
     const float inv_m = 1.f / ((float)n.P * n.cg);
-    float sum = 0.f, square = 0.f;
+    LongSum sum, square;
     for (int c = threadIdx.x; c < n.cg; c += kThreads)
-        for (long long p = 0; p < n.P; ++p) sum += na2d_vec::widen(x[p * n.x.p + c]);
-    const float mean = block_sum(sum, red) * inv_m;
+        for (long long p = 0; p < n.P; ++p) sum.add(na2d_vec::widen(x[p * n.x.p + c]));
+    const float mean = block_sum(sum.value(), red) * inv_m;
     for (int c = threadIdx.x; c < n.cg; c += kThreads)
         for (long long p = 0; p < n.P; ++p) {
             const float off = na2d_vec::widen(x[p * n.x.p + c]) - mean;
-            square = fmaf(off, off, square);
+            square.add(off * off);
         }
-    const float rstd = rsqrtf(fmaf(block_sum(square, red), inv_m, n.eps));
+    const float rstd = rsqrtf(fmaf(block_sum(square.value(), red), inv_m, n.eps));
     if (threadIdx.x == 0) {
         n.mean[blockIdx.x] = mean;
         n.rstd[blockIdx.x] = rstd;
@@ -982,15 +994,16 @@ __global__ void __launch_bounds__(kThreads) norm_wide_bwd_kernel(const Norm n, f
     };
     for (int c = threadIdx.x; c < n.cg; c += kThreads) {
         const float w = param<T>(n, n.w, g * n.cg + c, 1.f), bias = param<T>(n, n.bias, g * n.cg + c, 0.f);
-        float a = 0.f, d = 0.f, xhat;
+        LongSum a, d;
+        float xhat;
         for (long long p = 0; p < n.P; ++p) {
             const float dz = dz_of(p, c, w, bias, xhat);
-            a += dz;
-            d = fmaf(dz, xhat, d);
+            a.add(dz);
+            d.add(dz * xhat);
         }
-        if (sums) sums[(long long)b * n.C + g * n.cg + c] = make_float2(a, d);
-        s1 = fmaf(w, a, s1);
-        s2 = fmaf(w, d, s2);
+        if (sums) sums[(long long)b * n.C + g * n.cg + c] = make_float2(a.value(), d.value());
+        s1 = fmaf(w, a.value(), s1);
+        s2 = fmaf(w, d.value(), s2);
     }
     s1 = block_sum(s1, red) * inv_m;
     s2 = block_sum(s2, red) * inv_m;

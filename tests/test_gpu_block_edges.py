@@ -241,3 +241,16 @@ def test_fp16_gradients_without_a_workspace():
                 for name, ref, terms in (("q", want[2], want[5]), ("k", want[3], want[6]), ("v", want[4], torch.zeros(B))):
                     if name in halves:
                         near(out[name][b], ref[b], float(terms[b]), 1.5, f"d{name} {b} {size}")
+
+
+# ---- sums over very many pixels ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shape,groups,shift", [((1, 256, 256, 1028), 1, 0.0), ((1, 256, 256, 1028), 1, 300.0), ((1, 300, 333, 301), 1, 0.0)], ids=str)
+def test_group_norm_of_wide_groups_on_large_maps(shape, groups, shift):
+    """A group's values by the hundred thousand in one thread: the statistics are as near as the other forms'.  (With a mean of
+    300 spreads x - mean itself is exact to 1.8e-5, as in test_group_norm_far_from_zero.)"""
+    C = shape[-1]
+    x, d_y = rand(*shape, shift=shift), rand(*shape, seed=3) + 0.5
+    if shift:
+        check_norm(x, groups, None, None, d_y, None, units=8)
+    else:
+        check_norm(x, groups, rand(C, seed=1, scale=0.3, shift=1.0), rand(C, seed=2), d_y)
