@@ -375,6 +375,7 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor& x_in, const Tensor& weight
     const Tensor x = pixels(x_in);
     na2d_norm_args a = norm_args(x, weight, bias, stats, call);
     a.y = y.data_ptr();
+    check(abi.poll(a.device, nullptr));                  // (the two passes wait for one another)
     const Tensor workspace = scratch(abi.norm_workspace(&a, 0), x);
     if (workspace.defined()) {
         a.workspace = workspace.data_ptr();
@@ -411,6 +412,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& x_in, const Tenso
     a.d_x = d_x.defined() ? d_x.data_ptr() : nullptr;
     a.d_weight = need_w ? d_w.data_ptr() : nullptr;
     a.d_bias = need_b ? d_b.data_ptr() : nullptr;
+    check(abi.poll(a.device, nullptr));
     const Tensor workspace = scratch(abi.norm_workspace(&a, 1), x);
     a.workspace = workspace.data_ptr();
     a.workspace_bytes = workspace.numel();

@@ -254,3 +254,19 @@ def test_group_norm_of_wide_groups_on_large_maps(shape, groups, shift):
         check_norm(x, groups, None, None, d_y, None, units=8)
     else:
         check_norm(x, groups, rand(C, seed=1, scale=0.3, shift=1.0), rand(C, seed=2), d_y)
+
+
+# ---- waits that gave up ---------------------------------------------------------------------------------------------
+def test_group_norm_raises_what_an_earlier_wait_reported():
+    """Its kernels of two passes wait for one another; one that gave up wrote wrong values, and the next call, forward or backward, says so."""
+    na.check_kernels(DEV)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    x = rand(1, 4, 4, 8).requires_grad_()
+    y = na.group_norm(x, 2)
+    for call in (lambda: na.group_norm(x.detach(), 2), lambda: na.group_norm(x, 2), lambda: torch.autograd.grad(y, x, y.detach(), retain_graph=True)):
+        _lib.check(_lib.lib.na2d_selftest_wait_timeout(0, stream, 1000))
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="bounded wait"):
+            call()
+        call()
+    na.check_kernels(DEV)
