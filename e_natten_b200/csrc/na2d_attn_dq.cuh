@@ -410,6 +410,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 if (ok && !none)
                     scale *= exp2i(-ds_shift(__ldg(bounds.row + row_index(g, tile.b, n, t)), __ldg(bounds.unit + 2 * (tile.b * g.Nk + tile.m) + 1)));
             }
+            const bool blind = g.causal && keys_seen(g, tile.count, t) == 0;         // (beside rows that see: dS = 0 meets any key of theirs)
             if (!none) {
                 mbar_wait(dq_full, it & 1, wctx, kErrMmaWait);
                 tc_fence_after();
@@ -425,7 +426,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                         __syncwarp();
                         if (lane == 0) mbar_arrive(dq_free);
                     }
-                } else {
+                }
+                if (none || blind) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[e] = 0u;
                 }

@@ -160,6 +160,7 @@ struct Sums {
     }
 };
 
+// (a scale of 0: a row that sees nothing, whose products may be 0 times infinity)
 template <typename DT, int CP, int BM>
 __device__ __forceinline__ void store_rows(DT* dst, long long stride, int row0, int rows, int C,
                                            const Sums<CP, BM>& acc, const float (&scale)[BM / 16], int tx, int ty) {
@@ -173,7 +174,8 @@ __device__ __forceinline__ void store_rows(DT* dst, long long stride, int row0, 
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int c = out_col<CP>(tx, k) + e;
-                if (c < C) dst[r * stride + c] = narrow<DT>((e ? na2d_ptx::hi2(acc.at[i][k]) : na2d_ptx::lo2(acc.at[i][k])) * scale[i]);
+                const float x = (e ? na2d_ptx::hi2(acc.at[i][k]) : na2d_ptx::lo2(acc.at[i][k])) * scale[i];
+                if (c < C) dst[r * stride + c] = narrow<DT>(scale[i] == 0.f ? 0.f : x);
             }
     }
 }
@@ -302,7 +304,7 @@ simt_dq_kernel(const Operand q, const Operand k, const Operand v, const Operand 
         const bool row = t < g.Tq && keys_seen(g, count, t) > 0;
         neg[i] = row ? -lse[row_index(g, b, n, t)] * na2d_tc::kLog2e : 0.f;
         del[i] = row ? delta[row_index(g, b, n, t)] : 0.f;
-        scale[i] = g.scale;
+        scale[i] = row ? g.scale : 0.f;
     }
     for (int k0 = 0; k0 < keys; k0 += S::BT) {
         __syncthreads();

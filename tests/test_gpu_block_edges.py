@@ -270,3 +270,34 @@ def test_group_norm_raises_what_an_earlier_wait_reported():
             call()
         call()
     na.check_kernels(DEV)
+
+
+# ---- not finite beside what sees nothing ---------------------------------------------------------------------------------
+FORMS = [(F32, 32), (F32, 200), (BF16, 7), (BF16, 64), (F16, 128)]
+
+
+@pytest.mark.parametrize("Tq", [7, 150])
+@pytest.mark.parametrize("dtype,C", FORMS)
+def test_rows_that_see_nothing_beside_infinite_keys(dtype, C, Tq):
+    """o = 0 and dq = 0, although a visible key of their tile has a value that is not finite."""
+    q, k, v = rand(1, 2, Tq, C, dtype=dtype), rand(1, 1, 40, C, dtype=dtype, seed=1), rand(1, 1, 40, C, dtype=dtype, seed=2)
+    k[0, 0, 1, 0], v[0, 0, 0, 1], v[0, 0, 1, 2] = math.inf, math.inf, math.nan
+    lengths = torch.tensor([3], device=DEV)                       # the last three rows see keys
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    o, lse = na.attention_with_lse(q, k, v, 0.25, True, lengths)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), torch.ones_like(o))
+    assert (o[:, :, :Tq - 3] == 0).all() and (lse[:, :, :Tq - 3] == -math.inf).all()
+    assert (dq[:, :, :Tq - 3] == 0).all()
+
+
+@pytest.mark.parametrize("Tq", [3, 40])
+@pytest.mark.parametrize("dtype,C", FORMS)
+def test_tokens_that_see_nothing_beside_infinite_keys(dtype, C, Tq):
+    """The form of serving, caches of different lengths."""
+    q, k, v = rand(3, 4, Tq, C, dtype=dtype), rand(3, 2, 300, C, dtype=dtype, seed=1), rand(3, 2, 300, C, dtype=dtype, seed=2)
+    k[:, :, 0, 0], v[:, :, 0, 1] = math.inf, math.inf
+    lengths = torch.tensor([1, 0, 300], device=DEV)
+    with torch.no_grad():
+        o, lse = na.attention_with_lse(q, k, v, 0.25, True, lengths)
+    for b, blind in enumerate((Tq - 1, Tq, 0)):
+        assert (o[b, :, :blind] == 0).all() and (lse[b, :, :blind] == -math.inf).all()
