@@ -401,6 +401,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const KeyItem k = walk.get(g, cut, before);
             walk.next(k);
             const int first = k.k0 + quarter * 32, key = first + lane;
+            const bool there = k.n > 0 && key < k.count;     // else no query sees the tile, or the key is none (its weights of 0 meet any dO and Q)
             const float scale_dk = g.scale * exp2i(-unit_shift<DT>(g, bounds, k));
             if (k.n > 0) {
                 mbar_wait(acc_full, it & 1, wctx, kErrMmaWait);
@@ -419,7 +420,8 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                         __syncwarp();
                         if (lane == 0) mbar_arrive(acc_free);
                     }
-                } else {                                                 // no query sees the tile
+                }
+                if (!there) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) v[e] = 0u;
                 }

@@ -160,7 +160,7 @@ struct Sums {
     }
 };
 
-// (a scale of 0: a row that sees nothing, whose products may be 0 times infinity)
+// (a scale of 0: a row that sees nothing, or a key that is none, whose products may be 0 times infinity)
 template <typename DT, int CP, int BM>
 __device__ __forceinline__ void store_rows(DT* dst, long long stride, int row0, int rows, int C,
                                            const Sums<CP, BM>& acc, const float (&scale)[BM / 16], int tx, int ty) {
@@ -360,8 +360,9 @@ simt_dkdv_kernel(const Operand q, const Operand k, const Operand v, const Operan
     float scale_k[S::R], scale_v[S::R];
 #pragma unroll
     for (int i = 0; i < S::R; ++i) {
-        scale_k[i] = g.scale;
-        scale_v[i] = 1.f;
+        const bool there = k0 + ty + 16 * i < count;
+        scale_k[i] = there ? g.scale : 0.f;
+        scale_v[i] = there ? 1.f : 0.f;
     }
     const int first = t_min / S::BT * S::BT;
     const bool any = k0 < count && first < g.Tq;

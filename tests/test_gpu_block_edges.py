@@ -301,3 +301,19 @@ def test_tokens_that_see_nothing_beside_infinite_keys(dtype, C, Tq):
         o, lse = na.attention_with_lse(q, k, v, 0.25, True, lengths)
     for b, blind in enumerate((Tq - 1, Tq, 0)):
         assert (o[b, :, :blind] == 0).all() and (lse[b, :, :blind] == -math.inf).all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype,C", FORMS)
+@pytest.mark.parametrize("B,N,Nk,Tq,Tk", [(1, 2, 1, 20, 90), (1, 2, 2, 1100, 200), (2, 4, 2, 9, 300)])
+def test_keys_beyond_a_length_beside_infinite_gradients(B, N, Nk, Tq, Tk, dtype, C, causal):
+    """dk = 0 and dv = 0 there, although the queries and the gradients that meet their tile are not finite."""
+    q, k, v = rand(B, N, Tq, C, dtype=dtype), rand(B, Nk, Tk, C, dtype=dtype, seed=1), rand(B, Nk, Tk, C, dtype=dtype, seed=2)
+    d_o = rand(B, N, Tq, C, dtype=dtype, seed=3)
+    q[:, 0, Tq - 1, 0], d_o[:, 0, Tq - 2, 1], d_o[:, -1, Tq - 1, 3] = math.nan, math.inf, -math.inf
+    lengths = torch.tensor([Tk - 70, 5][:B], device=DEV)
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    o = na.attention(q, k, v, 0.25, causal, lengths)
+    _, dk, dv = torch.autograd.grad(o, (q, k, v), d_o)
+    for b in range(B):
+        assert (dk[b, :, lengths[b]:] == 0).all() and (dv[b, :, lengths[b]:] == 0).all()
