@@ -140,7 +140,7 @@ struct KeyCfg : TileCfg<D> {
     static constexpr int NST = D == 128 ? 2 : 4;                         // chunks of Q and dO
     static constexpr int NKV = D == 128 ? 1 : 2;                         // tiles of K and V: the next one's while this one's are read
     static constexpr int OUT_BYTES = 4 * 2 * OutStage<32>::BYTES;
-    static constexpr int X_BYTES = NST * 2 * kRows * 4;                  // [ring slot]{-lse * log2(e), -delta}[row]
+    static constexpr int X_BYTES = NST * 2 * kRows * 4 + NST * 8;        // [ring slot]{-lse * log2(e), -delta}[row]; [ring slot] what dP is scaled by, twice
     static constexpr int SMEM = 2 * NKV * T::BYTES + 2 * NST * T::BYTES + OUT_BYTES + X_BYTES + 512 /*barriers*/ + 1024 /*alignment*/;
     static constexpr int TMEM_S = 0, TMEM_DP = 128, TMEM_DV = 256, TMEM_DK = 384;
     static_assert(SMEM <= kSmemLimit, "dK/dV kernel shared memory");
@@ -276,6 +276,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                     x[lane + 32 * u] = x_lse[u] == -CUDART_INF_F ? -CUDART_INF_F : Weight<DT>::kShift - x_lse[u] * kLog2e;
                     x[kRows + lane + 32 * u] = -x_delta[u] * unit;
                 }
+                if (!IsBf16<DT>::value && lane == 0) reinterpret_cast<uint64_t*>(s_x + NST * 2 * kRows)[ring.at] = pair2(unit, unit);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(x_full + ring.at);
                 ring.next(NST);
@@ -458,8 +459,6 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const int key = k.k0 + row;
             // the first token that sees this key
             const int t_lo = key >= k.count ? 0x7fffffff : g.causal ? max(key + g.Tq - k.count, 0) : 0;
-            const float unit = exp2i(unit_shift<DT>(g, bounds, k) - Weight<DT>::kBits);
-            const uint64_t unit2 = pair2(unit, unit);
             int h0, t0;
             k.start(g, h0, t0);
             for (int i = 0; i < k.n; ++i, ++m, k.step(g, h0, t0)) {
@@ -507,6 +506,7 @@ attn_dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 tmem_ld_32x32(dp_addr, s[0]);
                 tmem_ld_32x32(dp_addr + 32, s[1]);
                 tmem_ld_wait();
+                const uint64_t unit2 = reinterpret_cast<const uint64_t*>(s_x + NST * 2 * kRows)[ring.at];
 #pragma unroll
                 for (int e4 = 0; e4 < 16; ++e4) {
                     const ulonglong2 nd = *reinterpret_cast<const ulonglong2*>(x_delta + 4 * e4);
