@@ -317,3 +317,101 @@ def test_keys_beyond_a_length_beside_infinite_gradients(B, N, Nk, Tq, Tk, dtype,
     _, dk, dv = torch.autograd.grad(o, (q, k, v), d_o)
     for b in range(B):
         assert (dk[b, :, lengths[b]:] == 0).all() and (dv[b, :, lengths[b]:] == 0).all()
+
+
+# ---- group norm in several sets of units -----------------------------------------------------------------------------
+SETS = [  # shape, groups, type: several sets of the two passes, several units a set, a last set of fewer, slabs of several entries
+    ((9, 128, 128, 256), 8, F32), ((9, 128, 128, 256), 8, BF16), ((4, 256, 256, 256), 16, F32), ((4, 256, 256, 256), 16, F16),
+    ((40, 100, 100, 64), 2, F32), ((40, 100, 100, 64), 2, BF16), ((5, 256, 257, 100), 5, F32), ((3, 300, 300, 384), 12, BF16), ((10, 64, 64, 1024), 2, F16),
+]
+
+
+@pytest.mark.parametrize("shape,groups,dtype", SETS, ids=str)
+def test_group_norm_in_several_sets(shape, groups, dtype):
+    """Blocks wait for one another, reuse the runs' places and add to their rows of channel sums: right, the same bits every time, and
+    the same parameter gradients where d_x is not wanted."""
+    gen = torch.Generator(DEV).manual_seed(7)
+    normal = lambda *s: torch.randn(s, generator=gen, device=DEV)
+    C = shape[-1]
+    x, d_y = (normal(*shape) * 1.5 + normal(shape[0], 1, 1, C)).to(dtype), normal(*shape).to(dtype)
+    w, b = normal(C) * 0.3 + 1, normal(C)
+    check_norm(x, groups, w, b, d_y)
+
+    def step(wanted):
+        leaves = [t.detach().requires_grad_(i in wanted) for i, t in enumerate((x, w, b))]
+        y = na.group_norm(leaves[0], groups, leaves[1], leaves[2], activation="silu")
+        return [y.detach()] + list(torch.autograd.grad(y, [leaves[i] for i in wanted], d_y))
+    first = step((0, 1, 2))
+    for _ in range(3):
+        same(step((0, 1, 2)), first)
+    same(step((1, 2)), [first[0]] + first[2:])
+    same(step((0,)), first[:2])
+    na.check_kernels(DEV)
+
+
+# ---- graphs ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("which", ["norm", "attention", "tokens", "rotary"])
+def test_calls_in_a_graph(which):
+    """Captured once, replayed on other values: the cooperative launch and its cleared counts, fp16's norms, parts of caches."""
+    table = na.rotary_table(torch.arange(50, device=DEV), na.rotary_frequencies(32))
+    shapes, call = {
+        "norm": (((9, 128, 128, 128), (128,), (128,)), lambda x, w, b: na.group_norm(x, 8, w, b, activation="silu")),
+        "attention": (((2, 4, 150, 64), (2, 2, 700, 64), (2, 2, 700, 64)), lambda q, k, v: na.attention(q.half(), k.half(), v.half(), 0.125)),
+        "tokens": (((5, 8, 1, 64), (5, 4, 900, 64), (5, 4, 900, 64)),
+                   lambda q, k, v: na.attention(q.bfloat16(), k.bfloat16(), v.bfloat16(), 0.125, True, torch.arange(5, device=DEV) * 200)),
+        "rotary": (((2, 3, 50, 32), (2, 1, 50, 32)), lambda q, k: torch.cat(na.rotary(q, k, table), 1)),
+    }[which]
+    inputs = [torch.randn(s, device=DEV).requires_grad_() for s in shapes]
+
+    def step():
+        y = call(*inputs)
+        return [y, *torch.autograd.grad(y, inputs, torch.ones_like(y))] if which != "tokens" else [y]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.set_grad_enabled(which != "tokens"):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), torch.set_grad_enabled(which != "tokens"):
+        out = step()
+    for _ in range(3):
+        with torch.no_grad():
+            for t in inputs:
+                t.normal_()
+        graph.replay()
+        got = [t.detach().clone() for t in out]
+        with torch.set_grad_enabled(which != "tokens"):
+            same(got, [t.detach() for t in step()])
+    na.check_kernels(DEV)
+
+
+# ---- sizes of serving --------------------------------------------------------------------------------------------------------
+def check_tokens(B, N, Nk, Tq, Tk, C, dtype, lengths=None):
+    q, k, v = rand(B, N, Tq, C, dtype=dtype), rand(B, Nk, Tk, C, dtype=dtype, seed=1), rand(B, Nk, Tk, C, dtype=dtype, seed=2)
+    lengths = None if lengths is None else torch.tensor(lengths, device=DEV)
+    with torch.no_grad():
+        o, lse = na.attention_with_lse(q, k, v, C ** -0.5, True, lengths)
+    na.check_kernels(DEV)
+    want = plain_attention(q, k, v, q, C ** -0.5, True, lengths)
+    close(o, want[0], dtype, 1, "o")
+    seen = want[1] > -math.inf
+    assert torch.equal(lse == -math.inf, ~seen) and (lse.double() - want[1])[seen].abs().max() < 1e-4
+
+
+@pytest.mark.parametrize("dtype,C", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("B,N,Nk,Tq", [(37, 8, 8, 1), (36, 8, 8, 1), (20, 32, 16, 1), (37, 16, 8, 5), (38, 32, 8, 9)])
+def test_tokens_of_many_units(B, N, Nk, Tq, dtype, C):
+    """On both sides of the number of units from which they are items by themselves."""
+    check_tokens(B, N, Nk, Tq, 333, C, dtype, [333 * b // (B - 1) for b in range(B)])
+    check_tokens(B, N, Nk, Tq, 260, C, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("G", [6, 7, 8, 9, 16])
+def test_tokens_of_as_many_heads_as_three_stages_take(G, dtype):
+    check_tokens(2, 2 * G, 2, 1, 1500, 128, dtype, [1500, 700])
+
+
+@pytest.mark.parametrize("N,Nk,Tq,C", [(4, 2, 1, 64), (2, 2, 2, 128), (6, 1, 1, 40)])
+def test_tokens_in_32_bits_on_long_caches(N, Nk, Tq, C):
+    check_tokens(2, N, Nk, Tq, 20000, C, F32, [20000, 4097])
