@@ -164,15 +164,15 @@ int vector_of(const Rotary& r, int esize) {
 }
 
 template <typename T, int N>
-int launch_rotary(Rotary r, cudaStream_t st) {
+int launch_rotary(Rotary r, int sms, cudaStream_t st) {
     r.turned = r.interleaved && N > 1 ? (2 * r.half / N + 1) / 2 : r.half / N;
     r.items = r.turned + ((r.C - 2 * r.half) / N + 1) / 2;
     const long long threads = (long long)r.B * r.T * r.items;
     const long long blocks = (threads + kThreads - 1) / kThreads;
     if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
-    // heads of a thread: 8, fewer where that would leave SMs without a block
+    // heads of a thread: 8, fewer where that would leave SMs without four blocks
     const int heads = r.side[0].heads + r.side[1].heads;
-    r.step = (int)std::max(1LL, std::min(8LL, blocks * heads / (4 * 148)));
+    r.step = (int)std::max(1LL, std::min(8LL, blocks * heads / (4 * sms)));
     const long long parts = (heads + r.step - 1) / r.step;
     if (parts > 65535) return NA2D_ERR_TOO_LARGE;
     const cudaError_t e = na2d_launch::launch(true, rotary_kernel<T, N>, dim3((unsigned)blocks, (unsigned)parts), kThreads, 0, st, r);
@@ -182,10 +182,10 @@ int launch_rotary(Rotary r, cudaStream_t st) {
 }
 
 template <typename T>
-int by_vector(const Rotary& r, cudaStream_t st) {
+int by_vector(const Rotary& r, int sms, cudaStream_t st) {
     constexpr int kFull = 16 / (int)sizeof(T), kSmall = 4 / (int)sizeof(T);
     const int v = vector_of(r, sizeof(T));
-    return v == kFull ? launch_rotary<T, kFull>(r, st) : v == kSmall ? launch_rotary<T, kSmall>(r, st) : launch_rotary<T, 1>(r, st);
+    return v == kFull ? launch_rotary<T, kFull>(r, sms, st) : v == kSmall ? launch_rotary<T, kSmall>(r, sms, st) : launch_rotary<T, 1>(r, sms, st);
 }
 
 }  // namespace
@@ -219,7 +219,10 @@ int na2d_rotary(const na2d_rotary_args* a) {
     r.index = a->index;
     return na2d_host::on_device(a->device, [&]() -> int {
         const cudaStream_t st = (cudaStream_t)a->stream;
-        return a->dtype == NA2D_F32 ? by_vector<float>(r, st) : a->dtype == NA2D_BF16 ? by_vector<__nv_bfloat16>(r, st) : by_vector<__half>(r, st);
+        const int sms = na2d_host::sm_count(a->device);
+        return a->dtype == NA2D_F32    ? by_vector<float>(r, sms, st)
+               : a->dtype == NA2D_BF16 ? by_vector<__nv_bfloat16>(r, sms, st)
+                                       : by_vector<__half>(r, sms, st);
     });
 }
 
