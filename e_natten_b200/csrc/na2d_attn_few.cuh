@@ -249,7 +249,7 @@ int launch_few_as(const Place& at, const Geom& g, const FwdCut& cut, const Opera
     return launch_combine<DT>(at, g, cut, o, lse);
 }
 
-// (three stages of 16 keys a warp at head dim 128, two where the rows' sums take their room, from 7 rows on; twice, and four times as many
+// (three stages of 16 keys a warp at head dim 128, two where the rows' sums take their room, from 8 rows on; twice, and four times as many
 // of the narrower ones)
 template <typename DT, int D>
 int launch_few(const Place& at, const Geom& g, const FwdCut& cut, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse) {

@@ -6,11 +6,10 @@
 // of threads fall into different banks; neighbouring lanes are two rows of one column, because a warp's 16-byte loads are shared between
 // neighbours only (with 16 columns side by side each load took its full four turns: 1305 us against 1209).
 // What bounds it: the multiply-adds, and beside them the loads from shared memory.  Batch 4, 4 heads of 128, 1024 tokens, fp32, forward and
-// backward: 1130 us, 34 TFLOP/s over the nine products that are done (the seven that have to be: 406 us at the measured rate).
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
+// backward: 1130 us, 34 TFLOP/s over the nine products that are done (the seven that have to be: 406 us at the 74 TFLOP/s that 148 SMs of 128
+// multiply-adds come to at 1965 MHz).
 #include "na2d_attn_entry.h"
+#include "na2d_vec.cuh"
 
 namespace na2d_attn {
 
@@ -18,13 +17,8 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float widen(float x) { return x; }
-__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
-template <typename T> __device__ __forceinline__ T narrow(float x);
-template <> __device__ __forceinline__ float narrow<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
+using na2d_vec::narrow;
+using na2d_vec::widen;
 
 // BM rows of one side stay, tiles of BT of the other pass by.
 template <int CP, int BM>

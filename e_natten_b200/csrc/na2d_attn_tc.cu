@@ -29,7 +29,11 @@ int by_head_dim(int C, F&& f) {
     return f(std::integral_constant<int, 128>{});
 }
 
-// Whether the chunks of all units go on one line: units of one tile, fewer than the groups of the SMs (two a CTA).
+// Whether the chunks of all units go on one line: units of one tile, fewer than the groups of the SMs (two a CTA).  The line against units as
+// items, bf16, 128 channels, lengths from none to the largest: 16 x 4 caches of up to 32768 keys with 4 heads each 98 us for 683, with 40 rows
+// (16 x 4 of up to 8192) 65 for 176; 36 x 8 caches of up to 8192, one head each, 117 for 189.  With more units the 128-row kernel has items
+// enough (64 x 8 of up to 4096, 40 rows: 146 us, 204 on the line).  The kernel for few rows would win there, too, where caches are long
+// (32 x 16 of up to 8192: 188 for 273) and lose where they are short (64 x 8 of up to 512: 48 for 34): it has the bound of the other.
 bool on_line(const Geom& g, int sms) { return g.tiles == 1 && g.units < 2 * sms && g.B <= kLineEntries && g.Tk > kRows; }
 
 // Whether the kernel for few rows takes them.
@@ -43,7 +47,9 @@ int line_groups(const Geom& g, int sms) {
 }
 
 // Parts of the keys in the forward of units of several tiles: where the tiles are fewer than the groups, so many that each group has about
-// four, since where lengths differ many of them are empty; of at least 4 chunks each.
+// four, since where lengths differ many of them are empty; of at least 4 chunks each.  In parts and whole, bf16, 128 channels, 8 heads: 512
+// rows on 16384 keys 86 us for 266, 1024 rows 141 for 298; 4 heads x 2048, causal, 38 for 44.  Near the bound the whole tiles, one round of
+// nearly all SMs, would be faster: 2 x 8 heads x 2048 rows on 8192 keys 240 for 158, 8 heads x 4096, causal, 121 for 80.
 int forward_parts(const Geom& g, int sms) {
     const long long tiles = (long long)g.units * g.tiles;
     const int chunks = (g.Tk + kRows - 1) / kRows;
@@ -52,7 +58,9 @@ int forward_parts(const Geom& g, int sms) {
 }
 
 // CTAs that share the line of the key half's chunks, at least 4 chunks each; 0 where every tile is a CTA's item.  By items a CTA has a
-// whole number of tiles, and with lengths some of them are empty; the line costs its parts' way through memory, about 4 chunks' time.
+// whole number of tiles, and with lengths some of them are empty; the line costs its parts' way through memory.  Line and items, bf16,
+// backward of the key half: 4 x 4 heads x 4096 x 128 290 us for 309, 8 x 4 x 3136 x 4 rows on 333 keys of 64 161 for 205, with lengths 117
+// for 213; lengths of up to 1024 keys of 64, 8 x 16 heads: 2048 rows 176 for 191, 1024 rows 116 for 106, 512 rows 77 for 63 (not on the line).
 int key_line(const Geom& g, int sms) {
     const long long tiles = (long long)g.units * ((g.Tk + kRows - 1) / kRows), chunks = tiles * g.tiles;
     if (g.causal || g.B > kLineEntries || chunks + sms > 0x7fffffffLL) return 0;
@@ -60,7 +68,8 @@ int key_line(const Geom& g, int sms) {
     return pays ? (int)std::max(1LL, std::min<long long>(sms, chunks / 4)) : 0;
 }
 
-// The same for the query half, whose tiles are of rows and whose chunks of keys.
+// The same for the query half, whose tiles are of rows and whose chunks of keys: 4 x 4 heads x 4096 x 128 238 us for 275, 2 x 4 heads x 512 rows
+// on 8192 keys 51 for 123; where whole rounds of items do as well, 4 x 4 x 3136 x 8 rows on 333 keys of 64, 190 for 139 (not on the line).
 int row_line(const Geom& g, int sms) {
     const long long tiles = (long long)g.units * g.tiles, each = (g.Tk + kRows - 1) / kRows, chunks = tiles * each;
     if (g.causal || g.B > kLineEntries || chunks + sms > 0x7fffffffLL) return 0;
@@ -68,7 +77,9 @@ int row_line(const Geom& g, int sms) {
     return pays ? (int)std::max(1LL, std::min<long long>(sms, chunks / 4)) : 0;
 }
 
-// Parts of the queries in the key half of causal calls, where tiles are fewer than CTAs: a part costs its sums' way through memory.
+// Parts of the queries in the key half of causal calls, where tiles are fewer than CTAs: a part costs its sums' way through memory.  In parts
+// and whole, bf16, 128 channels: 2 x 4 heads on one key head x 4096 181 us for 270, 2 heads x 4096 71 for 77; 8 heads x 2048 79 for 52, which
+// whole tiles would do better; 8 heads x 4096, more tiles than CTAs, 111 whole for 146.
 int key_parts(const Geom& g, int sms) {
     const long long tiles = (long long)g.units * ((g.Tk + kRows - 1) / kRows);
     if (!g.causal || tiles >= sms) return 1;
