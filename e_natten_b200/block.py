@@ -1,7 +1,8 @@
 """What stands around neighborhood attention in a model: group normalisation of channels-last feature maps,
 rotary positions on queries and keys, and attention over all keys for the stages, and the conditioning, that want
 no window.  Differentiable, in float32, bfloat16 and float16, on the caller's stream; like the windowed operators
-they run in libna2d.so and have no CPU path.
+they run in libna2d.so and have no CPU path.  ``torch.jit.trace`` and dispatch modes record them as operators
+of ``torch.ops.e_natten_b200``.
 
 They take the windowed operators' layouts: ``(B, heads, T, C)`` or ``(B, heads, H, W, C)`` queries, keys and
 values, strided views of a packed projection among them, and ``(B, ..., C)`` feature maps.
@@ -40,7 +41,12 @@ def attention(q, k, v, scale=None, causal=False, key_lengths=None):
     single query is the newest token of a cache.  A row that sees no key gives zeros.
 
     A value of ``v`` (``k``, ``q`` or the gradient) that is not finite reaches rows that a causal mask hides it
-    from if they lie in the same tile of 128: it meets a weight of zero there.
+    from if they lie in the same tile of 128: it meets a weight of zero there.  Rows that see no key, and keys
+    beyond a length, get their zeros all the same.
+
+    Scores, weights and sums are float32.  For 16-bit types the weights are rounded to the type for their products
+    with ``v`` and with the gradient: ``o`` and the gradient of ``v`` are up to 1.4 times as far off as rounding
+    them once puts them.  Head dims go up to 256; ``scale`` is positive.
     """
     return torch_ext.attention(q, k, v, 1.0 if scale is None else scale, causal, key_lengths, _lib.PATH_AUTO)[0]
 
@@ -50,7 +56,9 @@ def group_norm(x, num_groups: int, weight=None, bias=None, eps: float = 1e-5, ac
     """Group normalisation of a channels-last map ``(B, ..., C)``, with ``activation`` (None or "silu") fused in.
 
     Every batch entry's groups of ``C / num_groups`` consecutive channels are normalised over all their positions.
-    ``weight`` and ``bias`` are ``(C,)``, in float32 or the map's dtype.  Statistics are taken in float32.
+    ``weight`` and ``bias`` are ``(C,)``, in float32 or the map's dtype.  Statistics are taken in float32.  Maps have
+    up to 65535 entries, 16384 channels and 2^29 positions; groups of more than 1024 channels (2048 in 16 bits, 256
+    of an odd number of channels) take a block each, however many positions there are.
     """
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be None or 'silu'; got {activation!r}")

@@ -4,8 +4,9 @@
 //     P^T = exp(S^T - lse),  dS^T = P^T (dP^T - delta)     (softmax warps)
 //     dV += P^T dO_c,  dK += dS^T Q_c                      (P^T, dS^T from tensor memory, 16 bit)
 // over the query chunks of every head that shares the key head, accumulated in tensor memory: no atomics, and the order of the sums is
-// the same in every call.  P is rounded once to 16 bits for its product; dS goes into its own as what it rounds to and the rest, as in the
-// query half, in fp16 times a power of two (ds_shift, one for all rows of a unit, since they are summed).
+// the same in every call.  P is rounded once to 16 bits for its product (dV is 1.4 times as far from 64 bits as its own rounding puts it, like
+// o); dS goes into its own as what it rounds to and the rest, as in the query half, in fp16 times a power of two (ds_shift, one for all
+// rows of a unit, since they are summed).
 //
 // Bound by the chain from a chunk's scores to its dS: the tensor pipe works about half of the time (8 heads x 16384 x 128, causal: 1340 us,
 // 820 TFLOP/s over four products; 4 x 4 heads x 4096 x 128: 284 us; 8 x 16 heads on 4 key heads, 3136 rows on up to 333 keys of 64: 102 us.
@@ -140,7 +141,8 @@ struct KeyCfg : TileCfg<D> {
     static constexpr int NST = D == 128 ? 2 : 4;                         // chunks of Q and dO
     static constexpr int NKV = D == 128 ? 1 : 2;                         // tiles of K and V: the next one's while this one's are read
     static constexpr int OUT_BYTES = 4 * 2 * OutStage<32>::BYTES;
-    static constexpr int X_BYTES = NST * 2 * kRows * 4 + NST * 8;        // [ring slot]{-lse * log2(e), -delta}[row]; [ring slot] what dP is scaled by, twice
+    // [ring slot]{-lse * log2(e), -delta}[row]; [ring slot] what dP is scaled by, twice
+    static constexpr int X_BYTES = NST * 2 * kRows * 4 + NST * 8;
     static constexpr int SMEM = 2 * NKV * T::BYTES + 2 * NST * T::BYTES + OUT_BYTES + X_BYTES + 512 /*barriers*/ + 1024 /*alignment*/;
     static constexpr int TMEM_S = 0, TMEM_DP = 128, TMEM_DV = 256, TMEM_DK = 384;
     static_assert(SMEM <= kSmemLimit, "dK/dV kernel shared memory");
@@ -629,8 +631,8 @@ int launch_dkdv(const Place& at, const Geom& g, const KeyCut& cut, const Operand
     if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted[cut.line > 0]) != cudaSuccess) return NA2D_ERR_CUDA;
     const int sms = na2d_tc::sm_count(at.device);
     *at.launched += 1;
-    if (na2d_launch::launch(true, kern, cut.line ? cut.line : cut.items < sms ? cut.items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdk, tdv, lse, delta, bounds,
-                            at.errors, g, cut) != cudaSuccess)
+    if (na2d_launch::launch(true, kern, cut.line ? cut.line : cut.items < sms ? cut.items : sms, 512, C::SMEM, at.st, tq, tg, tk, tv, tdk, tdv,
+                            lse, delta, bounds, at.errors, g, cut) != cudaSuccess)
         return NA2D_ERR_CUDA;
     if (cut.line) {
         *at.launched += 1;

@@ -26,8 +26,9 @@
 
 namespace na2d_attn {
 
-// delta = dO . o of each row, 8 channels a lane; fp16: the norms of dO and, by the blocks behind row_blocks, of V, too.  LPR lanes a row: C / 8, rounded up to a power of two.  A lane has kDeltaRows rows of one
-// head, 256 / LPR apart, all under way at once (8 x 16 heads x 3136 x 64: 16.5 us, 6.2 TB/s; with one row a lane 24).
+// delta = dO . o of each row, 8 channels a lane; fp16: the norms of dO and, by the blocks behind row_blocks, of V, too.  LPR lanes a row:
+// C / 8, rounded up to a power of two.  A lane has kDeltaRows rows of one head, 256 / LPR apart, all under way at once (8 x 16 heads x 3136 x
+// 64: 16.5 us, 6.2 TB/s, with the norms 19; with one row a lane 24).
 constexpr int kDeltaRows = 4;
 template <typename DT, int LPR>
 __global__ void __launch_bounds__(256)

@@ -4,7 +4,7 @@
 // and how short the chain from a key to its weight is.  On tcgen05 a tile has 128 rows and its scores go through tensor memory: 5000
 // cycles a chunk for a group, two groups an SM, 60 % of the bandwidth (16 x 4 caches of up to 32768 keys of 128, 16 heads: 137 us).  Here
 // a warp takes 16 keys at a time by itself: mma.sync of 16 x 8 x 16 on registers, the scores' own registers being the next product's
-// operand, its keys and values in stages of shared memory that no other warp touches.
+// operand (rounded once to 16 bits, as in na2d_attn_fwd.cuh), its keys and values in stages of shared memory that no other warp touches.
 //
 // Measured: 16 x 16 heads on 4 key heads, caches of up to 32768 keys of 128, bf16: 95 us with the joining of the parts, 87 % of the copy
 // bandwidth over the caches' bytes.

@@ -10,6 +10,10 @@
 // units' chunks lie on one line, of which every group takes the same length, wherever units begin and end; with parts of a unit for
 // items, caches of different lengths left some CTAs 1.4 times the mean's work (16 x 4 caches of up to 32768 keys: 141 us).
 //
+// P goes into its product rounded once to 16 bits, as tensor memory and the pipe take it: o is 1.3 to 1.4 times as far from its 64-bit value as
+// its own rounding puts it (bf16 2.3e-3 for 1.7e-3, fp16 2.9e-4 for 2.1e-4), the two roundings' sum of squares.  A second number, as the
+// backward's dS has, would be a third product to these two.  Sums and maxima are of the weights in 32 bits.
+//
 // Bound by the chain S - maximum - exponentials - P V of a group, of which the other group's covers all but about 700 of 3700 cycles a pair of
 // chunks; the special-function unit is at 60 % (a polynomial for a quarter of the exponentials: 179 us for 155).  8 heads x 16384 x 128,
 // causal, bf16: 620-643 us, 870 TFLOP/s; 4 x 4 heads x 4096 x 128: 156 us.

@@ -926,6 +926,8 @@ __global__ void __launch_bounds__(2 * kHalf, 1) norm_bwd_kernel(const Norm n, co
 }
 
 // ---- groups wider than a block of vectors: a block a group, a thread a channel at a time ---------------------------------
+// (Made for odd widths on small maps: 1 x 64^2 x 1542 in 3 groups, bf16, 3.1 + 3.2 ms.  4 x 64^2 x 4096 in one group takes 43 + 48 ms on 4 of
+// the SMs.)
 // A sum of any number of values, with what its roundings lost (a thread has all pixels of its channels, hundreds of thousands of values:
 // without, the variance of 2^20 came out 5e-4 too small).
 struct LongSum {

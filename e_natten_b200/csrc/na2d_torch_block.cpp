@@ -102,12 +102,12 @@ c10::TypedOperatorHandle<F> operator_of(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
 }
 using AttentionForward = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const MaybeTensor&, double, bool, int64_t);
-using AttentionBackward = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const MaybeTensor&,
-                                              double, bool, int64_t, bool, bool);
+using AttentionBackward = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                              const MaybeTensor&, double, bool, int64_t, bool, bool);
 using Norm = Tensor(const Tensor&, const MaybeTensor&, const MaybeTensor&, int64_t, double, int64_t);
 using NormForward = std::tuple<Tensor, Tensor>(const Tensor&, const MaybeTensor&, const MaybeTensor&, int64_t, double, int64_t);
-using NormBackward = std::vector<Tensor>(const Tensor&, const MaybeTensor&, const MaybeTensor&, const Tensor&, const Tensor&, int64_t, double, int64_t, bool,
-                                         bool, bool);
+using NormBackward = std::vector<Tensor>(const Tensor&, const MaybeTensor&, const MaybeTensor&, const Tensor&, const Tensor&, int64_t, double,
+                                         int64_t, bool, bool, bool);
 using Turn = std::vector<Tensor>(const Tensor&, const MaybeTensor&, const Tensor&, const MaybeTensor&, bool, bool);
 using Table = Tensor(const Tensor&, const Tensor&, double);
 

@@ -297,6 +297,7 @@ typedef struct na2d_heads {
  *   A row that sees no key has o = 0, lse = -infinity and no gradient.
  *   path         AUTO: tensor cores for 16-bit types with C <= 128 a multiple of 8 and operands on 16-byte boundaries, else
  *                CUDA cores (C <= 256, any strides).  SIMT and TENSOR ask for one of them.
+ *   Tq, Tk <= 2^29, B * N <= 2^24, else NA2D_ERR_TOO_LARGE.
  *   o, d_q, d_k, d_v dense.  lse, delta: fp32 (B, N, Tq), dense; delta is scratch of the backward.
  *   d_q, or d_k and d_v together, may be NULL: that half is left out.  No atomics: the same call gives the same bits.
  *   workspace    scratch, 16-byte aligned, of na2d_attention_workspace bytes: where the tiles of rows, or of keys, do not share out evenly
@@ -329,6 +330,7 @@ size_t na2d_attention_workspace(const na2d_attention_args* a, int backward);
  *   activation   NA2D_ACT_NONE or NA2D_ACT_SILU (z * sigmoid(z)).
  *   mean, rstd   fp32 (B, groups): written by the forward, read by the backward.
  *   workspace    scratch, 16-byte aligned, at least na2d_group_norm_workspace bytes.
+ *   B <= 65535, C <= 16384, P <= 2^29, else NA2D_ERR_TOO_LARGE.
  * Statistics and sums are in fp32, variances about the mean; no atomics. */
 typedef enum na2d_activation {
     NA2D_ACT_NONE = 0,
