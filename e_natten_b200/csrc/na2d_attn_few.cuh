@@ -178,7 +178,7 @@ attn_few_kernel(const Operand q, const Operand k, const Operand v, const Geom g,
             uint32_t p[4];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const float base = top[half] == -CUDART_INF_F ? 0.f : top[half];
+                const float base = (top[half] == -CUDART_INF_F ? 0.f : top[half]) - kLift<DT>;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const float p0 = fast_exp2(s[j][2 * half] - base), p1 = fast_exp2(s[j][2 * half + 1] - base);
@@ -231,7 +231,7 @@ attn_few_kernel(const Operand q, const Operand k, const Operand v, const Geom g,
             }
             const float inv = all == 0.f ? 0.f : 1.f / all;
             if (c < g.C) *reinterpret_cast<float4*>(cut.part_o + (part + r) * g.C + c) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-            if (c == 0) cut.part_lse[part + r] = all == 0.f ? -CUDART_INF_F : (base + log2f(all)) * kLn2;
+            if (c == 0) cut.part_lse[part + r] = all == 0.f ? -CUDART_INF_F : (base - kLift<DT> + log2f(all)) * kLn2;
         }
         __syncthreads();
         here.next(g, before);

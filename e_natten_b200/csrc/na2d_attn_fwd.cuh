@@ -212,6 +212,9 @@ struct FwdCfg : TileCfg<D> {
 // Logarithm (base 2) by which a row's maximum may grow before its sums are rescaled: the weights stay below 2^8, within fp16 by far,
 // and most chunks after the first rescale nothing.
 constexpr float kGrow = 8.f;
+// Weights go into their sums and products times 2^kLift: fp16 ends at 2^-24, and 2^17 keys whose weights rounded to nothing, or to twice what they
+// are, beside one of large weight were a result off by hundredths.  kGrow + kLift stays within its 2^16.
+template <typename DT> constexpr float kLift = IsBf16<DT>::value ? 0.f : 7.f;
 
 // What rounding a pair to `w` left of it, rounded itself: the two together have 16 (22) bits.
 template <typename DT>
@@ -646,7 +649,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     run_sum *= alpha;
                 }
                 if (grow) run_max = cmax;
-                const float safe_max = run_max == -CUDART_INF_F ? 0.f : run_max;
+                const float safe_max = (run_max == -CUDART_INF_F ? 0.f : run_max) - kLift<DT>;
                 if ((tid & 127) == 0) NA2D_TR(group ? 0 : 3, 2, m);
                 bar_sync(my_turn, 256);
                 if ((tid & 127) == 0) NA2D_TR(group ? 0 : 3, 3, m);

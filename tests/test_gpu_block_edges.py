@@ -415,3 +415,25 @@ def test_tokens_of_as_many_heads_as_three_stages_take(G, dtype):
 @pytest.mark.parametrize("N,Nk,Tq,C", [(4, 2, 1, 64), (2, 2, 2, 128), (6, 1, 1, 40)])
 def test_tokens_in_32_bits_on_long_caches(N, Nk, Tq, C):
     check_tokens(2, N, Nk, Tq, 20000, C, F32, [20000, 4097])
+
+
+# ---- fp16 weights far below the largest ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("below", [22.0, 24.5, 26.0])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("N,Tq,Tk,C", [(1, 1, 131072, 64), (2, 3, 65536, 128), (1, 40, 65536, 64), (1, 300, 32768, 128)])
+def test_many_keys_of_small_weight_beside_one_of_large(N, Tq, Tk, C, dtype, below):
+    """One key has nearly all weight and a value of zero; the others, 2^-below of it each, and a spread about that, make up the
+    result.  Rounding them is unbiased as long as they are numbers of the type: one rounding's bound."""
+    q, k = rand(1, N, Tq, C, dtype=dtype), rand(1, 1, Tk, C, dtype=dtype, seed=1, scale=0.3)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[:, :, 0] = 0.0
+    k[:, :, 0, 0] = 16.0
+    scale = below * math.log(2.0) / 128
+    v = rand(1, 1, Tk, C, dtype=dtype, seed=2, scale=300.0, shift=1000.0)
+    v[:, :, 0] = 0.0
+    with torch.no_grad():
+        o, lse = na.attention_with_lse(q, k, v, scale)
+    na.check_kernels(DEV)
+    want = plain_attention(q, k, v, q, scale, False, None)
+    close(o, want[0], dtype, 1, "o")
+    assert (lse.double() - want[1]).abs().max() < 1e-4
