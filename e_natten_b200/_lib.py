@@ -81,6 +81,36 @@ class RotaryArgs(C.Structure):
                 ("table", C.c_void_p), ("table_rows", C.c_int64), ("index", C.c_void_p)]
 
 
+class PrefixAttentionArgs(C.Structure):
+    """Mirror of ``na2d_prefix_attention_args``."""
+    _fields_ = [("struct_size", C.c_size_t),
+                *[(n, C.c_int) for n in ("B", "S", "N", "Nk", "Tq", "Tk", "P", "C", "dtype", "path", "device", "causal")],
+                ("scale", C.c_float), ("stream", C.c_void_p),
+                *[(n, Heads) for n in ("q", "k", "v", "prefix_k", "prefix_v", "o", "d_o", "d_q", "d_k", "d_v", "d_prefix_k", "d_prefix_v")],
+                ("key_lengths", C.c_void_p), ("prefix_lengths", C.c_void_p), ("lse", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class BeamSelectArgs(C.Structure):
+    """Mirror of ``na2d_beam_select_args``."""
+    _fields_ = [("struct_size", C.c_size_t), *[(n, C.c_int) for n in ("B", "K", "V", "count", "dtype", "device")],
+                ("end", C.c_int64), ("stream", C.c_void_p), ("logits", C.c_void_p), ("stride_b", C.c_int64), ("stride_k", C.c_int64),
+                *[(n, C.c_void_p) for n in ("scores", "finished", "out_scores", "out_parents", "out_words", "workspace")],
+                ("workspace_bytes", C.c_size_t)]
+
+
+class Cache(C.Structure):
+    """Mirror of ``na2d_cache``."""
+    _fields_ = [("ptr", C.c_void_p), ("stride_e", C.c_int64), ("stride_h", C.c_int64), ("stride_t", C.c_int64),
+                ("heads", C.c_int), ("tokens", C.c_int), ("row_bytes", C.c_int64)]
+
+
+class BeamReorderArgs(C.Structure):
+    """Mirror of ``na2d_beam_reorder_args``."""
+    _fields_ = [("struct_size", C.c_size_t), *[(n, C.c_int) for n in ("B", "K", "caches", "parents_64", "lengths_64", "device")],
+                ("stream", C.c_void_p), ("cache", C.POINTER(Cache)), ("parents", C.c_void_p), ("lengths", C.c_void_p)]
+
+
 OP_2D, OP_1D = 0, 1
 FLAG_DKDV_F32 = 1
 
@@ -123,6 +153,12 @@ SIGNATURES = {
     "na2d_group_norm_workspace": (C.c_size_t, [C.POINTER(NormArgs), C.c_int]),
     "na2d_rotary": (C.c_int, [C.POINTER(RotaryArgs)]),
     "na2d_rotary_table": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_double, C.c_void_p, C.c_int, C.c_void_p]),
+    "na2d_prefix_attention_forward": (C.c_int, [C.POINTER(PrefixAttentionArgs)]),
+    "na2d_prefix_attention_backward": (C.c_int, [C.POINTER(PrefixAttentionArgs)]),
+    "na2d_prefix_attention_workspace": (C.c_size_t, [C.POINTER(PrefixAttentionArgs), C.c_int]),
+    "na2d_beam_select": (C.c_int, [C.POINTER(BeamSelectArgs)]),
+    "na2d_beam_select_workspace": (C.c_size_t, [C.POINTER(BeamSelectArgs)]),
+    "na2d_beam_reorder": (C.c_int, [C.POINTER(BeamReorderArgs)]),
     "na2d_check": (C.c_int, [C.c_int, C.c_void_p]),
     "na2d_poll": (C.c_int, [C.c_int, C.c_void_p]),
     "na2d_selftest_wait_timeout": (C.c_int, [C.c_int, C.c_void_p, C.c_uint]),
@@ -158,6 +194,9 @@ def _load_torch_ext():
     _na2d_torch.bind_block_abi(*(C.cast(fn, C.c_void_p).value for fn in (
         lib.na2d_attention_forward, lib.na2d_attention_backward, lib.na2d_attention_workspace, lib.na2d_group_norm_forward,
         lib.na2d_group_norm_backward, lib.na2d_group_norm_workspace, lib.na2d_rotary, lib.na2d_rotary_table, lib.na2d_poll)))
+    _na2d_torch.bind_answers_abi(*(C.cast(fn, C.c_void_p).value for fn in (
+        lib.na2d_prefix_attention_forward, lib.na2d_prefix_attention_backward, lib.na2d_prefix_attention_workspace, lib.na2d_beam_select,
+        lib.na2d_beam_select_workspace, lib.na2d_beam_reorder, lib.na2d_poll)))
     return _na2d_torch
 
 

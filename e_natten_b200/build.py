@@ -3,10 +3,10 @@
     python e_natten_b200/build.py [--force] [--verbose]
 
 The library is plain CUDA C++ behind a C ABI (include/na2d.h); it needs no framework headers.
-Its kernels are compiled as seventeen translation units in parallel (the API with the SIMT kernels, the
+Its kernels are compiled as nineteen translation units in parallel (the API with the SIMT kernels, the
 tiled CUDA-core kernels once per element type, the fp32 box kernels, each of the three tcgen05 kernel families once per
-16-bit element type, attention over all keys on tensor cores once per 16-bit type, on CUDA cores and its entry points, group norm and
-rotary positions) and linked into one shared object.  The Python package's extension module
+16-bit element type, attention over all keys on tensor cores once per 16-bit type, on CUDA cores and its entry points, group norm,
+rotary positions, attention over shared prefixes and beam search) and linked into one shared object.  The Python package's extension module
 (_na2d_torch.so, host code over PyTorch's C++ API) is compiled beside it with g++; it belongs to one
 PyTorch and one Python version and is compiled again when either changes.
 """
@@ -44,6 +44,8 @@ UNITS = [
     ("na2d_attn_api.cu", [], "na2d_attn_api.o"),
     ("na2d_norm.cu", [], "na2d_norm.o"),
     ("na2d_rotary.cu", [], "na2d_rotary.o"),
+    ("na2d_prefix.cu", [], "na2d_prefix.o"),
+    ("na2d_beam.cu", [], "na2d_beam.o"),
 ]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 
@@ -55,8 +57,8 @@ def _nvcc() -> str:
     return exe
 
 
-EXT_SOURCES = ("na2d_torch.cpp", "na2d_torch_block.cpp")
-EXT_HEADERS = ("na2d_torch.h",)
+EXT_SOURCES = ("na2d_torch.cpp", "na2d_torch_block.cpp", "na2d_torch_answers.cpp")
+EXT_HEADERS = ("na2d_torch.h", "na2d_torch_call.h")
 
 
 def _deps(ext: bool):

@@ -162,6 +162,7 @@ struct Place {
 struct Operand {
     void* ptr;
     long long b, n, t;
+    bool wide = false;      // a result in fp32, dense, whatever the operands' type: a sum that others join
 };
 
 // Tensor map with coordinates (channel, token, head, batch, 0) and boxes of box_t tokens of box_n heads.

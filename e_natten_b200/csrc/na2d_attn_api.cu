@@ -15,14 +15,6 @@ struct Problem {
     Operand q, k, v, o, d_o, d_q, d_k, d_v;
 };
 
-// What a tensor map needs of an operand: a base and strides on 16-byte boundaries, strides below 2^40 bytes.
-bool tma_ready(const Operand& x) {
-    if (reinterpret_cast<uintptr_t>(x.ptr) & 15u) return false;
-    for (long long s : {x.b, x.n, x.t})
-        if (s <= 0 || (s & 7) != 0 || s >= (1ll << 39)) return false;
-    return true;
-}
-
 int make_problem(const na2d_attention_args* a, Problem* p) {
     if (!a || a->struct_size < sizeof(na2d_attention_args)) return NA2D_ERR_BAD_ARG;
     if (a->B <= 0 || a->N <= 0 || a->Nk <= 0 || a->Tq <= 0 || a->Tk <= 0 || a->C <= 0 || a->N % a->Nk != 0) return NA2D_ERR_BAD_ARG;
@@ -60,7 +52,7 @@ int make_problem(const na2d_attention_args* a, Problem* p) {
             if (got.b != d.b || got.n != d.n || got.t != d.t) return NA2D_ERR_UNSUPPORTED;
         }
     bool fits = a->dtype != NA2D_F32 && a->C <= 128 && a->C % 8 == 0;
-    for (const Operand* x : {&p->q, &p->k, &p->v, &p->o, &p->d_o, &p->d_q, &p->d_k, &p->d_v}) fits = fits && (!x->ptr || tma_ready(*x));
+    for (const Operand* x : {&p->q, &p->k, &p->v, &p->o, &p->d_o, &p->d_q, &p->d_k, &p->d_v}) fits = fits && (!x->ptr || na2d_attn::tma_ready(*x));
     if (a->path == NA2D_PATH_TENSOR && !fits) return NA2D_ERR_UNSUPPORTED;
     p->tensor = fits && a->path != NA2D_PATH_SIMT;
     if (!p->tensor && a->C > na2d_attn::kSimtMaxC) return NA2D_ERR_UNSUPPORTED;

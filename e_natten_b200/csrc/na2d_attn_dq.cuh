@@ -105,6 +105,7 @@ struct RowCut {
     int items;              // tiles
     int line;               // the chunks of all tiles on one line, that many CTAs take; 0: an item is a tile
     float* part;            // line: (2 a CTA, rows of a tile, C)
+    float* sums;            // dQ in fp32, (B, N, Tq, C); null: in the operands' type
 };
 
 // One item: chunks [c0, c0 + n) of a tile of rows.
@@ -446,6 +447,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                         if (ok && 32 * j + 4 * e < g.C)
                             dst[e] = make_float4(__uint_as_float(v[4 * e]) * scale, __uint_as_float(v[4 * e + 1]) * scale,
                                                  __uint_as_float(v[4 * e + 2]) * scale, __uint_as_float(v[4 * e + 3]) * scale);
+                } else if (cut.sums) {
+                    float4* dst = reinterpret_cast<float4*>(cut.sums + row_index(g, tile.b, n, t) * g.C + 32 * j);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (ok && 32 * j + 4 * e < g.C)
+                            dst[e] = make_float4(__uint_as_float(v[4 * e]) * scale, __uint_as_float(v[4 * e + 1]) * scale,
+                                                 __uint_as_float(v[4 * e + 2]) * scale, __uint_as_float(v[4 * e + 3]) * scale);
                 } else if (g.hp == 1) {
                     if (t_first < g.Tq)
                         na2d_tc::stage_and_store<DT, 32, 2>(&tm_dq, stage, v, scale, 32 * j, t_first, tile.h0, tile.b, 0, lane, &seq);
@@ -597,9 +605,9 @@ int launch_delta(const Place& at, const Geom& g, const Operand& d_o, const Opera
 // Line: a block joins the parts of an eighth of one tile of rows, or writes zeros where the batch entry has no keys.  (A block a tile
 // read sixteen times one after the other: 24 us for 19 MB.)
 constexpr int kJoinBlocks = 8, kJoinRows = kRows / kJoinBlocks;
-template <typename DT>
+template <typename OT>
 __global__ void __launch_bounds__(256)
-attn_join_rows_kernel(const float* __restrict__ part, DT* __restrict__ dq, const Operand st, const Geom g, const RowCut cut) {
+attn_join_rows_kernel(const float* __restrict__ part, OT* __restrict__ dq, const Operand st, const Geom g, const RowCut cut) {
     after_previous_grid();
     next_grid_may_start();
     int which, m, before = 0, all = 0;                   // chunks of a tile of the entries before b, and of all
@@ -635,7 +643,7 @@ attn_join_rows_kernel(const float* __restrict__ part, DT* __restrict__ dq, const
                 acc.w += v.w;
             }
         }
-        *reinterpret_cast<uint2*>(dq + tile.b * st.b + n * st.n + t * st.t + c) = make_uint2(pack2<DT>(acc.x, acc.y), pack2<DT>(acc.z, acc.w));
+        store_4(dq + tile.b * st.b + n * st.n + t * st.t + c, acc);
     }
 }
 
@@ -648,7 +656,7 @@ int launch_dq(const Place& at, const Geom& g, RowCut cut, const Operand& q, cons
     if (rc == NA2D_OK) rc = operand_map(&tg, d_o, at.dtype, g.B, g.N, g.Tq, g.C, g.tt, g.hp, C::SLAB_C);
     if (rc == NA2D_OK) rc = operand_map(&tk, k, at.dtype, g.B, g.Nk, g.Tk, g.C, kRows, 1, C::SLAB_C);
     if (rc == NA2D_OK) rc = operand_map(&tv, v, at.dtype, g.B, g.Nk, g.Tk, g.C, kRows, 1, C::SLAB_C);
-    if (rc == NA2D_OK) rc = operand_map(&tdq, d_q, at.dtype, g.B, g.N, g.Tq, g.C, 32, 1, 32);
+    if (rc == NA2D_OK) rc = operand_map(&tdq, d_q.wide ? q : d_q, at.dtype, g.B, g.N, g.Tq, g.C, 32, 1, 32);
     if (rc != NA2D_OK) return rc;
     const long long items = (long long)g.units * g.tiles;
     if (items > 0x3fffffffLL) return NA2D_ERR_TOO_LARGE;
@@ -663,10 +671,12 @@ int launch_dq(const Place& at, const Geom& g, RowCut cut, const Operand& q, cons
         return NA2D_ERR_CUDA;
     if (!cut.line) return NA2D_OK;
     *at.launched += 1;
-    return na2d_launch::launch(true, attn_join_rows_kernel<DT>, dim3((unsigned)items, kJoinBlocks), 256, 0, at.st, (const float*)cut.part, (DT*)d_q.ptr, d_q, g,
-                               cut) == cudaSuccess
-               ? NA2D_OK
-               : NA2D_ERR_CUDA;
+    const dim3 grid((unsigned)items, kJoinBlocks);
+    const cudaError_t e = d_q.wide ? na2d_launch::launch(true, attn_join_rows_kernel<float>, grid, 256, 0, at.st, (const float*)cut.part,
+                                                         (float*)d_q.ptr, d_q, g, cut)
+                                   : na2d_launch::launch(true, attn_join_rows_kernel<DT>, grid, 256, 0, at.st, (const float*)cut.part, (DT*)d_q.ptr,
+                                                         d_q, g, cut);
+    return e == cudaSuccess ? NA2D_OK : NA2D_ERR_CUDA;
 }
 
 }  // namespace na2d_attn

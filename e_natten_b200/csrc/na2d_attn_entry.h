@@ -15,7 +15,16 @@ struct Scratch {
 size_t forward_floats(const Geom& g, int sms);
 size_t backward_floats(const Geom& g, int sms, bool f16, bool d_q, bool d_k);
 
-// 16 bits, C a multiple of 8 up to 128, every operand on 16-byte boundaries; o, d_q, d_k and d_v dense.
+// What a tensor map needs of an operand: a base and strides on 16-byte boundaries, strides below 2^40 bytes.
+inline bool tma_ready(const Operand& x) {
+    if (reinterpret_cast<uintptr_t>(x.ptr) & 15u) return false;
+    for (long long s : {x.b, x.n, x.t})
+        if (s <= 0 || (s & 7) != 0 || s >= (1ll << 39)) return false;
+    return true;
+}
+
+// 16 bits, C a multiple of 8 up to 128, every operand on 16-byte boundaries; o, d_q, d_k and d_v dense.  o and d_q may be `wide`; of a wide o only
+// rows with a finite lse are written, where rows are not in parts.
 int forward_bf16(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);
 int forward_f16(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);
 

@@ -53,8 +53,9 @@ struct FwdCut {
     int items;
     int each;               // chunks of a part
     int line;               // not PAIR: the chunks of all units on one line, that many groups take; 0: not
+    int keep;               // the whole rows, too, as parts: o in fp32, of rows that see a key
     Div by_splits, by_pairs;
-    float* part_o;          // (splits, B, N, Tq, C), where splits > 1; line: (groups + units, rows of a unit, C)
+    float* part_o;          // (splits, B, N, Tq, C), where splits > 1 or keep; line: (groups + units, rows of a unit, C)
     float* part_lse;        // (splits, B, N, Tq); line: (groups + units, rows of a unit)
 };
 
@@ -488,7 +489,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const int row = quarter * 32 + lane;                 // row of the tile = tensor-memory lane
         const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         uint8_t* stage = sOut + quarter * 2 * OutStage<32>::BYTES;
-        const bool in_parts = cut.splits > 1 || cut.line, by_tma = g.hp == 1 && !in_parts;
+        const bool in_parts = cut.splits > 1 || cut.line || cut.keep, by_tma = g.hp == 1 && !in_parts;
         const size_t part_rows = cut.line ? (size_t)g.G * g.Tq : static_cast<size_t>(g.B) * g.N * g.Tq;     // of the workspace
         uint32_t it[2] = {0, 0}, seq = 0;
         for (FwdWalk<PAIR> walk(g, cut, before); walk.more(cut); walk.next(g, cut, before)) {
@@ -701,11 +702,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     }
 }
 
+// 4 channels of a result.
+template <typename OT>
+__device__ __forceinline__ void store_4(OT* to, const float4& x) {
+    if constexpr (sizeof(OT) == 4) *reinterpret_cast<float4*>(to) = x;
+    else *reinterpret_cast<uint2*>(to) = make_uint2(pack2<OT>(x.x, x.y), pack2<OT>(x.z, x.w));
+}
+
 // Joins the parts of a row: lse = ln sum_s e^lse_s, o = sum_s e^(lse_s - lse) o_s.  A block a row: its four warps share the parts, 4 channels
 // a lane.
-template <typename DT>
+template <typename OT>
 __global__ void __launch_bounds__(128)
-attn_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse, DT* __restrict__ o, const Operand o_st,
+attn_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse, OT* __restrict__ o, const Operand o_st,
                     float* __restrict__ lse, const Geom g, const int splits, const int line_groups) {
     __shared__ float4 sums[3][32];
     after_previous_grid();
@@ -770,19 +778,22 @@ attn_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ 
         acc.z += sums[w][lane].z;
         acc.w += sums[w][lane].w;
     }
-    DT* dst = o + b * o_st.b + n * o_st.n + t * o_st.t;
-    *reinterpret_cast<uint2*>(dst + c) = make_uint2(pack2<DT>(acc.x, acc.y), pack2<DT>(acc.z, acc.w));
+    store_4(o + b * o_st.b + n * o_st.n + t * o_st.t + c, acc);
     if (lane == 0) lse[row] = total == 0.f ? -CUDART_INF_F : base + logf(total);
 }
 
-template <typename DT>
-int launch_combine(const Place& at, const Geom& g, const FwdCut& cut, const Operand& o, float* lse) {
+template <typename OT>
+int launch_combine_as(const Place& at, const Geom& g, const FwdCut& cut, const Operand& o, float* lse) {
     const long long rows = (long long)g.B * g.N * g.Tq;
     *at.launched += 1;
-    return na2d_launch::launch(true, attn_combine_kernel<DT>, (unsigned)rows, 128, 0, at.st, (const float*)cut.part_o,
-                               (const float*)cut.part_lse, (DT*)o.ptr, o, lse, g, cut.splits, cut.line) == cudaSuccess
+    return na2d_launch::launch(true, attn_combine_kernel<OT>, (unsigned)rows, 128, 0, at.st, (const float*)cut.part_o,
+                               (const float*)cut.part_lse, (OT*)o.ptr, o, lse, g, cut.splits, cut.line) == cudaSuccess
                ? NA2D_OK
                : NA2D_ERR_CUDA;
+}
+template <typename DT>
+int launch_combine(const Place& at, const Geom& g, const FwdCut& cut, const Operand& o, float* lse) {
+    return o.wide ? launch_combine_as<float>(at, g, cut, o, lse) : launch_combine_as<DT>(at, g, cut, o, lse);
 }
 
 template <typename DT, int D, bool PAIR>
@@ -793,7 +804,7 @@ int launch_fwd_as(const Place& at, const Geom& g, const FwdCut& cut, const Opera
     int rc = operand_map(&tq, q, at.dtype, g.B, g.N, g.Tq, g.C, g.tt, g.hp, C::SLAB_C);
     if (rc == NA2D_OK) rc = operand_map(&tk, k, at.dtype, g.B, g.Nk, g.Tk, g.C, kRows, 1, C::SLAB_C);
     if (rc == NA2D_OK) rc = operand_map(&tv, v, at.dtype, g.B, g.Nk, g.Tk, g.C, kRows, 1, C::SLAB_C);
-    if (rc == NA2D_OK) rc = operand_map(&to, o, at.dtype, g.B, g.N, g.Tq, g.C, 32, 1, 32);
+    if (rc == NA2D_OK) rc = operand_map(&to, o.wide ? q : o, at.dtype, g.B, g.N, g.Tq, g.C, 32, 1, 32);      // (parts do not go by it)
     if (rc != NA2D_OK) return rc;
     auto kern = attn_fwd_kernel<DT, D, PAIR>;
     static std::atomic<unsigned long long> opted{0};

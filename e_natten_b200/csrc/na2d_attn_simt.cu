@@ -155,8 +155,8 @@ struct Sums {
 };
 
 // (a scale of 0: a row that sees nothing, or a key that is none, whose products may be 0 times infinity)
-template <typename DT, int CP, int BM>
-__device__ __forceinline__ void store_rows(DT* dst, long long stride, int row0, int rows, int C,
+template <typename OT, int CP, int BM>
+__device__ __forceinline__ void store_rows(OT* dst, long long stride, int row0, int rows, int C,
                                            const Sums<CP, BM>& acc, const float (&scale)[BM / 16], int tx, int ty) {
     using S = SimtCfg<CP, BM>;
 #pragma unroll
@@ -169,7 +169,7 @@ __device__ __forceinline__ void store_rows(DT* dst, long long stride, int row0, 
             for (int e = 0; e < 2; ++e) {
                 const int c = out_col<CP>(tx, k) + e;
                 const float x = (e ? na2d_ptx::hi2(acc.at[i][k]) : na2d_ptx::lo2(acc.at[i][k])) * scale[i];
-                if (c < C) dst[r * stride + c] = narrow<DT>(scale[i] == 0.f ? 0.f : x);
+                if (c < C) dst[r * stride + c] = narrow<OT>(scale[i] == 0.f ? 0.f : x);
             }
     }
 }
@@ -190,7 +190,7 @@ template <typename DT>
 __device__ __forceinline__ DT* rows_of(const Operand& x, int b, int n) { return static_cast<DT*>(x.ptr) + b * x.b + n * x.n; }
 
 // ---- forward: a block has BT queries of one head ------------------------------------------------------------------
-template <typename DT, int CP, int BM>
+template <typename DT, typename OT, int CP, int BM>
 __global__ void __launch_bounds__(kThreads)
 simt_fwd_kernel(const Operand q, const Operand k, const Operand v, const Operand o, float* __restrict__ lse, const Geom g, const int tiles, const int vec) {
     using S = SimtCfg<CP, BM>;
@@ -256,7 +256,7 @@ simt_fwd_kernel(const Operand q, const Operand k, const Operand v, const Operand
         if (tx == 0 && t < g.Tq)
             lse[row_index(g, b, n, t)] = sum == 0.f ? -CUDART_INF_F : (top[i] + log2f(sum)) * na2d_tc::kLn2;
     }
-    store_rows<DT, CP, BM>(rows_of<DT>(o, b, n), o.t, t0, g.Tq, g.C, acc, inv, tx, ty);
+    store_rows<OT, CP, BM>(rows_of<OT>(o, b, n), o.t, t0, g.Tq, g.C, acc, inv, tx, ty);
 }
 
 // ---- delta = dO . o, a warp a row -------------------------------------------------------------------------------------
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kThreads) simt_delta_kernel(const Operand d_o,
 }
 
 // ---- query half of the backward -----------------------------------------------------------------------------------------
-template <typename DT, int CP, int BM>
+template <typename DT, typename OT, int CP, int BM>
 __global__ void __launch_bounds__(kThreads)
 simt_dq_kernel(const Operand q, const Operand k, const Operand v, const Operand d_o, const Operand d_q, const float* __restrict__ lse,
                const float* __restrict__ delta, const Geom g, const int tiles, const int vec) {
@@ -328,7 +328,7 @@ simt_dq_kernel(const Operand q, const Operand k, const Operand v, const Operand 
         __syncwarp();
         acc.add(sP, sKV, tx, ty);
     }
-    store_rows<DT, CP, BM>(rows_of<DT>(d_q, b, n), d_q.t, t0, g.Tq, g.C, acc, scale, tx, ty);
+    store_rows<OT, CP, BM>(rows_of<OT>(d_q, b, n), d_q.t, t0, g.Tq, g.C, acc, scale, tx, ty);
 }
 
 // ---- key half: a block has BT keys of one key head and walks the queries of every head that shares it ------------------------
@@ -446,7 +446,7 @@ int by_rows(const Place& at, const Geom& g, F&& f) {
     }
 }
 
-template <typename DT, int CP, int BM>
+template <typename DT, typename OT, int CP, int BM>
 int forward_as(const Place& at, const Geom& g, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse) {
     using S = SimtCfg<CP, BM>;
     static std::atomic<unsigned long long> opted{0};
@@ -454,17 +454,17 @@ int forward_as(const Place& at, const Geom& g, const Operand& q, const Operand& 
     int tiles = 0;
     unsigned blocks = 0;
     if (int rc = blocks_of((long long)g.B * g.N, g.Tq, BM, &tiles, &blocks)) return rc;
-    return start(at, simt_fwd_kernel<DT, CP, BM>, blocks, S::HELD + S::TILE + S::SCORES, opted, q, k, v, o, lse, g, tiles, vec);
+    return start(at, simt_fwd_kernel<DT, OT, CP, BM>, blocks, S::HELD + S::TILE + S::SCORES, opted, q, k, v, o, lse, g, tiles, vec);
 }
 
-template <typename DT, int CP, int BM>
+template <typename DT, typename OT, int CP, int BM>
 int queries_as(const Place& at, const Geom& g, const Backward& x, int vec) {
     using S = SimtCfg<CP, BM>;
     static std::atomic<unsigned long long> opted{0};
     int tiles = 0;
     unsigned blocks = 0;
     if (int rc = blocks_of((long long)g.B * g.N, g.Tq, BM, &tiles, &blocks)) return rc;
-    return start(at, simt_dq_kernel<DT, CP, BM>, blocks, 2 * S::HELD + S::TILE + S::SCORES, opted, x.q, x.k, x.v, x.d_o, x.d_q, x.lse,
+    return start(at, simt_dq_kernel<DT, OT, CP, BM>, blocks, 2 * S::HELD + S::TILE + S::SCORES, opted, x.q, x.k, x.v, x.d_o, x.d_q, x.lse,
                  (const float*)x.delta, g, tiles, vec);
 }
 
@@ -481,7 +481,11 @@ int backward_as(const Place& at, const Geom& g, const Backward& x) {
     *at.launched += 1;
     if (cudaGetLastError() != cudaSuccess) return NA2D_ERR_CUDA;
     if (x.d_q.ptr) {
-        if (int rc = by_rows<CP>(at, g, [&](auto bm) { return queries_as<DT, CP, decltype(bm)::value>(at, g, x, vec); })) return rc;
+        const int rc = by_rows<CP>(at, g, [&](auto bm) {
+            constexpr int kRowsOf = decltype(bm)::value;
+            return x.d_q.wide ? queries_as<DT, float, CP, kRowsOf>(at, g, x, vec) : queries_as<DT, DT, CP, kRowsOf>(at, g, x, vec);
+        });
+        if (rc != NA2D_OK) return rc;
     }
     if (!x.d_k.ptr) return NA2D_OK;
     unsigned blocks = 0;
@@ -497,7 +501,10 @@ int simt_forward(const Place& at, const Geom& g, const Operand& q, const Operand
         using DT = decltype(type);
         return by_channels<DT>(g.C, [&](auto cp) {
             constexpr int CP = decltype(cp)::value;
-            return by_rows<CP>(at, g, [&](auto bm) { return forward_as<DT, CP, decltype(bm)::value>(at, g, q, k, v, o, lse); });
+            return by_rows<CP>(at, g, [&](auto bm) {
+                constexpr int kRowsOf = decltype(bm)::value;
+                return o.wide ? forward_as<DT, float, CP, kRowsOf>(at, g, q, k, v, o, lse) : forward_as<DT, DT, CP, kRowsOf>(at, g, q, k, v, o, lse);
+            });
         });
     };
     return at.dtype == NA2D_F32 ? run(float{}) : at.dtype == NA2D_BF16 ? run(__nv_bfloat16{}) : run(__half{});

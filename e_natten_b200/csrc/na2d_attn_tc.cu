@@ -111,6 +111,11 @@ int NA2D_TC_NAME(forward)(const Place& at, const Geom& g, const Scratch& scratch
         cut.part_o = scratch.at;
         cut.part_lse = scratch.at + cut.splits * all_rows(g) * g.C;
     }
+    if (o.wide && cut.splits == 1 && !cut.line) {
+        cut.keep = 1;
+        cut.part_o = static_cast<float*>(o.ptr);
+        cut.part_lse = lse;
+    }
     const int chunks = (g.Tk + kRows - 1) / kRows;
     cut.each = (chunks + cut.splits - 1) / cut.splits;
     cut.by_splits = Div(cut.splits);
@@ -157,6 +162,7 @@ int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Scratch& given,
             row_cut.line = rows;
             row_cut.part = scratch.at;
         }
+        if (x.d_q.wide) row_cut.sums = static_cast<float*>(x.d_q.ptr);
         if (x.d_q.ptr) rc = launch_dq<NA2D_TC_TYPE, D>(at, g, row_cut, x.q, x.k, x.v, x.d_o, x.lse, x.delta, bounds, x.d_q);
         if (rc != NA2D_OK || !x.d_k.ptr) return rc;
         Geom gk = g;

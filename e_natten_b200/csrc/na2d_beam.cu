@@ -1,0 +1,521 @@
+// Beam search (include/na2d.h): the choice among all beams' next words, and caches that follow their beams.
+//
+// Choice.  Candidate (i, w) of a batch entry is worth  scores_i + logits_iw - ln sum_w e^logits_iw.
+// Bound by memory: the logits are read once, by select_rows_kernel: a block holds a segment of one beam's words in registers, forms
+// the segment's maximum and sum of exponentials, and finds its best words without sorting: with r = ceil(count / 8), the least of the
+// eight warps' r-th largest thread maxima is a bound that at least `count` words reach and few more do; those go to shared
+// memory, where each counts the better ones.  select_beams_kernel joins an entry's segments: sums in 64 bits, candidates by the
+// same bound.  (value, lowest beam, lowest word) is a total order, so nothing depends on the order in which candidates arrive.
+//
+// Reordering.  cache[g K + i] <- cache[g K + parent_gi] for all beams of a group at once, in place: a thread has the same few bytes of
+// all K beams, reads what moves and then writes it, so that no second copy of a cache exists and beams that keep their place cost
+// nothing.  Bound by memory: each beam that others follow is read once (again from L1 where several follow it), each entry that moves
+// written once.
+#include <algorithm>
+
+#include "../../include/na2d.h"
+#include "na2d_host.h"
+#include "na2d_launch.h"
+#include "na2d_ptx.cuh"
+#include "na2d_vec.cuh"
+
+namespace {
+
+using na2d_vec::Vec;
+using na2d_vec::widen;
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMostBeams = 32, kMostCount = 64;
+constexpr int kKept = 512;                              // candidates of a block that are ranked by counting
+constexpr float kInf = __builtin_huge_valf();
+
+// ---- choice ---------------------------------------------------------------------------------------------------------------
+// Numbers in the order of floats; 0 is below all of them.
+__device__ __forceinline__ unsigned ordered(float x) {
+    const unsigned u = __float_as_uint(x == 0.f ? 0.f : x);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered(unsigned u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+__device__ __forceinline__ unsigned long long ordered(double x) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(x == 0.0 ? 0.0 : x);
+    return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double from_ordered(unsigned long long u) {
+    return __longlong_as_double((long long)(u >> 63 ? u & 0x7fffffffffffffffull : ~u));
+}
+
+// The r-th largest of a warp's 32 numbers, equal ones counted one by one.
+__device__ __forceinline__ unsigned nth_largest(unsigned x, int r) {
+    unsigned top = 0;
+    for (int i = 0; i < r; ++i) {
+        top = __reduce_max_sync(0xffffffffu, x);
+        const unsigned at = __ballot_sync(0xffffffffu, x == top);
+        if ((threadIdx.x & 31) == __ffs(at) - 1) x = 0;
+    }
+    return top;
+}
+
+// A bound that at least `count` of the block's numbers reach (0 where there are fewer), from each thread's largest.  Every thread calls.
+__device__ __forceinline__ unsigned bound_of(unsigned largest, int count, unsigned* warps) {
+    const unsigned own = nth_largest(largest, (count + kWarps - 1) / kWarps);
+    if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = own;
+    __syncthreads();
+    unsigned least = warps[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) least = min(least, warps[w]);
+    return least;
+}
+
+struct Select {
+    const void* logits;
+    long long stride_b, stride_k;
+    const float* scores;                // (B, K)
+    const unsigned char* finished;      // (B, K), or null
+    int B, K, V, count;
+    long long end;
+    int segments, each;                 // of a row, words of one
+    float2* sums;                       // (B K, segments): maximum, sum of e^(logit - maximum)
+    unsigned long long* best;           // (B K, segments, count): ordered logit, ~word; 0 where there is none
+    float* out_scores;
+    long long *out_parents, *out_words;
+};
+
+// e^x for x <= 0.  (1 / ln 2 in two numbers: sums of many beams are compared with one another.)
+__device__ __forceinline__ float exp_of(float x) {
+    const float y = fmaf(x, 1.44269502f, x * 1.92596303e-8f);
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+    return r;
+}
+
+// E words a thread; N words a load, 1 where rows do not start on 16-byte boundaries.  Which thread has a word depends on the word and
+// N alone, so that equal rows have equal sums.
+template <typename T, int N, int E>
+__global__ void __launch_bounds__(kThreads) select_rows_kernel(const Select x) {
+    __shared__ unsigned warps[kWarps];
+    __shared__ float tops[kWarps], totals[kWarps];
+    __shared__ unsigned long long kept[kKept];
+    __shared__ int kept_count;
+    na2d_ptx::after_previous_grid();
+    na2d_ptx::next_grid_may_start();
+    const int row = blockIdx.x / x.segments, segment = blockIdx.x - row * x.segments, b = row / x.K, k = row - b * x.K;
+    if (x.finished && x.finished[row]) return;           // (nothing of it is read)
+    const int first = segment * x.each, words = min(x.each, x.V - first), tid = threadIdx.x;
+    const T* src = static_cast<const T*>(x.logits) + b * x.stride_b + k * x.stride_k + first;
+    float v[E];
+#pragma unroll
+    for (int j = 0; j < E / N; ++j) {
+        const int at = (j * kThreads + tid) * N;
+        if (N > 1 && at + N <= words) {
+            Vec<T, N> piece;
+            piece.load(src + at);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[j * N + i] = widen(piece.at[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[j * N + i] = at + i < words ? widen(src[at + i]) : -kInf;
+        }
+    }
+    if (tid == 0) kept_count = 0;
+    float high = -kInf;
+#pragma unroll
+    for (int j = 0; j < E; ++j) high = fmaxf(high, v[j]);
+    const unsigned bound = bound_of(high == -kInf ? 0u : ordered(high), x.count, warps);
+    {   // maximum and sum
+        float top = high;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (tid % 32 == 0) tops[tid / 32] = top;
+    }
+    __syncthreads();
+    float top = tops[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, tops[w]);
+    const float base = top == -kInf ? 0.f : top;
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < E; ++j) sum[j & 1] += exp_of(v[j] - base);
+    float total = sum[0] + sum[1];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    if (tid % 32 == 0) totals[tid / 32] = total;
+    // the words that reach the bound
+    const float least = bound ? from_ordered(bound) : -kInf;
+    auto word_of = [&](int j) { return first + ((j / N) * kThreads + tid) * N + j % N; };
+    auto key_of = [&](int j) { return ((unsigned long long)ordered(v[j]) << 32) | (unsigned)~word_of(j); };
+    if (high >= least) {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (v[j] >= least && v[j] > -kInf) {
+                const int at = atomicAdd(&kept_count, 1);
+                if (at < kKept) kept[at] = key_of(j);
+            }
+    }
+    __syncthreads();
+    const size_t place = (size_t)row * x.segments + segment;
+    unsigned long long* best = x.best + place * x.count;
+    const int n = kept_count;
+    if (tid == 0) {
+        total = 0.f;
+        for (int w = 0; w < kWarps; ++w) total += totals[w];
+        x.sums[place] = make_float2(top, total);
+    }
+    if (n <= kKept) {
+        for (int i = tid; i < n; i += kThreads) {
+            const unsigned long long own = kept[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += kept[j] > own;
+            if (rank < x.count) best[rank] = own;
+        }
+        for (int i = n + tid; i < x.count; i += kThreads) best[i] = 0;
+        return;
+    }
+    // many equal words: the best of those below the last one, `count` times
+    unsigned long long below = ~0ull;
+    for (int r = 0; r < x.count; ++r) {
+        unsigned long long own = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const unsigned long long key = v[j] > -kInf ? key_of(j) : 0;
+            if (key < below && key > own) own = key;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) own = max(own, __shfl_xor_sync(0xffffffffu, own, d));
+        __syncthreads();
+        if (tid % 32 == 0) kept[tid / 32] = own;
+        __syncthreads();
+        below = kept[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) below = max(below, kept[w]);
+        if (tid == 0) best[r] = below;                   // (n > count: there is one)
+    }
+}
+
+// A block an entry.
+__global__ void __launch_bounds__(kThreads) select_beams_kernel(const Select x) {
+    __shared__ double offset[kMostBeams];                // scores_i - lse_i; NaN: the beam has no candidates
+    __shared__ unsigned warps[kWarps];
+    __shared__ unsigned long long kept[kKept];
+    __shared__ long long names[kKept];                   // beam V + word
+    __shared__ int kept_count;
+    na2d_ptx::after_previous_grid();
+    na2d_ptx::next_grid_may_start();
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 32;
+    const double nan = __longlong_as_double(0x7ff8000000000000ll);
+    for (int i = tid / 32; i < x.K; i += kWarps) {
+        const int row = b * x.K + i;
+        const float score = x.scores[row];
+        const bool counts = score > -kInf && score < kInf;
+        if (x.finished && x.finished[row]) {
+            if (lane == 0) offset[i] = nan;
+            continue;
+        }
+        const float2* sums = x.sums + (size_t)row * x.segments;
+        float top = -kInf;
+        for (int s = lane; s < x.segments; s += 32) top = fmaxf(top, sums[s].x);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        double total = 0.0;
+        for (int s = lane; s < x.segments; s += 32) {
+            const float2 part = sums[s];
+            total += (double)part.y * (part.x == -kInf ? 1.0 : exp((double)part.x - (double)top));       // (a sum of nothing is 0, or NaN)
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+        if (lane == 0) offset[i] = counts && total > 0.0 ? (double)score - ((double)top + log(total)) : nan;
+    }
+    if (tid == 0) kept_count = 0;
+    __syncthreads();
+    const int per_beam = x.segments * x.count, n = x.K * per_beam;
+    const unsigned long long* best = x.best + (size_t)b * n;
+    // worth of candidate c (0: none) and its name
+    auto worth = [&](int c, long long& name) -> unsigned long long {
+        const int i = c / per_beam;
+        const double by = offset[i];
+        if (!(by == by)) {
+            const int row = b * x.K + i;
+            if (c != i * per_beam || !x.finished || !x.finished[row]) return 0;
+            const float score = x.scores[row];           // a beam that has ended: itself
+            name = (long long)i * x.V + x.end;
+            return score > -kInf && score < kInf ? ordered((double)score) : 0;
+        }
+        const unsigned long long key = best[c];
+        if (!key) return 0;
+        name = (long long)i * x.V + (unsigned)~(unsigned)key;
+        return ordered(by + (double)from_ordered((unsigned)(key >> 32)));
+    };
+    long long name = 0;
+    unsigned high = 0;
+    for (int c = tid; c < n; c += kThreads) high = max(high, (unsigned)(worth(c, name) >> 32));
+    const unsigned bound = max(bound_of(high, x.count, warps), 1u);
+    if (high >= bound)
+        for (int c = tid; c < n; c += kThreads) {
+            const unsigned long long own = worth(c, name);
+            if ((unsigned)(own >> 32) < bound) continue;
+            const int at = atomicAdd(&kept_count, 1);
+            if (at >= kKept) continue;
+            kept[at] = own;
+            names[at] = name;
+        }
+    __syncthreads();
+    const int m = kept_count;
+    auto put = [&](int r, unsigned long long own, long long called) {
+        const size_t at = (size_t)b * x.count + r;
+        x.out_scores[at] = own ? (float)from_ordered(own) : -kInf;
+        x.out_parents[at] = own ? called / x.V : 0;
+        x.out_words[at] = own ? called % x.V : 0;
+    };
+    if (m <= kKept) {
+        for (int i = tid; i < m; i += kThreads) {
+            int rank = 0;
+            for (int j = 0; j < m; ++j) rank += kept[j] > kept[i] || (kept[j] == kept[i] && names[j] < names[i]);
+            if (rank < x.count) put(rank, kept[i], names[i]);
+        }
+        for (int i = m + tid; i < x.count; i += kThreads) put(i, 0, 0);
+        return;
+    }
+    // many of nearly equal worth: the best behind the last one, `count` times
+    unsigned long long last = ~0ull;
+    long long last_name = -1;
+    for (int r = 0; r < x.count; ++r) {
+        unsigned long long own = 0;
+        long long called = 0;
+        auto take = [&](unsigned long long w, long long who) {
+            if (w > own || (w == own && w && who < called)) {
+                own = w;
+                called = who;
+            }
+        };
+        for (int c = tid; c < n; c += kThreads) {
+            const unsigned long long w = worth(c, name);
+            if (w < last || (w == last && name > last_name)) take(w, name);
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            const unsigned long long w = __shfl_xor_sync(0xffffffffu, own, d);
+            const long long who = __shfl_xor_sync(0xffffffffu, called, d);
+            take(w, who);
+        }
+        __syncthreads();
+        if (lane == 0) {
+            kept[tid / 32] = own;
+            names[tid / 32] = called;
+        }
+        __syncthreads();
+        for (int w = 0; w < kWarps; ++w) take(kept[w], names[w]);
+        last = own;
+        last_name = called;
+        if (tid == 0) put(r, own, called);
+    }
+}
+
+// Segments of a row: as many words as a block holds, fewer where that would leave SMs without two blocks.
+struct Cut {
+    int words, segments, each;          // words: a block's
+};
+Cut cut_of(int rows, int V, int sms) {
+    Cut c;
+    c.words = (long long)rows * ((V + 8191) / 8192) >= 2 * sms ? 8192 : 2048;
+    c.segments = (V + c.words - 1) / c.words;
+    c.each = ((V + c.segments - 1) / c.segments + 7) / 8 * 8;
+    c.segments = (V + c.each - 1) / c.each;
+    return c;
+}
+size_t bytes_of(int rows, const Cut& c, int count) { return (size_t)rows * c.segments * (sizeof(float2) + sizeof(unsigned long long) * count); }
+
+int check_select(const na2d_beam_select_args* a) {
+    if (!a || a->struct_size < sizeof(na2d_beam_select_args)) return NA2D_ERR_BAD_ARG;
+    if (a->B <= 0 || a->K <= 0 || a->V <= 0 || a->count <= 0 || a->end < 0 || a->end >= a->V) return NA2D_ERR_BAD_ARG;
+    if (a->dtype != NA2D_F32 && a->dtype != NA2D_BF16 && a->dtype != NA2D_F16) return NA2D_ERR_UNSUPPORTED;
+    if (a->K > kMostBeams || a->count > kMostCount) return NA2D_ERR_UNSUPPORTED;
+    if (a->V > (1 << 24) || (long long)a->B * a->K > (1 << 20)) return NA2D_ERR_TOO_LARGE;
+    return NA2D_OK;
+}
+
+template <typename T, int N>
+int launch_rows(const Select& x, const Cut& c, cudaStream_t st) {
+    const unsigned blocks = (unsigned)((long long)x.B * x.K * c.segments);
+    const cudaError_t e = c.words == 8192 ? na2d_launch::launch(true, select_rows_kernel<T, N, 32>, blocks, kThreads, 0, st, x)
+                                          : na2d_launch::launch(true, select_rows_kernel<T, N, 8>, blocks, kThreads, 0, st, x);
+    return e == cudaSuccess ? NA2D_OK : na2d_host::cuda_fail(e, "beam selection launch");
+}
+template <typename T>
+int by_alignment(const Select& x, const Cut& c, cudaStream_t st) {
+    constexpr int kFull = 16 / (int)sizeof(T);
+    const bool aligned = reinterpret_cast<uintptr_t>(x.logits) % 16 == 0 && x.stride_b % kFull == 0 && x.stride_k % kFull == 0;
+    return aligned ? launch_rows<T, kFull>(x, c, st) : launch_rows<T, 1>(x, c, st);
+}
+
+// ---- reordering -----------------------------------------------------------------------------------------------------------
+constexpr int kMostCaches = 64;                         // of a launch
+struct Cache {
+    char* at;
+    long long e, h, t;                  // strides, bytes
+    int heads, tokens, pieces;          // pieces: of a row
+    int heads_first;                    // heads lie closer together than tokens
+};
+struct Reorder {
+    Cache cache[kMostCaches];
+    int B, K;
+    const void* parents;                // (B, K)
+    const void* lengths;                // (B K,), or null
+    int parents_64, lengths_64;
+    int blocks;                         // of a group
+};
+
+// V: the piece that a thread has of every beam.
+template <typename V, int MOST>
+__global__ void __launch_bounds__(kThreads) reorder_kernel(const __grid_constant__ Reorder x) {
+    __shared__ int from[kMostBeams], length[kMostBeams];
+    __shared__ int longest;
+    na2d_ptx::after_previous_grid();
+    na2d_ptx::next_grid_may_start();
+    const Cache& c = x.cache[blockIdx.y];
+    const int group = blockIdx.x / x.blocks, part = blockIdx.x - group * x.blocks;
+    if (threadIdx.x < 32) {
+        const int i = threadIdx.x;
+        int parent = i, tokens = 0;
+        if (i < x.K) {
+            const size_t at = (size_t)group * x.K + i;
+            const long long p = x.parents_64 ? static_cast<const long long*>(x.parents)[at] : static_cast<const int*>(x.parents)[at];
+            parent = p >= 0 && p < x.K ? (int)p : i;     // (no such beam: it stays)
+            if (parent != i) {
+                const size_t of = (size_t)group * x.K + parent;
+                const long long n = !x.lengths ? c.tokens : x.lengths_64 ? static_cast<const long long*>(x.lengths)[of] : static_cast<const int*>(x.lengths)[of];
+                tokens = (int)min(max(n, 0ll), (long long)c.tokens);
+            }
+        }
+        from[i] = parent;
+        length[i] = tokens;                              // that move
+        const int most = __reduce_max_sync(0xffffffffu, tokens);
+        if (i == 0) longest = most;
+    }
+    __syncthreads();
+    const unsigned pieces = c.pieces, tokens = longest, heads = c.heads;
+    const unsigned all = pieces * tokens * heads;        // (below 2^31)
+    char* base = c.at + (long long)group * x.K * c.e;
+    for (unsigned i = part * kThreads + threadIdx.x; i < all; i += x.blocks * kThreads) {
+        const unsigned row = i / pieces, p = i - row * pieces;
+        unsigned h, t;
+        if (c.heads_first) {
+            t = row / heads;
+            h = row - t * heads;
+        } else {
+            h = row / tokens;
+            t = row - h * tokens;
+        }
+        char* at = base + h * c.h + t * c.t + (long long)p * sizeof(V);
+        V v[MOST];
+#pragma unroll
+        for (int k = 0; k < MOST; ++k)
+            if (k < x.K && (int)t < length[k]) v[k] = *reinterpret_cast<const V*>(at + from[k] * c.e);
+#pragma unroll
+        for (int k = 0; k < MOST; ++k)
+            if (k < x.K && (int)t < length[k]) *reinterpret_cast<V*>(at + k * c.e) = v[k];
+    }
+}
+
+template <typename V>
+int launch_reorder(const Reorder& x, int caches, cudaStream_t st) {
+    const dim3 grid((unsigned)(x.B * x.blocks), (unsigned)caches);
+    auto kern = x.K <= 4 ? reorder_kernel<V, 4> : x.K <= 8 ? reorder_kernel<V, 8> : x.K <= 16 ? reorder_kernel<V, 16> : reorder_kernel<V, 32>;
+    const cudaError_t e = na2d_launch::launch(true, kern, grid, kThreads, 0, st, x);
+    if (e != cudaSuccess) return na2d_host::cuda_fail(e, "beam reordering launch");
+    na2d_host::count_launches(1);
+    return NA2D_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t na2d_beam_select_workspace(const na2d_beam_select_args* a) {
+    if (check_select(a) != NA2D_OK) return 0;
+    return bytes_of(a->B * a->K, cut_of(a->B * a->K, a->V, na2d_host::sm_count(a->device)), a->count);
+}
+
+int na2d_beam_select(const na2d_beam_select_args* a) {
+    if (int rc = check_select(a)) return rc;
+    if (!a->logits || !a->scores || !a->out_scores || !a->out_parents || !a->out_words) return NA2D_ERR_BAD_ARG;
+    Select x{};
+    x.logits = a->logits;
+    const bool dense = a->stride_b == 0 && a->stride_k == 0;
+    x.stride_k = dense || a->K == 1 ? a->V : a->stride_k;
+    x.stride_b = dense || a->B == 1 ? a->K * x.stride_k : a->stride_b;
+    x.scores = a->scores;
+    x.finished = a->finished;
+    x.B = a->B;
+    x.K = a->K;
+    x.V = a->V;
+    x.count = a->count;
+    x.end = a->end;
+    const int rows = a->B * a->K;
+    const Cut c = cut_of(rows, a->V, na2d_host::sm_count(a->device));
+    if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_bytes < bytes_of(rows, c, a->count)) return NA2D_ERR_BAD_ARG;
+    if ((long long)rows * c.segments > 0x7fffffffLL || (long long)x.K * c.segments * x.count > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+    x.segments = c.segments;
+    x.each = c.each;
+    x.best = static_cast<unsigned long long*>(a->workspace);
+    x.sums = reinterpret_cast<float2*>(x.best + (size_t)rows * c.segments * a->count);
+    x.out_scores = a->out_scores;
+    x.out_parents = reinterpret_cast<long long*>(a->out_parents);
+    x.out_words = reinterpret_cast<long long*>(a->out_words);
+    return na2d_host::on_device(a->device, [&]() -> int {
+        const cudaStream_t st = (cudaStream_t)a->stream;
+        const int rc = a->dtype == NA2D_F32    ? by_alignment<float>(x, c, st)
+                       : a->dtype == NA2D_BF16 ? by_alignment<__nv_bfloat16>(x, c, st)
+                                               : by_alignment<__half>(x, c, st);
+        if (rc != NA2D_OK) return rc;
+        const cudaError_t e = na2d_launch::launch(true, select_beams_kernel, (unsigned)x.B, kThreads, 0, st, x);
+        if (e != cudaSuccess) return na2d_host::cuda_fail(e, "beam selection launch");
+        na2d_host::count_launches(2);
+        return NA2D_OK;
+    });
+}
+
+int na2d_beam_reorder(const na2d_beam_reorder_args* a) {
+    if (!a || a->struct_size < sizeof(na2d_beam_reorder_args)) return NA2D_ERR_BAD_ARG;
+    if (a->B <= 0 || a->K <= 0 || a->caches < 0 || (a->caches > 0 && !a->cache) || !a->parents) return NA2D_ERR_BAD_ARG;
+    if (a->K > kMostBeams) return NA2D_ERR_UNSUPPORTED;
+    if ((long long)a->B * a->K > (1 << 24)) return NA2D_ERR_TOO_LARGE;
+    int piece = 16;
+    long long most = 0;                                  // bytes of a beam in a cache
+    for (int i = 0; i < a->caches; ++i) {
+        const na2d_cache& c = a->cache[i];
+        if (!c.ptr || c.heads <= 0 || c.tokens <= 0 || c.row_bytes <= 0) return NA2D_ERR_BAD_ARG;
+        if (c.row_bytes > (1ll << 40) / ((long long)c.heads * c.tokens)) return NA2D_ERR_TOO_LARGE;
+        most = std::max<long long>(most, c.row_bytes * c.heads * c.tokens);
+        const long long bits = (long long)reinterpret_cast<uintptr_t>(c.ptr) | c.stride_e | c.stride_h | c.stride_t | c.row_bytes;
+        piece = bits % 16 == 0 ? piece : bits % 4 == 0 ? std::min(piece, 4) : 1;
+    }
+    if (!a->caches || a->K == 1) return NA2D_OK;
+    if (most / piece > 0x3fffffffLL) return NA2D_ERR_TOO_LARGE;
+    return na2d_host::on_device(a->device, [&]() -> int {
+        const int sms = na2d_host::sm_count(a->device);
+        for (int first = 0; first < a->caches; first += kMostCaches) {
+            Reorder x{};
+            const int n = std::min(kMostCaches, a->caches - first);
+            for (int i = 0; i < n; ++i) {
+                const na2d_cache& c = a->cache[first + i];
+                x.cache[i] = Cache{static_cast<char*>(c.ptr), c.stride_e, c.stride_h, c.stride_t, c.heads, c.tokens, (int)(c.row_bytes / piece),
+                                   c.stride_h < c.stride_t};
+            }
+            x.B = a->B;
+            x.K = a->K;
+            x.parents = a->parents;
+            x.lengths = a->lengths;
+            x.parents_64 = a->parents_64 != 0;
+            x.lengths_64 = a->lengths_64 != 0;
+            // a block for each of the largest cache's stretches of 256 pieces, at most four rounds of eight blocks an SM in all
+            const long long needed = (most / piece + kThreads - 1) / kThreads, room = std::max(1LL, 32LL * sms / ((long long)n * a->B));
+            x.blocks = (int)std::min(needed, room);
+            const int rc = piece == 16  ? launch_reorder<uint4>(x, n, (cudaStream_t)a->stream)
+                           : piece == 4 ? launch_reorder<uint32_t>(x, n, (cudaStream_t)a->stream)
+                                        : launch_reorder<uint8_t>(x, n, (cudaStream_t)a->stream);
+            if (rc != NA2D_OK) return rc;
+        }
+        return NA2D_OK;
+    });
+}
+
+}  // extern "C"

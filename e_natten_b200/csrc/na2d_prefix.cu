@@ -1,0 +1,473 @@
+// Attention over a prefix that several batch entries share, and each entry's own keys (include/na2d.h).
+//
+//   s_ij = scale q_i . k_j over the prefix's keys and the own keys that row i sees, one softmax over both:
+//   o_i = sum_x e^(lse_x - lse) o_x,   lse = ln sum_x e^lse_x,   x in {prefix, own}
+//
+// The rows of all entries of a prefix are the rows of one attention problem, (S, N, A Tq, C) for S prefixes of A entries: the prefix's
+// keys and values are read once for all of them, and its tiles of 128 rows are full where entries have few rows.  Own keys are another
+// problem, (B, N, Tq, C).  Both run on the kernels of attention over all keys, with results in fp32, which are joined here.
+// The backward forms the weights of both from the joint lse, so that each half's dQ is a summand, and dK and dV are final: the prefix's
+// are sums over the rows of all its entries without atomics.
+#include <algorithm>
+
+#include "na2d_attn_entry.h"
+#include "na2d_host.h"
+#include "na2d_launch.h"
+#include "na2d_vec.cuh"
+
+namespace {
+
+using na2d_attn::Geom;
+using na2d_attn::Operand;
+using na2d_attn::Scratch;
+using na2d_vec::narrow;
+using na2d_vec::Vec;
+
+constexpr int kThreads = 256;
+
+// Rows of the whole batch: entry b = s A + a has prefix s.
+struct Rows {
+    int A, N, Tq, C;
+    long long all;          // B N Tq
+};
+// Place of row `r` of (B, N, Tq) in (S, N, A, Tq).
+__device__ __forceinline__ long long by_prefix(const Rows& g, long long r) {
+    const long long bn = r / g.Tq, b = bn / g.N, s = b / g.A;
+    const int t = (int)(r - bn * g.Tq), n = (int)(bn - b * g.N), a = (int)(b - s * g.A);
+    return ((s * g.N + n) * g.A + a) * g.Tq + t;
+}
+
+// ---- rows in the prefixes' order ----------------------------------------------------------------------------------------
+struct Gather {
+    const void* from[3];    // (B, N, Tq, C), bytes
+    long long b[3], n[3], t[3];
+    void* to[3];            // (S, N, A Tq, C), dense
+    const float* lse;       // null: none
+    float* lse_to;
+    int tensors;
+    int row_bytes;
+};
+template <typename V>
+__global__ void __launch_bounds__(kThreads) gather_rows_kernel(const Rows g, const Gather x) {
+    na2d_ptx::after_previous_grid();
+    na2d_ptx::next_grid_may_start();
+    const int which = blockIdx.y, per = which < x.tensors ? x.row_bytes / (int)sizeof(V) : 1;
+    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x, r = i / per;
+    if (r >= g.all) return;
+    const int c = (int)(i - r * per);
+    const long long to = by_prefix(g, r);
+    if (which == x.tensors) {
+        x.lse_to[to] = x.lse[r];
+        return;
+    }
+    const long long bn = r / g.Tq, b = bn / g.N;
+    const char* row = static_cast<const char*>(x.from[which]) + b * x.b[which] + (bn - b * g.N) * x.n[which] + (r - bn * g.Tq) * x.t[which];
+    reinterpret_cast<V*>(x.to[which])[to * per + c] = __ldg(reinterpret_cast<const V*>(row) + c);
+}
+
+// ---- joins ----------------------------------------------------------------------------------------------------------------
+// o and lse of a row from the prefix's and its own; a thread has N channels.
+template <typename DT, int N>
+__global__ void __launch_bounds__(kThreads)
+join_outputs_kernel(const Rows g, const float* __restrict__ o_prefix, const float* __restrict__ lse_prefix, const float* __restrict__ o_own,
+                    const float* __restrict__ lse_own, DT* __restrict__ o, float* __restrict__ lse) {
+    na2d_ptx::after_previous_grid();
+    na2d_ptx::next_grid_may_start();
+    const int per = g.C / N;
+    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x, r = i / per;
+    if (r >= g.all) return;
+    const int c = (int)(i - r * per) * N;
+    const long long p = by_prefix(g, r);
+    const float x = lse_prefix[p], y = lse_own ? lse_own[r] : -CUDART_INF_F;
+    // (a NaN stays one: the maximum skips it, its weight does not)
+    const float top = fmaxf(x, y), base = top == -CUDART_INF_F ? 0.f : top;
+    const float wx = expf(x - base), wy = expf(y - base), total = wx + wy, inv = total == 0.f ? 0.f : 1.f / total;
+    float out[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) out[k] = 0.f;
+    Vec<float, N> v;
+    if (x != -CUDART_INF_F) {                            // (of rows that see nothing, nothing was written)
+        v.load(o_prefix + p * g.C + c);
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] = v.at[k] * (wx * inv);
+    }
+    if (y != -CUDART_INF_F) {
+        v.load(o_own + r * g.C + c);
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] = fmaf(v.at[k], wy * inv, out[k]);
+    }
+    Vec<DT, N> to;
+    to.round(out);
+    to.store(o + r * g.C + c);
+    if (c == 0) lse[r] = total == 0.f ? -CUDART_INF_F : base + logf(total);
+}
+
+// dq of a row: the sum of the prefix's and its own.
+template <typename DT, int N>
+__global__ void __launch_bounds__(kThreads)
+join_gradients_kernel(const Rows g, const float* __restrict__ prefix, const float* __restrict__ own, DT* __restrict__ d_q) {
+    na2d_ptx::after_previous_grid();
+    na2d_ptx::next_grid_may_start();
+    const int per = g.C / N;
+    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x, r = i / per;
+    if (r >= g.all) return;
+    const int c = (int)(i - r * per) * N;
+    Vec<float, N> x, y;
+    x.load(prefix + by_prefix(g, r) * g.C + c);
+    float out[N];
+    if (own) y.load(own + r * g.C + c);
+#pragma unroll
+    for (int k = 0; k < N; ++k) out[k] = own ? x.at[k] + y.at[k] : x.at[k];
+    Vec<DT, N> to;
+    to.round(out);
+    to.store(d_q + r * g.C + c);
+}
+
+// ---- the problem ------------------------------------------------------------------------------------------------------------
+struct Problem {
+    Rows rows;
+    Geom prefix, own;       // own: unused without own keys
+    bool any_own, tensor;
+    int B, S, dtype;
+    Operand q, k, v, pk, pv, o, d_o;       // as given
+    bool follow[3];         // whether q's (o's, d_o's) rows of an entry follow those of the one before
+};
+
+int make_problem(const na2d_prefix_attention_args* a, Problem* p) {
+    if (!a || a->struct_size < sizeof(na2d_prefix_attention_args)) return NA2D_ERR_BAD_ARG;
+    if (a->B <= 0 || a->S <= 0 || a->N <= 0 || a->Nk <= 0 || a->Tq <= 0 || a->P <= 0 || a->Tk < 0 || a->C <= 0) return NA2D_ERR_BAD_ARG;
+    if (a->B % a->S != 0 || a->N % a->Nk != 0) return NA2D_ERR_BAD_ARG;
+    if (a->dtype != NA2D_F32 && a->dtype != NA2D_BF16 && a->dtype != NA2D_F16) return NA2D_ERR_UNSUPPORTED;
+    if (a->path != NA2D_PATH_AUTO && a->path != NA2D_PATH_SIMT && a->path != NA2D_PATH_TENSOR) return NA2D_ERR_BAD_ARG;
+    if (!(a->scale > 0.f) || !(a->scale < 3.0e38f)) return NA2D_ERR_BAD_ARG;
+    const int A = a->B / a->S;
+    if (a->Tk > (1 << 29) || a->P > (1 << 29) || (long long)A * a->Tq > (1 << 29) || (long long)a->B * a->N > (1 << 24)) return NA2D_ERR_TOO_LARGE;
+    if (a->C > na2d_attn::kSimtMaxC) return NA2D_ERR_UNSUPPORTED;
+    p->any_own = a->Tk > 0;
+    p->B = a->B;
+    p->S = a->S;
+    p->dtype = a->dtype;
+    p->rows = Rows{A, a->N, a->Tq, a->C, (long long)a->B * a->N * a->Tq};
+    auto geometry = [&](int B, int Tq, int Tk, bool causal, const int* lengths) {
+        Geom g{};
+        g.B = B; g.N = a->N; g.Nk = a->Nk; g.Tq = Tq; g.Tk = Tk; g.C = a->C;
+        g.causal = causal;
+        g.lengths = lengths;
+        g.scale = a->scale;
+        g.sl2 = a->scale * 1.4426950408889634f;
+        na2d_attn::cut_rows(g);
+        return g;
+    };
+    p->prefix = geometry(a->S, A * a->Tq, a->P, false, a->prefix_lengths);
+    if (p->any_own) p->own = geometry(a->B, a->Tq, a->Tk, a->causal != 0, a->key_lengths);
+    auto operand = [&](const na2d_heads& x, int B, int heads, int T) {
+        const na2d_host::HeadStrides s = na2d_host::head_strides(x, B, heads, T, a->C);
+        return Operand{x.ptr, s.b, s.n, s.t};
+    };
+    p->q = operand(a->q, a->B, a->N, a->Tq);
+    p->o = operand(a->o, a->B, a->N, a->Tq);
+    p->d_o = operand(a->d_o, a->B, a->N, a->Tq);
+    p->pk = operand(a->prefix_k, a->S, a->Nk, a->P);
+    p->pv = operand(a->prefix_v, a->S, a->Nk, a->P);
+    if (p->any_own) {
+        p->k = operand(a->k, a->B, a->Nk, a->Tk);
+        p->v = operand(a->v, a->B, a->Nk, a->Tk);
+    }
+    const Operand* by_rows[3] = {&p->q, &p->o, &p->d_o};
+    for (int i = 0; i < 3; ++i) p->follow[i] = A == 1 || a->Tq == 1 || by_rows[i]->b == a->Tq * by_rows[i]->t;
+    bool fits = a->dtype != NA2D_F32 && a->C <= 128 && a->C % 8 == 0;
+    for (const Operand* x : {&p->q, &p->k, &p->v, &p->pk, &p->pv, &p->o, &p->d_o}) fits = fits && (!x->ptr || na2d_attn::tma_ready(*x));
+    if (a->path == NA2D_PATH_TENSOR && !fits) return NA2D_ERR_UNSUPPORTED;
+    p->tensor = fits && a->path != NA2D_PATH_SIMT;
+    return NA2D_OK;
+}
+
+size_t esize_of(const Problem& p) { return p.dtype == NA2D_F32 ? 4 : 2; }
+
+// Where things lie in the workspace, in bytes; every part on a 256-byte boundary.
+struct Layout {
+    size_t size = 0;
+    size_t take(size_t bytes) {
+        const size_t at = size;
+        size += (bytes + 255) / 256 * 256;
+        return at;
+    }
+};
+struct ForwardLayout {
+    size_t q, o_prefix, lse_prefix, o_own, lse_own, scratch, scratch_bytes, size;
+};
+ForwardLayout forward_layout(const Problem& p, int sms) {
+    Layout l;
+    ForwardLayout f{};
+    const size_t rows = p.rows.all, values = rows * p.rows.C;
+    if (!p.follow[0]) f.q = l.take(values * esize_of(p));
+    f.o_prefix = l.take(values * 4);
+    f.lse_prefix = l.take(rows * 4);
+    if (p.any_own) {
+        f.o_own = l.take(values * 4);
+        f.lse_own = l.take(rows * 4);
+    }
+    if (p.tensor) {
+        f.scratch_bytes = na2d_attn::forward_floats(p.prefix, sms) * 4;
+        if (p.any_own) f.scratch_bytes = std::max(f.scratch_bytes, na2d_attn::forward_floats(p.own, sms) * 4);
+    }
+    f.scratch = l.take(f.scratch_bytes);
+    f.size = l.size;
+    return f;
+}
+struct BackwardLayout {
+    size_t rows[3], lse, delta_prefix, delta, dq_prefix, dq_own, scratch, scratch_bytes, size;
+};
+// (own or prefix: whether that half's keys have gradients)
+BackwardLayout backward_layout(const Problem& p, int sms, bool d_q, bool d_prefix, bool d_own) {
+    Layout l;
+    BackwardLayout f{};
+    const size_t rows = p.rows.all, values = rows * p.rows.C;
+    const bool f16 = p.dtype == NA2D_F16;
+    for (int i = 0; i < 3; ++i)
+        if (!p.follow[i]) f.rows[i] = l.take(values * esize_of(p));
+    f.lse = l.take(rows * 4);
+    f.delta_prefix = l.take(rows * 4);
+    f.delta = l.take(rows * 4);
+    if (d_q) {
+        f.dq_prefix = l.take(values * 4);
+        if (p.any_own) f.dq_own = l.take(values * 4);
+    }
+    if (p.tensor) {
+        f.scratch_bytes = na2d_attn::backward_floats(p.prefix, sms, f16, d_q, d_prefix) * 4;
+        if (p.any_own) f.scratch_bytes = std::max(f.scratch_bytes, na2d_attn::backward_floats(p.own, sms, f16, d_q, d_own) * 4);
+    }
+    f.scratch = l.take(f.scratch_bytes);
+    f.size = l.size;
+    return f;
+}
+
+// x as the prefixes' problem sees it: (S, N, A Tq, C).
+Operand merged(const Problem& p, const Operand& x) {
+    const Rows& g = p.rows;
+    if (g.A == 1) return x;
+    return Operand{x.ptr, g.A * x.b, x.n, g.Tq == 1 ? x.b : x.t};
+}
+Operand merged_copy(const Problem& p, void* at) {
+    const Rows& g = p.rows;
+    const long long row = g.C, head = (long long)g.A * g.Tq * row;
+    return Operand{at, g.N * head, head, row};
+}
+// A dense result in fp32 of B entries with Tq rows a head.
+Operand sums(const Problem& p, float* at, int Tq) {
+    const long long head = (long long)Tq * p.rows.C;
+    Operand x{at, p.rows.N * head, head, p.rows.C};
+    x.wide = true;
+    return x;
+}
+
+int place(int dtype, int device, void* stream, int* launched, na2d_attn::Place* at) {
+    *at = na2d_attn::Place{dtype, device, (cudaStream_t)stream, nullptr, launched};
+    return na2d_host::error_state(device, &at->errors);
+}
+int finish(int rc, int launched, const char* what) {
+    na2d_host::count_launches(launched);
+    return rc == NA2D_ERR_CUDA ? na2d_host::launch_fail(what) : rc;
+}
+
+int forward_of(const Problem& p, const na2d_attn::Place& at, const Geom& g, const Scratch& s, const Operand& q, const Operand& k, const Operand& v,
+               const Operand& o, float* lse) {
+    if (!p.tensor) return na2d_attn::simt_forward(at, g, q, k, v, o, lse);
+    return p.dtype == NA2D_BF16 ? na2d_attn::forward_bf16(at, g, s, q, k, v, o, lse) : na2d_attn::forward_f16(at, g, s, q, k, v, o, lse);
+}
+int backward_of(const Problem& p, const na2d_attn::Place& at, const Geom& g, const Scratch& s, const na2d_attn::Backward& x) {
+    if (!p.tensor) return na2d_attn::simt_backward(at, g, x);
+    return p.dtype == NA2D_BF16 ? na2d_attn::backward_bf16(at, g, s, x) : na2d_attn::backward_f16(at, g, s, x);
+}
+
+// Copies of those operands whose rows do not follow one another, and of lse.
+int gather(const na2d_attn::Place& at, const Problem& p, const Operand* const* from, char* const* to, int tensors, const float* lse, float* lse_to) {
+    Gather x{};
+    const long long esize = (long long)esize_of(p);
+    x.tensors = tensors;
+    x.row_bytes = (int)(p.rows.C * esize);
+    x.lse = lse;
+    x.lse_to = lse_to;
+    bool by_16 = x.row_bytes % 16 == 0;
+    for (int i = 0; i < tensors; ++i) {
+        x.from[i] = from[i]->ptr;
+        x.to[i] = to[i];
+        x.b[i] = from[i]->b * esize;
+        x.n[i] = from[i]->n * esize;
+        x.t[i] = from[i]->t * esize;
+        by_16 = by_16 && reinterpret_cast<uintptr_t>(from[i]->ptr) % 16 == 0 && x.b[i] % 16 == 0 && x.n[i] % 16 == 0 && x.t[i] % 16 == 0;
+    }
+    const int sides = tensors + (lse ? 1 : 0);
+    if (!sides) return NA2D_OK;
+    const long long per = tensors ? x.row_bytes / (by_16 ? 16 : esize) : 1, blocks = (p.rows.all * per + kThreads - 1) / kThreads;
+    if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+    const dim3 grid((unsigned)blocks, (unsigned)sides);
+    *at.launched += 1;
+    const cudaError_t e = by_16        ? na2d_launch::launch(true, gather_rows_kernel<uint4>, grid, kThreads, 0, at.st, p.rows, x)
+                          : esize == 4 ? na2d_launch::launch(true, gather_rows_kernel<uint32_t>, grid, kThreads, 0, at.st, p.rows, x)
+                                       : na2d_launch::launch(true, gather_rows_kernel<uint16_t>, grid, kThreads, 0, at.st, p.rows, x);
+    return e == cudaSuccess ? NA2D_OK : NA2D_ERR_CUDA;
+}
+
+template <typename DT, int N>
+int join_outputs(const na2d_attn::Place& at, const Problem& p, const float* o_prefix, const float* lse_prefix, const float* o_own,
+                 const float* lse_own, void* o, float* lse) {
+    const long long blocks = (p.rows.all * (p.rows.C / N) + kThreads - 1) / kThreads;
+    if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+    *at.launched += 1;
+    return na2d_launch::launch(true, join_outputs_kernel<DT, N>, (unsigned)blocks, kThreads, 0, at.st, p.rows, o_prefix, lse_prefix, o_own, lse_own,
+                               static_cast<DT*>(o), lse) == cudaSuccess
+               ? NA2D_OK
+               : NA2D_ERR_CUDA;
+}
+template <typename DT, int N>
+int join_gradients(const na2d_attn::Place& at, const Problem& p, const float* prefix, const float* own, void* d_q) {
+    const long long blocks = (p.rows.all * (p.rows.C / N) + kThreads - 1) / kThreads;
+    if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+    *at.launched += 1;
+    return na2d_launch::launch(true, join_gradients_kernel<DT, N>, (unsigned)blocks, kThreads, 0, at.st, p.rows, prefix, own,
+                               static_cast<DT*>(d_q)) == cudaSuccess
+               ? NA2D_OK
+               : NA2D_ERR_CUDA;
+}
+// f(element type, channels of a vector)
+template <typename F>
+int by_type(const Problem& p, F&& f) {
+    using One = std::integral_constant<int, 1>;
+    using Four = std::integral_constant<int, 4>;
+    const bool four = p.rows.C % 4 == 0;
+    if (p.dtype == NA2D_F32) return four ? f(float{}, Four{}) : f(float{}, One{});
+    if (p.dtype == NA2D_BF16) return four ? f(__nv_bfloat16{}, Four{}) : f(__nv_bfloat16{}, One{});
+    return four ? f(__half{}, Four{}) : f(__half{}, One{});
+}
+
+bool dense(const na2d_heads& x) { return x.stride_b == 0 && x.stride_n == 0 && x.stride_t == 0; }
+bool enough(const na2d_prefix_attention_args* a, size_t bytes) {
+    return a->workspace && reinterpret_cast<uintptr_t>(a->workspace) % 256 == 0 && a->workspace_bytes >= bytes;
+}
+
+}  // namespace
+
+extern "C" {
+
+int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a) {
+    if (!a || !a->q.ptr || !a->prefix_k.ptr || !a->prefix_v.ptr || !a->o.ptr || !a->lse) return NA2D_ERR_BAD_ARG;
+    Problem p{};
+    if (int rc = make_problem(a, &p)) return rc;
+    if (p.any_own && (!a->k.ptr || !a->v.ptr)) return NA2D_ERR_BAD_ARG;
+    if (!dense(a->o)) return NA2D_ERR_UNSUPPORTED;
+    const ForwardLayout f = forward_layout(p, na2d_host::sm_count(a->device));
+    if (!enough(a, f.size)) return NA2D_ERR_BAD_ARG;
+    return na2d_host::on_device(a->device, [&]() -> int {
+        int launched = 0;
+        na2d_attn::Place at;
+        if (int rc = place(a->dtype, a->device, a->stream, &launched, &at)) return rc;
+        char* ws = static_cast<char*>(a->workspace);
+        auto floats = [&](size_t where) { return reinterpret_cast<float*>(ws + where); };
+        const Scratch scratch{floats(f.scratch), f.scratch_bytes / 4};
+        auto run = [&]() -> int {
+            Operand q = p.follow[0] ? merged(p, p.q) : merged_copy(p, ws + f.q);
+            if (!p.follow[0]) {
+                const Operand* from = &p.q;
+                char* to = ws + f.q;
+                if (int rc = gather(at, p, &from, &to, 1, nullptr, nullptr)) return rc;
+            }
+            if (int rc = forward_of(p, at, p.prefix, scratch, q, p.pk, p.pv, sums(p, floats(f.o_prefix), p.prefix.Tq), floats(f.lse_prefix))) return rc;
+            if (p.any_own)
+                if (int rc = forward_of(p, at, p.own, scratch, p.q, p.k, p.v, sums(p, floats(f.o_own), p.own.Tq), floats(f.lse_own))) return rc;
+            const float *o_own = p.any_own ? floats(f.o_own) : nullptr, *lse_own = p.any_own ? floats(f.lse_own) : nullptr;
+            return by_type(p, [&](auto type, auto n) {
+                return join_outputs<decltype(type), decltype(n)::value>(at, p, floats(f.o_prefix), floats(f.lse_prefix), o_own, lse_own, a->o.ptr, a->lse);
+            });
+        };
+        return finish(run(), launched, "prefix attention forward launch");
+    });
+}
+
+int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a) {
+    if (!a || !a->q.ptr || !a->prefix_k.ptr || !a->prefix_v.ptr || !a->o.ptr || !a->d_o.ptr || !a->lse) return NA2D_ERR_BAD_ARG;
+    const bool d_prefix = a->d_prefix_k.ptr != nullptr, d_own = a->d_k.ptr != nullptr, d_q = a->d_q.ptr != nullptr;
+    if (d_prefix != (a->d_prefix_v.ptr != nullptr) || d_own != (a->d_v.ptr != nullptr) || !(d_q || d_prefix || d_own)) return NA2D_ERR_BAD_ARG;
+    Problem p{};
+    if (int rc = make_problem(a, &p)) return rc;
+    if (p.any_own ? !a->k.ptr || !a->v.ptr : d_own) return NA2D_ERR_BAD_ARG;
+    for (const na2d_heads* x : {&a->d_q, &a->d_k, &a->d_v, &a->d_prefix_k, &a->d_prefix_v})
+        if (!dense(*x)) return NA2D_ERR_UNSUPPORTED;
+    const BackwardLayout f = backward_layout(p, na2d_host::sm_count(a->device), d_q, d_prefix, d_own);
+    if (!enough(a, f.size)) return NA2D_ERR_BAD_ARG;
+    return na2d_host::on_device(a->device, [&]() -> int {
+        int launched = 0;
+        na2d_attn::Place at;
+        if (int rc = place(a->dtype, a->device, a->stream, &launched, &at)) return rc;
+        char* ws = static_cast<char*>(a->workspace);
+        auto floats = [&](size_t where) { return reinterpret_cast<float*>(ws + where); };
+        const Scratch scratch{floats(f.scratch), f.scratch_bytes / 4};
+        auto result = [&](void* ptr, int B, int T) {     // a dense gradient of keys
+            const long long head = (long long)T * a->C;
+            return Operand{ptr, a->Nk * head, head, a->C};
+        };
+        auto run = [&]() -> int {
+            const float* lse = a->lse;
+            if (d_q || d_prefix) {
+                const Operand* given[3] = {&p.q, &p.o, &p.d_o};
+                Operand x[3];
+                const Operand* from[3];
+                char* to[3];
+                int copies = 0;
+                for (int i = 0; i < 3; ++i) {
+                    x[i] = p.follow[i] ? merged(p, *given[i]) : merged_copy(p, ws + f.rows[i]);
+                    if (p.follow[i]) continue;
+                    from[copies] = given[i];
+                    to[copies++] = ws + f.rows[i];
+                }
+                const bool lse_apart = p.rows.A > 1 && p.rows.N > 1;
+                if (int rc = gather(at, p, from, to, copies, lse_apart ? lse : nullptr, floats(f.lse))) return rc;
+                na2d_attn::Backward b{};
+                b.q = x[0];
+                b.o = x[1];
+                b.d_o = x[2];
+                b.k = p.pk;
+                b.v = p.pv;
+                b.lse = lse_apart ? floats(f.lse) : lse;
+                b.delta = floats(f.delta_prefix);
+                if (d_q) b.d_q = sums(p, floats(f.dq_prefix), p.prefix.Tq);
+                if (d_prefix) {
+                    b.d_k = result(a->d_prefix_k.ptr, a->S, a->P);
+                    b.d_v = result(a->d_prefix_v.ptr, a->S, a->P);
+                }
+                if (int rc = backward_of(p, at, p.prefix, scratch, b)) return rc;
+            }
+            if (p.any_own && (d_q || d_own)) {
+                na2d_attn::Backward b{};
+                b.q = p.q;
+                b.o = p.o;
+                b.d_o = p.d_o;
+                b.k = p.k;
+                b.v = p.v;
+                b.lse = lse;
+                b.delta = floats(f.delta);
+                if (d_q) b.d_q = sums(p, floats(f.dq_own), p.own.Tq);
+                if (d_own) {
+                    b.d_k = result(a->d_k.ptr, a->B, a->Tk);
+                    b.d_v = result(a->d_v.ptr, a->B, a->Tk);
+                }
+                if (int rc = backward_of(p, at, p.own, scratch, b)) return rc;
+            }
+            if (!d_q) return NA2D_OK;
+            return by_type(p, [&](auto type, auto n) {
+                return join_gradients<decltype(type), decltype(n)::value>(at, p, floats(f.dq_prefix), p.any_own ? floats(f.dq_own) : nullptr, a->d_q.ptr);
+            });
+        };
+        return finish(run(), launched, "prefix attention backward launch");
+    });
+}
+
+size_t na2d_prefix_attention_workspace(const na2d_prefix_attention_args* a, int backward) {
+    Problem p{};
+    if (make_problem(a, &p) != NA2D_OK) return 0;
+    const int sms = na2d_host::sm_count(a->device);
+    return backward ? backward_layout(p, sms, a->d_q.ptr != nullptr, a->d_prefix_k.ptr != nullptr, a->d_k.ptr != nullptr).size
+                    : forward_layout(p, sms).size;
+}
+
+}  // extern "C"

@@ -294,4 +294,5 @@ PYBIND11_MODULE(_na2d_torch, m) {
     m.def("forward", &forward, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("backward", &backward, pybind11::call_guard<pybind11::gil_scoped_release>());
     na2d_torch::add_block_operators(m);
+    na2d_torch::add_answer_operators(m);
 }

@@ -62,5 +62,7 @@ inline bool ordinary(const Tensor& t) {
 
 // group_norm, rotary and attention (na2d_torch_block.cpp).
 void add_block_operators(pybind11::module_& m);
+// prefix_attention, beam_select and beam_reorder (na2d_torch_answers.cpp).
+void add_answer_operators(pybind11::module_& m);
 
 }  // namespace na2d_torch

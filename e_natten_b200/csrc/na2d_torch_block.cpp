@@ -5,18 +5,14 @@
 // whoever records calls sees one, with its arguments, and can make it again.  What the functions here do for themselves is not seen; a
 // trace of them would be the allocation of their results and nothing else.  Ordinary calls do without the dispatcher.
 #include <torch/csrc/autograd/custom_function.h>
-#include <ATen/core/dispatch/Dispatcher.h>
-#include <ATen/core/grad_mode.h>
 #include <ATen/core/LegacyTypeDispatch.h>
-#include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
 #include <cstring>
-#include <limits>
 #include <tuple>
 #include <vector>
 
-#include "na2d_torch.h"
+#include "na2d_torch_call.h"
 
 namespace na2d_torch {
 namespace {
@@ -49,58 +45,7 @@ void bind_block_abi(uintptr_t attention_forward, uintptr_t attention_backward, u
     abi.poll = reinterpret_cast<decltype(abi.poll)>(poll);
 }
 
-// ---- checks and layouts ---------------------------------------------------------------------------------------------
-int dtype_of(const Tensor& t) {
-    return t.scalar_type() == at::kFloat ? NA2D_F32 : t.scalar_type() == at::kBFloat16 ? NA2D_BF16 : NA2D_F16;
-}
-// What t says of itself is in its memory.
-void check_plain(const Tensor& t, const char* name) {
-    TORCH_CHECK_VALUE(!t.is_neg() && !t._is_zerotensor(), name, ": a lazily negated or zero tensor is not supported");
-}
-void check_map(const Tensor& t, const char* name) {
-    TORCH_CHECK_VALUE(t.is_cuda() && t.layout() == at::kStrided, name, ": e_natten_b200 runs on CUDA tensors only (there is no CPU path)");
-    TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, name, ": dtype ",
-                      t.scalar_type(), " not supported (float32, bfloat16, float16)");
-    check_plain(t, name);
-}
-void check_like(const Tensor& t, const Tensor& first, const char* name, const char* first_name) {
-    check_map(t, name);
-    TORCH_CHECK_VALUE(t.device() == first.device() && t.scalar_type() == first.scalar_type(), name, " must be on ", first_name,
-                      "'s device, of its dtype");
-}
-int extent(int64_t n, const char* what) {
-    TORCH_CHECK_VALUE(n <= std::numeric_limits<int>::max(), what, " of ", n, " is too large");
-    return (int)n;
-}
-void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
-void check_once(const char* name) {
-    TORCH_CHECK(!at::GradMode::is_enabled(), name, " is not differentiable twice");
-}
-// (an absent tensor goes to an autograd function as none: it has no edge of the graph then)
-MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
-bool wants_grad(std::initializer_list<Tensor> tensors) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor& t : tensors)
-        if (t.defined() && (t.requires_grad() || t._fw_grad(0).defined())) return true;
-    return false;
-}
-Tensor scratch(size_t bytes, const Tensor& like) {
-    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
-}
-
 // ---- operators of the dispatcher ------------------------------------------------------------------------------------
-// Whether a call on these tensors goes through the dispatcher.
-bool goes_through(std::initializer_list<Tensor> tensors) {
-    if (looked_into()) return true;
-    for (const Tensor& t : tensors)
-        if (t.defined() && !ordinary(t) && !t.is_neg() && !t._is_zerotensor()) return true;      // (those two are refused)
-    return false;
-}
-// The operator of that name, on arguments of F.
-template <typename F>
-c10::TypedOperatorHandle<F> operator_of(const char* name) {
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
-}
 using AttentionForward = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const MaybeTensor&, double, bool, int64_t);
 using AttentionBackward = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                                               const MaybeTensor&, double, bool, int64_t, bool, bool);
@@ -110,18 +55,6 @@ using NormBackward = std::vector<Tensor>(const Tensor&, const MaybeTensor&, cons
                                          int64_t, bool, bool, bool);
 using Turn = std::vector<Tensor>(const Tensor&, const MaybeTensor&, const Tensor&, const MaybeTensor&, bool, bool);
 using Table = Tensor(const Tensor&, const Tensor&, double);
-
-// (B, heads, T, C), of (B, heads, H, W, C) too: a view where the grid's rows follow one another.
-Tensor tokens(const Tensor& t, const char* name) {
-    TORCH_CHECK_VALUE(t.dim() == 4 || t.dim() == 5, name, " must be (B, heads, T, C) or (B, heads, H, W, C); got ", t.sizes());
-    TORCH_CHECK_VALUE(t.size(-1) > 0, name, " has no channels");
-    return t.dim() == 5 ? t.flatten(2, 3) : t;
-}
-na2d_heads heads_of(const Tensor& t) {
-    const auto s = t.strides();
-    return {t.data_ptr(), at_least_one(s[0]), at_least_one(s[1]), at_least_one(s[2])};
-}
-na2d_heads dense_heads(const Tensor& t) { return {t.data_ptr(), 0, 0, 0}; }
 
 // ---- attention -----------------------------------------------------------------------------------------------------------
 struct AttentionCall {

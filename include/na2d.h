@@ -382,6 +382,91 @@ int na2d_rotary(const na2d_rotary_args* a);
 int na2d_rotary_table(const double* positions, const double* frequencies, int64_t P, int axes, int pairs, double magnitude,
                       float* table, int device, void* stream);
 
+/* ---- Several answers to one prompt ---------------------------------------------------------------
+ *
+ * Attention over a prefix that entries share and their own keys, the choice of beam search, and caches that follow their beams.  No
+ * reference counterparts.
+ *
+ * Attention over a prefix: S prefixes of P keys, prefix_k and prefix_v (S, Nk, P, C); each is shared by the B / S entries that follow one
+ * another, entry b has prefix b / (B / S).  s_ij = scale * q_i . k_j over the prefix's keys and then the own keys that row i sees, one
+ * softmax over both.
+ *   prefix_lengths  int32 (S,) on the device, or NULL: prefix s has the first prefix_lengths[s] of the P keys (clamped to [0, P]).
+ *   Tk              0: no own keys (k, v, d_k, d_v unused).
+ *   key_lengths, causal  of the own keys, as in na2d_attention_args; every row sees all of its prefix.
+ *   lse             fp32 (B, N, Tq), dense, over both; -infinity for a row that sees nothing, which has o = 0 and no gradient.
+ *   d_q; d_k and d_v; d_prefix_k and d_prefix_v: may be NULL.  The prefix's are sums over its entries.  Results dense.
+ *   workspace       scratch, 256-byte aligned, at least na2d_prefix_attention_workspace bytes (for the same results wanted).
+ *   B / S * Tq, P, Tk <= 2^29, B * N <= 2^24, else NA2D_ERR_TOO_LARGE.  P > 0.
+ * Types, head dims, path, strides as in na2d_attention_args.  No atomics: the same call gives the same bits. */
+typedef struct na2d_prefix_attention_args {
+    size_t struct_size;
+    int B, S, N, Nk, Tq, Tk, P, C, dtype, path, device, causal;
+    float scale;
+    void* stream;
+    na2d_heads q, k, v, prefix_k, prefix_v, o, d_o, d_q, d_k, d_v, d_prefix_k, d_prefix_v;
+    const int32_t *key_lengths, *prefix_lengths;
+    float* lse;
+    void* workspace;
+    size_t workspace_bytes;
+} na2d_prefix_attention_args;
+int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a);
+int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a);
+size_t na2d_prefix_attention_workspace(const na2d_prefix_attention_args* a, int backward);
+
+/* The choice of beam search.  Candidate (i, w) of entry b, beam i followed by word w, is worth
+ *   scores[b][i] + logits[b][i][w] - ln sum_w e^logits[b][i][w];
+ * the `count` best, by worth, then lowest beam, then lowest word.
+ *   logits       (B, K, V) of dtype; element strides of entry and beam, words contiguous; both zero means dense.
+ *   scores       fp32 (B, K), dense.  A beam whose score is not finite has no candidates, nor has one with a logit of NaN or +infinity;
+ *                a word whose logit is -infinity is none.
+ *   finished     (B, K) bytes, or NULL: a beam with a non-zero one has one candidate, itself: word `end` at its score.  Its logits are
+ *                not looked at.
+ *   out_scores fp32, out_parents, out_words (B, count): worth, beam and word.  Places that are left over have -infinity, 0 and 0.
+ *   workspace    scratch, 16-byte aligned, at least na2d_beam_select_workspace bytes.
+ *   K <= 32, count <= 64 (NA2D_ERR_UNSUPPORTED); V <= 2^24, B * K <= 2^20 (NA2D_ERR_TOO_LARGE); 0 <= end < V.
+ * Exponentials are in 32 bits, their sums' joins and the worths in 64. */
+typedef struct na2d_beam_select_args {
+    size_t struct_size;
+    int B, K, V, count, dtype, device;
+    int64_t end;
+    void* stream;
+    const void* logits;
+    int64_t stride_b, stride_k;
+    const float* scores;
+    const uint8_t* finished;
+    float* out_scores;
+    int64_t *out_parents, *out_words;
+    void* workspace;
+    size_t workspace_bytes;
+} na2d_beam_select_args;
+int na2d_beam_select(const na2d_beam_select_args* a);
+size_t na2d_beam_select_workspace(const na2d_beam_select_args* a);
+
+/* Caches that follow their beams: entry g K + i of each cache becomes what entry g K + parents[g][i] was, for all i of a group at once,
+ * in place.
+ *   cache        host array of `caches` caches of B K entries, of any type: (entries, heads, tokens) rows of row_bytes bytes, strides in
+ *                bytes.  No two rows may share memory, within a cache or between them.
+ *   parents      (B, K), dense, int32 or (parents_64) int64.  One outside [0, K) leaves its entry as it is.
+ *   lengths      (B K,), dense, int32 or (lengths_64) int64, or NULL: how many tokens an entry holds (clamped to [0, tokens]).  Only the
+ *                parent's are copied; rows behind them stay as they are.
+ *   K <= 32 (NA2D_ERR_UNSUPPORTED); B * K <= 2^24, 2^30 pieces of 16 bytes (of 4, or 1, where rows or strides are not multiples of them)
+ *   a beam in one cache (NA2D_ERR_TOO_LARGE). */
+typedef struct na2d_cache {
+    void* ptr;
+    int64_t stride_e, stride_h, stride_t;
+    int heads, tokens;
+    int64_t row_bytes;
+} na2d_cache;
+typedef struct na2d_beam_reorder_args {
+    size_t struct_size;
+    int B, K, caches, parents_64, lengths_64, device;
+    void* stream;
+    const na2d_cache* cache;
+    const void* parents;
+    const void* lengths;
+} na2d_beam_reorder_args;
+int na2d_beam_reorder(const na2d_beam_reorder_args* a);
+
 /* Reads and clears the error word that a kernel sets when a bounded wait
  * (mbarrier) ran out.  Synchronises the stream.  Returns NA2D_OK or NA2D_ERR_KERNEL_WAIT.
  * No reference counterpart. */
