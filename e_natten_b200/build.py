@@ -3,7 +3,7 @@
     python e_natten_b200/build.py [--force] [--verbose]
 
 The library is plain CUDA C++ behind a C ABI (include/na2d.h); it needs no framework headers.
-Its kernels are compiled as nineteen translation units in parallel (the API with the SIMT kernels, the
+Its kernels are compiled as twenty-one translation units in parallel (the API with the SIMT kernels, the
 tiled CUDA-core kernels once per element type, the fp32 box kernels, each of the three tcgen05 kernel families once per
 16-bit element type, attention over all keys on tensor cores once per 16-bit type, on CUDA cores and its entry points, group norm,
 rotary positions, attention over shared prefixes and beam search) and linked into one shared object.  The Python package's extension module
@@ -45,6 +45,8 @@ UNITS = [
     ("na2d_norm.cu", [], "na2d_norm.o"),
     ("na2d_rotary.cu", [], "na2d_rotary.o"),
     ("na2d_prefix.cu", [], "na2d_prefix.o"),
+    ("na2d_prefix_tc.cu", ["-DNA2D_TC_DT=1"], "na2d_prefix_tc_bf16.o"),
+    ("na2d_prefix_tc.cu", ["-DNA2D_TC_DT=2"], "na2d_prefix_tc_f16.o"),
     ("na2d_beam.cu", [], "na2d_beam.o"),
 ]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]

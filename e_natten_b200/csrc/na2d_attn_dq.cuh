@@ -105,7 +105,7 @@ struct RowCut {
     int items;              // tiles
     int line;               // the chunks of all tiles on one line, that many CTAs take; 0: an item is a tile
     float* part;            // line: (2 a CTA, rows of a tile, C)
-    float* sums;            // dQ in fp32, (B, N, Tq, C); null: in the operands' type
+    float* sums;            // a wide dQ, (B, N, Tq, C)
 };
 
 // One item: chunks [c0, c0 + n) of a tile of rows.
@@ -173,7 +173,8 @@ struct DqCfg : TileCfg<D> {
     static_assert(SMEM <= kSmemLimit, "dQ kernel shared memory");
 };
 
-template <typename DT, int D, bool LINE>
+// WIDE: dQ in fp32.
+template <typename DT, int D, bool LINE, bool WIDE>
 __global__ void __launch_bounds__(512, 1)
 attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -447,13 +448,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                         if (ok && 32 * j + 4 * e < g.C)
                             dst[e] = make_float4(__uint_as_float(v[4 * e]) * scale, __uint_as_float(v[4 * e + 1]) * scale,
                                                  __uint_as_float(v[4 * e + 2]) * scale, __uint_as_float(v[4 * e + 3]) * scale);
-                } else if (cut.sums) {
-                    float4* dst = reinterpret_cast<float4*>(cut.sums + row_index(g, tile.b, n, t) * g.C + 32 * j);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (ok && 32 * j + 4 * e < g.C)
-                            dst[e] = make_float4(__uint_as_float(v[4 * e]) * scale, __uint_as_float(v[4 * e + 1]) * scale,
-                                                 __uint_as_float(v[4 * e + 2]) * scale, __uint_as_float(v[4 * e + 3]) * scale);
+                } else if (WIDE) {
+                    store_wide(stage, v, scale, ok ? cut.sums + row_index(g, tile.b, n, t) * g.C + 32 * j : nullptr, g.C - 32 * j, lane);
                 } else if (g.hp == 1) {
                     if (t_first < g.Tq)
                         na2d_tc::stage_and_store<DT, 32, 2>(&tm_dq, stage, v, scale, 32 * j, t_first, tile.h0, tile.b, 0, lane, &seq);
@@ -647,9 +643,9 @@ attn_join_rows_kernel(const float* __restrict__ part, OT* __restrict__ dq, const
     }
 }
 
-template <typename DT, int D>
-int launch_dq(const Place& at, const Geom& g, RowCut cut, const Operand& q, const Operand& k, const Operand& v, const Operand& d_o, const float* lse,
-              const float* delta, const Bounds& bounds, const Operand& d_q) {
+template <typename DT, int D, bool WIDE>
+int launch_dq_as(const Place& at, const Geom& g, RowCut cut, const Operand& q, const Operand& k, const Operand& v, const Operand& d_o, const float* lse,
+                 const float* delta, const Bounds& bounds, const Operand& d_q) {
     using C = DqCfg<D>;
     CUtensorMap tq, tg, tk, tv, tdq;
     int rc = operand_map(&tq, q, at.dtype, g.B, g.N, g.Tq, g.C, g.tt, g.hp, C::SLAB_C);
@@ -661,7 +657,7 @@ int launch_dq(const Place& at, const Geom& g, RowCut cut, const Operand& q, cons
     const long long items = (long long)g.units * g.tiles;
     if (items > 0x3fffffffLL) return NA2D_ERR_TOO_LARGE;
     cut.items = (int)items;
-    auto kern = cut.line ? attn_dq_kernel<DT, D, true> : attn_dq_kernel<DT, D, false>;
+    auto kern = cut.line ? attn_dq_kernel<DT, D, true, WIDE> : attn_dq_kernel<DT, D, false, WIDE>;
     static std::atomic<unsigned long long> opted[2]{};
     if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted[cut.line > 0]) != cudaSuccess) return NA2D_ERR_CUDA;
     const int sms = na2d_tc::sm_count(at.device);
@@ -671,12 +667,16 @@ int launch_dq(const Place& at, const Geom& g, RowCut cut, const Operand& q, cons
         return NA2D_ERR_CUDA;
     if (!cut.line) return NA2D_OK;
     *at.launched += 1;
-    const dim3 grid((unsigned)items, kJoinBlocks);
-    const cudaError_t e = d_q.wide ? na2d_launch::launch(true, attn_join_rows_kernel<float>, grid, 256, 0, at.st, (const float*)cut.part,
-                                                         (float*)d_q.ptr, d_q, g, cut)
-                                   : na2d_launch::launch(true, attn_join_rows_kernel<DT>, grid, 256, 0, at.st, (const float*)cut.part, (DT*)d_q.ptr,
-                                                         d_q, g, cut);
+    using OT = std::conditional_t<WIDE, float, DT>;
+    const cudaError_t e = na2d_launch::launch(true, attn_join_rows_kernel<OT>, dim3((unsigned)items, kJoinBlocks), 256, 0, at.st, (const float*)cut.part,
+                                              (OT*)d_q.ptr, d_q, g, cut);
     return e == cudaSuccess ? NA2D_OK : NA2D_ERR_CUDA;
+}
+template <typename DT, int D>
+int launch_dq(const Place& at, const Geom& g, const RowCut& cut, const Operand& q, const Operand& k, const Operand& v, const Operand& d_o, const float* lse,
+              const float* delta, const Bounds& bounds, const Operand& d_q) {
+    return d_q.wide ? launch_dq_as<DT, D, true>(at, g, cut, q, k, v, d_o, lse, delta, bounds, d_q)
+                    : launch_dq_as<DT, D, false>(at, g, cut, q, k, v, d_o, lse, delta, bounds, d_q);
 }
 
 }  // namespace na2d_attn

@@ -23,10 +23,19 @@ inline bool tma_ready(const Operand& x) {
     return true;
 }
 
+// How a wide result lies, where whoever asked for it joins the parts itself: `count` of them, each of the rows (B, N, Tq), one behind
+// the other.
+struct Parts {
+    const float *o, *lse;
+    int count;
+};
+
 // 16 bits, C a multiple of 8 up to 128, every operand on 16-byte boundaries; o, d_q, d_k and d_v dense.  o and d_q may be `wide`; of a wide o only
 // rows with a finite lse are written, where rows are not in parts.
-int forward_bf16(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);
-int forward_f16(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);
+int forward_bf16(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse,
+                 Parts* parts = nullptr);
+int forward_f16(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse,
+                Parts* parts = nullptr);
 
 // d_q.ptr or d_k.ptr (with d_v.ptr) may be null: that half is left out.  Writes delta.
 struct Backward {

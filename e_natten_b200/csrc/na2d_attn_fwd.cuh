@@ -53,9 +53,10 @@ struct FwdCut {
     int items;
     int each;               // chunks of a part
     int line;               // not PAIR: the chunks of all units on one line, that many groups take; 0: not
-    int keep;               // the whole rows, too, as parts: o in fp32, of rows that see a key
+    int even;               // a wide result's parts of a unit share out its own keys; else all units' parts are `each` chunks
+    int open;               // the parts are not joined here
     Div by_splits, by_pairs;
-    float* part_o;          // (splits, B, N, Tq, C), where splits > 1 or keep; line: (groups + units, rows of a unit, C)
+    float* part_o;          // (splits, B, N, Tq, C), where splits > 1 or the result is wide; line: (groups + units, rows of a unit, C)
     float* part_lse;        // (splits, B, N, Tq); line: (groups + units, rows of a unit)
 };
 
@@ -116,7 +117,7 @@ struct Stretch {
 };
 
 // The items of a CTA, which every role walks by itself.
-template <bool PAIR>
+template <bool PAIR, bool WIDE>
 struct FwdWalk {
     int item;
     Stretch s[2];
@@ -160,7 +161,8 @@ struct FwdWalk {
                 chunks[x] = p[x].any ? (p[x].tile.keys(g) + kRows - 1) / kRows : 0;
                 most = max(most, chunks[x]);
             }
-            const int c0 = min(split * cut.each, most), c1 = min(c0 + cut.each, most);
+            const int each = WIDE && cut.even ? cut.by_splits.quotient(most + cut.splits - 1) : cut.each;
+            const int c0 = min(split * each, most), c1 = min(c0 + each, most);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 p[x].slot = split;
@@ -231,10 +233,40 @@ __device__ __forceinline__ uint32_t pack_rest(uint64_t pair, uint32_t w) {
     return pack2<DT>(na2d_ptx::lo2(rest), na2d_ptx::hi2(rest));
 }
 
+// Stores 32 columns, held as fp32 bit patterns, times `scale` in fp32: row `lane` at `to` (null: none), of which there are `cols`, a multiple
+// of 4.  Through shared memory (4 KB): a store of 16 bytes of each of 32 rows touches 32 lines, one of 128 bytes of four rows
+// touches four.
+__device__ __forceinline__ void store_wide(uint8_t* stage, const uint32_t (&v)[32], float scale, float* to, int cols, int lane) {
+    const uint32_t base = smem_u32(stage);
+    if (lane == 0) bulk_wait_read<0>();                  // a store of results in 16 bits may still read the buffer
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        na2d_tc::st_shared_v4(base + lane * 128 + ((c ^ (lane & 7)) << 4), __float_as_uint(__uint_as_float(v[4 * c]) * scale),
+                              __float_as_uint(__uint_as_float(v[4 * c + 1]) * scale), __float_as_uint(__uint_as_float(v[4 * c + 2]) * scale),
+                              __float_as_uint(__uint_as_float(v[4 * c + 3]) * scale));
+    __syncwarp();
+    const unsigned long long own = reinterpret_cast<unsigned long long>(to);
+    const int c = lane & 7;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int row = 4 * i + (lane >> 3);
+        float* dst = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, own, row));
+        if (dst && 4 * c < cols) {
+            uint4 x;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                         : "r"(base + row * 128 + ((c ^ (row & 7)) << 4)) : "memory");
+            *reinterpret_cast<uint4*>(dst + 4 * c) = x;
+        }
+    }
+    __syncwarp();
+}
+
 // Columns of P whose product starts ahead of the others (64: 166 us for 156).
 constexpr int kMost = 96;
 
-template <typename DT, int D, bool PAIR>
+// WIDE: the results are fp32, of whole rows, too; they lie in part_o and part_lse, and rows that see nothing have no o.
+template <typename DT, int D, bool PAIR, bool WIDE>
 __global__ void __launch_bounds__(512, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, DT* __restrict__ o_rows,
@@ -335,7 +367,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     rv.next(NST);
                 }
             };
-            for (FwdWalk<PAIR> walk(g, cut, before); walk.more(cut) && lt.ok; walk.next(g, cut, before)) {
+            for (FwdWalk<PAIR, WIDE> walk(g, cut, before); walk.more(cut) && lt.ok; walk.next(g, cut, before)) {
                 FwdPart p[2];
                 walk.parts(g, cut, before, p);
                 const int most = max(p[0].n, p[1].n);
@@ -366,7 +398,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         reg_dec<kDkvRegsCtl>();
         if (g.lengths) {
             Ring ring;
-            for (FwdWalk<PAIR> walk(g, cut, before); walk.more(cut); walk.next(g, cut, before)) {
+            for (FwdWalk<PAIR, WIDE> walk(g, cut, before); walk.more(cut); walk.next(g, cut, before)) {
                 FwdPart p[2];
                 walk.parts(g, cut, before, p);
                 const int most = max(p[0].n, p[1].n);
@@ -399,7 +431,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         // Loads of the item that come before the group's chunk c.
         struct Item {
             int n, other;                    // chunks of the group, and of the other one
-            __device__ __forceinline__ Item(const Geom& g, const FwdCut& cut, const int* before, const FwdWalk<PAIR>& walk, int x) {
+            __device__ __forceinline__ Item(const Geom& g, const FwdCut& cut, const int* before, const FwdWalk<PAIR, WIDE>& walk, int x) {
                 n = other = 0;
                 if (!walk.more(cut)) return;
                 FwdPart p[2];
@@ -427,7 +459,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         auto key_wait = [&](const Item& t, int c) {
             mbar_wait(k_full + (base + t.ahead(c, x)) % NST, ((base + t.ahead(c, x)) / NST) & 1, wctx, kErrLoadWait);
         };
-        FwdWalk<PAIR> walk(g, cut, before);
+        FwdWalk<PAIR, WIDE> walk(g, cut, before);
         Item t(g, cut, before, walk, x);
         while (walk.more(cut)) {
             if (t.n > 0) {
@@ -489,30 +521,34 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const int row = quarter * 32 + lane;                 // row of the tile = tensor-memory lane
         const uint32_t tmem_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         uint8_t* stage = sOut + quarter * 2 * OutStage<32>::BYTES;
-        const bool in_parts = cut.splits > 1 || cut.line || cut.keep, by_tma = g.hp == 1 && !in_parts;
+        const bool in_parts = WIDE || cut.splits > 1 || cut.line, by_tma = g.hp == 1 && !in_parts;
         const size_t part_rows = cut.line ? (size_t)g.G * g.Tq : static_cast<size_t>(g.B) * g.N * g.Tq;     // of the workspace
-        uint32_t it[2] = {0, 0}, seq = 0;
-        for (FwdWalk<PAIR> walk(g, cut, before); walk.more(cut); walk.next(g, cut, before)) {
+        uint32_t it0 = 0, it1 = 0, seq = 0;
+        for (FwdWalk<PAIR, WIDE> walk(g, cut, before); walk.more(cut); walk.next(g, cut, before)) {
             FwdPart p[2];
             walk.parts(g, cut, before, p);
-#pragma unroll
+            // (wide results are those of short calls, too, where fetching unrolled code, met once for each piece of each tile, took longer than
+            // the stores: a call of one chunk 42 thousand cycles for 24)
+#pragma unroll (WIDE ? 1 : 2)
             for (int x = 0; x < 2; ++x) {
-                if (!p[x].any) continue;
+                const FwdPart part = x ? p[1] : p[0];
+                if (!part.any) continue;
+                const uint32_t turn = x ? it1 : it0;
                 int n, t;
-                const bool ok = p[x].tile.row(g, row, n, t);
-                const size_t at = row_index(g, p[x].tile.b, n, t);
-                const size_t part_at = p[x].slot * part_rows + (cut.line ? (size_t)(n - p[x].tile.m * g.G) * g.Tq + t : at);
-                const bool none = p[x].n == 0;               // no key: zeros
+                const bool ok = part.tile.row(g, row, n, t);
+                const size_t at = row_index(g, part.tile.b, n, t);
+                const size_t part_at = part.slot * part_rows + (cut.line ? (size_t)(n - part.tile.m * g.G) * g.Tq + t : at);
+                const bool none = part.n == 0;               // no key: zeros
                 float total = 0.f, fin = 0.f;
                 if (!none) {
-                    mbar_wait(o_full + x, it[x] & 1, wctx, kErrMmaWait);          // also: the group's sums are written
+                    mbar_wait(o_full + x, turn & 1, wctx, kErrMmaWait);          // also: the group's sums are written
                     tc_fence_after();
-                    total = x_sum[(x * 2 + (it[x] & 1)) * kRows + row];
-                    fin = x_fin[(x * 2 + (it[x] & 1)) * kRows + row];
+                    total = x_sum[(x * 2 + (turn & 1)) * kRows + row];
+                    fin = x_fin[(x * 2 + (turn & 1)) * kRows + row];
                 }
                 const float inv = total == 0.f ? 0.f : 1.f / total;
-                const int h_first = p[x].tile.h0, t_first = p[x].tile.t0 + quarter * 32;
-#pragma unroll
+                const int h_first = part.tile.h0, t_first = part.tile.t0 + quarter * 32;
+#pragma unroll (WIDE ? 1 : D / 32)
                 for (int j = 0; j < D / 32; ++j) {
                     uint32_t v[32];
                     if (!none) {
@@ -534,9 +570,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     if (32 * j >= g.C) continue;
                     if (by_tma) {
                         if (t_first < g.Tq)
-                            na2d_tc::stage_and_store<DT, 32, 2>(&tm_o, stage, v, inv, 32 * j, t_first, h_first, p[x].tile.b, 0, lane, &seq);
+                            na2d_tc::stage_and_store<DT, 32, 2>(&tm_o, stage, v, inv, 32 * j, t_first, h_first, part.tile.b, 0, lane, &seq);
                     } else if (ok && !in_parts) {
-                        uint4* dst = reinterpret_cast<uint4*>(o_rows + p[x].tile.b * o_st.b + n * o_st.n + t * o_st.t + 32 * j);
+                        uint4* dst = reinterpret_cast<uint4*>(o_rows + part.tile.b * o_st.b + n * o_st.n + t * o_st.t + 32 * j);
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (32 * j + 8 * e < g.C) {
@@ -546,20 +582,25 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                                     w[i] = pack2<DT>(__uint_as_float(v[8 * e + 2 * i]) * inv, __uint_as_float(v[8 * e + 2 * i + 1]) * inv);
                                 dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
                             }
-                    } else if (ok && !none) {
+                    } else if (!WIDE && ok && !none) {
                         float4* dst = reinterpret_cast<float4*>(cut.part_o + part_at * g.C + 32 * j);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             if (32 * j + 4 * e < g.C)
                                 dst[e] = make_float4(__uint_as_float(v[4 * e]) * inv, __uint_as_float(v[4 * e + 1]) * inv,
                                                      __uint_as_float(v[4 * e + 2]) * inv, __uint_as_float(v[4 * e + 3]) * inv);
+                    } else if (WIDE && !none) {
+                        store_wide(stage, v, inv, ok ? cut.part_o + part_at * g.C + 32 * j : nullptr, g.C - 32 * j, lane);
                     }
                 }
                 if (ok) {
                     float* to = in_parts ? cut.part_lse + part_at : lse + at;
                     *to = total == 0.f ? -CUDART_INF_F : (fin + log2f(total)) * kLn2;
                 }
-                if (!none) ++it[x];
+                if (!none) {
+                    if (x) ++it1;
+                    else ++it0;
+                }
             }
         }
         if (lane == 0) bulk_wait<0>();                       // the staging buffers have been read, the rows written
@@ -576,7 +617,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         // waiting for their MMAs (4 x 4 x 4096 x 128: 4640 cycles a chunk of either).  Both go through the turns of an item's longer half.
         const uint32_t my_turn = 1 + group, other_turn = 2 - group;
         if (group) bar_arrive(other_turn, 256);              // a goes first
-        for (FwdWalk<PAIR> walk(g, cut, before); walk.more(cut); walk.next(g, cut, before)) {
+        for (FwdWalk<PAIR, WIDE> walk(g, cut, before); walk.more(cut); walk.next(g, cut, before)) {
             FwdPart both[2];
             walk.parts(g, cut, before, both);
             const FwdPart p = group ? both[1] : both[0];
@@ -796,7 +837,7 @@ int launch_combine(const Place& at, const Geom& g, const FwdCut& cut, const Oper
     return o.wide ? launch_combine_as<float>(at, g, cut, o, lse) : launch_combine_as<DT>(at, g, cut, o, lse);
 }
 
-template <typename DT, int D, bool PAIR>
+template <typename DT, int D, bool PAIR, bool WIDE>
 int launch_fwd_as(const Place& at, const Geom& g, const FwdCut& cut, const Operand& q, const Operand& k, const Operand& v,
                   const Operand& o, float* lse) {
     using C = FwdCfg<D>;
@@ -806,7 +847,7 @@ int launch_fwd_as(const Place& at, const Geom& g, const FwdCut& cut, const Opera
     if (rc == NA2D_OK) rc = operand_map(&tv, v, at.dtype, g.B, g.Nk, g.Tk, g.C, kRows, 1, C::SLAB_C);
     if (rc == NA2D_OK) rc = operand_map(&to, o.wide ? q : o, at.dtype, g.B, g.N, g.Tq, g.C, 32, 1, 32);      // (parts do not go by it)
     if (rc != NA2D_OK) return rc;
-    auto kern = attn_fwd_kernel<DT, D, PAIR>;
+    auto kern = attn_fwd_kernel<DT, D, PAIR, WIDE>;
     static std::atomic<unsigned long long> opted{0};
     if (na2d_tc::opt_in_smem(kern, C::SMEM, at.device, opted) != cudaSuccess) return NA2D_ERR_CUDA;
     const int sms = na2d_tc::sm_count(at.device);
@@ -815,14 +856,15 @@ int launch_fwd_as(const Place& at, const Geom& g, const FwdCut& cut, const Opera
     if (na2d_launch::launch(false, kern, grid, 512, C::SMEM, at.st, tq, tk, tv, to, (DT*)o.ptr, o, lse,
                             at.errors, g, cut) != cudaSuccess)
         return NA2D_ERR_CUDA;
-    return cut.splits == 1 && !cut.line ? NA2D_OK : launch_combine<DT>(at, g, cut, o, lse);
+    return (cut.splits == 1 && !cut.line) || cut.open ? NA2D_OK : launch_combine<DT>(at, g, cut, o, lse);
 }
 
 template <typename DT, int D>
 int launch_fwd(const Place& at, const Geom& g, const FwdCut& cut, const Operand& q, const Operand& k, const Operand& v,
                const Operand& o, float* lse) {
-    if (g.tiles > 1) return launch_fwd_as<DT, D, true>(at, g, cut, q, k, v, o, lse);
-    return launch_fwd_as<DT, D, false>(at, g, cut, q, k, v, o, lse);
+    if (o.wide)
+        return g.tiles > 1 ? launch_fwd_as<DT, D, true, true>(at, g, cut, q, k, v, o, lse) : launch_fwd_as<DT, D, false, true>(at, g, cut, q, k, v, o, lse);
+    return g.tiles > 1 ? launch_fwd_as<DT, D, true, false>(at, g, cut, q, k, v, o, lse) : launch_fwd_as<DT, D, false, false>(at, g, cut, q, k, v, o, lse);
 }
 
 }  // namespace na2d_attn

@@ -54,6 +54,7 @@ int forward_parts(const Geom& g, int sms) {
     const long long tiles = (long long)g.units * g.tiles;
     const int chunks = (g.Tk + kRows - 1) / kRows;
     if (g.tiles == 1 || tiles >= 2 * sms) return 1;
+    if (g.parts > 0) return std::max(1, std::min(g.parts, chunks));
     return (int)std::max(1LL, std::min<long long>((8LL * sms + tiles - 1) / tiles, chunks / 4));
 }
 
@@ -97,7 +98,7 @@ size_t line_part(const Geom& g, int line) { return (size_t)line * 2 * 2 * kRows 
 }  // namespace
 
 int NA2D_TC_NAME(forward)(const Place& at, const Geom& g, const Scratch& scratch, const Operand& q, const Operand& k, const Operand& v,
-                          const Operand& o, float* lse) {
+                          const Operand& o, float* lse, Parts* parts) {
     const int sms = na2d_tc::sm_count(at.device);
     FwdCut cut{};
     cut.pairs = (g.tiles + 1) / 2;
@@ -112,7 +113,6 @@ int NA2D_TC_NAME(forward)(const Place& at, const Geom& g, const Scratch& scratch
         cut.part_lse = scratch.at + cut.splits * all_rows(g) * g.C;
     }
     if (o.wide && cut.splits == 1 && !cut.line) {
-        cut.keep = 1;
         cut.part_o = static_cast<float*>(o.ptr);
         cut.part_lse = lse;
     }
@@ -120,6 +120,11 @@ int NA2D_TC_NAME(forward)(const Place& at, const Geom& g, const Scratch& scratch
     cut.each = (chunks + cut.splits - 1) / cut.splits;
     cut.by_splits = Div(cut.splits);
     cut.by_pairs = Div(cut.pairs);
+    cut.even = g.parts > 0;
+    if (parts) {
+        *parts = cut.splits > 1 ? Parts{cut.part_o, cut.part_lse, cut.splits} : Parts{static_cast<const float*>(o.ptr), lse, 1};
+        cut.open = cut.splits > 1;
+    }
     const long long items = g.tiles > 1 ? (long long)g.units * cut.pairs * cut.splits : ((long long)g.units + 1) / 2;
     if (items > 0x3fffffffLL) return NA2D_ERR_TOO_LARGE;
     cut.items = (int)items;

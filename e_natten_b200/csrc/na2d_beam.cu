@@ -1,16 +1,16 @@
 // Beam search (include/na2d.h): the choice among all beams' next words, and caches that follow their beams.
 //
 // Choice.  Candidate (i, w) of a batch entry is worth  scores_i + logits_iw - ln sum_w e^logits_iw.
-// Bound by memory: the logits are read once, by select_rows_kernel: a block holds a segment of one beam's words in registers, forms
-// the segment's maximum and sum of exponentials, and finds its best words without sorting: with r = ceil(count / 8), the least of the
-// eight warps' r-th largest thread maxima is a bound that at least `count` words reach and few more do; those go to shared
-// memory, where each counts the better ones.  select_beams_kernel joins an entry's segments: sums in 64 bits, candidates by the
-// same bound.  (value, lowest beam, lowest word) is a total order, so nothing depends on the order in which candidates arrive.
+// Bound by memory: the logits are read once, by select_rows_kernel: a block takes a segment of one beam's words in chunks, the next one under
+// way, every thread with a running maximum and sum of exponentials of its own, and finds the best words without sorting: with r =
+// ceil(count / 8), the least of the eight warps' r-th largest thread maxima is a bound that at least `count` words reach and few more do;
+// those go to shared memory, where at the end each counts the better ones.  The bound is formed anew behind 1, 2, 4 ... chunks.
+// select_beams_kernel joins an entry's segments: sums in 64 bits, candidates by the same bound.  (value, lowest beam, lowest word) is a total order, so nothing depends on the order in which candidates arrive.
 //
 // Reordering.  cache[g K + i] <- cache[g K + parent_gi] for all beams of a group at once, in place: a thread has the same few bytes of
 // all K beams, reads what moves and then writes it, so that no second copy of a cache exists and beams that keep their place cost
-// nothing.  Bound by memory: each beam that others follow is read once (again from L1 where several follow it), each entry that moves
-// written once.
+// nothing.  Bound by memory: each beam that others follow is read once, each entry that moves written once.  Blocks of all
+// groups come in the order of their part of a beam, so that those behind the end of short groups, which have nothing to do, come last.
 #include <algorithm>
 
 #include "../../include/na2d.h"
@@ -66,6 +66,17 @@ __device__ __forceinline__ unsigned bound_of(unsigned largest, int count, unsign
     return least;
 }
 
+// The same for counts of at most 32, the best of the warps' bounds.
+__device__ __forceinline__ unsigned best_bound_of(unsigned largest, int count, unsigned* warps) {
+    const unsigned own = nth_largest(largest, count);
+    if (threadIdx.x % 32 == 0) warps[threadIdx.x / 32] = own;
+    __syncthreads();
+    unsigned most = warps[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) most = max(most, warps[w]);
+    return most;
+}
+
 struct Select {
     const void* logits;
     long long stride_b, stride_k;
@@ -80,17 +91,37 @@ struct Select {
     long long *out_parents, *out_words;
 };
 
-// e^x for x <= 0.  (1 / ln 2 in two numbers: sums of many beams are compared with one another.)
+// e^x for x <= 0.  (1 / ln 2 in one number: off by 1.4e-8 of x, the same way in every beam.)
 __device__ __forceinline__ float exp_of(float x) {
-    const float y = fmaf(x, 1.44269502f, x * 1.92596303e-8f);
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269502f));
     return r;
 }
 
-// E words a thread; N words a load, 1 where rows do not start on 16-byte boundaries.  Which thread has a word depends on the word and
-// N alone, so that equal rows have equal sums.
-template <typename T, int N, int E>
+constexpr int kEach = 16;                               // words that a thread has of a chunk
+constexpr int kChunk = kThreads * kEach;
+
+// N words a load, 1 where rows do not start on 16-byte boundaries.  Which thread has a word, and when, depends on the word and N
+// alone, so that equal rows have equal sums.
+template <typename T, int N>
+struct Piece {
+    Vec<T, N> part[kEach / N];
+    // words at + [0, kEach) of a row's `words`, N at a time, a chunk's threads side by side
+    __device__ __forceinline__ void load(const T* src, int chunk, int words) {
+#pragma unroll
+        for (int j = 0; j < kEach / N; ++j) {
+            const int at = chunk * kChunk + (j * kThreads + (int)threadIdx.x) * N;
+            if (at + N <= words) {
+                part[j].load(src + at);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) part[j].at[i] = at + i < words ? src[at + i] : na2d_vec::narrow<T>(-kInf);
+            }
+        }
+    }
+};
+
+template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) select_rows_kernel(const Select x) {
     __shared__ unsigned warps[kWarps];
     __shared__ float tops[kWarps], totals[kWarps];
@@ -102,54 +133,62 @@ __global__ void __launch_bounds__(kThreads) select_rows_kernel(const Select x) {
     if (x.finished && x.finished[row]) return;           // (nothing of it is read)
     const int first = segment * x.each, words = min(x.each, x.V - first), tid = threadIdx.x;
     const T* src = static_cast<const T*>(x.logits) + b * x.stride_b + k * x.stride_k + first;
-    float v[E];
+    const int chunks = (words + kChunk - 1) / kChunk;
+    auto key_of = [&](int chunk, int j, float v) {
+        const int word = first + chunk * kChunk + ((j / N) * kThreads + tid) * N + j % N;
+        return ((unsigned long long)ordered(v) << 32) | (unsigned)~word;
+    };
+    Piece<T, N> next;
+    next.load(src, 0, words);
+    if (tid == 0) kept_count = 0;
+    float high = -kInf, total = 0.f, least = -kInf;      // this thread's maximum and sum; what the block's best reach
+    int renew = 1;                                       // the bound is formed anew behind that many chunks
+    for (int c = 0; c < chunks; ++c) {
+        float v[kEach];
 #pragma unroll
-    for (int j = 0; j < E / N; ++j) {
-        const int at = (j * kThreads + tid) * N;
-        if (N > 1 && at + N <= words) {
-            Vec<T, N> piece;
-            piece.load(src + at);
+        for (int j = 0; j < kEach; ++j) v[j] = widen(next.part[j / N].at[j % N]);
+        if (c + 1 < chunks) next.load(src, c + 1, words);
+        float most = -kInf;
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[j * N + i] = widen(piece.at[i]);
-        } else {
+        for (int j = 0; j < kEach; ++j) most = fmaxf(most, v[j]);
+        if (most > high) {
+            total *= exp_of(high - most);                // (from -infinity on: a sum of nothing)
+            high = most;
+        }
+        const float base = high == -kInf ? 0.f : high;
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[j * N + i] = at + i < words ? widen(src[at + i]) : -kInf;
+        for (int j = 0; j < kEach; ++j) sum[j & 1] += exp_of(v[j] - base);
+        total += sum[0] + sum[1];
+        if (c + 1 == renew) {
+            __syncthreads();                             // (`warps` has been read)
+            const unsigned bound = bound_of(high == -kInf ? 0u : ordered(high), x.count, warps);
+            least = bound ? from_ordered(bound) : -kInf;
+            renew *= 2;
+        }
+        if (most >= least) {
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+                if (v[j] >= least && v[j] > -kInf) {
+                    const int at = atomicAdd(&kept_count, 1);
+                    if (at < kKept) kept[at] = key_of(c, j, v[j]);
+                }
         }
     }
-    if (tid == 0) kept_count = 0;
-    float high = -kInf;
-#pragma unroll
-    for (int j = 0; j < E; ++j) high = fmaxf(high, v[j]);
-    const unsigned bound = bound_of(high == -kInf ? 0u : ordered(high), x.count, warps);
-    {   // maximum and sum
+    {   // the block's maximum and sum
         float top = high;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         if (tid % 32 == 0) tops[tid / 32] = top;
-    }
-    __syncthreads();
-    float top = tops[0];
+        __syncthreads();
+        top = tops[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, tops[w]);
-    const float base = top == -kInf ? 0.f : top;
-    float sum[2] = {0.f, 0.f};
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, tops[w]);
+        total *= high == -kInf ? 1.f : exp_of(high - top);       // (a NaN among words of -infinity stays one)
 #pragma unroll
-    for (int j = 0; j < E; ++j) sum[j & 1] += exp_of(v[j] - base);
-    float total = sum[0] + sum[1];
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    if (tid % 32 == 0) totals[tid / 32] = total;
-    // the words that reach the bound
-    const float least = bound ? from_ordered(bound) : -kInf;
-    auto word_of = [&](int j) { return first + ((j / N) * kThreads + tid) * N + j % N; };
-    auto key_of = [&](int j) { return ((unsigned long long)ordered(v[j]) << 32) | (unsigned)~word_of(j); };
-    if (high >= least) {
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (v[j] >= least && v[j] > -kInf) {
-                const int at = atomicAdd(&kept_count, 1);
-                if (at < kKept) kept[at] = key_of(j);
-            }
+        for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+        if (tid % 32 == 0) totals[tid / 32] = total;
+        high = top;
     }
     __syncthreads();
     const size_t place = (size_t)row * x.segments + segment;
@@ -158,7 +197,7 @@ __global__ void __launch_bounds__(kThreads) select_rows_kernel(const Select x) {
     if (tid == 0) {
         total = 0.f;
         for (int w = 0; w < kWarps; ++w) total += totals[w];
-        x.sums[place] = make_float2(top, total);
+        x.sums[place] = make_float2(high, total);
     }
     if (n <= kKept) {
         for (int i = tid; i < n; i += kThreads) {
@@ -170,14 +209,18 @@ __global__ void __launch_bounds__(kThreads) select_rows_kernel(const Select x) {
         for (int i = n + tid; i < x.count; i += kThreads) best[i] = 0;
         return;
     }
-    // many equal words: the best of those below the last one, `count` times
+    // many words reach the bound (equal ones, ascending ones): the best of those below the last one, `count` times
     unsigned long long below = ~0ull;
     for (int r = 0; r < x.count; ++r) {
         unsigned long long own = 0;
+        for (int c = 0; c < chunks; ++c) {
+            next.load(src, c, words);
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            const unsigned long long key = v[j] > -kInf ? key_of(j) : 0;
-            if (key < below && key > own) own = key;
+            for (int j = 0; j < kEach; ++j) {
+                const float v = widen(next.part[j / N].at[j % N]);
+                const unsigned long long key = v > -kInf ? key_of(c, j, v) : 0;
+                if (key < below && key > own) own = key;
+            }
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) own = max(own, __shfl_xor_sync(0xffffffffu, own, d));
@@ -193,7 +236,10 @@ __global__ void __launch_bounds__(kThreads) select_rows_kernel(const Select x) {
 
 // A block an entry.
 __global__ void __launch_bounds__(kThreads) select_beams_kernel(const Select x) {
-    __shared__ double offset[kMostBeams];                // scores_i - lse_i; NaN: the beam has no candidates
+    // scores_i - ln sum_w e^(logits_iw - top_i), and top_i, which a logit's difference goes before all else (exact, whatever their size);
+    // NaN: the beam has no candidates
+    __shared__ double offset[kMostBeams];
+    __shared__ float tops[kMostBeams];
     __shared__ unsigned warps[kWarps];
     __shared__ unsigned long long kept[kKept];
     __shared__ long long names[kKept];                   // beam V + word
@@ -201,6 +247,20 @@ __global__ void __launch_bounds__(kThreads) select_beams_kernel(const Select x) 
     na2d_ptx::after_previous_grid();
     na2d_ptx::next_grid_may_start();
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 32;
+    const int lists = x.K * x.segments, n = lists * x.count;
+    const unsigned long long* best = x.best + (size_t)b * n;
+    auto key_at = [&](int c) { return best[(size_t)(c % lists) * x.count + c / lists]; };
+    // a thread's candidates are own_c, own_c + 256, ...; the keys of the first few are on their way meanwhile
+    constexpr int kHeld = 4;
+    const bool by_warp = x.count <= 32;
+    const int own_c = by_warp ? tid : tid % kWarps * 32 + tid / kWarps;
+    unsigned long long held[kHeld];
+    long long names_held[kHeld];
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+        held[u] = own_c + u * kThreads < n ? key_at(own_c + u * kThreads) : 0;
+        names_held[u] = 0;
+    }
     const double nan = __longlong_as_double(0x7ff8000000000000ll);
     for (int i = tid / 32; i < x.K; i += kWarps) {
         const int row = b * x.K + i;
@@ -222,41 +282,54 @@ __global__ void __launch_bounds__(kThreads) select_beams_kernel(const Select x) 
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-        if (lane == 0) offset[i] = counts && total > 0.0 ? (double)score - ((double)top + log(total)) : nan;
+        if (lane == 0) {
+            offset[i] = counts && total > 0.0 ? (double)score - log(total) : nan;
+            tops[i] = top;
+        }
     }
     if (tid == 0) kept_count = 0;
     __syncthreads();
-    const int per_beam = x.segments * x.count, n = x.K * per_beam;
-    const unsigned long long* best = x.best + (size_t)b * n;
-    // worth of candidate c (0: none) and its name
-    auto worth = [&](int c, long long& name) -> unsigned long long {
-        const int i = c / per_beam;
+    // worth of candidate c (0: none) and its name, from its key.  Candidates lie list after list, a list a segment's best; c counts through all
+    // lists' first ones, then their second ones.
+    auto worth = [&](int c, unsigned long long key, long long& name) -> unsigned long long {
+        const int list = c % lists, i = list / x.segments;
         const double by = offset[i];
         if (!(by == by)) {
             const int row = b * x.K + i;
-            if (c != i * per_beam || !x.finished || !x.finished[row]) return 0;
+            if (c != i * x.segments || !x.finished || !x.finished[row]) return 0;
             const float score = x.scores[row];           // a beam that has ended: itself
             name = (long long)i * x.V + x.end;
             return score > -kInf && score < kInf ? ordered((double)score) : 0;
         }
-        const unsigned long long key = best[c];
         if (!key) return 0;
         name = (long long)i * x.V + (unsigned)~(unsigned)key;
-        return ordered(by + (double)from_ordered((unsigned)(key >> 32)));
+        return ordered(by + ((double)from_ordered((unsigned)(key >> 32)) - (double)tops[i]));
     };
-    long long name = 0;
     unsigned high = 0;
-    for (int c = tid; c < n; c += kThreads) high = max(high, (unsigned)(worth(c, name) >> 32));
-    const unsigned bound = max(bound_of(high, x.count, warps), 1u);
-    if (high >= bound)
-        for (int c = tid; c < n; c += kThreads) {
-            const unsigned long long own = worth(c, name);
-            if ((unsigned)(own >> 32) < bound) continue;
-            const int at = atomicAdd(&kept_count, 1);
-            if (at >= kKept) continue;
-            kept[at] = own;
-            names[at] = name;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+        held[u] = own_c + u * kThreads < n ? worth(own_c + u * kThreads, held[u], names_held[u]) : 0;
+        high = max(high, (unsigned)(held[u] >> 32));
+    }
+    long long name = 0;
+    for (int c = own_c + kHeld * kThreads; c < n; c += kThreads) high = max(high, (unsigned)(worth(c, key_at(c), name) >> 32));
+    // (up to 32 candidates: a warp's `count`-th largest is a bound by itself, and the warp of the lists' first ones has a good one)
+    const unsigned bound = max(by_warp ? best_bound_of(high, x.count, warps) : bound_of(high, x.count, warps), 1u);
+    auto keep = [&](unsigned long long own, long long called) {
+        if ((unsigned)(own >> 32) < bound) return;
+        const int at = atomicAdd(&kept_count, 1);
+        if (at >= kKept) return;
+        kept[at] = own;
+        names[at] = called;
+    };
+    if (high >= bound) {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) keep(held[u], names_held[u]);
+        for (int c = own_c + kHeld * kThreads; c < n; c += kThreads) {
+            const unsigned long long own = worth(c, key_at(c), name);
+            keep(own, name);
         }
+    }
     __syncthreads();
     const int m = kept_count;
     auto put = [&](int r, unsigned long long own, long long called) {
@@ -287,7 +360,7 @@ __global__ void __launch_bounds__(kThreads) select_beams_kernel(const Select x) 
             }
         };
         for (int c = tid; c < n; c += kThreads) {
-            const unsigned long long w = worth(c, name);
+            const unsigned long long w = worth(c, key_at(c), name);
             if (w < last || (w == last && name > last_name)) take(w, name);
         }
 #pragma unroll
@@ -309,14 +382,15 @@ __global__ void __launch_bounds__(kThreads) select_beams_kernel(const Select x) 
     }
 }
 
-// Segments of a row: as many words as a block holds, fewer where that would leave SMs without two blocks.
+// Segments of a row: so many chunks each, up to 16, as give all SMs their four blocks.  A block that lives long has its loads under way for more of
+// its time: 64 x 8 rows of 131072 words in fp32 take 56 us with 16 chunks a block (1024 blocks), 63 with 7.
 struct Cut {
-    int words, segments, each;          // words: a block's
+    int segments, each;                 // each: words of one
 };
 Cut cut_of(int rows, int V, int sms) {
+    const long long chunks = (V + kChunk - 1) / kChunk, of_block = std::max(1LL, std::min(16LL, rows * chunks / (4LL * sms)));
     Cut c;
-    c.words = (long long)rows * ((V + 8191) / 8192) >= 2 * sms ? 8192 : 2048;
-    c.segments = (V + c.words - 1) / c.words;
+    c.segments = (int)((chunks + of_block - 1) / of_block);
     c.each = ((V + c.segments - 1) / c.segments + 7) / 8 * 8;
     c.segments = (V + c.each - 1) / c.each;
     return c;
@@ -334,9 +408,7 @@ int check_select(const na2d_beam_select_args* a) {
 
 template <typename T, int N>
 int launch_rows(const Select& x, const Cut& c, cudaStream_t st) {
-    const unsigned blocks = (unsigned)((long long)x.B * x.K * c.segments);
-    const cudaError_t e = c.words == 8192 ? na2d_launch::launch(true, select_rows_kernel<T, N, 32>, blocks, kThreads, 0, st, x)
-                                          : na2d_launch::launch(true, select_rows_kernel<T, N, 8>, blocks, kThreads, 0, st, x);
+    const cudaError_t e = na2d_launch::launch(true, select_rows_kernel<T, N>, (unsigned)((long long)x.B * x.K * c.segments), kThreads, 0, st, x);
     return e == cudaSuccess ? NA2D_OK : na2d_host::cuda_fail(e, "beam selection launch");
 }
 template <typename T>
@@ -363,62 +435,88 @@ struct Reorder {
     int blocks;                         // of a group
 };
 
-// V: the piece that a thread has of every beam.
-template <typename V, int MOST>
+// V: the piece that a thread has of every beam, kPieces of them under way at once.
+constexpr int kRuns = 8;                                // of 256 pieces, that a block takes
+template <typename V, int MOST, int PIECES>
 __global__ void __launch_bounds__(kThreads) reorder_kernel(const __grid_constant__ Reorder x) {
-    __shared__ int from[kMostBeams], length[kMostBeams];
-    __shared__ int longest;
+    __shared__ unsigned takers[kMostBeams];              // of a beam: bit i for beam i
+    __shared__ int length[kMostBeams];
     na2d_ptx::after_previous_grid();
     na2d_ptx::next_grid_may_start();
     const Cache& c = x.cache[blockIdx.y];
-    const int group = blockIdx.x / x.blocks, part = blockIdx.x - group * x.blocks;
-    if (threadIdx.x < 32) {
-        const int i = threadIdx.x;
-        int parent = i, tokens = 0;
+    const int group = blockIdx.x % x.B, part = blockIdx.x / x.B;
+    int longest = 0;                                     // of the beams that others follow (every warp by itself)
+    {
+        const int i = threadIdx.x & 31;
+        int parent = i;
         if (i < x.K) {
             const size_t at = (size_t)group * x.K + i;
             const long long p = x.parents_64 ? static_cast<const long long*>(x.parents)[at] : static_cast<const int*>(x.parents)[at];
             parent = p >= 0 && p < x.K ? (int)p : i;     // (no such beam: it stays)
-            if (parent != i) {
-                const size_t of = (size_t)group * x.K + parent;
-                const long long n = !x.lengths ? c.tokens : x.lengths_64 ? static_cast<const long long*>(x.lengths)[of] : static_cast<const int*>(x.lengths)[of];
-                tokens = (int)min(max(n, 0ll), (long long)c.tokens);
-            }
         }
-        from[i] = parent;
-        length[i] = tokens;                              // that move
-        const int most = __reduce_max_sync(0xffffffffu, tokens);
-        if (i == 0) longest = most;
+        unsigned mine = 0;
+        for (int k = 0; k < x.K; ++k) {
+            const int of = __shfl_sync(0xffffffffu, parent, k);
+            if (of == i && k != i) mine |= 1u << k;
+        }
+        int tokens = 0;
+        if (mine) {
+            const size_t at = (size_t)group * x.K + i;
+            const long long n = !x.lengths ? c.tokens : x.lengths_64 ? static_cast<const long long*>(x.lengths)[at] : static_cast<const int*>(x.lengths)[at];
+            tokens = (int)min(max(n, 0ll), (long long)c.tokens);
+        }
+        longest = __reduce_max_sync(0xffffffffu, tokens);
+        if (threadIdx.x < 32) {
+            takers[i] = mine;
+            length[i] = tokens;
+        }
     }
-    __syncthreads();
     const unsigned pieces = c.pieces, tokens = longest, heads = c.heads;
-    const unsigned all = pieces * tokens * heads;        // (below 2^31)
+    const unsigned all = pieces * tokens * heads;        // (at most 2^30)
+    const unsigned begin = part * (kRuns * kThreads), end = min(all, begin + kRuns * kThreads);
+    if (begin >= all) return;
+    __syncthreads();
     char* base = c.at + (long long)group * x.K * c.e;
-    for (unsigned i = part * kThreads + threadIdx.x; i < all; i += x.blocks * kThreads) {
-        const unsigned row = i / pieces, p = i - row * pieces;
-        unsigned h, t;
-        if (c.heads_first) {
-            t = row / heads;
-            h = row - t * heads;
-        } else {
-            h = row / tokens;
-            t = row - h * tokens;
+    for (unsigned first = begin + threadIdx.x; first < end; first += PIECES * kThreads) {
+        char* at[PIECES];
+        int t[PIECES];
+        V v[PIECES][MOST];
+#pragma unroll
+        for (int u = 0; u < PIECES; ++u) {
+            const unsigned i = first + u * kThreads, row = i / pieces, p = i - row * pieces;
+            unsigned h;
+            if (c.heads_first) {
+                t[u] = row / heads;
+                h = row - t[u] * heads;
+            } else {
+                h = row / tokens;
+                t[u] = row - h * tokens;
+            }
+            if (i >= end) t[u] = 0x7fffffff;             // no piece
+            at[u] = base + h * c.h + t[u] * c.t + (long long)p * sizeof(V);
         }
-        char* at = base + h * c.h + t * c.t + (long long)p * sizeof(V);
-        V v[MOST];
 #pragma unroll
         for (int k = 0; k < MOST; ++k)
-            if (k < x.K && (int)t < length[k]) v[k] = *reinterpret_cast<const V*>(at + from[k] * c.e);
+            if (k < x.K && takers[k]) {
+#pragma unroll
+                for (int u = 0; u < PIECES; ++u)
+                    if (t[u] < length[k]) v[u][k] = *reinterpret_cast<const V*>(at[u] + k * c.e);
+            }
 #pragma unroll
         for (int k = 0; k < MOST; ++k)
-            if (k < x.K && (int)t < length[k]) *reinterpret_cast<V*>(at + k * c.e) = v[k];
+            for (unsigned left = k < x.K ? takers[k] : 0u; left; left &= left - 1) {
+                const int i = __ffs(left) - 1;
+#pragma unroll
+                for (int u = 0; u < PIECES; ++u)
+                    if (t[u] < length[k]) *reinterpret_cast<V*>(at[u] + i * c.e) = v[u][k];
+            }
     }
 }
 
 template <typename V>
 int launch_reorder(const Reorder& x, int caches, cudaStream_t st) {
     const dim3 grid((unsigned)(x.B * x.blocks), (unsigned)caches);
-    auto kern = x.K <= 4 ? reorder_kernel<V, 4> : x.K <= 8 ? reorder_kernel<V, 8> : x.K <= 16 ? reorder_kernel<V, 16> : reorder_kernel<V, 32>;
+    auto kern = x.K <= 4 ? reorder_kernel<V, 4, 4> : x.K <= 8 ? reorder_kernel<V, 8, 2> : x.K <= 16 ? reorder_kernel<V, 16, 1> : reorder_kernel<V, 32, 1>;
     const cudaError_t e = na2d_launch::launch(true, kern, grid, kThreads, 0, st, x);
     if (e != cudaSuccess) return na2d_host::cuda_fail(e, "beam reordering launch");
     na2d_host::count_launches(1);
@@ -506,9 +604,8 @@ int na2d_beam_reorder(const na2d_beam_reorder_args* a) {
             x.lengths = a->lengths;
             x.parents_64 = a->parents_64 != 0;
             x.lengths_64 = a->lengths_64 != 0;
-            // a block for each of the largest cache's stretches of 256 pieces, at most four rounds of eight blocks an SM in all
-            const long long needed = (most / piece + kThreads - 1) / kThreads, room = std::max(1LL, 32LL * sms / ((long long)n * a->B));
-            x.blocks = (int)std::min(needed, room);
+            x.blocks = (int)((most / piece + kRuns * kThreads - 1) / (kRuns * kThreads));
+            if ((long long)x.blocks * x.B > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
             const int rc = piece == 16  ? launch_reorder<uint4>(x, n, (cudaStream_t)a->stream)
                            : piece == 4 ? launch_reorder<uint32_t>(x, n, (cudaStream_t)a->stream)
                                         : launch_reorder<uint8_t>(x, n, (cudaStream_t)a->stream);

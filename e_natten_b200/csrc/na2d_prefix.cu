@@ -13,6 +13,7 @@
 #include "na2d_attn_entry.h"
 #include "na2d_host.h"
 #include "na2d_launch.h"
+#include "na2d_prefix_entry.h"
 #include "na2d_vec.cuh"
 
 namespace {
@@ -133,6 +134,14 @@ struct Problem {
     bool follow[3];         // whether q's (o's, d_o's) rows of an entry follow those of the one before
 };
 
+// Parts of a prefix's keys where the tiles of rows, two an item, are at most half as many as the SMs: as many as make one round.  32 heads on 8
+// key heads of 16384 keys, 64 answers of one token: 90 us with one round, 101 with two, 122 with four, 100 with attention's own rule.
+int even_parts(const Geom& g, int sms) {
+    const long long items = (long long)g.units * ((g.tiles + 1) / 2);
+    if (g.tiles == 1 || items > sms / 2) return 0;
+    return (int)(sms / items);
+}
+
 int make_problem(const na2d_prefix_attention_args* a, Problem* p) {
     if (!a || a->struct_size < sizeof(na2d_prefix_attention_args)) return NA2D_ERR_BAD_ARG;
     if (a->B <= 0 || a->S <= 0 || a->N <= 0 || a->Nk <= 0 || a->Tq <= 0 || a->P <= 0 || a->Tk < 0 || a->C <= 0) return NA2D_ERR_BAD_ARG;
@@ -159,6 +168,7 @@ int make_problem(const na2d_prefix_attention_args* a, Problem* p) {
         return g;
     };
     p->prefix = geometry(a->S, A * a->Tq, a->P, false, a->prefix_lengths);
+    p->prefix.parts = even_parts(p->prefix, na2d_host::sm_count(a->device));
     if (p->any_own) p->own = geometry(a->B, a->Tq, a->Tk, a->causal != 0, a->key_lengths);
     auto operand = [&](const na2d_heads& x, int B, int heads, int T) {
         const na2d_host::HeadStrides s = na2d_host::head_strides(x, B, heads, T, a->C);
@@ -193,25 +203,48 @@ struct Layout {
         return at;
     }
 };
+// Which kind of keys goes on the line of few rows (na2d_prefix_tokens.cuh): its units' rows fit.
+struct OnLine {
+    bool prefix, own;
+    bool any() const { return prefix || own; }
+};
+OnLine on_line(const Problem& p) {
+    const Rows& g = p.rows;
+    const long long most = na2d_prefix::kTokenRows, own = (long long)p.prefix.G * g.Tq;
+    const long long steps = (p.S * ((p.prefix.Tk + 15LL) / 16 + 1) + (p.any_own ? p.B * ((p.own.Tk + 15LL) / 16 + 1) : 0)) * p.prefix.Nk;
+    if (!p.tensor || (long long)p.S + p.B > na2d_prefix::kTokenEntries || steps > (1 << 30)) return {false, false};
+    return {own * g.A <= most, p.any_own && own <= most};
+}
+// Rows of the parts of one side on the line: from part to part either the warp or the unit is one more.
+size_t line_rows(const Geom& g, int sms) { return ((size_t)g.units + na2d_prefix::token_warps(sms)) * g.G * g.Tq; }
+
 struct ForwardLayout {
-    size_t q, o_prefix, lse_prefix, o_own, lse_own, scratch, scratch_bytes, size;
+    size_t q, o_prefix, lse_prefix, o_own, lse_own, scratch, scratch_bytes, own_scratch, own_scratch_bytes, table, part_o, part_lse, size;
 };
 ForwardLayout forward_layout(const Problem& p, int sms) {
     Layout l;
     ForwardLayout f{};
     const size_t rows = p.rows.all, values = rows * p.rows.C;
-    if (!p.follow[0]) f.q = l.take(values * esize_of(p));
-    f.o_prefix = l.take(values * 4);
-    f.lse_prefix = l.take(rows * 4);
-    if (p.any_own) {
+    const OnLine line = on_line(p);
+    if (!line.prefix) {
+        if (!p.follow[0]) f.q = l.take(values * esize_of(p));
+        f.o_prefix = l.take(values * 4);
+        f.lse_prefix = l.take(rows * 4);
+        if (p.tensor) f.scratch_bytes = na2d_attn::forward_floats(p.prefix, sms) * 4;
+    }
+    if (p.any_own && !line.own) {
         f.o_own = l.take(values * 4);
         f.lse_own = l.take(rows * 4);
-    }
-    if (p.tensor) {
-        f.scratch_bytes = na2d_attn::forward_floats(p.prefix, sms) * 4;
-        if (p.any_own) f.scratch_bytes = std::max(f.scratch_bytes, na2d_attn::forward_floats(p.own, sms) * 4);
+        if (p.tensor) f.own_scratch_bytes = na2d_attn::forward_floats(p.own, sms) * 4;
     }
     f.scratch = l.take(f.scratch_bytes);
+    f.own_scratch = l.take(f.own_scratch_bytes);
+    if (line.any()) {
+        const size_t parts = (line.prefix ? line_rows(p.prefix, sms) : 0) + (line.own ? line_rows(p.own, sms) : 0);
+        f.table = l.take((na2d_prefix::kTokenEntries + 2) * sizeof(int));
+        f.part_o = l.take(parts * p.rows.C * 4);
+        f.part_lse = l.take(parts * 4);
+    }
     f.size = l.size;
     return f;
 }
@@ -271,9 +304,9 @@ int finish(int rc, int launched, const char* what) {
 }
 
 int forward_of(const Problem& p, const na2d_attn::Place& at, const Geom& g, const Scratch& s, const Operand& q, const Operand& k, const Operand& v,
-               const Operand& o, float* lse) {
+               const Operand& o, float* lse, na2d_attn::Parts* parts = nullptr) {
     if (!p.tensor) return na2d_attn::simt_forward(at, g, q, k, v, o, lse);
-    return p.dtype == NA2D_BF16 ? na2d_attn::forward_bf16(at, g, s, q, k, v, o, lse) : na2d_attn::forward_f16(at, g, s, q, k, v, o, lse);
+    return p.dtype == NA2D_BF16 ? na2d_attn::forward_bf16(at, g, s, q, k, v, o, lse, parts) : na2d_attn::forward_f16(at, g, s, q, k, v, o, lse, parts);
 }
 int backward_of(const Problem& p, const na2d_attn::Place& at, const Geom& g, const Scratch& s, const na2d_attn::Backward& x) {
     if (!p.tensor) return na2d_attn::simt_backward(at, g, x);
@@ -364,17 +397,49 @@ int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a) {
         if (int rc = place(a->dtype, a->device, a->stream, &launched, &at)) return rc;
         char* ws = static_cast<char*>(a->workspace);
         auto floats = [&](size_t where) { return reinterpret_cast<float*>(ws + where); };
-        const Scratch scratch{floats(f.scratch), f.scratch_bytes / 4};
+        const Scratch scratch{floats(f.scratch), f.scratch_bytes / 4}, own_scratch{floats(f.own_scratch), f.own_scratch_bytes / 4};
+        const OnLine line = on_line(p);
         auto run = [&]() -> int {
-            Operand q = p.follow[0] ? merged(p, p.q) : merged_copy(p, ws + f.q);
-            if (!p.follow[0]) {
-                const Operand* from = &p.q;
-                char* to = ws + f.q;
-                if (int rc = gather(at, p, &from, &to, 1, nullptr, nullptr)) return rc;
+            na2d_attn::Parts prefix{}, own{};
+            if (!line.prefix) {
+                Operand q = p.follow[0] ? merged(p, p.q) : merged_copy(p, ws + f.q);
+                if (!p.follow[0]) {
+                    const Operand* from = &p.q;
+                    char* to = ws + f.q;
+                    if (int rc = gather(at, p, &from, &to, 1, nullptr, nullptr)) return rc;
+                }
+                if (int rc = forward_of(p, at, p.prefix, scratch, q, p.pk, p.pv, sums(p, floats(f.o_prefix), p.prefix.Tq), floats(f.lse_prefix),
+                                        line.any() ? &prefix : nullptr))
+                    return rc;
             }
-            if (int rc = forward_of(p, at, p.prefix, scratch, q, p.pk, p.pv, sums(p, floats(f.o_prefix), p.prefix.Tq), floats(f.lse_prefix))) return rc;
-            if (p.any_own)
-                if (int rc = forward_of(p, at, p.own, scratch, p.q, p.k, p.v, sums(p, floats(f.o_own), p.own.Tq), floats(f.lse_own))) return rc;
+            if (p.any_own && !line.own)
+                if (int rc = forward_of(p, at, p.own, own_scratch, p.q, p.k, p.v, sums(p, floats(f.o_own), p.own.Tq), floats(f.lse_own),
+                                        line.any() ? &own : nullptr))
+                    return rc;
+            if (line.any()) {
+                na2d_prefix::Tokens x{};
+                auto side = [&](int which, const Geom& g, const Operand& k, const Operand& v, int share, size_t first_row) {
+                    x.side[which] = na2d_prefix::TokenSide{k, v, g.lengths, g.B, g.Tk, share, g.G * g.Tq, first_row};
+                };
+                const size_t rows = line.prefix ? line_rows(p.prefix, na2d_host::sm_count(a->device)) : 0;
+                if (line.prefix) side(0, p.prefix, p.pk, p.pv, p.rows.A, 0);
+                if (line.own) side(1, p.own, p.k, p.v, 1, rows);
+                x.q = p.q;
+                x.N = p.rows.N;
+                x.Nk = p.prefix.Nk;
+                x.G = p.prefix.G;
+                x.Tq = p.rows.Tq;
+                x.C = p.rows.C;
+                x.causal = p.any_own && p.own.causal;
+                x.sl2 = p.prefix.sl2;
+                x.table = reinterpret_cast<int*>(ws + f.table);
+                x.part_o = floats(f.part_o);
+                x.part_lse = floats(f.part_lse);
+                const size_t stride = (size_t)p.rows.all;
+                const na2d_prefix::JoinSide by_prefix{prefix.o, prefix.lse, stride, prefix.count, p.rows.A}, by_own{own.o, own.lse, stride, own.count, 1};
+                return p.dtype == NA2D_BF16 ? na2d_prefix::tokens_bf16(at, x, by_prefix, by_own, a->o.ptr, a->lse, p.B, launched > 0)
+                                            : na2d_prefix::tokens_f16(at, x, by_prefix, by_own, a->o.ptr, a->lse, p.B, launched > 0);
+            }
             const float *o_own = p.any_own ? floats(f.o_own) : nullptr, *lse_own = p.any_own ? floats(f.lse_own) : nullptr;
             return by_type(p, [&](auto type, auto n) {
                 return join_outputs<decltype(type), decltype(n)::value>(at, p, floats(f.o_prefix), floats(f.lse_prefix), o_own, lse_own, a->o.ptr, a->lse);

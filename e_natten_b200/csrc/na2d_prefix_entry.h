@@ -1,0 +1,46 @@
+// Host entry points of the kernels for few query rows on a shared prefix and own keys, compiled once per 16-bit element type
+// (na2d_prefix_tc.cu with -DNA2D_TC_DT=1 for bf16 and 2 for fp16).
+#pragma once
+
+#include "na2d_attn.cuh"
+
+namespace na2d_prefix {
+
+constexpr int kTokenEntries = 4096;     // prefixes and batch entries on the line, at most
+constexpr int kTokenLeast = 2;          // steps of 16 keys that a warp takes
+constexpr int kUnitSteps = 1;           // steps that a unit counts for beside those of its keys
+
+// One kind of keys: prefixes, or the entries' own.
+struct TokenSide {
+    na2d_attn::Operand k, v;            // (entries, Nk, T, C)
+    const int* lengths;
+    int entries, T;                     // entries 0: this side is not on the line
+    int share;                          // batch entries of one
+    int rows;                           // of a unit: G share Tq, row (h share + a) Tq + t
+    size_t first_row;                   // of its parts in the workspace
+};
+struct Tokens {
+    TokenSide side[2];                  // prefixes, own
+    na2d_attn::Operand q;               // (B, N, Tq, C)
+    int N, Nk, G, Tq, C, causal;
+    float sl2;
+    int* table;                         // steps before each entry, of all, and those of a warp
+    float *part_o, *part_lse;
+};
+// Where a row's sums of one kind of keys come from: the line (count 0), or another kernel's results, (count, entries, N, share Tq).
+struct JoinSide {
+    const float *o, *lse;
+    size_t stride;                      // rows from one to the next
+    int count, share;
+};
+
+// Query rows of a unit that the kernel takes, at most.
+constexpr int kTokenRows = 32;
+// Warps of the line.
+inline int token_warps(int sms) { return sms * 8; }
+
+// `behind`: another kernel of the same call has been launched before.
+int tokens_bf16(const na2d_attn::Place& at, const Tokens& x, const JoinSide& prefix, const JoinSide& own, void* o, float* lse, int B, bool behind);
+int tokens_f16(const na2d_attn::Place& at, const Tokens& x, const JoinSide& prefix, const JoinSide& own, void* o, float* lse, int B, bool behind);
+
+}  // namespace na2d_prefix

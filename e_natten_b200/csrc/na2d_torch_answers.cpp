@@ -44,7 +44,7 @@ using PrefixForward = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, c
 using PrefixBackward = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const MaybeTensor&, const MaybeTensor&, const Tensor&,
                                            const Tensor&, const Tensor&, const MaybeTensor&, const MaybeTensor&, double, bool, int64_t, bool, bool, bool);
 using Select = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, int64_t, const MaybeTensor&, int64_t);
-using Reorder = void(at::TensorList, const Tensor&, const MaybeTensor&);
+using Reordered = Tensor(const Tensor&, const Tensor&, const MaybeTensor&);
 
 bool is_whole(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
 
@@ -348,6 +348,7 @@ std::tuple<Tensor, Tensor, Tensor> select_op(const Tensor& logits_in, const Tens
     return {out_scores, parents, words};
 }
 std::tuple<Tensor, Tensor, Tensor> select(const Tensor& logits, const Tensor& scores, int64_t count, const MaybeTensor& finished, int64_t end) {
+    check_map(logits, "logits");
     TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(logits.requires_grad() || scores.requires_grad()), "beam_select has no gradient");
     if (goes_through({logits, scores, finished.value_or(Tensor())})) {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -387,7 +388,7 @@ bool rows_of_cache(const Tensor& t, int64_t entries, na2d_cache* c) {
     return true;
 }
 
-void reorder_op(at::TensorList caches, const Tensor& parents_in, const MaybeTensor& lengths_in) {
+void reorder_in_place(at::TensorList caches, const Tensor& parents_in, const MaybeTensor& lengths_in) {
     TORCH_CHECK_VALUE(parents_in.is_cuda() && parents_in.layout() == at::kStrided, "parents: e_natten_b200 runs on CUDA tensors only (there is no CPU path)");
     TORCH_CHECK_VALUE(parents_in.dim() == 2 && parents_in.size(1) > 0 && is_whole(parents_in), "parents must be an int32 or int64 tensor of (B, beams)");
     check_plain(parents_in, "parents");
@@ -455,16 +456,23 @@ void reorder_op(at::TensorList caches, const Tensor& parents_in, const MaybeTens
     }
 }
 void reorder(const std::vector<Tensor>& caches, const Tensor& parents, const MaybeTensor& lengths) {
+    TORCH_CHECK_VALUE(parents.is_cuda(), "parents: e_natten_b200 runs on CUDA tensors only (there is no CPU path)");
     bool through = goes_through({parents, lengths.value_or(Tensor())});
     for (const Tensor& t : caches) {
+        TORCH_CHECK_VALUE(t.is_cuda(), "caches must be on parents' device");
         TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !t.requires_grad(), "beam_reorder has no gradient");
         through = through || goes_through({t});
     }
-    if (through) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        return operator_of<Reorder>("e_natten_b200::beam_reorder_").call(caches, parents, lengths);
-    }
-    reorder_op(caches, parents, lengths);
+    if (!through) return reorder_in_place(caches, parents, lengths);
+    at::AutoDispatchBelowADInplaceOrView below;
+    for (Tensor t : caches) t.copy_(operator_of<Reordered>("e_natten_b200::beam_reordered").call(t, parents, lengths));
+}
+// The operator: a cache of its own.  (Whoever records calls follows what copy_ changes; an operator without a result is dropped from a trace.)
+Tensor reordered_op(const Tensor& cache, const Tensor& parents, const MaybeTensor& lengths) {
+    TORCH_CHECK_VALUE(cache.is_cuda() && cache.device() == parents.device(), "caches must be on parents' device");
+    Tensor mine = cache.clone();
+    reorder_in_place({mine}, parents, lengths);
+    return mine;
 }
 
 TORCH_LIBRARY_FRAGMENT(e_natten_b200, m) {
@@ -474,13 +482,13 @@ TORCH_LIBRARY_FRAGMENT(e_natten_b200, m) {
           "Tensor? key_lengths, Tensor? prefix_lengths, float scale, bool causal, int path, bool need_dq, bool need_dprefix, bool need_dkdv) "
           "-> Tensor[]");
     m.def("beam_select(Tensor logits, Tensor scores, int count, Tensor? finished, int end) -> (Tensor, Tensor, Tensor)");
-    m.def("beam_reorder_(Tensor(a!)[] caches, Tensor parents, Tensor? lengths) -> ()");
+    m.def("beam_reordered(Tensor cache, Tensor parents, Tensor? lengths) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(e_natten_b200, CUDA, m) {
     m.impl("prefix_attention", &prefix_forward_op);
     m.impl("prefix_attention_backward", &prefix_backward_op);
     m.impl("beam_select", &select_op);
-    m.impl("beam_reorder_", &reorder_op);
+    m.impl("beam_reordered", &reordered_op);
 }
 TORCH_LIBRARY_IMPL(e_natten_b200, Autograd, m) {
     m.impl("prefix_attention", &prefix_autograd);
