@@ -853,7 +853,7 @@ int launch_fwd_as(const Place& at, const Geom& g, const FwdCut& cut, const Opera
     const int sms = na2d_tc::sm_count(at.device);
     *at.launched += 1;
     const int grid = cut.line ? cut.line / 2 : cut.items < sms ? cut.items : sms;
-    if (na2d_launch::launch(false, kern, grid, 512, C::SMEM, at.st, tq, tk, tv, to, (DT*)o.ptr, o, lse,
+    if (na2d_launch::launch(WIDE, kern, grid, 512, C::SMEM, at.st, tq, tk, tv, to, (DT*)o.ptr, o, lse,
                             at.errors, g, cut) != cudaSuccess)
         return NA2D_ERR_CUDA;
     return (cut.splits == 1 && !cut.line) || cut.open ? NA2D_OK : launch_combine<DT>(at, g, cut, o, lse);

@@ -29,14 +29,29 @@ constexpr int kThreads = 256;
 // Rows of the whole batch: entry b = s A + a has prefix s.
 struct Rows {
     int A, N, Tq, C;
-    long long all;          // B N Tq
+    long long all;          // B N Tq, below 2^31
+    na2d_attn::Div by_a, by_n, by_tq;
 };
-// Place of row `r` of (B, N, Tq) in (S, N, A, Tq).
-__device__ __forceinline__ long long by_prefix(const Rows& g, long long r) {
-    const long long bn = r / g.Tq, b = bn / g.N, s = b / g.A;
-    const int t = (int)(r - bn * g.Tq), n = (int)(bn - b * g.N), a = (int)(b - s * g.A);
-    return ((s * g.N + n) * g.A + a) * g.Tq + t;
+struct Row {
+    int b, n, t;
+    long long by_prefix;    // its place in (S, N, A, Tq)
+};
+// Row `r` of (B, N, Tq).
+__device__ __forceinline__ Row row_of(const Rows& g, int r) {
+    Row x;
+    x.b = g.by_n.split(g.by_tq.split(r, x.t), x.n);
+    int a = 0, s = x.b;
+    if (g.A > 1) s = g.by_a.split(x.b, a);
+    x.by_prefix = (((long long)s * g.N + x.n) * g.A + a) * g.Tq + x.t;
+    return x;
 }
+// The row and the piece of it, of `by.d`, that a thread has; a block has whole rows.
+__device__ __forceinline__ bool piece_of(const Rows& g, const na2d_attn::Div& by, int& r, int& piece) {
+    const int rows = kThreads / (int)by.d, own = by.split(threadIdx.x, piece);
+    r = blockIdx.x * rows + own;
+    return own < rows && r < g.all;
+}
+unsigned blocks_of(const Rows& g, int pieces) { return (unsigned)((g.all + kThreads / pieces - 1) / (kThreads / pieces)); }
 
 // ---- rows in the prefixes' order ----------------------------------------------------------------------------------------
 struct Gather {
@@ -46,82 +61,78 @@ struct Gather {
     const float* lse;       // null: none
     float* lse_to;
     int tensors;
-    int row_bytes;
+    na2d_attn::Div by_pieces;           // of a row
 };
 template <typename V>
-__global__ void __launch_bounds__(kThreads) gather_rows_kernel(const Rows g, const Gather x) {
+__global__ void __launch_bounds__(kThreads) gather_rows_kernel(const __grid_constant__ Rows g, const __grid_constant__ Gather x) {
+    int r, c;
+    const bool there = piece_of(g, x.by_pieces, r, c);
+    const Row row = row_of(g, there ? r : 0);
     na2d_ptx::after_previous_grid();
     na2d_ptx::next_grid_may_start();
-    const int which = blockIdx.y, per = which < x.tensors ? x.row_bytes / (int)sizeof(V) : 1;
-    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x, r = i / per;
-    if (r >= g.all) return;
-    const int c = (int)(i - r * per);
-    const long long to = by_prefix(g, r);
+    if (!there) return;
+    const int which = blockIdx.y;
     if (which == x.tensors) {
-        x.lse_to[to] = x.lse[r];
+        if (c == 0) x.lse_to[row.by_prefix] = x.lse[r];
         return;
     }
-    const long long bn = r / g.Tq, b = bn / g.N;
-    const char* row = static_cast<const char*>(x.from[which]) + b * x.b[which] + (bn - b * g.N) * x.n[which] + (r - bn * g.Tq) * x.t[which];
-    reinterpret_cast<V*>(x.to[which])[to * per + c] = __ldg(reinterpret_cast<const V*>(row) + c);
+    const char* from = static_cast<const char*>(x.from[which]) + row.b * x.b[which] + row.n * x.n[which] + row.t * x.t[which];
+    reinterpret_cast<V*>(x.to[which])[row.by_prefix * (int)x.by_pieces.d + c] = __ldg(reinterpret_cast<const V*>(from) + c);
 }
 
 // ---- joins ----------------------------------------------------------------------------------------------------------------
 // o and lse of a row from the prefix's and its own; a thread has N channels.
 template <typename DT, int N>
 __global__ void __launch_bounds__(kThreads)
-join_outputs_kernel(const Rows g, const float* __restrict__ o_prefix, const float* __restrict__ lse_prefix, const float* __restrict__ o_own,
-                    const float* __restrict__ lse_own, DT* __restrict__ o, float* __restrict__ lse) {
+join_outputs_kernel(const __grid_constant__ Rows g, const na2d_attn::Div by_pieces, const float* __restrict__ o_prefix,
+                    const float* __restrict__ lse_prefix, const float* __restrict__ o_own, const float* __restrict__ lse_own, DT* __restrict__ o,
+                    float* __restrict__ lse) {
+    int r, c;
+    const bool there = piece_of(g, by_pieces, r, c);
+    const Row row = row_of(g, there ? r : 0);
     na2d_ptx::after_previous_grid();
     na2d_ptx::next_grid_may_start();
-    const int per = g.C / N;
-    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x, r = i / per;
-    if (r >= g.all) return;
-    const int c = (int)(i - r * per) * N;
-    const long long p = by_prefix(g, r);
-    const float x = lse_prefix[p], y = lse_own ? lse_own[r] : -CUDART_INF_F;
+    if (!there) return;
+    const float x = lse_prefix[row.by_prefix], y = lse_own ? lse_own[r] : -CUDART_INF_F;
+    // (of rows that see nothing, nothing was written)
+    Vec<float, N> u, v;
+    if (x != -CUDART_INF_F) u.load(o_prefix + row.by_prefix * g.C + c * N);
+    if (y != -CUDART_INF_F) v.load(o_own + (long long)r * g.C + c * N);
     // (a NaN stays one: the maximum skips it, its weight does not)
     const float top = fmaxf(x, y), base = top == -CUDART_INF_F ? 0.f : top;
     const float wx = expf(x - base), wy = expf(y - base), total = wx + wy, inv = total == 0.f ? 0.f : 1.f / total;
     float out[N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) out[k] = 0.f;
-    Vec<float, N> v;
-    if (x != -CUDART_INF_F) {                            // (of rows that see nothing, nothing was written)
-        v.load(o_prefix + p * g.C + c);
-#pragma unroll
-        for (int k = 0; k < N; ++k) out[k] = v.at[k] * (wx * inv);
-    }
-    if (y != -CUDART_INF_F) {
-        v.load(o_own + r * g.C + c);
-#pragma unroll
-        for (int k = 0; k < N; ++k) out[k] = fmaf(v.at[k], wy * inv, out[k]);
+    for (int k = 0; k < N; ++k) {
+        out[k] = x != -CUDART_INF_F ? u.at[k] * (wx * inv) : 0.f;
+        if (y != -CUDART_INF_F) out[k] = fmaf(v.at[k], wy * inv, out[k]);
     }
     Vec<DT, N> to;
     to.round(out);
-    to.store(o + r * g.C + c);
+    to.store(o + (long long)r * g.C + c * N);
     if (c == 0) lse[r] = total == 0.f ? -CUDART_INF_F : base + logf(total);
 }
 
 // dq of a row: the sum of the prefix's and its own.
 template <typename DT, int N>
 __global__ void __launch_bounds__(kThreads)
-join_gradients_kernel(const Rows g, const float* __restrict__ prefix, const float* __restrict__ own, DT* __restrict__ d_q) {
+join_gradients_kernel(const __grid_constant__ Rows g, const na2d_attn::Div by_pieces, const float* __restrict__ prefix, const float* __restrict__ own,
+                      DT* __restrict__ d_q) {
+    int r, c;
+    const bool there = piece_of(g, by_pieces, r, c);
+    const Row row = row_of(g, there ? r : 0);
     na2d_ptx::after_previous_grid();
     na2d_ptx::next_grid_may_start();
-    const int per = g.C / N;
-    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x, r = i / per;
-    if (r >= g.all) return;
-    const int c = (int)(i - r * per) * N;
+    if (!there) return;
     Vec<float, N> x, y;
-    x.load(prefix + by_prefix(g, r) * g.C + c);
+    x.load(prefix + row.by_prefix * g.C + c * N);
+    if (own) y.load(own + (long long)r * g.C + c * N);
     float out[N];
-    if (own) y.load(own + r * g.C + c);
 #pragma unroll
     for (int k = 0; k < N; ++k) out[k] = own ? x.at[k] + y.at[k] : x.at[k];
     Vec<DT, N> to;
     to.round(out);
-    to.store(d_q + r * g.C + c);
+    to.store(d_q + (long long)r * g.C + c * N);
 }
 
 // ---- the problem ------------------------------------------------------------------------------------------------------------
@@ -156,7 +167,8 @@ int make_problem(const na2d_prefix_attention_args* a, Problem* p) {
     p->B = a->B;
     p->S = a->S;
     p->dtype = a->dtype;
-    p->rows = Rows{A, a->N, a->Tq, a->C, (long long)a->B * a->N * a->Tq};
+    p->rows = Rows{A, a->N, a->Tq, a->C, (long long)a->B * a->N * a->Tq, na2d_attn::Div(A), na2d_attn::Div(a->N), na2d_attn::Div(a->Tq)};
+    if (p->rows.all > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
     auto geometry = [&](int B, int Tq, int Tk, bool causal, const int* lengths) {
         Geom g{};
         g.B = B; g.N = a->N; g.Nk = a->Nk; g.Tq = Tq; g.Tk = Tk; g.C = a->C;
@@ -318,10 +330,10 @@ int gather(const na2d_attn::Place& at, const Problem& p, const Operand* const* f
     Gather x{};
     const long long esize = (long long)esize_of(p);
     x.tensors = tensors;
-    x.row_bytes = (int)(p.rows.C * esize);
     x.lse = lse;
     x.lse_to = lse_to;
-    bool by_16 = x.row_bytes % 16 == 0;
+    const long long row_bytes = p.rows.C * esize;
+    bool by_16 = row_bytes % 16 == 0;
     for (int i = 0; i < tensors; ++i) {
         x.from[i] = from[i]->ptr;
         x.to[i] = to[i];
@@ -332,9 +344,9 @@ int gather(const na2d_attn::Place& at, const Problem& p, const Operand* const* f
     }
     const int sides = tensors + (lse ? 1 : 0);
     if (!sides) return NA2D_OK;
-    const long long per = tensors ? x.row_bytes / (by_16 ? 16 : esize) : 1, blocks = (p.rows.all * per + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
-    const dim3 grid((unsigned)blocks, (unsigned)sides);
+    const int pieces = tensors ? (int)(row_bytes / (by_16 ? 16 : esize)) : 1;
+    x.by_pieces = na2d_attn::Div(pieces);
+    const dim3 grid(blocks_of(p.rows, pieces), (unsigned)sides);
     *at.launched += 1;
     const cudaError_t e = by_16        ? na2d_launch::launch(true, gather_rows_kernel<uint4>, grid, kThreads, 0, at.st, p.rows, x)
                           : esize == 4 ? na2d_launch::launch(true, gather_rows_kernel<uint32_t>, grid, kThreads, 0, at.st, p.rows, x)
@@ -345,21 +357,19 @@ int gather(const na2d_attn::Place& at, const Problem& p, const Operand* const* f
 template <typename DT, int N>
 int join_outputs(const na2d_attn::Place& at, const Problem& p, const float* o_prefix, const float* lse_prefix, const float* o_own,
                  const float* lse_own, void* o, float* lse) {
-    const long long blocks = (p.rows.all * (p.rows.C / N) + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+    const int pieces = p.rows.C / N;
     *at.launched += 1;
-    return na2d_launch::launch(true, join_outputs_kernel<DT, N>, (unsigned)blocks, kThreads, 0, at.st, p.rows, o_prefix, lse_prefix, o_own, lse_own,
-                               static_cast<DT*>(o), lse) == cudaSuccess
+    return na2d_launch::launch(true, join_outputs_kernel<DT, N>, blocks_of(p.rows, pieces), kThreads, 0, at.st, p.rows, na2d_attn::Div(pieces), o_prefix,
+                               lse_prefix, o_own, lse_own, static_cast<DT*>(o), lse) == cudaSuccess
                ? NA2D_OK
                : NA2D_ERR_CUDA;
 }
 template <typename DT, int N>
 int join_gradients(const na2d_attn::Place& at, const Problem& p, const float* prefix, const float* own, void* d_q) {
-    const long long blocks = (p.rows.all * (p.rows.C / N) + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+    const int pieces = p.rows.C / N;
     *at.launched += 1;
-    return na2d_launch::launch(true, join_gradients_kernel<DT, N>, (unsigned)blocks, kThreads, 0, at.st, p.rows, prefix, own,
-                               static_cast<DT*>(d_q)) == cudaSuccess
+    return na2d_launch::launch(true, join_gradients_kernel<DT, N>, blocks_of(p.rows, pieces), kThreads, 0, at.st, p.rows, na2d_attn::Div(pieces), prefix,
+                               own, static_cast<DT*>(d_q)) == cudaSuccess
                ? NA2D_OK
                : NA2D_ERR_CUDA;
 }
@@ -432,13 +442,18 @@ int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a) {
                 x.C = p.rows.C;
                 x.causal = p.any_own && p.own.causal;
                 x.sl2 = p.prefix.sl2;
+                x.behind = launched > 0;
+                x.by_tq = na2d_attn::Div(p.rows.Tq);
+                x.by_n = na2d_attn::Div(p.rows.N);
+                x.by_g = na2d_attn::Div(p.prefix.G);
                 x.table = reinterpret_cast<int*>(ws + f.table);
                 x.part_o = floats(f.part_o);
                 x.part_lse = floats(f.part_lse);
                 const size_t stride = (size_t)p.rows.all;
-                const na2d_prefix::JoinSide by_prefix{prefix.o, prefix.lse, stride, prefix.count, p.rows.A}, by_own{own.o, own.lse, stride, own.count, 1};
-                return p.dtype == NA2D_BF16 ? na2d_prefix::tokens_bf16(at, x, by_prefix, by_own, a->o.ptr, a->lse, p.B, launched > 0)
-                                            : na2d_prefix::tokens_f16(at, x, by_prefix, by_own, a->o.ptr, a->lse, p.B, launched > 0);
+                const na2d_prefix::JoinSide by_prefix{prefix.o, prefix.lse, stride, prefix.count, p.rows.A, na2d_attn::Div(p.rows.A)},
+                    by_own{own.o, own.lse, stride, own.count, 1, na2d_attn::Div(1)};
+                return p.dtype == NA2D_BF16 ? na2d_prefix::tokens_bf16(at, x, by_prefix, by_own, a->o.ptr, a->lse, p.B)
+                                            : na2d_prefix::tokens_f16(at, x, by_prefix, by_own, a->o.ptr, a->lse, p.B);
             }
             const float *o_own = p.any_own ? floats(f.o_own) : nullptr, *lse_own = p.any_own ? floats(f.lse_own) : nullptr;
             return by_type(p, [&](auto type, auto n) {

@@ -23,7 +23,9 @@ struct Tokens {
     TokenSide side[2];                  // prefixes, own
     na2d_attn::Operand q;               // (B, N, Tq, C)
     int N, Nk, G, Tq, C, causal;
+    int behind;                         // another kernel of the call has been launched before
     float sl2;
+    na2d_attn::Div by_tq, by_n, by_g;
     int* table;                         // steps before each entry, of all, and those of a warp
     float *part_o, *part_lse;
 };
@@ -32,6 +34,7 @@ struct JoinSide {
     const float *o, *lse;
     size_t stride;                      // rows from one to the next
     int count, share;
+    na2d_attn::Div by_share;
 };
 
 // Query rows of a unit that the kernel takes, at most.
@@ -39,8 +42,7 @@ constexpr int kTokenRows = 32;
 // Warps of the line.
 inline int token_warps(int sms) { return sms * 8; }
 
-// `behind`: another kernel of the same call has been launched before.
-int tokens_bf16(const na2d_attn::Place& at, const Tokens& x, const JoinSide& prefix, const JoinSide& own, void* o, float* lse, int B, bool behind);
-int tokens_f16(const na2d_attn::Place& at, const Tokens& x, const JoinSide& prefix, const JoinSide& own, void* o, float* lse, int B, bool behind);
+int tokens_bf16(const na2d_attn::Place& at, const Tokens& x, const JoinSide& prefix, const JoinSide& own, void* o, float* lse, int B);
+int tokens_f16(const na2d_attn::Place& at, const Tokens& x, const JoinSide& prefix, const JoinSide& own, void* o, float* lse, int B);
 
 }  // namespace na2d_prefix

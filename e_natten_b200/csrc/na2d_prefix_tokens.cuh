@@ -80,8 +80,9 @@ __global__ void __launch_bounds__(kTokenThreads, 1) prefix_tokens_kernel(const _
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int E0 = x.side[0].entries, E = E0 + x.side[1].entries;
 
-    // (nothing here reads what the kernel before wrote, where that is another one of this call; the joins that follow do, and the wait for
-    // it at the end is theirs)
+    // (behind another kernel of this call nothing here reads what that one wrote; the join that follows does, and the wait at the end is
+    // for it)
+    if (!x.behind) after_previous_grid();
     {   // the table
         for (int e = threadIdx.x; e < E; e += kTokenThreads) {
             const int steps = (token_keys(x, e) + kStep - 1) / kStep;
@@ -182,17 +183,19 @@ __global__ void __launch_bounds__(kTokenThreads, 1) prefix_tokens_kernel(const _
     for (int i = 0; i < NST - 1; ++i) ask();
 
     const int r_lo = lane / 4, c_lo = 2 * (lane % 4);    // of a fragment: rows r_lo and r_lo + 8, columns c_lo, + 1
-    while (here.any()) {
+    int c0 = 0, c1 = 0;
+    auto settle = [&]() {                                // on to a unit of which the stretch has steps
+        for (; here.any(); here.next(before, x.Nk)) {
+            here.steps(before, x.Nk, c0, c1);
+            if (c0 < c1) return true;
+        }
+        return false;
+    };
+    while (settle()) {
         const bool second = here.e >= E0;
         const TokenSide& side = x.side[second];
         const int i0 = second ? here.e - E0 : here.e, m = here.m, count = token_keys(x, here.e), unit = i0 * x.Nk + m;
         const int tokens = side.share * x.Tq;            // of one head
-        int c0, c1;
-        here.steps(before, x.Nk, c0, c1);
-        if (c0 >= c1) {
-            here.next(before, x.Nk);
-            continue;
-        }
         // Q as the first product's operand, and the keys that the thread's rows see
         uint32_t qf[MT][D / 16][4];
         int seen[MT][2];
@@ -337,10 +340,10 @@ __global__ void __launch_bounds__(kTokenThreads, 1) prefix_tokens_kernel(const _
         here.next(before, x.Nk);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    after_previous_grid();
+    if (x.behind) after_previous_grid();
 }
 
-// A row's parts of one side: places first, first + stride, ... of part_o and part_lse.
+// A row's parts of one side: rows first, first + stride, ... of o and lse.
 struct PartList {
     const float *o, *lse;
     size_t first, stride;
@@ -349,86 +352,98 @@ struct PartList {
 __device__ __forceinline__ PartList parts_of(const Tokens& x, const JoinSide& j, int which, int b, int n, int t) {
     PartList l{};
     const TokenSide& s = x.side[which];
-    const int share = j.share, entry = b / share, a = b - entry * share;
+    int entry = b, a = 0;
+    if (j.share > 1) entry = j.by_share.split(b, a);
+    const size_t row = static_cast<size_t>(a) * x.Tq + t;
     if (j.count > 0) {                                   // of another kernel: rows of (entries, N, share Tq)
         l.o = j.o;
         l.lse = j.lse;
-        l.first = (static_cast<size_t>(entry) * x.N + n) * share * x.Tq + static_cast<size_t>(a) * x.Tq + t;
+        l.first = (static_cast<size_t>(entry) * x.N + n) * j.share * x.Tq + row;
         l.stride = j.stride;
         l.count = j.count;
         return l;
     }
     if (s.entries == 0) return l;
-    const int e = (which ? x.side[0].entries : 0) + entry, m = n / x.G, unit = entry * x.Nk + m;
-    const int E = x.side[0].entries + x.side[1].entries, each = x.table[E + 1], length = x.table[e + 1] - x.table[e];
+    int h;
+    const int e = (which ? x.side[0].entries : 0) + entry, m = x.by_g.split(n, h), unit = entry * x.Nk + m;
+    const int E = x.side[0].entries + x.side[1].entries, each = x.table[E + 1], before = x.table[e], length = x.table[e + 1] - before;
     if (length == 0) return l;
-    const int at = x.table[e] * x.Nk + m * length, lo = (at + kUnitSteps) / each, hi = (at + length - 1) / each;       // warps with steps of it
+    const int at = before * x.Nk + m * length, lo = (at + kUnitSteps) / each, hi = (at + length - 1) / each;       // warps with steps of it
     l.o = x.part_o;
     l.lse = x.part_lse;
     l.stride = s.rows;
-    l.first = s.first_row + static_cast<size_t>(lo + unit) * s.rows + static_cast<size_t>(n - m * x.G) * share * x.Tq + static_cast<size_t>(a) * x.Tq + t;
+    l.first = s.first_row + static_cast<size_t>(lo + unit) * s.rows + static_cast<size_t>(h) * j.share * x.Tq + row;
     l.count = hi - lo + 1;
     return l;
 }
 
-// lse = ln sum_s e^lse_s, o = sum_s e^(lse_s - lse) o_s over a row's parts of both sides.  W warps a row, 4 channels a lane.
-template <typename DT, int W>
-__global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Tokens x, const JoinSide prefix, const JoinSide own, DT* __restrict__ o,
-                                                          float* __restrict__ lse, const long long rows) {
-    __shared__ float4 sums[4][32];
+// lse = ln sum_s e^lse_s, o = sum_s e^(lse_s - lse) o_s over a row's parts of both sides.  A block a row: its warps share the parts, 4
+// channels a lane; where they lie and what they weigh, each lane of a warp works out for one of 32.
+template <typename DT>
+__global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Tokens x, const __grid_constant__ JoinSide prefix,
+                                                          const __grid_constant__ JoinSide own, DT* __restrict__ o, float* __restrict__ lse) {
+    constexpr int W = 4;
+    __shared__ float4 sums[W][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x, c = 4 * lane;
+    int t, n;
+    const int b = x.by_n.split(x.by_tq.split(row, t), n);
     after_previous_grid();
     next_grid_may_start();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % W;
-    const long long row = (long long)blockIdx.x * (4 / W) + warp / W;
-    if (W < 4 && row >= rows) return;                    // (with four warps a row there is a block for each)
-    const long long bn = row / x.Tq;
-    const int t = (int)(row - bn * x.Tq), c = 4 * lane, b = (int)(bn / x.N), n = (int)(bn - (long long)b * x.N);
-    const PartList list[2] = {parts_of(x, prefix, 0, b, n, t), parts_of(x, own, 1, b, n, t)};
-    float top = -CUDART_INF_F;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-        for (int i = lane; i < list[s].count; i += 32) top = fmaxf(top, list[s].lse[list[s].first + i * list[s].stride]);
+    const PartList first = parts_of(x, prefix, 0, b, n, t), second = parts_of(x, own, 1, b, n, t);
+    const int parts = first.count + second.count;
+    auto part = [&](int i, const float*& at) {           // lse of part i, and its o
+        const PartList& l = i < first.count ? first : second;
+        const size_t r = l.first + (i < first.count ? i : i - first.count) * l.stride;
+        at = l.o + r * x.C;
+        return l.lse[r];
+    };
+    const float* at = nullptr;
+    float of = lane < parts ? part(lane, at) : -CUDART_INF_F, top = of;
+    for (int i = lane + 32; i < parts; i += 32) {
+        const float* ignored;
+        top = fmaxf(top, part(i, ignored));
+    }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     // (a NaN of a part stays one: the maximum skips it, its weight does not)
     const float base = top == -CUDART_INF_F ? 0.f : top;
     float total = 0.f;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-        for (int i = lane; i < list[s].count; i += 32) total += expf(list[s].lse[list[s].first + i * list[s].stride] - base);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    const float inv = total == 0.f ? 0.f : 1.f / total;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c < x.C) {
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        if (i0 > 0) of = i0 + lane < parts ? part(i0 + lane, at) : -CUDART_INF_F;
+        const float w = of == -CUDART_INF_F ? 0.f : expf(of - base);
+        total += w;
+        const unsigned there = __ballot_sync(0xffffffffu, of != -CUDART_INF_F);      // of the others nothing was written
+        const unsigned long long place = reinterpret_cast<unsigned long long>(at);
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll 4
-            for (int i = part; i < list[s].count; i += W) {
-                const size_t at = list[s].first + i * list[s].stride;
-                const float of = list[s].lse[at];
-                if (of == -CUDART_INF_F) continue;       // nothing was written for it
-                const float w = expf(of - base) * inv;
-                const float4 v = *reinterpret_cast<const float4*>(list[s].o + at * x.C + c);
-                acc.x = fmaf(w, v.x, acc.x);
-                acc.y = fmaf(w, v.y, acc.y);
-                acc.z = fmaf(w, v.z, acc.z);
-                acc.w = fmaf(w, v.w, acc.w);
+        for (int k = 0; k < 32 / W; ++k) {
+            const int j = W * k + warp;
+            if (i0 + W * k >= parts) break;
+            const float by = __shfl_sync(0xffffffffu, w, j);
+            const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, place, j));
+            if ((there >> j & 1) && c < x.C) {
+                const float4 v = *reinterpret_cast<const float4*>(from + c);
+                acc.x = fmaf(by, v.x, acc.x);
+                acc.y = fmaf(by, v.y, acc.y);
+                acc.z = fmaf(by, v.z, acc.z);
+                acc.w = fmaf(by, v.w, acc.w);
             }
-    }
-    if constexpr (W > 1) {
-        if (part > 0) sums[warp][lane] = acc;
-        __syncthreads();
-        if (part > 0) return;
-#pragma unroll
-        for (int w = 1; w < W; ++w) {
-            acc.x += sums[w][lane].x;
-            acc.y += sums[w][lane].y;
-            acc.z += sums[w][lane].z;
-            acc.w += sums[w][lane].w;
         }
     }
-    if (c < x.C) store_4(o + row * x.C + c, acc);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    if (warp > 0) sums[warp][lane] = acc;
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+        acc.x += sums[w][lane].x;
+        acc.y += sums[w][lane].y;
+        acc.z += sums[w][lane].z;
+        acc.w += sums[w][lane].w;
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (c < x.C) store_4(o + static_cast<size_t>(row) * x.C + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     if (lane == 0) lse[row] = total == 0.f ? -CUDART_INF_F : base + logf(total);
 }
 
