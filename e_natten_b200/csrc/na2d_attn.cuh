@@ -45,7 +45,7 @@ struct Geom {
     const int* lengths;                     // (B,) on the device, or null
     float scale, sl2;                       // the softmax scale, and times log2(e)
     Div by_nk, by_tt, by_tiles_t, by_tiles, by_units;
-    int parts;                              // forward, units of several tiles: parts of each unit's keys, all of the same length; 0: by a rule
+    int parts = 0;                          // forward, units of several tiles: parts of each unit's keys, all of the same length; 0: by a rule
 };
 
 // Rows in tiles (host); several heads in one only with `pack`.

@@ -87,7 +87,8 @@ int na2d_attention_forward(const na2d_attention_args* a) {
         if (int rc = place(a, &launched, &at)) return rc;
         int rc;
         if (!p.tensor) {
-            rc = na2d_attn::simt_forward(at, p.g, p.q, p.k, p.v, p.o, a->lse);
+            const na2d_attn::Forward x{&p.g, p.q, p.k, p.v, p.o, a->lse};
+            rc = na2d_attn::simt_forward(at, &x, 1);
         } else {
             const na2d_attn::Scratch scratch = scratch_of(a);
             rc = a->dtype == NA2D_BF16 ? na2d_attn::forward_bf16(at, p.g, scratch, p.q, p.k, p.v, p.o, a->lse)
@@ -106,13 +107,13 @@ int na2d_attention_backward(const na2d_attention_args* a) {
         int launched = 0;
         na2d_attn::Place at;
         if (int rc = place(a, &launched, &at)) return rc;
-        const na2d_attn::Backward x{p.q, p.k, p.v, p.o, p.d_o, p.d_q, p.d_k, p.d_v, a->lse, a->delta};
+        const na2d_attn::Backward x{&p.g, p.q, p.k, p.v, p.o, p.d_o, p.d_q, p.d_k, p.d_v, a->lse, a->delta};
         int rc;
         if (!p.tensor) {
-            rc = na2d_attn::simt_backward(at, p.g, x);
+            rc = na2d_attn::simt_backward(at, &x, 1);
         } else {
             const na2d_attn::Scratch scratch = scratch_of(a);
-            rc = a->dtype == NA2D_BF16 ? na2d_attn::backward_bf16(at, p.g, scratch, x) : na2d_attn::backward_f16(at, p.g, scratch, x);
+            rc = a->dtype == NA2D_BF16 ? na2d_attn::backward_bf16(at, scratch, x) : na2d_attn::backward_f16(at, scratch, x);
         }
         return finish(rc, launched, "attention backward launch");
     });

@@ -39,16 +39,23 @@ int forward_f16(const Place& at, const Geom& g, const Scratch& scratch, const Op
 
 // d_q.ptr or d_k.ptr (with d_v.ptr) may be null: that half is left out.  Writes delta.
 struct Backward {
+    const Geom* g;
     Operand q, k, v, o, d_o, d_q, d_k, d_v;
     const float* lse;
     float* delta;
 };
-int backward_bf16(const Place& at, const Geom& g, const Scratch& scratch, const Backward& x);
-int backward_f16(const Place& at, const Geom& g, const Scratch& scratch, const Backward& x);
+int backward_bf16(const Place& at, const Scratch& scratch, const Backward& x);
+int backward_f16(const Place& at, const Scratch& scratch, const Backward& x);
 
 // CUDA cores: any strides, C up to kSimtMaxC, fp32 and 16 bits.
+// One problem, or two of one head dim whose results are alike, `wide` or not, in the same launches.
 constexpr int kSimtMaxC = 256;
-int simt_forward(const Place& at, const Geom& g, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse);
-int simt_backward(const Place& at, const Geom& g, const Backward& x);
+struct Forward {
+    const Geom* g;
+    Operand q, k, v, o;
+    float* lse;
+};
+int simt_forward(const Place& at, const Forward* x, int count);
+int simt_backward(const Place& at, const Backward* x, int count);
 
 }  // namespace na2d_attn

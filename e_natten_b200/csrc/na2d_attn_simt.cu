@@ -189,16 +189,41 @@ __device__ __forceinline__ float row_max(float x) {
 template <typename DT>
 __device__ __forceinline__ DT* rows_of(const Operand& x, int b, int n) { return static_cast<DT*>(x.ptr) + b * x.b + n * x.n; }
 
+// What a launch works on: one problem, or two whose blocks share it (a prefix's keys and the entries' own: small ones take as long alone as
+// together).  `out`: o, dQ or dK; out2: dV.
+struct SimtWork {
+    Operand q, k, v, d_o, out, out2;
+    float *lse, *delta;
+    Geom g;
+    int tiles, vec;
+    unsigned blocks;
+};
+struct SimtPair {
+    SimtWork at[2];
+};
+// The problem of this block, and its block of it.
+__device__ __forceinline__ const SimtWork& work_of(const SimtPair& p, unsigned& block) {
+    const bool second = blockIdx.x >= p.at[0].blocks;
+    block = blockIdx.x - (second ? p.at[0].blocks : 0u);
+    return p.at[second];
+}
+
 // ---- forward: a block has BT queries of one head ------------------------------------------------------------------
 template <typename DT, typename OT, int CP, int BM>
 __global__ void __launch_bounds__(kThreads)
-simt_fwd_kernel(const Operand q, const Operand k, const Operand v, const Operand o, float* __restrict__ lse, const Geom g, const int tiles, const int vec) {
+simt_fwd_kernel(const __grid_constant__ SimtPair pair) {
     using S = SimtCfg<CP, BM>;
+    unsigned block;
+    const SimtWork& work = work_of(pair, block);
+    const Operand q = work.q, k = work.k, v = work.v, o = work.out;
+    float* __restrict__ lse = work.lse;
+    const Geom g = work.g;
+    const int tiles = work.tiles, vec = work.vec;
     extern __shared__ __align__(16) float smem[];
     float *sQ = smem, *sKV = sQ + S::HELD, *sP = sKV + S::TILE;
     const int tx = threadIdx.x % 32 / 2, ty = threadIdx.x / 32 * 2 + threadIdx.x % 2;
-    const int bn = blockIdx.x / tiles, b = bn / g.N, n = bn - b * g.N, m = n / g.G;
-    const int t0 = (g.causal ? tiles - 1 - (int)(blockIdx.x % tiles) : (int)(blockIdx.x % tiles)) * BM;
+    const int bn = block / tiles, b = bn / g.N, n = bn - b * g.N, m = n / g.G;
+    const int t0 = (g.causal ? tiles - 1 - (int)(block % tiles) : (int)(block % tiles)) * BM;
     const int count = key_count(g, b), keys = keys_seen(g, count, min(t0 + BM, g.Tq) - 1);
     Tile<DT, CP, BM>::bring(sQ, rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
     Tile<DT, CP, S::BT> tile;
@@ -261,8 +286,13 @@ simt_fwd_kernel(const Operand q, const Operand k, const Operand v, const Operand
 
 // ---- delta = dO . o, a warp a row -------------------------------------------------------------------------------------
 template <typename DT>
-__global__ void __launch_bounds__(kThreads) simt_delta_kernel(const Operand d_o, const Operand o, float* __restrict__ delta, const Geom g) {
-    const long long rows = (long long)g.B * g.N * g.Tq, row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
+__global__ void __launch_bounds__(kThreads) simt_delta_kernel(const __grid_constant__ SimtPair pair) {
+    unsigned block;
+    const SimtWork& work = work_of(pair, block);
+    const Operand d_o = work.d_o, o = work.out;
+    float* __restrict__ delta = work.delta;
+    const Geom& g = work.g;
+    const long long rows = (long long)g.B * g.N * g.Tq, row = (long long)block * 8 + threadIdx.x / 32;
     if (row >= rows) return;
     const long long bn = row / g.Tq;
     const int t = (int)(row % g.Tq), b = (int)(bn / g.N), n = (int)(bn % g.N);
@@ -277,14 +307,19 @@ __global__ void __launch_bounds__(kThreads) simt_delta_kernel(const Operand d_o,
 // ---- query half of the backward -----------------------------------------------------------------------------------------
 template <typename DT, typename OT, int CP, int BM>
 __global__ void __launch_bounds__(kThreads)
-simt_dq_kernel(const Operand q, const Operand k, const Operand v, const Operand d_o, const Operand d_q, const float* __restrict__ lse,
-               const float* __restrict__ delta, const Geom g, const int tiles, const int vec) {
+simt_dq_kernel(const __grid_constant__ SimtPair pair) {
     using S = SimtCfg<CP, BM>;
+    unsigned block;
+    const SimtWork& work = work_of(pair, block);
+    const Operand q = work.q, k = work.k, v = work.v, d_o = work.d_o, d_q = work.out;
+    const float *__restrict__ lse = work.lse, *__restrict__ delta = work.delta;
+    const Geom g = work.g;
+    const int tiles = work.tiles, vec = work.vec;
     extern __shared__ __align__(16) float smem[];
     float *sQ = smem, *sG = sQ + S::HELD, *sKV = sG + S::HELD, *sP = sKV + S::TILE;
     const int tx = threadIdx.x % 32 / 2, ty = threadIdx.x / 32 * 2 + threadIdx.x % 2;
-    const int bn = blockIdx.x / tiles, b = bn / g.N, n = bn - b * g.N, m = n / g.G;
-    const int t0 = (g.causal ? tiles - 1 - (int)(blockIdx.x % tiles) : (int)(blockIdx.x % tiles)) * BM;
+    const int bn = block / tiles, b = bn / g.N, n = bn - b * g.N, m = n / g.G;
+    const int t0 = (g.causal ? tiles - 1 - (int)(block % tiles) : (int)(block % tiles)) * BM;
     const int count = key_count(g, b), keys = keys_seen(g, count, min(t0 + BM, g.Tq) - 1);
     Tile<DT, CP, BM>::bring(sQ, rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
     Tile<DT, CP, BM>::bring(sG, rows_of<DT>(d_o, b, n), d_o.t, t0, g.Tq, g.C, vec);
@@ -334,15 +369,20 @@ simt_dq_kernel(const Operand q, const Operand k, const Operand v, const Operand 
 // ---- key half: a block has BT keys of one key head and walks the queries of every head that shares it ------------------------
 template <typename DT, int CP>
 __global__ void __launch_bounds__(kThreads)
-simt_dkdv_kernel(const Operand q, const Operand k, const Operand v, const Operand d_o, const Operand d_k, const Operand d_v,
-                 const float* __restrict__ lse, const float* __restrict__ delta, const Geom g, const int tiles, const int vec) {
+simt_dkdv_kernel(const __grid_constant__ SimtPair pair) {
     constexpr int BM = CP <= 128 ? 64 : 32;
     using S = SimtCfg<CP, BM>;
+    unsigned block;
+    const SimtWork& work = work_of(pair, block);
+    const Operand q = work.q, k = work.k, v = work.v, d_o = work.d_o, d_k = work.out, d_v = work.out2;
+    const float *__restrict__ lse = work.lse, *__restrict__ delta = work.delta;
+    const Geom g = work.g;
+    const int tiles = work.tiles, vec = work.vec;
     extern __shared__ __align__(16) float smem[];
     float *sK = smem, *sV = sK + S::TILE, *sX = sV + S::TILE, *sY = sX + S::TILE, *sP = sY + S::TILE;
     const int tx = threadIdx.x % 32 / 2, ty = threadIdx.x / 32 * 2 + threadIdx.x % 2;
-    const int unit = blockIdx.x / tiles, b = unit / g.Nk, m = unit - b * g.Nk;
-    const int k0 = (blockIdx.x % tiles) * S::BT;
+    const int unit = block / tiles, b = unit / g.Nk, m = unit - b * g.Nk;
+    const int k0 = (block % tiles) * S::BT;
     const int count = key_count(g, b);
     const int t_min = g.causal ? max(k0 + g.Tq - count, 0) : 0;      // the first token that sees the tile
     Tile<DT, CP, BM> tile;
@@ -418,17 +458,21 @@ bool vectors(const Operand& x, int dtype, int C) {
 }
 
 // Blocks of `rows` in tiles, for each of `units`.
-int blocks_of(long long units, int rows, int tile, int* tiles, unsigned* blocks) {
-    *tiles = (rows + tile - 1) / tile;
-    if (units * *tiles > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
-    *blocks = (unsigned)(units * *tiles);
+int cut_work(SimtWork* w, long long units, int rows, int tile) {
+    w->tiles = (rows + tile - 1) / tile;
+    if (units * w->tiles > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+    w->blocks = (unsigned)(units * w->tiles);
     return NA2D_OK;
 }
 
-template <typename K, typename... A>
-int start(const Place& at, K kernel, unsigned blocks, int floats, std::atomic<unsigned long long>& opted, A... args) {
-    if (na2d_tc::opt_in_smem(kernel, floats * 4, at.device, opted) != cudaSuccess) return NA2D_ERR_CUDA;
-    kernel<<<blocks, kThreads, floats * 4, at.st>>>(args...);
+// floats: of dynamic shared memory, 0: none.
+template <typename K>
+int start(const Place& at, K kernel, const SimtPair& pair, int floats, std::atomic<unsigned long long>& opted) {
+    const unsigned long long blocks = (unsigned long long)pair.at[0].blocks + pair.at[1].blocks;
+    if (blocks == 0) return NA2D_OK;
+    if (blocks > 0x7fffffffULL) return NA2D_ERR_TOO_LARGE;
+    if (floats > 0 && na2d_tc::opt_in_smem(kernel, floats * 4, at.device, opted) != cudaSuccess) return NA2D_ERR_CUDA;
+    kernel<<<(unsigned)blocks, kThreads, floats * 4, at.st>>>(pair);
     *at.launched += 1;
     return cudaGetLastError() == cudaSuccess ? NA2D_OK : NA2D_ERR_CUDA;
 }
@@ -437,9 +481,11 @@ int start(const Place& at, K kernel, unsigned blocks, int floats, std::atomic<un
 // memory for its 32 products, one of 4 x 4 reads 8 for 16.  Forward and query half with 256 blocks of 64: 277 and 417 us; with 128 of 128:
 // 244 and 365 us.
 template <int CP, typename F>
-int by_rows(const Place& at, const Geom& g, F&& f) {
+int by_rows(const Place& at, const SimtPair& pair, F&& f) {
     if constexpr (CP <= 128) {
-        if ((long long)g.B * g.N * ((g.Tq + 63) / 64) > na2d_tc::sm_count(at.device)) return f(std::integral_constant<int, 128>{});
+        long long blocks = 0;
+        for (const SimtWork& w : pair.at) blocks += (long long)w.g.B * w.g.N * ((w.g.Tq + 63) / 64);
+        if (blocks > na2d_tc::sm_count(at.device)) return f(std::integral_constant<int, 128>{});
         return f(std::integral_constant<int, 64>{});
     } else {
         return f(std::integral_constant<int, 32>{});
@@ -447,73 +493,100 @@ int by_rows(const Place& at, const Geom& g, F&& f) {
 }
 
 template <typename DT, typename OT, int CP, int BM>
-int forward_as(const Place& at, const Geom& g, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse) {
+int forward_as(const Place& at, SimtPair pair) {
     using S = SimtCfg<CP, BM>;
     static std::atomic<unsigned long long> opted{0};
-    const int vec = vectors(q, at.dtype, g.C) && vectors(k, at.dtype, g.C) && vectors(v, at.dtype, g.C);
-    int tiles = 0;
-    unsigned blocks = 0;
-    if (int rc = blocks_of((long long)g.B * g.N, g.Tq, BM, &tiles, &blocks)) return rc;
-    return start(at, simt_fwd_kernel<DT, OT, CP, BM>, blocks, S::HELD + S::TILE + S::SCORES, opted, q, k, v, o, lse, g, tiles, vec);
+    for (SimtWork& w : pair.at) {
+        if (!w.q.ptr) continue;
+        w.vec = vectors(w.q, at.dtype, w.g.C) && vectors(w.k, at.dtype, w.g.C) && vectors(w.v, at.dtype, w.g.C);
+        if (int rc = cut_work(&w, (long long)w.g.B * w.g.N, w.g.Tq, BM)) return rc;
+    }
+    return start(at, simt_fwd_kernel<DT, OT, CP, BM>, pair, S::HELD + S::TILE + S::SCORES, opted);
 }
 
 template <typename DT, typename OT, int CP, int BM>
-int queries_as(const Place& at, const Geom& g, const Backward& x, int vec) {
+int queries_as(const Place& at, SimtPair pair) {
     using S = SimtCfg<CP, BM>;
     static std::atomic<unsigned long long> opted{0};
-    int tiles = 0;
-    unsigned blocks = 0;
-    if (int rc = blocks_of((long long)g.B * g.N, g.Tq, BM, &tiles, &blocks)) return rc;
-    return start(at, simt_dq_kernel<DT, OT, CP, BM>, blocks, 2 * S::HELD + S::TILE + S::SCORES, opted, x.q, x.k, x.v, x.d_o, x.d_q, x.lse,
-                 (const float*)x.delta, g, tiles, vec);
+    for (SimtWork& w : pair.at)
+        if (w.q.ptr)
+            if (int rc = cut_work(&w, (long long)w.g.B * w.g.N, w.g.Tq, BM)) return rc;
+    return start(at, simt_dq_kernel<DT, OT, CP, BM>, pair, 2 * S::HELD + S::TILE + S::SCORES, opted);
 }
 
 template <typename DT, int CP>
-int backward_as(const Place& at, const Geom& g, const Backward& x) {
+int backward_as(const Place& at, const Backward* x, int count) {
     constexpr int BM = CP <= 128 ? 64 : 32;
     using S = SimtCfg<CP, BM>;
     static std::atomic<unsigned long long> opted{0};
-    int vec = 1, tiles = 0;
-    for (const Operand* t : {&x.q, &x.k, &x.v, &x.d_o}) vec = vec && vectors(*t, at.dtype, g.C);
-    const long long rows = (long long)g.B * g.N * g.Tq;
-    if ((rows + 7) / 8 > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
-    simt_delta_kernel<DT><<<(unsigned)((rows + 7) / 8), kThreads, 0, at.st>>>(x.d_o, x.o, x.delta, g);
-    *at.launched += 1;
-    if (cudaGetLastError() != cudaSuccess) return NA2D_ERR_CUDA;
-    if (x.d_q.ptr) {
-        const int rc = by_rows<CP>(at, g, [&](auto bm) {
-            constexpr int kRowsOf = decltype(bm)::value;
-            return x.d_q.wide ? queries_as<DT, float, CP, kRowsOf>(at, g, x, vec) : queries_as<DT, DT, CP, kRowsOf>(at, g, x, vec);
-        });
-        if (rc != NA2D_OK) return rc;
+    SimtPair delta{}, queries{}, keys{};
+    bool wide = false;
+    for (int i = 0; i < count; ++i) {
+        SimtWork w{};
+        w.q = x[i].q;
+        w.k = x[i].k;
+        w.v = x[i].v;
+        w.d_o = x[i].d_o;
+        w.lse = const_cast<float*>(x[i].lse);
+        w.delta = x[i].delta;
+        w.g = *x[i].g;
+        w.vec = 1;
+        for (const Operand* t : {&w.q, &w.k, &w.v, &w.d_o}) w.vec = w.vec && vectors(*t, at.dtype, w.g.C);
+        delta.at[i] = w;
+        delta.at[i].out = x[i].o;
+        const long long blocks = ((long long)w.g.B * w.g.N * w.g.Tq + 7) / 8;        // a warp a row
+        if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+        delta.at[i].blocks = (unsigned)blocks;
+        if (x[i].d_q.ptr) {
+            queries.at[i] = w;
+            queries.at[i].out = x[i].d_q;
+            wide = x[i].d_q.wide;
+        }
+        if (x[i].d_k.ptr) {
+            keys.at[i] = w;
+            keys.at[i].out = x[i].d_k;
+            keys.at[i].out2 = x[i].d_v;
+            if (int rc = cut_work(&keys.at[i], w.g.units, w.g.Tk, BM)) return rc;
+        }
     }
-    if (!x.d_k.ptr) return NA2D_OK;
-    unsigned blocks = 0;
-    if (int rc = blocks_of(g.units, g.Tk, BM, &tiles, &blocks)) return rc;
-    return start(at, simt_dkdv_kernel<DT, CP>, blocks, 4 * S::TILE + S::SCORES, opted, x.q, x.k, x.v, x.d_o, x.d_k, x.d_v, x.lse,
-                 (const float*)x.delta, g, tiles, vec);
+    if (int rc = start(at, simt_delta_kernel<DT>, delta, 0, opted)) return rc;
+    const int rc = by_rows<CP>(at, queries, [&](auto bm) {
+        constexpr int kRowsOf = decltype(bm)::value;
+        return wide ? queries_as<DT, float, CP, kRowsOf>(at, queries) : queries_as<DT, DT, CP, kRowsOf>(at, queries);
+    });
+    return rc != NA2D_OK ? rc : start(at, simt_dkdv_kernel<DT, CP>, keys, 4 * S::TILE + S::SCORES, opted);
 }
 
 }  // namespace
 
-int simt_forward(const Place& at, const Geom& g, const Operand& q, const Operand& k, const Operand& v, const Operand& o, float* lse) {
+int simt_forward(const Place& at, const Forward* x, int count) {
+    SimtPair pair{};
+    for (int i = 0; i < count; ++i) {
+        SimtWork& w = pair.at[i];
+        w.q = x[i].q;
+        w.k = x[i].k;
+        w.v = x[i].v;
+        w.out = x[i].o;
+        w.lse = x[i].lse;
+        w.g = *x[i].g;
+    }
     auto run = [&](auto type) {
         using DT = decltype(type);
-        return by_channels<DT>(g.C, [&](auto cp) {
+        return by_channels<DT>(x[0].g->C, [&](auto cp) {
             constexpr int CP = decltype(cp)::value;
-            return by_rows<CP>(at, g, [&](auto bm) {
+            return by_rows<CP>(at, pair, [&](auto bm) {
                 constexpr int kRowsOf = decltype(bm)::value;
-                return o.wide ? forward_as<DT, float, CP, kRowsOf>(at, g, q, k, v, o, lse) : forward_as<DT, DT, CP, kRowsOf>(at, g, q, k, v, o, lse);
+                return x[0].o.wide ? forward_as<DT, float, CP, kRowsOf>(at, pair) : forward_as<DT, DT, CP, kRowsOf>(at, pair);
             });
         });
     };
     return at.dtype == NA2D_F32 ? run(float{}) : at.dtype == NA2D_BF16 ? run(__nv_bfloat16{}) : run(__half{});
 }
 
-int simt_backward(const Place& at, const Geom& g, const Backward& x) {
+int simt_backward(const Place& at, const Backward* x, int count) {
     auto run = [&](auto type) {
         using DT = decltype(type);
-        return by_channels<DT>(g.C, [&](auto cp) { return backward_as<DT, decltype(cp)::value>(at, g, x); });
+        return by_channels<DT>(x[0].g->C, [&](auto cp) { return backward_as<DT, decltype(cp)::value>(at, x, count); });
     };
     return at.dtype == NA2D_F32 ? run(float{}) : at.dtype == NA2D_BF16 ? run(__nv_bfloat16{}) : run(__half{});
 }

@@ -134,7 +134,8 @@ int NA2D_TC_NAME(forward)(const Place& at, const Geom& g, const Scratch& scratch
     });
 }
 
-int NA2D_TC_NAME(backward)(const Place& at, const Geom& g, const Scratch& given, const Backward& x) {
+int NA2D_TC_NAME(backward)(const Place& at, const Scratch& given, const Backward& x) {
+    const Geom& g = *x.g;
     // fp16's bounds come first in the workspace; without one they lie in the stream's memory pool for the time of the call
     struct Own {
         float* at = nullptr;

@@ -326,12 +326,13 @@ int finish(int rc, int launched, const char* what) {
 
 int forward_of(const Problem& p, const na2d_attn::Place& at, const Geom& g, const Scratch& s, const Operand& q, const Operand& k, const Operand& v,
                const Operand& o, float* lse, na2d_attn::Parts* parts = nullptr) {
-    if (!p.tensor) return na2d_attn::simt_forward(at, g, q, k, v, o, lse);
     return p.dtype == NA2D_BF16 ? na2d_attn::forward_bf16(at, g, s, q, k, v, o, lse, parts) : na2d_attn::forward_f16(at, g, s, q, k, v, o, lse, parts);
 }
-int backward_of(const Problem& p, const na2d_attn::Place& at, const Geom& g, const Scratch& s, const na2d_attn::Backward& x) {
-    if (!p.tensor) return na2d_attn::simt_backward(at, g, x);
-    return p.dtype == NA2D_BF16 ? na2d_attn::backward_bf16(at, g, s, x) : na2d_attn::backward_f16(at, g, s, x);
+int backward_of(const Problem& p, const na2d_attn::Place& at, const Scratch& s, const na2d_attn::Backward* x, int count) {
+    if (!p.tensor) return count ? na2d_attn::simt_backward(at, x, count) : NA2D_OK;
+    for (int i = 0; i < count; ++i)
+        if (int rc = p.dtype == NA2D_BF16 ? na2d_attn::backward_bf16(at, s, x[i]) : na2d_attn::backward_f16(at, s, x[i])) return rc;
+    return NA2D_OK;
 }
 
 // Copies of those operands whose rows do not follow one another, and of lse.
@@ -427,11 +428,15 @@ int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a) {
                     char* to = ws + f.q;
                     if (int rc = gather(at, p, &from, &to, 1, nullptr, nullptr)) return rc;
                 }
-                if (int rc = forward_of(p, at, p.prefix, scratch, q, p.pk, p.pv, sums(p, floats(f.o_prefix), p.prefix.Tq), floats(f.lse_prefix),
+                if (!p.tensor) {
+                    const na2d_attn::Forward x[2] = {{&p.prefix, q, p.pk, p.pv, sums(p, floats(f.o_prefix), p.prefix.Tq), floats(f.lse_prefix)},
+                                                     {&p.own, p.q, p.k, p.v, sums(p, floats(f.o_own), p.own.Tq), floats(f.lse_own)}};
+                    if (int rc = na2d_attn::simt_forward(at, x, p.any_own ? 2 : 1)) return rc;
+                } else if (int rc = forward_of(p, at, p.prefix, scratch, q, p.pk, p.pv, sums(p, floats(f.o_prefix), p.prefix.Tq), floats(f.lse_prefix),
                                         line.any() ? &prefix : nullptr))
                     return rc;
             }
-            if (p.any_own && !line.own)
+            if (p.tensor && p.any_own && !line.own)
                 if (int rc = forward_of(p, at, p.own, own_scratch, p.q, p.k, p.v, sums(p, floats(f.o_own), p.own.Tq), floats(f.lse_own),
                                         line.any() ? &own : nullptr))
                     return rc;
@@ -498,6 +503,8 @@ int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a) {
         };
         auto run = [&]() -> int {
             const float* lse = a->lse;
+            na2d_attn::Backward x_of[2]{};
+            int count = 0;
             if (d_q || d_prefix) {
                 const Operand* given[3] = {&p.q, &p.o, &p.d_o};
                 Operand x[3];
@@ -512,7 +519,8 @@ int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a) {
                 }
                 const bool lse_apart = p.rows.A > 1 && p.rows.N > 1;
                 if (int rc = gather(at, p, from, to, copies, lse_apart ? lse : nullptr, floats(f.lse))) return rc;
-                na2d_attn::Backward b{};
+                na2d_attn::Backward& b = x_of[count++];
+                b.g = &p.prefix;
                 b.q = x[0];
                 b.o = x[1];
                 b.d_o = x[2];
@@ -525,10 +533,10 @@ int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a) {
                     b.d_k = result(a->d_prefix_k.ptr, a->S, a->P);
                     b.d_v = result(a->d_prefix_v.ptr, a->S, a->P);
                 }
-                if (int rc = backward_of(p, at, p.prefix, scratch, b)) return rc;
             }
             if (p.any_own && (d_q || d_own)) {
-                na2d_attn::Backward b{};
+                na2d_attn::Backward& b = x_of[count++];
+                b.g = &p.own;
                 b.q = p.q;
                 b.o = p.o;
                 b.d_o = p.d_o;
@@ -541,8 +549,8 @@ int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a) {
                     b.d_k = result(a->d_k.ptr, a->B, a->Tk);
                     b.d_v = result(a->d_v.ptr, a->B, a->Tk);
                 }
-                if (int rc = backward_of(p, at, p.own, scratch, b)) return rc;
             }
+            if (int rc = backward_of(p, at, scratch, x_of, count)) return rc;
             if (!d_q) return NA2D_OK;
             return by_type(p, [&](auto type, auto n) {
                 return join_gradients<decltype(type), decltype(n)::value>(at, p, floats(f.dq_prefix), p.any_own ? floats(f.dq_own) : nullptr, a->d_q.ptr);
