@@ -477,15 +477,18 @@ int start(const Place& at, K kernel, const SimtPair& pair, int floats, std::atom
     return cudaGetLastError() == cudaSuccess ? NA2D_OK : NA2D_ERR_CUDA;
 }
 
-// 128 query rows a block where blocks of 64 would take the SMs more than one round: a piece of 8 x 4 scores reads 12 operands from shared
-// memory for its 32 products, one of 4 x 4 reads 8 for 16.  Forward and query half with 256 blocks of 64: 277 and 417 us; with 128 of 128:
-// 244 and 365 us.
+// 128 query rows a block where blocks of 64 would take the SMs more than one round, and where that adds no more than an eighth of rows that are
+// none: a piece of 8 x 4 scores reads 12 operands from shared memory for its 32 products, one of 4 x 4 reads 8 for 16.  Forward and query
+// half with 256 blocks of 64: 277 and 417 us; with 128 of 128: 244 and 365 us.  Of 36 rows a head, blocks of 128 do twice the work.
 template <int CP, typename F>
 int by_rows(const Place& at, const SimtPair& pair, F&& f) {
     if constexpr (CP <= 128) {
-        long long blocks = 0;
-        for (const SimtWork& w : pair.at) blocks += (long long)w.g.B * w.g.N * ((w.g.Tq + 63) / 64);
-        if (blocks > na2d_tc::sm_count(at.device)) return f(std::integral_constant<int, 128>{});
+        long long small = 0, large = 0;
+        for (const SimtWork& w : pair.at) {
+            small += (long long)w.g.B * w.g.N * ((w.g.Tq + 63) / 64);
+            large += (long long)w.g.B * w.g.N * ((w.g.Tq + 127) / 128);
+        }
+        if (small > na2d_tc::sm_count(at.device) && 16 * large <= 9 * small) return f(std::integral_constant<int, 128>{});
         return f(std::integral_constant<int, 64>{});
     } else {
         return f(std::integral_constant<int, 32>{});
