@@ -43,6 +43,7 @@ struct Backward {
     Operand q, k, v, o, d_o, d_q, d_k, d_v;
     const float* lse;
     float* delta;
+    float* key_sums = nullptr;          // CUDA cores: room for simt_row_parts dK and dV, fp32; null: the key half is not taken in parts
 };
 int backward_bf16(const Place& at, const Scratch& scratch, const Backward& x);
 int backward_f16(const Place& at, const Scratch& scratch, const Backward& x);
@@ -56,6 +57,9 @@ struct Forward {
     float* lse;
 };
 int simt_forward(const Place& at, const Forward* x, int count);
+// Parts of the keys, whose wide o and lse, or wide d_q, lie one behind the other, and of the rows in the key half.
+int simt_key_parts(const Geom& g, int sms);
+int simt_row_parts(const Geom& g, int sms);
 int simt_backward(const Place& at, const Backward* x, int count);
 
 }  // namespace na2d_attn

@@ -190,44 +190,56 @@ template <typename DT>
 __device__ __forceinline__ DT* rows_of(const Operand& x, int b, int n) { return static_cast<DT*>(x.ptr) + b * x.b + n * x.n; }
 
 // What a launch works on: one problem, or two whose blocks share it (a prefix's keys and the entries' own: small ones take as long alone as
-// together).  `out`: o, dQ or dK; out2: dV.
+// together).  `out`: o, dQ or dK; out2: dV.  WIDE kernels take the other side (keys; rows in the key half) in `splits` parts of `each` tiles,
+// whose fp32 results lie `part` values apart, and lse B N Tq; sums and sums2 are those of the key half.
 struct SimtWork {
     Operand q, k, v, d_o, out, out2;
-    float *lse, *delta;
+    float *lse, *delta, *sums, *sums2;
     Geom g;
-    int tiles, vec;
-    unsigned blocks;
+    int tiles, vec, splits, each;
+    size_t part;
+    unsigned blocks;                    // of all parts
 };
 struct SimtPair {
     SimtWork at[2];
 };
-// The problem of this block, and its block of it.
-__device__ __forceinline__ const SimtWork& work_of(const SimtPair& p, unsigned& block) {
+// The problem of this block, its block of a part, and which part.
+template <bool WIDE>
+__device__ __forceinline__ const SimtWork& work_of(const SimtPair& p, unsigned& block, int& split) {
     const bool second = blockIdx.x >= p.at[0].blocks;
     block = blockIdx.x - (second ? p.at[0].blocks : 0u);
+    split = 0;
+    if constexpr (WIDE) {
+        const unsigned each = p.at[second].blocks / p.at[second].splits;
+        split = block / each;
+        block -= split * each;
+    }
     return p.at[second];
 }
 
 // ---- forward: a block has BT queries of one head ------------------------------------------------------------------
-template <typename DT, typename OT, int CP, int BM>
+template <typename DT, bool WIDE, int CP, int BM>
 __global__ void __launch_bounds__(kThreads)
 simt_fwd_kernel(const __grid_constant__ SimtPair pair) {
     using S = SimtCfg<CP, BM>;
+    using OT = std::conditional_t<WIDE, float, DT>;
     unsigned block;
-    const SimtWork& work = work_of(pair, block);
+    int split;
+    const SimtWork& work = work_of<WIDE>(pair, block, split);
     const Operand q = work.q, k = work.k, v = work.v, o = work.out;
-    float* __restrict__ lse = work.lse;
     const Geom g = work.g;
+    float* __restrict__ lse = work.lse + (WIDE ? split * ((size_t)g.B * g.N * g.Tq) : 0);
     const int tiles = work.tiles, vec = work.vec;
     extern __shared__ __align__(16) float smem[];
     float *sQ = smem, *sKV = sQ + S::HELD, *sP = sKV + S::TILE;
     const int tx = threadIdx.x % 32 / 2, ty = threadIdx.x / 32 * 2 + threadIdx.x % 2;
     const int bn = block / tiles, b = bn / g.N, n = bn - b * g.N, m = n / g.G;
     const int t0 = (g.causal ? tiles - 1 - (int)(block % tiles) : (int)(block % tiles)) * BM;
-    const int count = key_count(g, b), keys = keys_seen(g, count, min(t0 + BM, g.Tq) - 1);
+    const int count = key_count(g, b), all_keys = keys_seen(g, count, min(t0 + BM, g.Tq) - 1);
+    const int from = WIDE ? split * work.each * S::BT : 0, keys = WIDE ? min(all_keys, from + work.each * S::BT) : all_keys;
     Tile<DT, CP, BM>::bring(sQ, rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
     Tile<DT, CP, S::BT> tile;
-    if (keys > 0) tile.fetch(rows_of<DT>(k, b, m), k.t, 0, count, g.C, vec);
+    if (keys > from) tile.fetch(rows_of<DT>(k, b, m), k.t, from, count, g.C, vec);
     Sums<CP, BM> acc;
     float top[S::RM], total[S::RM];
 #pragma unroll
@@ -235,7 +247,7 @@ simt_fwd_kernel(const __grid_constant__ SimtPair pair) {
         top[i] = -CUDART_INF_F;
         total[i] = 0.f;
     }
-    for (int k0 = 0; k0 < keys; k0 += S::BT) {
+    for (int k0 = from; k0 < keys; k0 += S::BT) {
         __syncthreads();
         tile.put(sKV);
         tile.fetch(rows_of<DT>(v, b, m), v.t, k0, count, g.C, vec);
@@ -281,14 +293,15 @@ simt_fwd_kernel(const __grid_constant__ SimtPair pair) {
         if (tx == 0 && t < g.Tq)
             lse[row_index(g, b, n, t)] = sum == 0.f ? -CUDART_INF_F : (top[i] + log2f(sum)) * na2d_tc::kLn2;
     }
-    store_rows<OT, CP, BM>(rows_of<OT>(o, b, n), o.t, t0, g.Tq, g.C, acc, inv, tx, ty);
+    store_rows<OT, CP, BM>(rows_of<OT>(o, b, n) + (WIDE ? split * work.part : 0), o.t, t0, g.Tq, g.C, acc, inv, tx, ty);
 }
 
 // ---- delta = dO . o, a warp a row -------------------------------------------------------------------------------------
 template <typename DT>
 __global__ void __launch_bounds__(kThreads) simt_delta_kernel(const __grid_constant__ SimtPair pair) {
     unsigned block;
-    const SimtWork& work = work_of(pair, block);
+    int split;
+    const SimtWork& work = work_of<false>(pair, block, split);
     const Operand d_o = work.d_o, o = work.out;
     float* __restrict__ delta = work.delta;
     const Geom& g = work.g;
@@ -305,12 +318,14 @@ __global__ void __launch_bounds__(kThreads) simt_delta_kernel(const __grid_const
 }
 
 // ---- query half of the backward -----------------------------------------------------------------------------------------
-template <typename DT, typename OT, int CP, int BM>
+template <typename DT, bool WIDE, int CP, int BM>
 __global__ void __launch_bounds__(kThreads)
 simt_dq_kernel(const __grid_constant__ SimtPair pair) {
     using S = SimtCfg<CP, BM>;
+    using OT = std::conditional_t<WIDE, float, DT>;
     unsigned block;
-    const SimtWork& work = work_of(pair, block);
+    int split;
+    const SimtWork& work = work_of<WIDE>(pair, block, split);
     const Operand q = work.q, k = work.k, v = work.v, d_o = work.d_o, d_q = work.out;
     const float *__restrict__ lse = work.lse, *__restrict__ delta = work.delta;
     const Geom g = work.g;
@@ -320,11 +335,12 @@ simt_dq_kernel(const __grid_constant__ SimtPair pair) {
     const int tx = threadIdx.x % 32 / 2, ty = threadIdx.x / 32 * 2 + threadIdx.x % 2;
     const int bn = block / tiles, b = bn / g.N, n = bn - b * g.N, m = n / g.G;
     const int t0 = (g.causal ? tiles - 1 - (int)(block % tiles) : (int)(block % tiles)) * BM;
-    const int count = key_count(g, b), keys = keys_seen(g, count, min(t0 + BM, g.Tq) - 1);
+    const int count = key_count(g, b), all_keys = keys_seen(g, count, min(t0 + BM, g.Tq) - 1);
+    const int from = WIDE ? split * work.each * S::BT : 0, keys = WIDE ? min(all_keys, from + work.each * S::BT) : all_keys;
     Tile<DT, CP, BM>::bring(sQ, rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
     Tile<DT, CP, BM>::bring(sG, rows_of<DT>(d_o, b, n), d_o.t, t0, g.Tq, g.C, vec);
     Tile<DT, CP, S::BT> tile;
-    if (keys > 0) tile.fetch(rows_of<DT>(v, b, m), v.t, 0, count, g.C, vec);
+    if (keys > from) tile.fetch(rows_of<DT>(v, b, m), v.t, from, count, g.C, vec);
     Sums<CP, BM> acc;
     float neg[S::RM], del[S::RM], scale[S::RM];
 #pragma unroll
@@ -335,7 +351,7 @@ simt_dq_kernel(const __grid_constant__ SimtPair pair) {
         del[i] = row ? delta[row_index(g, b, n, t)] : 0.f;
         scale[i] = row ? g.scale : 0.f;
     }
-    for (int k0 = 0; k0 < keys; k0 += S::BT) {
+    for (int k0 = from; k0 < keys; k0 += S::BT) {
         __syncthreads();
         tile.put(sKV);
         tile.fetch(rows_of<DT>(k, b, m), k.t, k0, count, g.C, vec);
@@ -363,17 +379,18 @@ simt_dq_kernel(const __grid_constant__ SimtPair pair) {
         __syncwarp();
         acc.add(sP, sKV, tx, ty);
     }
-    store_rows<OT, CP, BM>(rows_of<OT>(d_q, b, n), d_q.t, t0, g.Tq, g.C, acc, scale, tx, ty);
+    store_rows<OT, CP, BM>(rows_of<OT>(d_q, b, n) + (WIDE ? split * work.part : 0), d_q.t, t0, g.Tq, g.C, acc, scale, tx, ty);
 }
 
 // ---- key half: a block has BT keys of one key head and walks the queries of every head that shares it ------------------------
-template <typename DT, int CP>
+template <typename DT, bool WIDE, int CP>
 __global__ void __launch_bounds__(kThreads)
 simt_dkdv_kernel(const __grid_constant__ SimtPair pair) {
     constexpr int BM = CP <= 128 ? 64 : 32;
     using S = SimtCfg<CP, BM>;
     unsigned block;
-    const SimtWork& work = work_of(pair, block);
+    int split;
+    const SimtWork& work = work_of<WIDE>(pair, block, split);
     const Operand q = work.q, k = work.k, v = work.v, d_o = work.d_o, d_k = work.out, d_v = work.out2;
     const float *__restrict__ lse = work.lse, *__restrict__ delta = work.delta;
     const Geom g = work.g;
@@ -400,48 +417,77 @@ simt_dkdv_kernel(const __grid_constant__ SimtPair pair) {
     }
     const int first = t_min / S::BT * S::BT;
     const bool any = k0 < count && first < g.Tq;
-    if (any) tile.fetch(rows_of<DT>(q, b, m * g.G), q.t, first, g.Tq, g.C, vec);
-    for (int n = m * g.G; any && n < (m + 1) * g.G; ++n) {
-        for (int t0 = first; t0 < g.Tq; t0 += S::BT) {
-            // rows of a piece are keys (ty), columns queries (tx).  Q stays in sX, dO goes to sY.
-            __syncthreads();
-            tile.put(sX);
-            tile.fetch(rows_of<DT>(d_o, b, n), d_o.t, t0, g.Tq, g.C, vec);
-            __syncthreads();
-            float p[S::R][S::R], dp[S::R][S::R];
-            dot_tile<CP, BM>(sK, sX, p, tx, ty);
-            float del[S::R];
-#pragma unroll
-            for (int j = 0; j < S::R; ++j) {
-                const int t = t0 + tx + 16 * j, seen = t < g.Tq ? keys_seen(g, count, t) : 0;
-                const float neg = seen ? -lse[row_index(g, b, n, t)] * na2d_tc::kLog2e : 0.f;
-                del[j] = seen ? delta[row_index(g, b, n, t)] : 0.f;
-#pragma unroll
-                for (int i = 0; i < S::R; ++i) p[i][j] = k0 + ty + 16 * i < seen ? exp2f(fmaf(p[i][j], g.sl2, neg)) : 0.f;
-            }
-            tile.put(sY);                                // (last read before the first barrier of this round)
-            const bool more = t0 + S::BT < g.Tq;
-            if (more || n + 1 < (m + 1) * g.G)
-                tile.fetch(rows_of<DT>(q, b, more ? n : n + 1), q.t, more ? t0 + S::BT : first, g.Tq, g.C, vec);
-#pragma unroll
-            for (int i = 0; i < S::R; ++i)
-#pragma unroll
-                for (int j = 0; j < S::R; ++j) sP[(ty + 16 * i) * S::LS + tx + 16 * j] = p[i][j];
-            __syncthreads();
-            dot_tile<CP, BM>(sV, sY, dp, tx, ty);
-            acc_v.add(sP, sY, tx, ty);
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < S::R; ++i)
-#pragma unroll
-                for (int j = 0; j < S::R; ++j)       // (by selection: what is not seen may hold anything)
-                    sP[(ty + 16 * i) * S::LS + tx + 16 * j] = p[i][j] == 0.f ? 0.f : p[i][j] * (dp[i][j] - del[j]);
-            __syncthreads();
-            acc_k.add(sP, sX, tx, ty);
+    // tiles of rows, of one head after the other: the part's first one and how many it has
+    int n = m * g.G, t0 = first, left = any ? g.G * ((g.Tq - first + S::BT - 1) / S::BT) : 0;
+    if constexpr (WIDE) {
+        const int per_head = (g.Tq - first + S::BT - 1) / S::BT, at = min(split * work.each, left);
+        left = min(left - at, work.each);
+        if (left > 0) {
+            n += at / per_head;
+            t0 += at % per_head * S::BT;
         }
+    }
+    if (left > 0) tile.fetch(rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
+    for (; left > 0; --left) {
+        // rows of a piece are keys (ty), columns queries (tx).  Q stays in sX, dO goes to sY.
+        __syncthreads();
+        tile.put(sX);
+        tile.fetch(rows_of<DT>(d_o, b, n), d_o.t, t0, g.Tq, g.C, vec);
+        __syncthreads();
+        float p[S::R][S::R], dp[S::R][S::R];
+        dot_tile<CP, BM>(sK, sX, p, tx, ty);
+        float del[S::R];
+#pragma unroll
+        for (int j = 0; j < S::R; ++j) {
+            const int t = t0 + tx + 16 * j, seen = t < g.Tq ? keys_seen(g, count, t) : 0;
+            const float neg = seen ? -lse[row_index(g, b, n, t)] * na2d_tc::kLog2e : 0.f;
+            del[j] = seen ? delta[row_index(g, b, n, t)] : 0.f;
+#pragma unroll
+            for (int i = 0; i < S::R; ++i) p[i][j] = k0 + ty + 16 * i < seen ? exp2f(fmaf(p[i][j], g.sl2, neg)) : 0.f;
+        }
+        tile.put(sY);                                // (last read before the first barrier of this round)
+        t0 += S::BT;
+        if (t0 >= g.Tq) {
+            t0 = first;
+            ++n;
+        }
+        if (left > 1) tile.fetch(rows_of<DT>(q, b, n), q.t, t0, g.Tq, g.C, vec);
+#pragma unroll
+        for (int i = 0; i < S::R; ++i)
+#pragma unroll
+            for (int j = 0; j < S::R; ++j) sP[(ty + 16 * i) * S::LS + tx + 16 * j] = p[i][j];
+        __syncthreads();
+        dot_tile<CP, BM>(sV, sY, dp, tx, ty);
+        acc_v.add(sP, sY, tx, ty);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < S::R; ++i)
+#pragma unroll
+            for (int j = 0; j < S::R; ++j)       // (by selection: what is not seen may hold anything)
+                sP[(ty + 16 * i) * S::LS + tx + 16 * j] = p[i][j] == 0.f ? 0.f : p[i][j] * (dp[i][j] - del[j]);
+        __syncthreads();
+        acc_k.add(sP, sX, tx, ty);
+    }
+    if (WIDE && work.splits > 1) {                       // summed by simt_sum_kernel
+        const size_t at = split * work.part + ((size_t)b * g.Nk + m) * g.Tk * g.C;
+        store_rows<float, CP, BM>(work.sums + at, g.C, k0, g.Tk, g.C, acc_k, scale_k, tx, ty);
+        store_rows<float, CP, BM>(work.sums2 + at, g.C, k0, g.Tk, g.C, acc_v, scale_v, tx, ty);
+        return;
     }
     store_rows<DT, CP, BM>(rows_of<DT>(d_k, b, m), d_k.t, k0, g.Tk, g.C, acc_k, scale_k, tx, ty);
     store_rows<DT, CP, BM>(rows_of<DT>(d_v, b, m), d_v.t, k0, g.Tk, g.C, acc_v, scale_v, tx, ty);
+}
+
+// dK and dV (the second row of blocks) from their parts, in the parts' order.
+template <typename DT>
+__global__ void __launch_bounds__(kThreads)
+simt_sum_kernel(const float* __restrict__ sums, const float* __restrict__ sums2, DT* __restrict__ d_k, DT* __restrict__ d_v, const size_t part, const int splits) {
+    const size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= part) return;
+    const float* from = blockIdx.y ? sums2 : sums;
+    float acc = 0.f;
+    for (int s = 0; s < splits; ++s) acc += from[s * part + i];
+    (blockIdx.y ? d_v : d_k)[i] = narrow<DT>(acc);
 }
 
 // ---- launchers ---------------------------------------------------------------------------------------------------------
@@ -495,7 +541,16 @@ int by_rows(const Place& at, const SimtPair& pair, F&& f) {
     }
 }
 
-template <typename DT, typename OT, int CP, int BM>
+// Parts of a WIDE kernel's other side.
+void cut_parts(SimtWork* w, int tiles, int splits) {
+    w->splits = splits;
+    w->each = (tiles + splits - 1) / splits;
+    w->blocks *= splits;
+}
+int tile_of(int C) { return C <= 128 ? 64 : 32; }
+size_t dense_rows(const Geom& g) { return (size_t)g.B * g.N * g.Tq * g.C; }
+
+template <typename DT, bool WIDE, int CP, int BM>
 int forward_as(const Place& at, SimtPair pair) {
     using S = SimtCfg<CP, BM>;
     static std::atomic<unsigned long long> opted{0};
@@ -503,27 +558,32 @@ int forward_as(const Place& at, SimtPair pair) {
         if (!w.q.ptr) continue;
         w.vec = vectors(w.q, at.dtype, w.g.C) && vectors(w.k, at.dtype, w.g.C) && vectors(w.v, at.dtype, w.g.C);
         if (int rc = cut_work(&w, (long long)w.g.B * w.g.N, w.g.Tq, BM)) return rc;
+        if (WIDE) cut_parts(&w, (w.g.Tk + S::BT - 1) / S::BT, simt_key_parts(w.g, na2d_tc::sm_count(at.device)));
+        w.part = dense_rows(w.g);
     }
-    return start(at, simt_fwd_kernel<DT, OT, CP, BM>, pair, S::HELD + S::TILE + S::SCORES, opted);
+    return start(at, simt_fwd_kernel<DT, WIDE, CP, BM>, pair, S::HELD + S::TILE + S::SCORES, opted);
 }
 
-template <typename DT, typename OT, int CP, int BM>
+template <typename DT, bool WIDE, int CP, int BM>
 int queries_as(const Place& at, SimtPair pair) {
     using S = SimtCfg<CP, BM>;
     static std::atomic<unsigned long long> opted{0};
-    for (SimtWork& w : pair.at)
-        if (w.q.ptr)
-            if (int rc = cut_work(&w, (long long)w.g.B * w.g.N, w.g.Tq, BM)) return rc;
-    return start(at, simt_dq_kernel<DT, OT, CP, BM>, pair, 2 * S::HELD + S::TILE + S::SCORES, opted);
+    for (SimtWork& w : pair.at) {
+        if (!w.q.ptr) continue;
+        if (int rc = cut_work(&w, (long long)w.g.B * w.g.N, w.g.Tq, BM)) return rc;
+        if (WIDE) cut_parts(&w, (w.g.Tk + S::BT - 1) / S::BT, simt_key_parts(w.g, na2d_tc::sm_count(at.device)));
+        w.part = dense_rows(w.g);
+    }
+    return start(at, simt_dq_kernel<DT, WIDE, CP, BM>, pair, 2 * S::HELD + S::TILE + S::SCORES, opted);
 }
 
 template <typename DT, int CP>
 int backward_as(const Place& at, const Backward* x, int count) {
     constexpr int BM = CP <= 128 ? 64 : 32;
     using S = SimtCfg<CP, BM>;
-    static std::atomic<unsigned long long> opted{0};
+    static std::atomic<unsigned long long> opted[2]{};
     SimtPair delta{}, queries{}, keys{};
-    bool wide = false;
+    bool wide = false, parts = false;
     for (int i = 0; i < count; ++i) {
         SimtWork w{};
         w.q = x[i].q;
@@ -533,6 +593,7 @@ int backward_as(const Place& at, const Backward* x, int count) {
         w.lse = const_cast<float*>(x[i].lse);
         w.delta = x[i].delta;
         w.g = *x[i].g;
+        w.splits = 1;
         w.vec = 1;
         for (const Operand* t : {&w.q, &w.k, &w.v, &w.d_o}) w.vec = w.vec && vectors(*t, at.dtype, w.g.C);
         delta.at[i] = w;
@@ -546,21 +607,57 @@ int backward_as(const Place& at, const Backward* x, int count) {
             wide = x[i].d_q.wide;
         }
         if (x[i].d_k.ptr) {
-            keys.at[i] = w;
-            keys.at[i].out = x[i].d_k;
-            keys.at[i].out2 = x[i].d_v;
-            if (int rc = cut_work(&keys.at[i], w.g.units, w.g.Tk, BM)) return rc;
+            SimtWork& y = keys.at[i];
+            y = w;
+            y.out = x[i].d_k;
+            y.out2 = x[i].d_v;
+            if (int rc = cut_work(&y, w.g.units, w.g.Tk, BM)) return rc;
+            const int splits = x[i].key_sums ? simt_row_parts(w.g, na2d_tc::sm_count(at.device)) : 1;
+            cut_parts(&y, w.g.G * ((w.g.Tq + S::BT - 1) / S::BT), splits);
+            y.part = (size_t)w.g.units * w.g.Tk * w.g.C;
+            y.sums = x[i].key_sums;
+            y.sums2 = x[i].key_sums + splits * y.part;
+            parts = parts || splits > 1;
         }
     }
-    if (int rc = start(at, simt_delta_kernel<DT>, delta, 0, opted)) return rc;
-    const int rc = by_rows<CP>(at, queries, [&](auto bm) {
-        constexpr int kRowsOf = decltype(bm)::value;
-        return wide ? queries_as<DT, float, CP, kRowsOf>(at, queries) : queries_as<DT, DT, CP, kRowsOf>(at, queries);
-    });
-    return rc != NA2D_OK ? rc : start(at, simt_dkdv_kernel<DT, CP>, keys, 4 * S::TILE + S::SCORES, opted);
+    if (int rc = start(at, simt_delta_kernel<DT>, delta, 0, opted[0])) return rc;
+    if (int rc = by_rows<CP>(at, queries, [&](auto bm) {
+            constexpr int kRowsOf = decltype(bm)::value;
+            return wide ? queries_as<DT, true, CP, kRowsOf>(at, queries) : queries_as<DT, false, CP, kRowsOf>(at, queries);
+        }))
+        return rc;
+    for (SimtWork& y : keys.at)
+        if (!y.splits) y.splits = 1;                     // (no blocks)
+    if (!parts) return start(at, simt_dkdv_kernel<DT, false, CP>, keys, 4 * S::TILE + S::SCORES, opted[0]);
+    if (int rc = start(at, simt_dkdv_kernel<DT, true, CP>, keys, 4 * S::TILE + S::SCORES, opted[1])) return rc;
+    for (const SimtWork& y : keys.at) {
+        if (y.splits == 1) continue;
+        const size_t blocks = (y.part + kThreads - 1) / kThreads;
+        if (blocks > 0x7fffffffULL) return NA2D_ERR_TOO_LARGE;
+        simt_sum_kernel<DT><<<dim3((unsigned)blocks, 2), kThreads, 0, at.st>>>(y.sums, y.sums2, static_cast<DT*>(y.out.ptr), static_cast<DT*>(y.out2.ptr),
+                                                                              y.part, y.splits);
+        *at.launched += 1;
+        if (cudaGetLastError() != cudaSuccess) return NA2D_ERR_CUDA;
+    }
+    return NA2D_OK;
+}
+
+// As many parts as give each SM two blocks where there are fewer blocks than SMs, of at least four tiles each.
+int parts_for(long long blocks, long long tiles, int sms) {
+    if (blocks >= sms) return 1;
+    return (int)std::max(1LL, std::min(2 * sms / std::max(1LL, blocks), tiles / 4));
 }
 
 }  // namespace
+
+int simt_key_parts(const Geom& g, int sms) {
+    return parts_for((long long)g.B * g.N * ((g.Tq + 63) / 64), (g.Tk + tile_of(g.C) - 1) / tile_of(g.C), sms);
+}
+int simt_row_parts(const Geom& g, int sms) {
+    if (g.causal) return 1;
+    const int tile = tile_of(g.C);
+    return parts_for((long long)g.units * ((g.Tk + tile - 1) / tile), (long long)g.G * ((g.Tq + tile - 1) / tile), sms);
+}
 
 int simt_forward(const Place& at, const Forward* x, int count) {
     SimtPair pair{};
@@ -573,13 +670,14 @@ int simt_forward(const Place& at, const Forward* x, int count) {
         w.lse = x[i].lse;
         w.g = *x[i].g;
     }
+    for (SimtWork& w : pair.at) w.splits = 1;
     auto run = [&](auto type) {
         using DT = decltype(type);
         return by_channels<DT>(x[0].g->C, [&](auto cp) {
             constexpr int CP = decltype(cp)::value;
             return by_rows<CP>(at, pair, [&](auto bm) {
                 constexpr int kRowsOf = decltype(bm)::value;
-                return x[0].o.wide ? forward_as<DT, float, CP, kRowsOf>(at, pair) : forward_as<DT, DT, CP, kRowsOf>(at, pair);
+                return x[0].o.wide ? forward_as<DT, true, CP, kRowsOf>(at, pair) : forward_as<DT, false, CP, kRowsOf>(at, pair);
             });
         });
     };

@@ -82,55 +82,69 @@ __global__ void __launch_bounds__(kThreads) gather_rows_kernel(const __grid_cons
 }
 
 // ---- joins ----------------------------------------------------------------------------------------------------------------
-// o and lse of a row from the prefix's and its own; a thread has N channels.
+// o and lse of a row from the prefix's and its own, either in parts of all rows; a thread has N channels.
 template <typename DT, int N>
 __global__ void __launch_bounds__(kThreads)
 join_outputs_kernel(const __grid_constant__ Rows g, const na2d_attn::Div by_pieces, const float* __restrict__ o_prefix,
-                    const float* __restrict__ lse_prefix, const float* __restrict__ o_own, const float* __restrict__ lse_own, DT* __restrict__ o,
-                    float* __restrict__ lse) {
+                    const float* __restrict__ lse_prefix, const float* __restrict__ o_own, const float* __restrict__ lse_own, const int prefix_parts,
+                    const int own_parts, DT* __restrict__ o, float* __restrict__ lse) {
     int r, c;
     const bool there = piece_of(g, by_pieces, r, c);
     const Row row = row_of(g, there ? r : 0);
     na2d_ptx::after_previous_grid();
     na2d_ptx::next_grid_may_start();
     if (!there) return;
-    const float x = lse_prefix[row.by_prefix], y = lse_own ? lse_own[r] : -CUDART_INF_F;
-    // (of rows that see nothing, nothing was written)
-    Vec<float, N> u, v;
-    if (x != -CUDART_INF_F) u.load(o_prefix + row.by_prefix * g.C + c * N);
-    if (y != -CUDART_INF_F) v.load(o_own + (long long)r * g.C + c * N);
+    const int parts = prefix_parts + own_parts;
+    auto place = [&](int i) { return i < prefix_parts ? i * g.all + row.by_prefix : (i - prefix_parts) * g.all + r; };
+    auto lse_of = [&](int i) { return (i < prefix_parts ? lse_prefix : lse_own)[place(i)]; };
+    float top = lse_of(0);
+    for (int i = 1; i < parts; ++i) top = fmaxf(top, lse_of(i));
     // (a NaN stays one: the maximum skips it, its weight does not)
-    const float top = fmaxf(x, y), base = top == -CUDART_INF_F ? 0.f : top;
-    const float wx = expf(x - base), wy = expf(y - base), total = wx + wy, inv = total == 0.f ? 0.f : 1.f / total;
-    float out[N];
+    const float base = top == -CUDART_INF_F ? 0.f : top;
+    float out[N], total = 0.f;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-        out[k] = x != -CUDART_INF_F ? u.at[k] * (wx * inv) : 0.f;
-        if (y != -CUDART_INF_F) out[k] = fmaf(v.at[k], wy * inv, out[k]);
+    for (int k = 0; k < N; ++k) out[k] = 0.f;
+#pragma unroll 2
+    for (int i = 0; i < parts; ++i) {
+        const float of = lse_of(i);
+        if (of == -CUDART_INF_F) continue;               // of rows that see nothing, nothing was written
+        Vec<float, N> v;
+        v.load((i < prefix_parts ? o_prefix : o_own) + place(i) * g.C + c * N);
+        const float w = expf(of - base);
+        total += w;
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] = fmaf(v.at[k], w, out[k]);
     }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int k = 0; k < N; ++k) out[k] *= inv;
     Vec<DT, N> to;
     to.round(out);
     to.store(o + (long long)r * g.C + c * N);
     if (c == 0) lse[r] = total == 0.f ? -CUDART_INF_F : base + logf(total);
 }
 
-// dq of a row: the sum of the prefix's and its own.
+// dq of a row: the sum of the prefix's parts and its own, in their order.
 template <typename DT, int N>
 __global__ void __launch_bounds__(kThreads)
 join_gradients_kernel(const __grid_constant__ Rows g, const na2d_attn::Div by_pieces, const float* __restrict__ prefix, const float* __restrict__ own,
-                      DT* __restrict__ d_q) {
+                      const int prefix_parts, const int own_parts, DT* __restrict__ d_q) {
     int r, c;
     const bool there = piece_of(g, by_pieces, r, c);
     const Row row = row_of(g, there ? r : 0);
     na2d_ptx::after_previous_grid();
     na2d_ptx::next_grid_may_start();
     if (!there) return;
-    Vec<float, N> x, y;
-    x.load(prefix + row.by_prefix * g.C + c * N);
-    if (own) y.load(own + (long long)r * g.C + c * N);
     float out[N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) out[k] = own ? x.at[k] + y.at[k] : x.at[k];
+    for (int k = 0; k < N; ++k) out[k] = 0.f;
+#pragma unroll 2
+    for (int i = 0; i < prefix_parts + own_parts; ++i) {
+        Vec<float, N> x;
+        x.load((i < prefix_parts ? prefix + (i * g.all + row.by_prefix) * g.C : own + ((i - prefix_parts) * g.all + r) * g.C) + c * N);
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] += x.at[k];
+    }
     Vec<DT, N> to;
     to.round(out);
     to.store(d_q + (long long)r * g.C + c * N);
@@ -239,6 +253,9 @@ int least_steps(const Problem& p) {
     return std::max(2, (int)(std::sqrt((double)longest) / 3 + 0.5));
 }
 
+// Parts that the kernels on CUDA cores take a half's keys in.
+int key_parts(const Problem& p, const Geom& g, int sms) { return p.tensor ? 1 : na2d_attn::simt_key_parts(g, sms); }
+
 struct ForwardLayout {
     size_t q, o_prefix, lse_prefix, o_own, lse_own, scratch, scratch_bytes, own_scratch, own_scratch_bytes, table, part_o, part_lse, size;
 };
@@ -249,13 +266,15 @@ ForwardLayout forward_layout(const Problem& p, int sms) {
     const OnLine line = on_line(p);
     if (!line.prefix) {
         if (!p.follow[0]) f.q = l.take(values * esize_of(p));
-        f.o_prefix = l.take(values * 4);
-        f.lse_prefix = l.take(rows * 4);
+        const int parts = key_parts(p, p.prefix, sms);
+        f.o_prefix = l.take(parts * values * 4);
+        f.lse_prefix = l.take(parts * rows * 4);
         if (p.tensor) f.scratch_bytes = na2d_attn::forward_floats(p.prefix, sms) * 4;
     }
     if (p.any_own && !line.own) {
-        f.o_own = l.take(values * 4);
-        f.lse_own = l.take(rows * 4);
+        const int parts = key_parts(p, p.own, sms);
+        f.o_own = l.take(parts * values * 4);
+        f.lse_own = l.take(parts * rows * 4);
         if (p.tensor) f.own_scratch_bytes = na2d_attn::forward_floats(p.own, sms) * 4;
     }
     f.scratch = l.take(f.scratch_bytes);
@@ -270,9 +289,9 @@ ForwardLayout forward_layout(const Problem& p, int sms) {
     return f;
 }
 struct BackwardLayout {
-    size_t rows[3], lse, delta_prefix, delta, dq_prefix, dq_own, scratch, scratch_bytes, size;
+    size_t rows[3], lse, delta_prefix, delta, dq_prefix, dq_own, scratch, scratch_bytes, prefix_sums, own_sums, size;
 };
-// (own or prefix: whether that half's keys have gradients)
+// d_prefix, d_own: whether that half's keys have gradients.
 BackwardLayout backward_layout(const Problem& p, int sms, bool d_q, bool d_prefix, bool d_own) {
     Layout l;
     BackwardLayout f{};
@@ -284,9 +303,14 @@ BackwardLayout backward_layout(const Problem& p, int sms, bool d_q, bool d_prefi
     f.delta_prefix = l.take(rows * 4);
     f.delta = l.take(rows * 4);
     if (d_q) {
-        f.dq_prefix = l.take(values * 4);
-        if (p.any_own) f.dq_own = l.take(values * 4);
+        f.dq_prefix = l.take(key_parts(p, p.prefix, sms) * values * 4);
+        if (p.any_own) f.dq_own = l.take(key_parts(p, p.own, sms) * values * 4);
     }
+    auto sums = [&](const Geom& g) {                     // of the key half on CUDA cores
+        return l.take(p.tensor ? 0 : 2 * (size_t)na2d_attn::simt_row_parts(g, sms) * g.units * g.Tk * g.C * 4);
+    };
+    if (d_prefix) f.prefix_sums = sums(p.prefix);
+    if (p.any_own && d_own) f.own_sums = sums(p.own);
     if (p.tensor) {
         f.scratch_bytes = na2d_attn::backward_floats(p.prefix, sms, f16, d_q, d_prefix) * 4;
         if (p.any_own) f.scratch_bytes = std::max(f.scratch_bytes, na2d_attn::backward_floats(p.own, sms, f16, d_q, d_own) * 4);
@@ -367,19 +391,20 @@ int gather(const na2d_attn::Place& at, const Problem& p, const Operand* const* f
 template <typename DT, int N>
 int join_outputs(const na2d_attn::Place& at, const Problem& p, const float* o_prefix, const float* lse_prefix, const float* o_own,
                  const float* lse_own, void* o, float* lse) {
-    const int pieces = p.rows.C / N;
+    const int pieces = p.rows.C / N, sms = na2d_host::sm_count(at.device);
     *at.launched += 1;
     return na2d_launch::launch(true, join_outputs_kernel<DT, N>, blocks_of(p.rows, pieces), kThreads, 0, at.st, p.rows, na2d_attn::Div(pieces), o_prefix,
-                               lse_prefix, o_own, lse_own, static_cast<DT*>(o), lse) == cudaSuccess
+                               lse_prefix, o_own, lse_own, key_parts(p, p.prefix, sms), p.any_own ? key_parts(p, p.own, sms) : 0, static_cast<DT*>(o),
+                               lse) == cudaSuccess
                ? NA2D_OK
                : NA2D_ERR_CUDA;
 }
 template <typename DT, int N>
 int join_gradients(const na2d_attn::Place& at, const Problem& p, const float* prefix, const float* own, void* d_q) {
-    const int pieces = p.rows.C / N;
+    const int pieces = p.rows.C / N, sms = na2d_host::sm_count(at.device);
     *at.launched += 1;
     return na2d_launch::launch(true, join_gradients_kernel<DT, N>, blocks_of(p.rows, pieces), kThreads, 0, at.st, p.rows, na2d_attn::Div(pieces), prefix,
-                               own, static_cast<DT*>(d_q)) == cudaSuccess
+                               own, key_parts(p, p.prefix, sms), p.any_own ? key_parts(p, p.own, sms) : 0, static_cast<DT*>(d_q)) == cudaSuccess
                ? NA2D_OK
                : NA2D_ERR_CUDA;
 }
@@ -532,6 +557,7 @@ int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a) {
                 if (d_prefix) {
                     b.d_k = result(a->d_prefix_k.ptr, a->S, a->P);
                     b.d_v = result(a->d_prefix_v.ptr, a->S, a->P);
+                    if (!p.tensor) b.key_sums = floats(f.prefix_sums);
                 }
             }
             if (p.any_own && (d_q || d_own)) {
@@ -548,6 +574,7 @@ int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a) {
                 if (d_own) {
                     b.d_k = result(a->d_k.ptr, a->B, a->Tk);
                     b.d_v = result(a->d_v.ptr, a->B, a->Tk);
+                    if (!p.tensor) b.key_sums = floats(f.own_sums);
                 }
             }
             if (int rc = backward_of(p, at, scratch, x_of, count)) return rc;
