@@ -674,6 +674,84 @@ def test_a_call_recorded_by_a_dispatch_mode_runs_again(which, grad):
     assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+# ---- beside and behind other work ---------------------------------------------------------------------------------------
+TOKENS = [(1, 64, 8, 2, 3000, 1, 200, 128), (16, 4, 16, 4, 1000, 1, 100, 64), (2, 6, 4, 2, 900, 5, 100, 128), (1, 2, 16, 2, 260, 5, 400, 64)]
+
+
+@pytest.mark.parametrize("shape", TOKENS, ids=str)
+def test_tokens_right_behind_what_writes_their_inputs(shape):
+    """Kernels start under the ones before them: every input, the lengths too, is written just before the call that reads it."""
+    S, A, N, Nk, P, Tq, Tk, C = shape
+    sources = [operands(*shape, BF16, seed=10 * i)[:5] for i in range(3)]
+    own = [torch.randint(Tq, Tk + 1, (S * A,), generator=torch.Generator().manual_seed(i)).int().to(DEV) for i in range(3)]
+    prompts = [torch.randint(1, P + 1, (S,), generator=torch.Generator().manual_seed(i)).int().to(DEV) for i in range(3)]
+    at = [t.clone() for t in sources[0]]
+    lengths, prefix_lengths = own[0].clone(), prompts[0].clone()
+
+    def call(i):
+        for t, source in zip(at, sources[i]):
+            t.copy_(source)
+        prefix_lengths.copy_(prompts[i])
+        lengths.copy_(own[i])
+        return na.prefix_attention(*at, C ** -0.5, True, lengths, prefix_lengths)
+    want = []
+    for i in range(3):
+        want.append(call(i))
+        torch.cuda.synchronize()
+    got = [call(i % 3) for i in range(30)]
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 3]), i
+    na.check_kernels(DEV)
+
+
+def test_calls_on_two_streams_at_once():
+    shapes = TOKENS[:2]
+    inputs = [operands(*shape, BF16, seed=i)[:5] for i, shape in enumerate(shapes)]
+    logits = [beams(8, 4, 30011, BF16, i) for i in range(2)]
+    caches = [torch.randn(8, 4, 500, 64, device=DEV) for _ in range(2)]
+    parents = [parents_of(2, 4, i) for i in range(2)]
+
+    def work(i):
+        o = na.prefix_attention(*inputs[i], 0.125, True)
+        moved = caches[i].clone()
+        na.beam_reorder([moved], parents[i])
+        return (o, *na.beam_select(*logits[i], 8), moved)
+    want = [work(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(work(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+    na.check_kernels(DEV)
+
+
+def test_choices_and_caches_right_behind_what_writes_them():
+    sources = [beams(6, 4, 40003, F16, i) for i in range(3)]
+    logits, scores = (t.clone() for t in sources[0])
+    cache, state = torch.zeros(24, 2, 300, 64, device=DEV), torch.randn(24, 2, 300, 64, device=DEV)
+
+    def call(i):
+        logits.copy_(sources[i][0])
+        scores.copy_(sources[i][1])
+        cache.copy_(state)
+        found = na.beam_select(logits, scores)
+        na.beam_reorder(cache, found[1])
+        return (*found, cache.clone())
+    want = []
+    for i in range(3):
+        want.append(call(i))
+        torch.cuda.synchronize()
+        assert torch.equal(want[-1][3], plain_reorder(state, want[-1][1]))
+    for i, out in enumerate([call(i % 3) for i in range(30)]):
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i % 3])), i
+
+
 # ---- refusals -------------------------------------------------------------------------------------------------------
 def test_prefix_attention_refuses():
     q, pk = torch.zeros(4, 4, 3, 32, device=DEV, dtype=BF16), torch.zeros(2, 2, 9, 32, device=DEV, dtype=BF16)
