@@ -8,7 +8,7 @@
 // select_beams_kernel joins an entry's segments: sums in 64 bits, candidates by the same bound.  (value, lowest beam, lowest word) is a
 // total order, so nothing depends on the order in which candidates arrive.  What a block keeps has room for 512: where more words reach
 // the bound (equal ones, ascending ones) it looks for the best below the last one, `count` times over.
-// Measured: 64 x 8 x 131072 fp32, 268 MB: 56 us, 73 % of the copy bandwidth (the rows 54, issue slots 61 %); 7 x 5 x 100003 fp16, rows on odd
+// Measured: 64 x 8 x 131072 fp32, 268 MB: 55 us, 74 % of the copy bandwidth (the rows 53, issue slots 54 %); 7 x 5 x 100003 fp16, rows on odd
 // places, 15 us, of which the rows are 8 and the joining 6; 16 x 4 x 32768 bf16 10.6, the host's time of the call.
 //
 // Reordering.  cache[g K + i] <- cache[g K + parent_gi] for all beams of a group at once, in place: a thread has the same few bytes of
@@ -98,9 +98,17 @@ struct Select {
 };
 
 // e^x for x <= 0.  (1 / ln 2 in one number: off by 1.4e-8 of x, the same way in every beam.)
-__device__ __forceinline__ float exp_of(float x) {
+constexpr float kLog2e = 1.44269502f;
+__device__ __forceinline__ float exp2_of(float x) {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269502f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float exp_of(float x) { return exp2_of(x * kLog2e); }
+// The largest of three that is a number.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -156,16 +164,21 @@ __global__ void __launch_bounds__(kThreads) select_rows_kernel(const Select x) {
         if (c + 1 < chunks) next.load(src, c + 1, words);
         float most = -kInf;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) most = fmaxf(most, v[j]);
+        for (int j = 0; j < kEach; j += 2) most = max3(most, v[j], v[j + 1]);
         if (most > high) {
             total *= exp_of(high - most);                // (from -infinity on: a sum of nothing)
             high = most;
         }
         const float base = high == -kInf ? 0.f : high;
-        float sum[2] = {0.f, 0.f};
+        // (two at a time: half the issue slots of all but the exponentials)
+        const uint64_t less = na2d_ptx::pair2(-base, -base), by = na2d_ptx::pair2(kLog2e, kLog2e);
+        uint64_t sum = 0;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) sum[j & 1] += exp_of(v[j] - base);
-        total += sum[0] + sum[1];
+        for (int j = 0; j < kEach; j += 2) {
+            const uint64_t y = na2d_ptx::mul2(na2d_ptx::add2(na2d_ptx::pair2(v[j], v[j + 1]), less), by);
+            sum = na2d_ptx::add2(sum, na2d_ptx::pair2(exp2_of(na2d_ptx::lo2(y)), exp2_of(na2d_ptx::hi2(y))));
+        }
+        total += na2d_ptx::lo2(sum) + na2d_ptx::hi2(sum);
         if (c + 1 == renew) {
             __syncthreads();                             // (`warps` has been read)
             const unsigned bound = bound_of(high == -kInf ? 0u : ordered(high), x.count, warps);
@@ -389,7 +402,7 @@ __global__ void __launch_bounds__(kThreads) select_beams_kernel(const Select x) 
 }
 
 // Segments of a row: so many chunks each, up to 16, as give all SMs their four blocks.  A block that lives long has its loads under way for more of
-// its time: 64 x 8 rows of 131072 words in fp32 take 56 us with 16 chunks a block (1024 blocks), 63 with 7.
+// its time: 64 x 8 rows of 131072 words in fp32 take 55 us with 16 chunks a block (1024 blocks), 63 with 7.
 struct Cut {
     int segments, each;                 // each: words of one
 };
