@@ -216,6 +216,7 @@ int make_problem(const na2d_prefix_attention_args* a, Problem* p) {
     for (int i = 0; i < 3; ++i) p->follow[i] = A == 1 || a->Tq == 1 || by_rows[i]->b == a->Tq * by_rows[i]->t;
     bool fits = a->dtype != NA2D_F32 && a->C <= 128 && a->C % 8 == 0;
     for (const Operand* x : {&p->q, &p->k, &p->v, &p->pk, &p->pv, &p->o, &p->d_o}) fits = fits && (!x->ptr || na2d_attn::tma_ready(*x));
+    for (const na2d_heads* x : {&a->d_k, &a->d_v, &a->d_prefix_k, &a->d_prefix_v}) fits = fits && reinterpret_cast<uintptr_t>(x->ptr) % 16 == 0;      // (dense)
     if (a->path == NA2D_PATH_TENSOR && !fits) return NA2D_ERR_UNSUPPORTED;
     p->tensor = fits && a->path != NA2D_PATH_SIMT;
     p->heads_as_rows = p->any_own && !p->tensor && a->Tq == 1 && a->N > a->Nk;
@@ -421,12 +422,12 @@ int join_gradients(const na2d_attn::Place& at, const Problem& p, const float* pr
                ? NA2D_OK
                : NA2D_ERR_CUDA;
 }
-// f(element type, channels of a vector)
+// f(element type, channels of a vector) for rows that are written at `to`
 template <typename F>
-int by_type(const Problem& p, F&& f) {
+int by_type(const Problem& p, const void* to, F&& f) {
     using One = std::integral_constant<int, 1>;
     using Four = std::integral_constant<int, 4>;
-    const bool four = p.rows.C % 4 == 0;
+    const bool four = p.rows.C % 4 == 0 && reinterpret_cast<uintptr_t>(to) % (4 * esize_of(p)) == 0;
     if (p.dtype == NA2D_F32) return four ? f(float{}, Four{}) : f(float{}, One{});
     if (p.dtype == NA2D_BF16) return four ? f(__nv_bfloat16{}, Four{}) : f(__nv_bfloat16{}, One{});
     return four ? f(__half{}, Four{}) : f(__half{}, One{});
@@ -509,7 +510,7 @@ int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a) {
                                             : na2d_prefix::tokens_f16(at, x, by_prefix, by_own, a->o.ptr, a->lse, p.B);
             }
             const float *o_own = p.any_own ? floats(f.o_own) : nullptr, *lse_own = p.any_own ? floats(f.lse_own) : nullptr;
-            return by_type(p, [&](auto type, auto n) {
+            return by_type(p, a->o.ptr, [&](auto type, auto n) {
                 return join_outputs<decltype(type), decltype(n)::value>(at, p, floats(f.o_prefix), floats(f.lse_prefix), o_own, lse_own, a->o.ptr, a->lse);
             });
         };
@@ -592,7 +593,7 @@ int na2d_prefix_attention_backward(const na2d_prefix_attention_args* a) {
             }
             if (int rc = backward_of(p, at, scratch, x_of, count)) return rc;
             if (!d_q) return NA2D_OK;
-            return by_type(p, [&](auto type, auto n) {
+            return by_type(p, a->d_q.ptr, [&](auto type, auto n) {
                 return join_gradients<decltype(type), decltype(n)::value>(at, p, floats(f.dq_prefix), p.any_own ? floats(f.dq_own) : nullptr, a->d_q.ptr);
             });
         };

@@ -88,6 +88,12 @@ def test_prefix_attention_refuses_bad_arguments_without_touching_cuda(backward):
     assert prefix(False, Tk=0, k=NOTHING, v=NOTHING) in GPU_WANTED
 
 
+@pytest.mark.parametrize("name", ["d_k", "d_v", "d_prefix_k", "d_prefix_v"])
+def test_prefix_attention_asks_for_key_gradients_on_16_bytes_for_tensor_cores(name):
+    assert prefix(True, **{name: _lib.Heads(258, 0, 0, 0)}, path=_lib.PATH_TENSOR) == _lib.ERR_UNSUPPORTED
+    assert prefix(True, d_q=_lib.Heads(258, 0, 0, 0), path=_lib.PATH_TENSOR) in GPU_WANTED        # (written by the join, in pieces that fit)
+
+
 def test_prefix_attention_workspaces():
     """Bounded by the rows and the device: the partial results of few rows do not grow with the keys."""
     room = lambda backward=0, **kw: lib.na2d_prefix_attention_workspace(C.byref(prefix_args(bool(backward), **kw)), backward)

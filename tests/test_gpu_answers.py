@@ -6,12 +6,14 @@ results once, and what is joined in between is fp32.  beam_select's words and pa
 its logarithm of a sum is off by less than 2^-22: exponentials by 2^-22 of themselves, of either sign, in sums of many.  beam_reorder
 moves bytes.
 """
+import ctypes
 import math
 
 import pytest
 import torch
 
 import e_natten_b200 as na
+from e_natten_b200 import _lib
 from test_gpu_block import BF16, DEV, F16, F32, close, differences, rand
 
 pytestmark = pytest.mark.gpu
@@ -324,6 +326,63 @@ def test_prefix_attention_infinities_and_nan():
     sign = q[2:, 1, :, 0].double() > 0                   # +infinity among the logits: NaN; -infinity: a weight of zero
     want[2:, 1] = sign
     assert torch.equal(bad, want)
+
+
+@pytest.mark.parametrize("odd", [("o",), ("d_q",), ("d_k",), ("d_prefix_v",), ("o", "d_q", "d_k", "d_v", "d_prefix_k", "d_prefix_v")])
+@pytest.mark.parametrize("dtype,C,Tq,Tk", [(F32, 32, 5, 7), (F32, 20, 1, 3), (BF16, 64, 40, 9), (BF16, 64, 1, 0), (F16, 20, 9, 7)])
+def test_prefix_attention_results_on_any_place(dtype, C, Tq, Tk, odd):
+    """Results of the C ABI that start one element behind a 16-byte boundary: what the same kernels write elsewhere, bit by bit, and
+    nothing beside them."""
+    B, S, N, Nk, P = 4, 2, 4, 2, 37
+    q, d_o = rand(B, N, Tq, C, dtype=dtype), rand(B, N, Tq, C, dtype=dtype, seed=1)
+    pk, pv = rand(S, Nk, P, C, dtype=dtype, seed=2), rand(S, Nk, P, C, dtype=dtype, seed=3)
+    k, v = rand(B, Nk, Tk, C, dtype=dtype, seed=4), rand(B, Nk, Tk, C, dtype=dtype, seed=5)
+    lse = torch.empty(B, N, Tq, device=DEV)
+
+    def call(odd, forward, backward):
+        a = _lib.PrefixAttentionArgs()
+        a.struct_size = ctypes.sizeof(a)
+        a.B, a.S, a.N, a.Nk, a.Tq, a.Tk, a.P, a.C = B, S, N, Nk, Tq, Tk, P, C
+        a.dtype, a.scale = {F32: 0, BF16: 1, F16: 2}[dtype], 0.3
+        a.stream = torch.cuda.current_stream(DEV).cuda_stream
+        for name, t in (("q", q), ("prefix_k", pk), ("prefix_v", pv)) + ((("k", k), ("v", v)) if Tk else ()):
+            setattr(a, name, _lib.Heads(t.data_ptr(), 0, 0, 0))
+        a.lse = lse.data_ptr()
+        out = {}
+
+        def give(name, like):
+            room = torch.full((like.numel() + 16,), 7.0, dtype=dtype, device=DEV)
+            at = 1 if name in odd else 0
+            out[name] = (room, room[at:at + like.numel()].view(like.shape))
+            setattr(a, name, _lib.Heads(out[name][1].data_ptr(), 0, 0, 0))
+
+        def run(path, of_backward):
+            a.path = path
+            need = _lib.lib.na2d_prefix_attention_workspace(ctypes.byref(a), of_backward)
+            assert need > 0
+            workspace = torch.empty(need, dtype=torch.uint8, device=DEV)
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), need
+            _lib.check((_lib.lib.na2d_prefix_attention_backward if of_backward else _lib.lib.na2d_prefix_attention_forward)(ctypes.byref(a)))
+            na.check_kernels(DEV)
+
+        give("o", q)
+        run(forward, 0)
+        a.d_o = _lib.Heads(d_o.data_ptr(), 0, 0, 0)
+        for name, like in (("d_q", q), ("d_prefix_k", pk), ("d_prefix_v", pv)) + ((("d_k", k), ("d_v", v)) if Tk else ()):
+            give(name, like)
+        run(backward, 1)
+        for name, (room, t) in out.items():
+            at = 1 if name in odd else 0
+            assert (room[:at] == 7).all() and (room[at + t.numel():] == 7).all(), name
+        return {name: t for name, (_, t) in out.items()}
+
+    # (o, and gradients of keys, that lie so are the CUDA cores'; a d_q is not)
+    simt = _lib.PATH_SIMT
+    forward = simt if "o" in odd else _lib.PATH_AUTO
+    backward = _lib.PATH_AUTO if odd == ("d_q",) or not Tk and odd == ("d_k",) else simt
+    want = call((), forward, backward)
+    for name, t in call(odd, _lib.PATH_AUTO, _lib.PATH_AUTO).items():
+        assert torch.equal(t, want[name]), name
 
 
 @pytest.mark.parametrize("Tq", [1, 40])
