@@ -46,6 +46,7 @@ struct Geom {
     float scale, sl2;                       // the softmax scale, and times log2(e)
     Div by_nk, by_tt, by_tiles_t, by_tiles, by_units;
     int parts = 0;                          // forward, units of several tiles: parts of each unit's keys, all of the same length; 0: by a rule
+    bool joint = false;                     // rows see other keys, too: o and lse are over all of them
 };
 
 // Rows in tiles (host); several heads in one only with `pack`.
@@ -132,22 +133,25 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int first, int lane) {
 
 #endif
 
-// fp16: what bounds |dO . V|, from which the backward takes the power of two that its dS go into their products with (ds_shift).
+// fp16: what bounds |dO . V| and |delta|, from which the backward takes the power of two that its dS go into their products with (ds_shift).
 struct Bounds {
     float* unit;            // (units, 2): the largest squared norms of the dO rows that see keys and of V's rows
     float* row;             // (B, N, Tq): the squared norm of a dO row
+    float* delta;           // joint rows: (units,): the largest square of the delta of rows that see keys; else null
 };
 
 #ifdef __CUDACC__
-// s so that |dS| 2^s stays below 2^15, given the squared norms of dO and V: |dP| and |delta| are at most the norms' product.  dS and
-// the rest that rounding leaves of it are then within fp16's 2^-24 of a largest value near its end, whatever the size of gradients
+// s so that |dS| 2^s stays below 2^15, given the squared norms of dO and V: |dP| and |delta| are at most the norms' product.  (Of joint rows
+// |delta| is not, o being of other values, too: they give the square of delta.)  dS and the rest that rounding leaves of it are then within fp16's 2^-24 of a largest value near its end, whatever the size of gradients
 // (unshifted, weights of 2^-14 times gradients of 1e-2 were half lost, and dS beyond 65504 infinite).
-__device__ __forceinline__ int ds_shift(float d_o_square, float v_square) {
-    const float square = d_o_square * v_square;              // 2^-96 to 2^78 for numbers of fp16
+__device__ __forceinline__ int ds_shift(float d_o_square, float v_square, float delta_square = 0.f) {
+    const float square = fmaxf(d_o_square * v_square, delta_square);         // 2^-96 to 2^78 for numbers of fp16
     if (!(square > 0.f) || square == CUDART_INF_F) return 0;
     const int e = (__float_as_int(square) >> 23) - 127;      // square < 2^(e + 1)
     return 14 - ((e + 2) >> 1);
 }
+// x^2, or 0 where that is infinite or no number: what such a delta gives is no number whatever the shift.
+__device__ __forceinline__ float finite_square(float x) { return x * x < CUDART_INF_F ? x * x : 0.f; }
 __device__ __forceinline__ float exp2i(int s) { return __int_as_float((s + 127) << 23); }      // |s| < 127
 #endif
 

@@ -158,7 +158,7 @@ template <typename DT>
 __device__ __forceinline__ int unit_shift(const Geom& g, const Bounds& bounds, const KeyItem& k) {
     if constexpr (IsBf16<DT>::value) return 0;
     const float2 squares = __ldg(reinterpret_cast<const float2*>(bounds.unit) + k.b * g.Nk + k.m);
-    return ds_shift(squares.x, squares.y);
+    return ds_shift(squares.x, squares.y, g.joint ? __ldg(bounds.delta + k.b * g.Nk + k.m) : 0.f);
 }
 
 template <typename DT, int D, bool LINE>

@@ -26,7 +26,8 @@
 
 namespace na2d_attn {
 
-// delta = dO . o of each row, 8 channels a lane; fp16: the norms of dO and, by the blocks behind row_blocks, of V, too.  LPR lanes a row:
+// delta = dO . o of each row, 8 channels a lane; fp16: the norms of dO and, by the blocks behind row_blocks, of V, too (and of joint rows
+// the largest delta).  LPR lanes a row:
 // C / 8, rounded up to a power of two.  A lane has kDeltaRows rows of one head, 256 / LPR apart, all under way at once (8 x 16 heads x 3136 x
 // 64: 16.5 us, 6.2 TB/s, with the norms 19; with one row a lane 24).
 constexpr int kDeltaRows = 4;
@@ -82,7 +83,7 @@ attn_delta_kernel(const DT* __restrict__ d_o, const Operand st_do, const DT* __r
         }
     }
     const int count = IsBf16<DT>::value ? 0 : key_count(g, b);
-    float top = 0.f;
+    float top = 0.f, top_delta = 0.f;
 #pragma unroll
     for (int i = 0; i < kDeltaRows; ++i) {
         float acc = na2d_delta::dot8<DT>(vx[i], vy[i], 0.f);
@@ -95,10 +96,20 @@ attn_delta_kernel(const DT* __restrict__ d_o, const Operand st_do, const DT* __r
 #pragma unroll
             for (int d = LPR / 2; d > 0; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
             if (part == 0 && t < g.Tq) bounds.row[static_cast<size_t>(bn) * g.Tq + t] = square;
-            if (t < g.Tq && keys_seen(g, count, t) > 0 && square < CUDART_INF_F) top = fmaxf(top, square);
+            if (t < g.Tq && keys_seen(g, count, t) > 0) {
+                if (square < CUDART_INF_F) top = fmaxf(top, square);
+                top_delta = fmaxf(top_delta, finite_square(acc));
+            }
         }
     }
-    if constexpr (!IsBf16<DT>::value) largest(top, bounds.unit + 2 * (b * g.Nk + n / g.G));
+    if constexpr (!IsBf16<DT>::value) {
+        const int unit = b * g.Nk + n / g.G;
+        largest(top, bounds.unit + 2 * unit);
+        if (g.joint) {
+            __syncthreads();                             // (`warps` has been read)
+            largest(top_delta, bounds.delta + unit);
+        }
+    }
 }
 
 struct RowCut {
@@ -417,7 +428,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             float scale = g.scale;
             if constexpr (!IsBf16<DT>::value) {
                 if (ok && !none)
-                    scale *= exp2i(-ds_shift(__ldg(bounds.row + row_index(g, tile.b, n, t)), __ldg(bounds.unit + 2 * (tile.b * g.Nk + tile.m) + 1)));
+                    scale *= exp2i(-ds_shift(__ldg(bounds.row + row_index(g, tile.b, n, t)), __ldg(bounds.unit + 2 * (tile.b * g.Nk + tile.m) + 1),
+                                             WIDE && g.joint ? finite_square(__ldg(delta + row_index(g, tile.b, n, t))) : 0.f));
             }
             const bool blind = g.causal && keys_seen(g, tile.count, t) == 0;         // (beside rows that see: dS = 0 meets any key of theirs)
             if (!none) {
@@ -504,7 +516,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         while (next.n >= 0) {
             const RowTile tile = next.tile;
             const int chunks = next.n, c0 = next.c0;
-            const float row_lse = next_lse, row_delta = next_delta, shift = IsBf16<DT>::value ? 0.f : (float)ds_shift(next_row, next_unit);
+            const float row_lse = next_lse, row_delta = next_delta;
+            const float shift = IsBf16<DT>::value ? 0.f : (float)ds_shift(next_row, next_unit, WIDE && g.joint ? finite_square(row_delta) : 0.f);
             fetch();
             if (chunks == 0) continue;
             int n, t;
@@ -589,7 +602,8 @@ int launch_delta(const Place& at, const Geom& g, const Operand& d_o, const Opera
     const int key_tiles = (g.Tk + rows - 1) / rows;
     const long long row_blocks = (long long)g.B * g.N * tiles, blocks = row_blocks + (IsBf16<DT>::value ? 0 : (long long)g.units * key_tiles);
     if (blocks > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
-    if (!IsBf16<DT>::value && cudaMemsetAsync(bounds.unit, 0, (size_t)g.units * 2 * sizeof(float), at.st) != cudaSuccess) return NA2D_ERR_CUDA;
+    // (bounds.delta, where it is one, follows unit)
+    if (!IsBf16<DT>::value && cudaMemsetAsync(bounds.unit, 0, (size_t)g.units * (g.joint ? 3 : 2) * sizeof(float), at.st) != cudaSuccess) return NA2D_ERR_CUDA;
     auto kern = lanes == 4 ? attn_delta_kernel<DT, 4> : lanes == 8 ? attn_delta_kernel<DT, 8> : attn_delta_kernel<DT, 16>;
     *at.launched += 1;
     return na2d_launch::launch(false, kern, (unsigned)blocks, 256, 0, at.st, (const DT*)d_o.ptr, d_o, (const DT*)o.ptr, o, delta, g, Div(tiles),

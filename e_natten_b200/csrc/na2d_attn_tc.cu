@@ -91,7 +91,7 @@ size_t line_rows(const Geom& g, int sms) { return (size_t)(line_groups(g, sms) +
 size_t all_rows(const Geom& g) { return (size_t)g.B * g.N * g.Tq; }
 size_t key_part(const Geom& g) { return (size_t)g.units * g.Tk * g.C; }
 size_t row_part(const Geom& g, int line) { return (size_t)line * 2 * kRows * g.C; }             // 2 a CTA
-size_t bound_units(const Geom& g) { return ((size_t)g.units * 2 + 3) / 4 * 4; }                 // floats, in whole 16 bytes
+size_t bound_units(const Geom& g) { return ((size_t)g.units * (g.joint ? 3 : 2) + 3) / 4 * 4; } // floats, in whole 16 bytes
 size_t bound_floats(const Geom& g) { return bound_units(g) + (all_rows(g) + 3) / 4 * 4; }
 size_t line_part(const Geom& g, int line) { return (size_t)line * 2 * 2 * kRows * g.C; }        // of dK and dV, 2 a CTA
 
@@ -156,6 +156,7 @@ int NA2D_TC_NAME(backward)(const Place& at, const Scratch& given, const Backward
             bounds.unit = own.at;
         }
         bounds.row = bounds.unit + bound_units(g);
+        if (g.joint) bounds.delta = bounds.unit + (size_t)g.units * 2;
     }
     int rc = launch_delta<NA2D_TC_TYPE>(at, g, x.d_o, x.o, x.v, x.delta, bounds);
     if (rc != NA2D_OK) return rc;

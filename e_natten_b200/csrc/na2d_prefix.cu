@@ -191,6 +191,7 @@ int make_problem(const na2d_prefix_attention_args* a, Problem* p) {
         g.B = B; g.N = a->N; g.Nk = a->Nk; g.Tq = Tq; g.Tk = Tk; g.C = a->C;
         g.causal = causal;
         g.lengths = lengths;
+        g.joint = a->Tk > 0;
         g.scale = a->scale;
         g.sl2 = a->scale * 1.4426950408889634f;
         na2d_attn::cut_rows(g);

@@ -1,0 +1,76 @@
+"""prefix_attention, beam_select and beam_reorder where one half, one cache or one candidate is quite unlike the others, and calls that
+something looks into."""
+import math
+
+import pytest
+import torch
+
+import e_natten_b200 as na
+from test_gpu_answers import operands
+from test_gpu_block import BF16, DEV, F16, rand
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- attention over a prefix: halves whose values differ in size --------------------------------------------------
+def gradients_and_bounds(q, pk, pv, k, v, d_o, scale):
+    """The gradients of q, pk, pv, k, v in 64 bits, all keys seen, and how far the kernels' may be off, element by element.
+
+    u, half a step of the operands' type, for each rounding: of the weights in the forward's product and of o, both of which reach dS through
+    delta = dO . o; of the weights in dV's product; of each result, with half a step of fp16's smallest numbers.  32 bits hold all else:
+    products of up to 128 channels within 2^-17 of their terms' sizes, weights within 2^-16 of themselves (exponents of up to 32 in
+    32 bits, and lse), sums of up to 512 terms within 2^-15 of the terms' sizes.  dS goes into its products as two numbers of 16 bits, u^2 of
+    itself, in fp16 on a grid of 2^-37 of the largest |dO| |V| that it may have."""
+    u, tiny = torch.finfo(q.dtype).eps / 2, 2.0 ** -25 if q.dtype == F16 else 0.0
+    S, A, G = len(pk), len(q) // len(pk), q.shape[1] // pk.shape[1]
+    P = pk.shape[2]
+    q, pk, pv, k, v, g = (t.double() for t in (q, pk, pv, k, v, d_o))
+    kk = torch.cat((pk.repeat_interleave(A, 0), k), 2).repeat_interleave(G, 1)
+    vv = torch.cat((pv.repeat_interleave(A, 0), v), 2).repeat_interleave(G, 1)
+    p = torch.softmax(q @ kk.mT * scale, -1)
+    dp = g @ vv.mT
+    o, delta = p @ vv, (p * dp).sum(-1, keepdim=True)
+    ds = p * (dp - delta) * scale
+    of_o = u * (p @ vv.abs()) + u * o.abs() + tiny
+    of_delta = (g.abs() * of_o).sum(-1, keepdim=True) + 2.0 ** -17 * (g * o).abs().sum(-1, keepdim=True)
+    grid = 2.0 ** -37 * (g.norm(dim=-1).amax() * vv.norm(dim=-1).amax()) if tiny else 0.0
+    of_ds = (p * (of_delta + 2.0 ** -17 * (g.abs() @ vv.abs().mT)) + (2.0 ** -16 + 2 * u * u) * p * (dp - delta).abs() + grid) * scale
+    of_p = u * p + (2.0 ** -31 if tiny else 0.0)
+
+    def keys(t):                                         # (B, heads, keys, C) -> prefix's, own
+        t = t.unflatten(1, (-1, G)).sum(2)
+        return t[:, :, :P].unflatten(0, (S, A)).sum(1), t[:, :, P:]
+    sums = 2.0 ** -15
+    dq, dq_off = ds @ kk, of_ds @ kk.abs() + sums * (ds.abs() @ kk.abs())
+    dk, dk_off = keys(ds.mT @ q), keys(of_ds.mT @ q.abs() + sums * (ds.abs().mT @ q.abs()))
+    dv, dv_off = keys(p.mT @ g), keys(of_p.mT @ g.abs() + sums * (p.mT @ g.abs()))
+    want = (dq, dk[0], dv[0], dk[1], dv[1])
+    return want, [off + u * t.abs() + tiny for off, t in zip((dq_off, dk_off[0], dv_off[0], dk_off[1], dv_off[1]), want)]
+
+
+@pytest.mark.parametrize("Tq", [1, 40])
+@pytest.mark.parametrize("of_prefix,of_own,of_do", [(2.0 ** -12, 1.0, 1.0), (1.0, 2.0 ** -12, 1.0), (0.0, 1.0, 1.0), (1.0, 0.0, 1.0), (0.0, 1.0, 2.0 ** -12),
+                                                    (1.0, 0.0, 2.0 ** -12), (2.0 ** 12, 1.0, 2.0 ** -8), (1.0, 2.0 ** 12, 2.0 ** -8), (2.0 ** -12, 2.0 ** 8, 2.0 ** -6),
+                                                    (0.0, 0.0, 1.0)])
+@pytest.mark.parametrize("scale", [0.125, 0.5], ids=["even", "peaked"])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+def test_prefix_attention_gradients_of_halves_of_any_size(dtype, scale, of_prefix, of_own, of_do, Tq):
+    """Values of the prompt far above, far below, and beside the answers' own, none of them (0) too: delta = dO . o holds both.  Values of a
+    half, and dO, point the same way, so that dP and delta are as large as their norms allow; queries are large and keys small, so that dS
+    of small values still count."""
+    S, A, N, Nk, P, Tk, C = 2, 3, 4, 2, 70, 40, 64
+    q, pk, pv, k, v, d_o = operands(S, A, N, Nk, P, Tq, Tk, C, dtype)
+    way = rand(2, 1, Nk, 1, C, seed=11)
+    large = 2.0 ** 8 if of_do < 1.0 and of_prefix * of_own == 0 else 1.0
+    q, pk, k = (q.float() * large).to(dtype), (pk.float() / large).to(dtype), (k.float() / large).to(dtype)
+    pv, v = ((way[i] + 0.1 * t.float()).mul(by).to(dtype) for i, t, by in ((0, pv, of_prefix), (1, v, of_own)))
+    d_o = (way.sum(0).repeat_interleave(N // Nk, 1) + 0.1 * d_o.float()).mul(of_do).to(dtype)
+    leaves = [t.requires_grad_() for t in (q, pk, pv, k, v)]
+    got = torch.autograd.grad(na.prefix_attention(*leaves, scale), leaves, d_o)
+    na.check_kernels(DEV)
+    want, off = gradients_and_bounds(*(t.detach() for t in leaves), d_o, scale)
+    for name, a, ref, most in zip(("dq", "dpk", "dpv", "dk", "dv"), got, want, off):
+        assert torch.isfinite(a).all(), name
+        assert ref.abs().max() < 60000, "the test's own values fit"
+        far = ((a.double() - ref).abs() / most.clamp_min(1e-300)).max()
+        assert far <= 1, f"{name}: {far:.3g} times as far off as roundings account for"
