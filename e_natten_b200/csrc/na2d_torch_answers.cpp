@@ -464,8 +464,16 @@ void reorder(const std::vector<Tensor>& caches, const Tensor& parents, const May
         through = through || goes_through({t});
     }
     if (!through) return reorder_in_place(caches, parents, lengths);
-    at::AutoDispatchBelowADInplaceOrView below;
-    for (Tensor t : caches) t.copy_(operator_of<Reordered>("e_natten_b200::beam_reordered").call(t, parents, lengths));
+    auto below = [](auto&& f) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        return f();
+    };
+    for (Tensor t : caches) {
+        const Tensor moved = below([&] { return operator_of<Reordered>("e_natten_b200::beam_reordered").call(t, parents, lengths); });
+        // (not below: autograd counts the cache's version there; an inference tensor has none)
+        if (t.is_inference()) below([&] { return t.copy_(moved); });
+        else t.copy_(moved);
+    }
 }
 // The operator: a cache of its own.  (Whoever records calls follows what copy_ changes; an operator without a result is dropped from a trace.)
 Tensor reordered_op(const Tensor& cache, const Tensor& parents, const MaybeTensor& lengths) {

@@ -4,9 +4,10 @@ import math
 
 import pytest
 import torch
+import torch.utils._python_dispatch
 
 import e_natten_b200 as na
-from test_gpu_answers import operands
+from test_gpu_answers import operands, parents_of, plain_reorder
 from test_gpu_block import BF16, DEV, F16, rand
 
 pytestmark = pytest.mark.gpu
@@ -74,3 +75,31 @@ def test_prefix_attention_gradients_of_halves_of_any_size(dtype, scale, of_prefi
         assert ref.abs().max() < 60000, "the test's own values fit"
         far = ((a.double() - ref).abs() / most.clamp_min(1e-300)).max()
         assert far <= 1, f"{name}: {far:.3g} times as far off as roundings account for"
+
+
+# ---- beam search: calls that something looks into --------------------------------------------------------------------
+class Through(torch.utils._python_dispatch.TorchDispatchMode):
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+def a_cache(seed=0, B=2, K=4):
+    return rand(B * K, 2, 30, 16, seed=seed), parents_of(B, K, seed)
+
+
+def test_beam_reorder_under_a_dispatch_mode_tells_autograd():
+    """What was recorded before is not differentiated with the values of after."""
+    cache, parents = a_cache()
+    want, version = plain_reorder(cache, parents), cache._version
+    w = rand(16).requires_grad_()
+    y = (cache * w).sum()
+    with Through():
+        na.beam_reorder(cache, parents)
+    assert torch.equal(cache, want) and cache._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        mine = cache.clone()
+    with Through():
+        na.beam_reorder(mine, parents)                   # (no version to count)
+    assert torch.equal(mine, plain_reorder(cache, parents))
