@@ -44,14 +44,14 @@ inline void check(int status) {
     pybind11::module_::import("e_natten_b200._lib").attr("check")(status);
 }
 
-// Whether anything looks into the calls of this thread: a functional transform, forward-mode gradients, a trace, a function or dispatch
-// mode.
-inline bool looked_into() {
+// Whether anything records or rewrites the calls of this thread: a functional transform, forward-mode gradients, a trace, a dispatch mode.
+inline bool recorded() {
     const auto tls = c10::impl::tls_local_dispatch_key_set();
     return tls.included_.has(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) || tls.included_.has(c10::DispatchKey::Functionalize) ||
-           tls.included_.has(c10::DispatchKey::Python) || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
-           at::impl::torch_function_mode_enabled() || torch::jit::tracer::isTracing();
+           tls.included_.has(c10::DispatchKey::Python) || c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing();
 }
+// Whether anything looks into them: that, or a function mode (a default device is one).
+inline bool looked_into() { return recorded() || at::impl::torch_function_mode_enabled(); }
 // Whether t is a tensor whose memory is all there is to it.
 inline bool ordinary(const Tensor& t) {
     return t.is_cuda() && t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.is_neg() && !t.is_conj() &&

@@ -457,11 +457,12 @@ void reorder_in_place(at::TensorList caches, const Tensor& parents_in, const May
 }
 void reorder(const std::vector<Tensor>& caches, const Tensor& parents, const MaybeTensor& lengths) {
     TORCH_CHECK_VALUE(parents.is_cuda(), "parents: e_natten_b200 runs on CUDA tensors only (there is no CPU path)");
-    bool through = goes_through({parents, lengths.value_or(Tensor())});
+    // (a function mode sees no calls of the dispatcher, and the operator, a cache of its own and a copy back, costs several times as much)
+    bool through = recorded() || any_special({parents, lengths.value_or(Tensor())});
     for (const Tensor& t : caches) {
         TORCH_CHECK_VALUE(t.is_cuda(), "caches must be on parents' device");
         TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !t.requires_grad(), "beam_reorder has no gradient");
-        through = through || goes_through({t});
+        through = through || any_special({t});
     }
     if (!through) return reorder_in_place(caches, parents, lengths);
     auto below = [](auto&& f) {

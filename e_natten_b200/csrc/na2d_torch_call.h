@@ -52,13 +52,13 @@ inline Tensor scratch(size_t bytes, const Tensor& like) {
 }
 
 // ---- operators of the dispatcher ------------------------------------------------------------------------------------
-// Whether a call on these tensors goes through the dispatcher.
-inline bool goes_through(std::initializer_list<Tensor> tensors) {
-    if (looked_into()) return true;
+// Whether any of them is more than its memory; whether a call on these tensors goes through the dispatcher.
+inline bool any_special(std::initializer_list<Tensor> tensors) {
     for (const Tensor& t : tensors)
         if (t.defined() && !ordinary(t) && !t.is_neg() && !t._is_zerotensor()) return true;      // (those two are refused)
     return false;
 }
+inline bool goes_through(std::initializer_list<Tensor> tensors) { return looked_into() || any_special(tensors); }
 // The operator of that name, on arguments of F.
 template <typename F>
 c10::TypedOperatorHandle<F> operator_of(const char* name) {

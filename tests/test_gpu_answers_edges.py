@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.overrides
 import torch.utils._python_dispatch
 
 import e_natten_b200 as na
@@ -103,3 +104,18 @@ def test_beam_reorder_under_a_dispatch_mode_tells_autograd():
     with Through():
         na.beam_reorder(mine, parents)                   # (no version to count)
     assert torch.equal(mine, plain_reorder(cache, parents))
+
+
+@pytest.mark.parametrize("mode", [lambda: torch.device("cuda"), torch.overrides.TorchFunctionMode])
+def test_beam_reorder_under_a_function_mode_is_in_place(mode):
+    """No second copy of a cache, as without one."""
+    cache = torch.randn(8, 4, 512, 256, device=DEV)
+    parents = parents_of(2, 4, 5)
+    want, version = plain_reorder(cache, parents), cache._version
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.max_memory_allocated()
+    with mode():
+        na.beam_reorder(cache, parents)
+    assert torch.cuda.max_memory_allocated() - before < cache.nbytes // 4
+    assert torch.equal(cache, want) and cache._version > version
