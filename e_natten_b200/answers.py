@@ -61,7 +61,7 @@ def beam_select(logits, scores, count: Optional[int] = None, finished=None, end:
     Exponentials are float32, so that worths of different beams that are nearer to one another than ``2 ** -22`` may come in either
     order; equal rows of logits have equal worths.
 
-    Up to 32 beams, 64 candidates and 2^24 words.  Not differentiable.
+    Up to 32 beams, 64 candidates and 2^24 words.  Not differentiable: what has a tangent is refused.
     """
     return torch_ext.beam_select(logits, scores, scores.shape[-1] if count is None else count, finished, end)
 
@@ -79,6 +79,6 @@ def beam_reorder(caches: Union[torch.Tensor, Sequence[torch.Tensor]], parents: t
     parent's, and what is stored behind those stays as it was.  (Lengths themselves do not move: ``lengths.view(B, K).gather(1,
     parents)`` are the new ones.)
 
-    Several caches move one after the other in effect: one that is given twice moves twice.  Up to 32 beams.  Not differentiable.
+    Several caches move one after the other in effect: one that is given twice moves twice.  Up to 32 beams.  Not differentiable: what has a tangent is refused.
     """
     torch_ext.beam_reorder([caches] if isinstance(caches, torch.Tensor) else list(caches), parents, lengths)

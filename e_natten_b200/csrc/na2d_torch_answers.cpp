@@ -299,6 +299,10 @@ std::tuple<Tensor, Tensor> prefix_attention(const Tensor& q_in, const Tensor& pk
 }
 
 // ---- beam search ------------------------------------------------------------------------------------------------------------
+// (a tangent would stay behind, or be dropped, without a word)
+void check_no_gradient(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined(), name, " has no gradient");
+}
 std::tuple<Tensor, Tensor, Tensor> select_op(const Tensor& logits_in, const Tensor& scores_in, int64_t count, const MaybeTensor& finished_in, int64_t end) {
     check_map(logits_in, "logits");
     TORCH_CHECK_VALUE(logits_in.dim() == 3 && logits_in.size(1) > 0 && logits_in.size(2) > 0, "logits must be (B, beams, words); got ", logits_in.sizes());
@@ -349,7 +353,8 @@ std::tuple<Tensor, Tensor, Tensor> select_op(const Tensor& logits_in, const Tens
 }
 std::tuple<Tensor, Tensor, Tensor> select(const Tensor& logits, const Tensor& scores, int64_t count, const MaybeTensor& finished, int64_t end) {
     check_map(logits, "logits");
-    TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(logits.requires_grad() || scores.requires_grad()), "beam_select has no gradient");
+    check_no_gradient(logits, "beam_select");
+    check_no_gradient(scores, "beam_select");
     if (goes_through({logits, scores, finished.value_or(Tensor())})) {
         at::AutoDispatchBelowADInplaceOrView below;
         return operator_of<Select>("e_natten_b200::beam_select").call(logits, scores, count, finished, end);
@@ -461,7 +466,7 @@ void reorder(const std::vector<Tensor>& caches, const Tensor& parents, const May
     bool through = recorded() || any_special({parents, lengths.value_or(Tensor())});
     for (const Tensor& t : caches) {
         TORCH_CHECK_VALUE(t.is_cuda(), "caches must be on parents' device");
-        TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !t.requires_grad(), "beam_reorder has no gradient");
+        check_no_gradient(t, "beam_reorder");
         through = through || any_special({t});
     }
     if (!through) return reorder_in_place(caches, parents, lengths);

@@ -8,7 +8,7 @@ import torch.overrides
 import torch.utils._python_dispatch
 
 import e_natten_b200 as na
-from test_gpu_answers import operands, parents_of, plain_reorder
+from test_gpu_answers import beams, operands, parents_of, plain_reorder
 from test_gpu_block import BF16, DEV, F16, rand
 
 pytestmark = pytest.mark.gpu
@@ -119,3 +119,16 @@ def test_beam_reorder_under_a_function_mode_is_in_place(mode):
         na.beam_reorder(cache, parents)
     assert torch.cuda.max_memory_allocated() - before < cache.nbytes // 4
     assert torch.equal(cache, want) and cache._version > version
+
+
+def test_beam_operators_refuse_tensors_with_tangents():
+    cache, parents = a_cache()
+    logits, scores = beams(2, 4, 50, torch.float32)
+    was = cache.clone()
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: na.beam_reorder(dual(cache), parents), lambda: na.beam_reorder([cache, dual(cache)], parents),
+                     lambda: na.beam_select(dual(logits), scores), lambda: na.beam_select(logits, dual(scores))):
+            with pytest.raises(ValueError, match="no gradient"):
+                call()
+    assert torch.equal(cache, was)
