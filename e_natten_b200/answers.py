@@ -79,6 +79,7 @@ def beam_reorder(caches: Union[torch.Tensor, Sequence[torch.Tensor]], parents: t
     parent's, and what is stored behind those stays as it was.  (Lengths themselves do not move: ``lengths.view(B, K).gather(1,
     parents)`` are the new ones.)
 
-    Several caches move one after the other in effect: one that is given twice moves twice.  Up to 32 beams.  Not differentiable: what has a tangent is refused.
+    Several caches move one after the other in effect: one that is given twice moves twice.  All are checked
+    before one moves.  Up to 32 beams.  Not differentiable: what has a tangent is refused.
     """
     torch_ext.beam_reorder([caches] if isinstance(caches, torch.Tensor) else list(caches), parents, lengths)

@@ -362,10 +362,9 @@ std::tuple<Tensor, Tensor, Tensor> select(const Tensor& logits, const Tensor& sc
     return select_op(logits, scores, count, finished, end);
 }
 
-// A cache of `entries` entries as rows; false where its rows cannot be told apart.
+// A cache of `entries` entries as rows, but for where it is; false where its rows cannot be told apart.
 bool rows_of_cache(const Tensor& t, int64_t entries, na2d_cache* c) {
     const int64_t esize = t.element_size();
-    c->ptr = t.data_ptr();
     if (t.dim() == 4 && (t.stride(3) == 1 || t.size(3) == 1)) {
         // strides that nest: sorted, each is at least what lies within it
         std::vector<std::pair<int64_t, int64_t>> dims;
@@ -393,27 +392,25 @@ bool rows_of_cache(const Tensor& t, int64_t entries, na2d_cache* c) {
     return true;
 }
 
-void reorder_in_place(at::TensorList caches, const Tensor& parents_in, const MaybeTensor& lengths_in) {
+// All that a call is refused for but what the library refuses; the rows of the caches that have any, without their places.
+std::vector<na2d_cache> check_reorder(at::TensorList caches, const Tensor& parents_in, const MaybeTensor& lengths_in) {
     TORCH_CHECK_VALUE(parents_in.is_cuda() && parents_in.layout() == at::kStrided, "parents: e_natten_b200 runs on CUDA tensors only (there is no CPU path)");
     TORCH_CHECK_VALUE(parents_in.dim() == 2 && parents_in.size(1) > 0 && is_whole(parents_in), "parents must be an int32 or int64 tensor of (B, beams)");
     check_plain(parents_in, "parents");
     const int64_t B = parents_in.size(0), K = parents_in.size(1), entries = B * K;
-    const Tensor parents = parents_in.contiguous();
-    Tensor lengths;
     if (lengths_in) {
-        TORCH_CHECK_VALUE(lengths_in->numel() == entries && is_whole(*lengths_in) && lengths_in->device() == parents.device() && lengths_in->dim() > 0 &&
+        TORCH_CHECK_VALUE(lengths_in->numel() == entries && is_whole(*lengths_in) && lengths_in->device() == parents_in.device() && lengths_in->dim() > 0 &&
                               lengths_in->dim() < 3,
                           "lengths must be an int32 or int64 tensor with a length for each of ", entries, " entries, on parents' device");
         check_plain(*lengths_in, "lengths");
-        lengths = lengths_in->contiguous();
     }
     std::vector<na2d_cache> rows;
     for (const Tensor& t : caches) {
-        TORCH_CHECK_VALUE(t.is_cuda() && t.layout() == at::kStrided && t.device() == parents.device(), "caches must be on parents' device");
+        TORCH_CHECK_VALUE(t.is_cuda() && t.layout() == at::kStrided && t.device() == parents_in.device(), "caches must be on parents' device");
         check_plain(t, "caches");
         TORCH_CHECK_VALUE(!t.is_conj(), "caches: a lazily conjugated tensor is not supported");
         TORCH_CHECK_VALUE(t.dim() > 0 && t.size(0) == entries, "caches must have an entry for each of ", B, " x ", K, " beams; got ", t.sizes());
-        TORCH_CHECK_VALUE(!lengths.defined() || t.dim() == 4, "with lengths, caches must be (entries, heads, tokens, channels); got ", t.sizes());
+        TORCH_CHECK_VALUE(!lengths_in || t.dim() == 4, "with lengths, caches must be (entries, heads, tokens, channels); got ", t.sizes());
         if (t.numel() == 0) continue;
         na2d_cache c;
         std::memset(&c, 0, sizeof(c));
@@ -421,6 +418,15 @@ void reorder_in_place(at::TensorList caches, const Tensor& parents_in, const May
                           "and no element twice; got sizes ", t.sizes(), " and strides ", t.strides());
         rows.push_back(c);
     }
+    return rows;
+}
+void reorder_in_place(at::TensorList caches, const Tensor& parents_in, const MaybeTensor& lengths_in) {
+    std::vector<na2d_cache> rows = check_reorder(caches, parents_in, lengths_in);
+    const int64_t B = parents_in.size(0), K = parents_in.size(1), entries = B * K;
+    const Tensor parents = parents_in.contiguous(), lengths = lengths_in ? lengths_in->contiguous() : Tensor();
+    auto next = rows.begin();
+    for (const Tensor& t : caches)
+        if (t.numel()) (next++)->ptr = t.data_ptr();
     for (const Tensor& t : caches)
         if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     if (rows.empty()) return;
@@ -470,6 +476,7 @@ void reorder(const std::vector<Tensor>& caches, const Tensor& parents, const May
         through = through || any_special({t});
     }
     if (!through) return reorder_in_place(caches, parents, lengths);
+    check_reorder(caches, parents, lengths);             // all of them, before the first one moves
     auto below = [](auto&& f) {
         at::AutoDispatchBelowADInplaceOrView guard;
         return f();

@@ -1,5 +1,6 @@
 """prefix_attention, beam_select and beam_reorder where one half, one cache or one candidate is quite unlike the others, and calls that
 something looks into."""
+import contextlib
 import math
 
 import pytest
@@ -132,3 +133,17 @@ def test_beam_operators_refuse_tensors_with_tangents():
             with pytest.raises(ValueError, match="no gradient"):
                 call()
     assert torch.equal(cache, was)
+
+
+@pytest.mark.parametrize("mode", [Through, contextlib.nullcontext])
+def test_beam_reorder_checks_every_cache_before_it_moves_one(mode):
+    good, parents = a_cache()
+    was = good.clone()
+    for bad in (good[:7].clone(), good[:1].clone().expand(8, 2, 30, 16), good.clone().transpose(2, 3), good.cpu(), torch._neg_view(good.clone())):
+        with mode(), pytest.raises(ValueError):
+            na.beam_reorder([good, bad], parents)
+    with mode(), pytest.raises(ValueError):
+        na.beam_reorder([good, good.flatten(2)], parents, torch.zeros(8, dtype=torch.int32, device=DEV))
+    with mode(), pytest.raises(ValueError):
+        na.beam_reorder([good, good.clone().requires_grad_()], parents)
+    assert torch.equal(good, was)
