@@ -450,7 +450,7 @@ size_t na2d_beam_select_workspace(const na2d_beam_select_args* a);
  *   parents      (B, K), dense, int32 or (parents_64) int64.  One outside [0, K) leaves its entry as it is.
  *   lengths      (B K,), dense, int32 or (lengths_64) int64, or NULL: how many tokens an entry holds (clamped to [0, tokens]).  Only the
  *                parent's are copied; rows behind them stay as they are.
- *   K <= 32 (NA2D_ERR_UNSUPPORTED); B * K <= 2^24, 2^30 pieces of 16 bytes (of 4, or 1, where rows or strides are not multiples of them)
+ *   K <= 32 (NA2D_ERR_UNSUPPORTED); B * K <= 2^24, 2^30 pieces of 16 bytes (of 4, or 1, where its rows or strides are not multiples of them)
  *   a beam in one cache (NA2D_ERR_TOO_LARGE). */
 typedef struct na2d_cache {
     void* ptr;

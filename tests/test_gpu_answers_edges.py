@@ -9,7 +9,7 @@ import torch.overrides
 import torch.utils._python_dispatch
 
 import e_natten_b200 as na
-from test_gpu_answers import beams, operands, parents_of, plain_reorder
+from test_gpu_answers import beams, bits, operands, parents_of, plain_reorder
 from test_gpu_block import BF16, DEV, F16, rand
 
 pytestmark = pytest.mark.gpu
@@ -147,3 +147,18 @@ def test_beam_reorder_checks_every_cache_before_it_moves_one(mode):
     with mode(), pytest.raises(ValueError):
         na.beam_reorder([good, good.clone().requires_grad_()], parents)
     assert torch.equal(good, was)
+
+
+def test_beam_reorder_of_caches_of_unlike_rows():
+    """Rows of 16 bytes' multiples, of 4's and of single bytes in one list, each in pieces of its own; more of one kind than a launch takes."""
+    B, K, T = 2, 4, 70
+    parents = parents_of(B, K, 9)
+    lengths = (torch.arange(B * K, device=DEV) * 11).int()
+    like = lambda: [bits(B * K, 2, T, 64, dtype=torch.int16, seed=1), bits(B * K, 1, T, 13, dtype=torch.int32, seed=2), bits(B * K, 3, T, 5, seed=3),
+                    bits(B * K, 1, T, 1, dtype=torch.bool, seed=4), bits(B * K, T, 2, 8, dtype=torch.int64, seed=5).transpose(1, 2),
+                    *(bits(B * K, 1, T, 3 + i % 2, dtype=torch.int32, seed=6 + i) for i in range(150))]
+    for n in (None, lengths):
+        caches = like()
+        want = [plain_reorder(c, parents, n) for c in caches]
+        na.beam_reorder(caches, parents, n)
+        assert all(torch.equal(a, b) for a, b in zip(caches, want))
