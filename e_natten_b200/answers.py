@@ -58,8 +58,9 @@ def beam_select(logits, scores, count: Optional[int] = None, finished=None, end:
     is not finite has none (scores of ``-inf`` for all beams but one start a search from one prompt), nor has a beam with a
     logit of NaN or ``+inf``.  Places that are left over have score ``-inf``, parent 0 and word 0.
 
-    Exponentials are float32, so that worths of different beams that are nearer to one another than ``2 ** -22`` may come in either
-    order; equal rows of logits have equal worths.
+    Exponentials are float32: a worth is off by less than ``2 ** -16`` (by up to ``2 ** -20`` in rows that were made to be hard), so
+    that those of different beams that are nearer to one another than ``2 ** -15`` may come in either order; equal rows of logits have
+    equal worths.
 
     Up to 32 beams, 64 candidates and 2^24 words.  Not differentiable: what has a tangent is refused.
     """

@@ -424,8 +424,9 @@ size_t na2d_prefix_attention_workspace(const na2d_prefix_attention_args* a, int 
  *   out_scores fp32, out_parents, out_words (B, count): worth, beam and word.  Places that are left over have -infinity, 0 and 0.
  *   workspace    scratch, 16-byte aligned, at least na2d_beam_select_workspace bytes.
  *   K <= 32, count <= 64 (NA2D_ERR_UNSUPPORTED); V <= 2^24, B * K <= 2^20 (NA2D_ERR_TOO_LARGE); 0 <= end < V.
- * Exponentials are in 32 bits, their sums' joins and the worths in 64: worths of different beams within 2^-22 of one another may come in
- * either order; equal rows have equal worths. */
+ * Exponentials and a block's sums are in 32 bits, their joins and the worths in 64: a worth is off by less than 2^-16 (by up to 2^-20 in rows
+ * that were made to be hard), so that those of different beams within 2^-15 of one another may come in either order; equal rows have equal
+ * worths. */
 typedef struct na2d_beam_select_args {
     size_t struct_size;
     int B, K, V, count, dtype, device;

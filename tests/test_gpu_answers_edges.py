@@ -162,3 +162,59 @@ def test_beam_reorder_of_caches_of_unlike_rows():
         want = [plain_reorder(c, parents, n) for c in caches]
         na.beam_reorder(caches, parents, n)
         assert all(torch.equal(a, b) for a, b in zip(caches, want))
+
+
+# ---- beam search: how far off a worth may be ---------------------------------------------------------------------------
+def most_off(logits):
+    """How far the logarithm of each row's sum may be off.  An exponent, a difference of 32 bits times 1 / ln 2 in 32 bits, is off by (2^-24 +
+    2^-24 + 2^-26) of itself: that, by the words' weights; an exponential by 2^-22 of itself, and a sum is multiplied by one for each chunk of a
+    block, up to 16, and once more; 52 roundings of 2^-24 (8 sums in a chunk, 16 chunks, their 15 factors, 13 to join a block's threads).  Blocks
+    are joined in 64 bits."""
+    x = logits.double()
+    distance = (torch.softmax(x, -1) * (x.amax(-1, keepdim=True) - x)).sum(-1)
+    return 2.25 * 2.0 ** -24 * distance + 17 * 2.0 ** -22 + 52 * 2.0 ** -24
+
+
+def rows_of_sums(V):
+    """Rows whose sums are hard: a peak before equal words far below it, words that climb from chunk to chunk, equal words."""
+    tails = [0.1, 1.7, 5.3, 8.9, 10.2, 11.37, 12.7, 13.1, 14.9, 15.9, 17.3, 20.1]
+    x = torch.zeros(len(tails) + 4, V, device=DEV)
+    for row, tail in zip(x, tails):
+        row[1:] = -tail
+        row[0] = 0.37
+    line = torch.arange(V, device=DEV, dtype=torch.float64) / V
+    x[-4], x[-3], x[-2], x[-1] = 1e-3 * line, 7.3 * line, 30 * line, -0.123
+    return x
+
+
+@pytest.mark.parametrize("V", [1000, 50257, 1 << 18, 1 << 22])
+def test_beam_select_worths_of_uneven_rows(V):
+    x = rows_of_sums(V)
+    for dtype in (torch.float32, BF16):
+        logits = x.to(dtype)
+        want = logits.double().amax(-1) - logits.double().logsumexp(-1)
+        got = na.beam_select(logits[:, None], torch.zeros(len(x), 1, device=DEV))[0][:, 0]
+        off = (got.double() - want).abs()
+        most = most_off(logits)
+        assert most.max() < 2.0 ** -16.5                 # what the documents say, and the score's own rounding
+        assert (off <= most + 2.0 ** -24 * want.abs()).all()
+
+
+def test_beam_select_orders_worths_that_are_far_enough_apart():
+    """Beams of one peak each before tails of their own, in the order that 64 bits give where worths are 2^-15 apart."""
+    V, apart = 1 << 18, 2.0 ** -15
+    x = rows_of_sums(V)
+    ends = x.double().amax(-1) - x.double().logsumexp(-1)
+    order = torch.randperm(len(x), generator=torch.Generator().manual_seed(3)).to(DEV)
+    worths = -1.0 - apart * 1.001 * order.double()       # of each beam's best
+    scores = (worths - ends).float()
+    have = scores.double() + ends                        # (scores are rounded to 32 bits)
+    best = torch.argsort(have, descending=True)
+    assert (have[best][:-1] - have[best][1:] > apart * 0.9).all()
+    parents = na.beam_select(x[None, :-4], scores[None, :-4], 1)[1]
+    kept = best[best < len(x) - 4]
+    assert parents[0, 0] == kept[0]
+    for _ in range(len(kept) - 1):                       # the best beam of those left, one after the other
+        scores[kept[0]] = -math.inf
+        kept = kept[1:]
+        assert na.beam_select(x[None, :-4], scores[None, :-4], 1)[1][0, 0] == kept[0]
