@@ -203,9 +203,14 @@ struct SimtWork {
 struct SimtPair {
     SimtWork at[2];
 };
-// The problem of this block, its block of a part, and which part.
-template <bool WIDE>
+// The problem of this block, its block of a part, and which part.  ONE: there is no second problem.
+template <bool WIDE, bool ONE = false>
 __device__ __forceinline__ const SimtWork& work_of(const SimtPair& p, unsigned& block, int& split) {
+    if constexpr (ONE) {
+        block = blockIdx.x;
+        split = 0;
+        return p.at[0];
+    }
     const bool second = blockIdx.x >= p.at[0].blocks;
     block = blockIdx.x - (second ? p.at[0].blocks : 0u);
     split = 0;
@@ -318,8 +323,10 @@ __global__ void __launch_bounds__(kThreads) simt_delta_kernel(const __grid_const
 }
 
 // ---- query half of the backward -----------------------------------------------------------------------------------------
+// Head dims above 128: 128 registers, with which an SM has two blocks.  2 x 8 heads x 1024 x 256, fp32: 953 us; 136 registers, one block, 1068.
+// (0: as many as the compiler takes.)
 template <typename DT, bool WIDE, int CP, int BM>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, CP > 128 ? 2 : 0)
 simt_dq_kernel(const __grid_constant__ SimtPair pair) {
     using S = SimtCfg<CP, BM>;
     using OT = std::conditional_t<WIDE, float, DT>;
@@ -383,6 +390,10 @@ simt_dq_kernel(const __grid_constant__ SimtPair pair) {
 }
 
 // ---- key half: a block has BT keys of one key head and walks the queries of every head that shares it ------------------------
+// Head dims above 128: calls of one problem that is not taken in parts have instances without the choice between two, whose operands then
+// stay in constant memory.  2 x 8 heads x 1024 x 256, fp32: 1422 us for 1510, fp16 causal 1032 for 1091.  (Below it is the other way round: 128
+// channels 1063 us for 1028.  Forward and query half are faster with the choice throughout.)
+template <int CP, bool WIDE> constexpr bool kOneProblem = CP > 128 && !WIDE;
 template <typename DT, bool WIDE, int CP>
 __global__ void __launch_bounds__(kThreads)
 simt_dkdv_kernel(const __grid_constant__ SimtPair pair) {
@@ -390,7 +401,7 @@ simt_dkdv_kernel(const __grid_constant__ SimtPair pair) {
     using S = SimtCfg<CP, BM>;
     unsigned block;
     int split;
-    const SimtWork& work = work_of<WIDE>(pair, block, split);
+    const SimtWork& work = work_of<WIDE, kOneProblem<CP, WIDE>>(pair, block, split);
     const Operand q = work.q, k = work.k, v = work.v, d_o = work.d_o, d_k = work.out, d_v = work.out2;
     const float *__restrict__ lse = work.lse, *__restrict__ delta = work.delta;
     const Geom g = work.g;
@@ -626,9 +637,11 @@ int backward_as(const Place& at, const Backward* x, int count) {
             return wide ? queries_as<DT, true, CP, kRowsOf>(at, queries) : queries_as<DT, false, CP, kRowsOf>(at, queries);
         }))
         return rc;
+    if (!keys.at[0].blocks) std::swap(keys.at[0], keys.at[1]);
     for (SimtWork& y : keys.at)
         if (!y.splits) y.splits = 1;                     // (no blocks)
-    if (!parts) return start(at, simt_dkdv_kernel<DT, false, CP>, keys, 4 * S::TILE + S::SCORES, opted[0]);
+    if (!parts && !(kOneProblem<CP, false> && keys.at[1].blocks))
+        return start(at, simt_dkdv_kernel<DT, false, CP>, keys, 4 * S::TILE + S::SCORES, opted[0]);
     if (int rc = start(at, simt_dkdv_kernel<DT, true, CP>, keys, 4 * S::TILE + S::SCORES, opted[1])) return rc;
     for (const SimtWork& y : keys.at) {
         if (y.splits == 1) continue;

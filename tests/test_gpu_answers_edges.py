@@ -9,7 +9,7 @@ import torch.overrides
 import torch.utils._python_dispatch
 
 import e_natten_b200 as na
-from test_gpu_answers import beams, bits, operands, parents_of, plain_reorder
+from test_gpu_answers import beams, bits, check, operands, parents_of, plain_reorder
 from test_gpu_block import BF16, DEV, F16, rand
 
 pytestmark = pytest.mark.gpu
@@ -77,6 +77,26 @@ def test_prefix_attention_gradients_of_halves_of_any_size(dtype, scale, of_prefi
         assert ref.abs().max() < 60000, "the test's own values fit"
         far = ((a.double() - ref).abs() / most.clamp_min(1e-300)).max()
         assert far <= 1, f"{name}: {far:.3g} times as far off as roundings account for"
+
+
+# ---- attention over a prefix: head dims above 128, whose key half has instances of its own --------------------------
+@pytest.mark.parametrize("dtype,C", [(torch.float32, 130), (BF16, 136), (F16, 256)])
+@pytest.mark.parametrize("S,A,N,Nk,P,Tq,Tk", [(2, 3, 4, 2, 66, 20, 21), (1, 8, 4, 1, 40, 100, 100), (2, 2, 2, 2, 130, 40, 0)])       # in the second the prompt's are in parts
+def test_prefix_attention_gradients_of_some_keys_at_wide_heads(S, A, N, Nk, P, Tq, Tk, dtype, C):
+    """Both halves' keys, and either half's alone: two problems of a launch, the first, the second."""
+    *x, d_o = operands(S, A, N, Nk, P, Tq, Tk, C, dtype)
+    _, want = check(*x, d_o, C ** -0.5, True)
+    names = ("q", "pk", "pv", "k", "v")[:5 if Tk else 3]
+    for some in (("pk", "pv"), ("k", "v"), ("q", "v"), ("q", "pk"), ("pv", "k")):
+        some = [n for n in some if n in names]
+        if not some:
+            continue
+        leaves = {n: t.detach().requires_grad_(n in some) for n, t in zip(names, x)}
+        o = na.prefix_attention(*leaves.values(), *((None, None) if not Tk else ()), C ** -0.5, True)
+        got = torch.autograd.grad(o, [leaves[n] for n in some], d_o)
+        for n, g in zip(some, got):
+            assert torch.equal(g, want[names.index(n)]), (some, n)
+    na.check_kernels(DEV)
 
 
 # ---- beam search: calls that something looks into --------------------------------------------------------------------
