@@ -242,7 +242,7 @@ struct Layout {
         return at;
     }
 };
-// Which kind of keys goes on the line of few rows (na2d_prefix_tokens.cuh): its units' rows fit.
+// Which kind of keys goes on the line of few rows (na2d_prefix_tokens.cuh): its units' rows fit.  Where a prefix's do, its entries' own do.
 struct OnLine {
     bool prefix, own;
     bool any() const { return prefix || own; }
@@ -460,7 +460,7 @@ int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a) {
         const Scratch scratch{floats(f.scratch), f.scratch_bytes / 4}, own_scratch{floats(f.own_scratch), f.own_scratch_bytes / 4};
         const OnLine line = on_line(p);
         auto run = [&]() -> int {
-            na2d_attn::Parts prefix{}, own{};
+            na2d_attn::Parts prefix{};
             if (!line.prefix) {
                 Operand q = p.follow[0] ? merged(p, p.q) : merged_copy(p, ws + f.q);
                 if (!p.follow[0]) {
@@ -477,9 +477,7 @@ int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a) {
                     return rc;
             }
             if (p.tensor && p.any_own && !line.own)
-                if (int rc = forward_of(p, at, p.own, own_scratch, p.q, p.k, p.v, sums(p.own, floats(f.o_own)), floats(f.lse_own),
-                                        line.any() ? &own : nullptr))
-                    return rc;
+                if (int rc = forward_of(p, at, p.own, own_scratch, p.q, p.k, p.v, sums(p.own, floats(f.o_own)), floats(f.lse_own))) return rc;
             if (line.any()) {
                 na2d_prefix::Tokens x{};
                 auto side = [&](int which, const Geom& g, const Operand& k, const Operand& v, int share, size_t first_row) {
@@ -504,11 +502,9 @@ int na2d_prefix_attention_forward(const na2d_prefix_attention_args* a) {
                 x.table = reinterpret_cast<int*>(ws + f.table);
                 x.part_o = floats(f.part_o);
                 x.part_lse = floats(f.part_lse);
-                const size_t stride = (size_t)p.rows.all;
-                const na2d_prefix::JoinSide by_prefix{prefix.o, prefix.lse, stride, prefix.count, p.rows.A, na2d_attn::Div(p.rows.A)},
-                    by_own{own.o, own.lse, stride, own.count, 1, na2d_attn::Div(1)};
-                return p.dtype == NA2D_BF16 ? na2d_prefix::tokens_bf16(at, x, by_prefix, by_own, a->o.ptr, a->lse, p.B)
-                                            : na2d_prefix::tokens_f16(at, x, by_prefix, by_own, a->o.ptr, a->lse, p.B);
+                const na2d_prefix::JoinPrefix by_prefix{prefix.o, prefix.lse, (size_t)p.rows.all, prefix.count, p.rows.A, na2d_attn::Div(p.rows.A)};
+                return p.dtype == NA2D_BF16 ? na2d_prefix::tokens_bf16(at, x, by_prefix, a->o.ptr, a->lse, p.B)
+                                            : na2d_prefix::tokens_f16(at, x, by_prefix, a->o.ptr, a->lse, p.B);
             }
             const float *o_own = p.any_own ? floats(f.o_own) : nullptr, *lse_own = p.any_own ? floats(f.lse_own) : nullptr;
             return by_type(p, a->o.ptr, [&](auto type, auto n) {

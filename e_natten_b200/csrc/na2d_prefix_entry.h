@@ -31,8 +31,9 @@ struct Tokens {
     int* table;                         // steps before each entry, of all, and those of a warp
     float *part_o, *part_lse;
 };
-// Where a row's sums of one kind of keys come from: the line (count 0), or another kernel's results, (count, entries, N, share Tq).
-struct JoinSide {
+// Where a row's sums over the prefix come from: the line (count 0), or another kernel's results, (count, entries, N, share Tq).  (Own keys are
+// on the line in every call that has one.)
+struct JoinPrefix {
     const float *o, *lse;
     size_t stride;                      // rows from one to the next
     int count, share;
@@ -44,7 +45,7 @@ constexpr int kTokenRows = 32;
 // Warps of the line.
 inline int token_warps(int sms) { return sms * 8; }
 
-int tokens_bf16(const na2d_attn::Place& at, const Tokens& x, const JoinSide& prefix, const JoinSide& own, void* o, float* lse, int B);
-int tokens_f16(const na2d_attn::Place& at, const Tokens& x, const JoinSide& prefix, const JoinSide& own, void* o, float* lse, int B);
+int tokens_bf16(const na2d_attn::Place& at, const Tokens& x, const JoinPrefix& prefix, void* o, float* lse, int B);
+int tokens_f16(const na2d_attn::Place& at, const Tokens& x, const JoinPrefix& prefix, void* o, float* lse, int B);
 
 }  // namespace na2d_prefix

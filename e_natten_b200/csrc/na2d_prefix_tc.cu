@@ -35,13 +35,13 @@ int by_rows(const Place& at, const Tokens& x) {
 }
 }  // namespace
 
-int NA2D_TC_NAME(tokens)(const Place& at, const Tokens& x, const JoinSide& prefix, const JoinSide& own, void* o, float* lse, int B) {
+int NA2D_TC_NAME(tokens)(const Place& at, const Tokens& x, const JoinPrefix& prefix, void* o, float* lse, int B) {
     const int rc = x.C <= 32 ? by_rows<32>(at, x) : x.C <= 64 ? by_rows<64>(at, x) : by_rows<128>(at, x);
     if (rc != NA2D_OK) return rc;
     const long long rows = (long long)B * x.N * x.Tq;
     if (rows > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
     *at.launched += 1;
-    return na2d_launch::launch(true, prefix_join_kernel<NA2D_TC_TYPE>, (unsigned)rows, 128, 0, at.st, x, prefix, own, (NA2D_TC_TYPE*)o, lse) == cudaSuccess
+    return na2d_launch::launch(true, prefix_join_kernel<NA2D_TC_TYPE>, (unsigned)rows, 128, 0, at.st, x, prefix, (NA2D_TC_TYPE*)o, lse) == cudaSuccess
                ? NA2D_OK
                : NA2D_ERR_CUDA;
 }

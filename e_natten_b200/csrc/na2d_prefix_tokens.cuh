@@ -350,30 +350,32 @@ struct PartList {
     size_t first, stride;
     int count;
 };
-__device__ __forceinline__ PartList parts_of(const Tokens& x, const JoinSide& j, int which, int b, int n, int t) {
+template <bool OWN>
+__device__ __forceinline__ PartList parts_of(const Tokens& x, const JoinPrefix& j, int b, int n, int t) {
     PartList l{};
-    const TokenSide& s = x.side[which];
+    const TokenSide& s = x.side[OWN];
+    const int share = OWN ? 1 : j.share;
     int entry = b, a = 0;
-    if (j.share > 1) entry = j.by_share.split(b, a);
+    if (share > 1) entry = j.by_share.split(b, a);
     const size_t row = static_cast<size_t>(a) * x.Tq + t;
-    if (j.count > 0) {                                   // of another kernel: rows of (entries, N, share Tq)
+    if (!OWN && j.count > 0) {                           // of another kernel: rows of (entries, N, share Tq)
         l.o = j.o;
         l.lse = j.lse;
-        l.first = (static_cast<size_t>(entry) * x.N + n) * j.share * x.Tq + row;
+        l.first = (static_cast<size_t>(entry) * x.N + n) * share * x.Tq + row;
         l.stride = j.stride;
         l.count = j.count;
         return l;
     }
     if (s.entries == 0) return l;
     int h;
-    const int e = (which ? x.side[0].entries : 0) + entry, m = x.by_g.split(n, h), unit = entry * x.Nk + m;
+    const int e = (OWN ? x.side[0].entries : 0) + entry, m = x.by_g.split(n, h), unit = entry * x.Nk + m;
     const int E = x.side[0].entries + x.side[1].entries, each = x.table[E + 1], before = x.table[e], length = x.table[e + 1] - before;
     if (length == 0) return l;
     const int at = before * x.Nk + m * length, lo = (at + kUnitSteps) / each, hi = (at + length - 1) / each;       // warps with steps of it
     l.o = x.part_o;
     l.lse = x.part_lse;
     l.stride = s.rows;
-    l.first = s.first_row + static_cast<size_t>(lo + unit) * s.rows + static_cast<size_t>(h) * j.share * x.Tq + row;
+    l.first = s.first_row + static_cast<size_t>(lo + unit) * s.rows + static_cast<size_t>(h) * share * x.Tq + row;
     l.count = hi - lo + 1;
     return l;
 }
@@ -381,8 +383,8 @@ __device__ __forceinline__ PartList parts_of(const Tokens& x, const JoinSide& j,
 // lse = ln sum_s e^lse_s, o = sum_s e^(lse_s - lse) o_s over a row's parts of both sides.  A block a row: its warps share the parts, 4
 // channels a lane; where they lie and what they weigh, each lane of a warp works out for one of 32.
 template <typename DT>
-__global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Tokens x, const __grid_constant__ JoinSide prefix,
-                                                          const __grid_constant__ JoinSide own, DT* __restrict__ o, float* __restrict__ lse) {
+__global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Tokens x, const __grid_constant__ JoinPrefix prefix,
+                                                          DT* __restrict__ o, float* __restrict__ lse) {
     constexpr int W = 4;
     __shared__ float4 sums[W][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x, c = 4 * lane;
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
     const int b = x.by_n.split(x.by_tq.split(row, t), n);
     after_previous_grid();
     next_grid_may_start();
-    const PartList first = parts_of(x, prefix, 0, b, n, t), second = parts_of(x, own, 1, b, n, t);
+    const PartList first = parts_of<false>(x, prefix, b, n, t), second = parts_of<true>(x, prefix, b, n, t);
     const int parts = first.count + second.count;
     auto part = [&](int i, const float*& at) {           // lse of part i, and its o
         const PartList& l = i < first.count ? first : second;
