@@ -81,6 +81,6 @@ def beam_reorder(caches: Union[torch.Tensor, Sequence[torch.Tensor]], parents: t
     parents)`` are the new ones.)
 
     Several caches move one after the other in effect: one that is given twice moves twice.  All are checked
-    before one moves.  Up to 32 beams.  Not differentiable: what has a tangent is refused.
+    before one moves; parents and lengths that are among them are taken as they were.  Up to 32 beams.  Not differentiable: what has a tangent is refused.
     """
     torch_ext.beam_reorder([caches] if isinstance(caches, torch.Tensor) else list(caches), parents, lengths)

@@ -466,7 +466,15 @@ void reorder_in_place(at::TensorList caches, const Tensor& parents_in, const May
         check(abi.reorder(&a));
     }
 }
-void reorder(const std::vector<Tensor>& caches, const Tensor& parents, const MaybeTensor& lengths) {
+// x, or a copy of it where it lies in the storage of a cache, which moves while x is read.
+Tensor apart_from(const std::vector<Tensor>& caches, const Tensor& x) {
+    for (const Tensor& t : caches)
+        if (x.has_storage() && t.has_storage() && x.is_alias_of(t)) return x.clone();
+    return x;
+}
+void reorder(const std::vector<Tensor>& caches, const Tensor& parents_in, const MaybeTensor& lengths_in) {
+    const Tensor parents = apart_from(caches, parents_in);
+    const MaybeTensor lengths = lengths_in ? MaybeTensor(apart_from(caches, *lengths_in)) : lengths_in;
     TORCH_CHECK_VALUE(parents.is_cuda(), "parents: e_natten_b200 runs on CUDA tensors only (there is no CPU path)");
     // (a function mode sees no calls of the dispatcher, and the operator, a cache of its own and a copy back, costs several times as much)
     bool through = recorded() || any_special({parents, lengths.value_or(Tensor())});

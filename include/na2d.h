@@ -448,7 +448,7 @@ size_t na2d_beam_select_workspace(const na2d_beam_select_args* a);
 /* Caches that follow their beams: entry g K + i of each cache becomes what entry g K + parents[g][i] was, for all i of a group at once,
  * in place.
  *   cache        host array of `caches` caches of B K entries, of any type: (entries, heads, tokens) rows of row_bytes bytes, strides in
- *                bytes.  No two rows may share memory, within a cache or between them.
+ *                bytes.  No two rows may share memory, within a cache or between them, nor a row with parents or lengths.
  *   parents      (B, K), dense, int32 or (parents_64) int64.  One outside [0, K) leaves its entry as it is.
  *   lengths      (B K,), dense, int32 or (lengths_64) int64, or NULL: how many tokens an entry holds (clamped to [0, tokens]).  Only the
  *                parent's are copied; rows behind them stay as they are.

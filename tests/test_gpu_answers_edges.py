@@ -238,3 +238,23 @@ def test_beam_select_orders_worths_that_are_far_enough_apart():
         scores[kept[0]] = -math.inf
         kept = kept[1:]
         assert na.beam_select(x[None, :-4], scores[None, :-4], 1)[1][0, 0] == kept[0]
+
+
+@pytest.mark.parametrize("mode", [contextlib.nullcontext, Through])
+def test_beam_reorder_of_what_says_how(mode):
+    """Parents, or lengths, that are themselves among the caches: all move by what they were."""
+    B, K, T = 4, 8, 4000
+    for seed in range(5):
+        parents, cache = parents_of(B, K, seed), bits(B * K, 1, T, 9, dtype=torch.int32, seed=seed)
+        lengths = torch.randint(0, T + 1, (B * K,), generator=torch.Generator().manual_seed(seed)).to(DEV)
+        said = parents.view(-1)
+        want = [plain_reorder(t, parents.clone()) for t in (said, cache)]
+        with mode():
+            na.beam_reorder([said, cache], parents)
+        assert torch.equal(said, want[0]) and torch.equal(cache, want[1])
+        parents = parents_of(B, K, seed + 10)
+        held = lengths.view(-1, 1, 1, 1)
+        want = [plain_reorder(t, parents, lengths.clone()) for t in (held, cache)]
+        with mode():
+            na.beam_reorder([held, cache], parents, lengths)
+        assert torch.equal(held, want[0]) and torch.equal(cache, want[1])
