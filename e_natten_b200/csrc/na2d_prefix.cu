@@ -31,7 +31,7 @@ constexpr int kThreads = 256;
 // Rows of the whole batch: entry b = s A + a has prefix s.
 struct Rows {
     int A, N, Tq, C;
-    long long all;          // B N Tq, below 2^31
+    long long all;          // B N Tq, at most 2^31 - kThreads
     na2d_attn::Div by_a, by_n, by_tq;
 };
 struct Row {
@@ -185,7 +185,7 @@ int make_problem(const na2d_prefix_attention_args* a, Problem* p) {
     p->S = a->S;
     p->dtype = a->dtype;
     p->rows = Rows{A, a->N, a->Tq, a->C, (long long)a->B * a->N * a->Tq, na2d_attn::Div(A), na2d_attn::Div(a->N), na2d_attn::Div(a->Tq)};
-    if (p->rows.all > 0x7fffffffLL) return NA2D_ERR_TOO_LARGE;
+    if (p->rows.all > (1LL << 31) - kThreads) return NA2D_ERR_TOO_LARGE;         // (the last block's rows that are none are counted, too)
     auto geometry = [&](int B, int Tq, int Tk, bool causal, const int* lengths) {
         Geom g{};
         g.B = B; g.N = a->N; g.Nk = a->Nk; g.Tq = Tq; g.Tk = Tk; g.C = a->C;

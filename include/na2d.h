@@ -397,7 +397,7 @@ int na2d_rotary_table(const double* positions, const double* frequencies, int64_
  *   d_q; d_k and d_v; d_prefix_k and d_prefix_v: may be NULL.  The prefix's are sums over its entries.  Results dense.
  *   workspace       scratch, 256-byte aligned, at least na2d_prefix_attention_workspace bytes.  That is asked with the call's own sizes, path,
  *                   pointers and strides, results included: where operands lie decides which kernels run, and null results are not computed.
- *   B / S * Tq, P, Tk <= 2^29, B * N <= 2^24, else NA2D_ERR_TOO_LARGE.  P > 0.
+ *   B / S * Tq, P, Tk <= 2^29, B * N <= 2^24, B * N * Tq <= 2^31 - 256, else NA2D_ERR_TOO_LARGE.  P > 0.
  * Types, head dims, path, strides as in na2d_attention_args.  No atomics: the same call gives the same bits. */
 typedef struct na2d_prefix_attention_args {
     size_t struct_size;

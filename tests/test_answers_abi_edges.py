@@ -30,3 +30,12 @@ def test_prefix_attention_workspace_goes_by_where_operands_lie(backward):
         assert prefix(backward, **kw, workspace_bytes=room(**kw) - 1) == _lib.ERR_BAD_ARG
     less, more = sorted((shape, odd), key=lambda kw: room(**kw))
     assert prefix(backward, **more, workspace_bytes=room(**less)) == _lib.ERR_BAD_ARG
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_prefix_attention_counts_rows_of_whole_blocks_in_32_bits(backward):
+    """A block of the joins has up to 256 rows, the last one some beyond the last row."""
+    rows = lambda Tq, **kw: prefix(backward, B=4, S=4, N=1, Nk=1, Tq=Tq, Tk=0, P=1, C=3, k=_lib.Heads(0, 0, 0, 0), v=_lib.Heads(0, 0, 0, 0),
+                                   **(dict(d_k=_lib.Heads(0, 0, 0, 0), d_v=_lib.Heads(0, 0, 0, 0)) if backward else {}), workspace_bytes=1 << 60, **kw)
+    assert rows((1 << 29) - 1) == _lib.ERR_TOO_LARGE     # 2^31 - 4
+    assert rows((1 << 29) - 64) in GPU_WANTED            # 2^31 - 256
