@@ -6,7 +6,7 @@
 // of threads fall into different banks; neighbouring lanes are two rows of one column, because a warp's 16-byte loads are shared between
 // neighbours only (with 16 columns side by side each load took its full four turns: 1305 us against 1209).
 // What bounds it: the multiply-adds, and beside them the loads from shared memory.  Batch 4, 4 heads of 128, 1024 tokens, fp32, forward and
-// backward: 1130 us, 34 TFLOP/s over the nine products that are done (the seven that have to be: 406 us at the 74 TFLOP/s that 148 SMs of 128
+// backward: 1077 us, 36 TFLOP/s over the nine products that are done (the seven that have to be: 406 us at the 74 TFLOP/s that 148 SMs of 128
 // multiply-adds come to at 1965 MHz).
 #include "na2d_attn_entry.h"
 #include "na2d_vec.cuh"
@@ -536,7 +536,9 @@ int start(const Place& at, K kernel, const SimtPair& pair, int floats, std::atom
 
 // 128 query rows a block where blocks of 64 would take the SMs more than one round, and where that adds no more than an eighth of rows that are
 // none: a piece of 8 x 4 scores reads 12 operands from shared memory for its 32 products, one of 4 x 4 reads 8 for 16.  Forward and query
-// half with 256 blocks of 64: 277 and 417 us; with 128 of 128: 244 and 365 us.  Of 36 rows a head, blocks of 128 do twice the work.
+// half (with delta), fp32: 16 heads x 1024 x 128, 256 blocks of 64: 258 and 384 us, 128 of 128: 233 and 349.  18 x 16 x 36 rows x 64, of which blocks of
+// 128 do twice the work, 18 and 32 with 64, 29 and 40 with 128; 16 x 16 x 129 x 128 160 and 237 for 191 and 283.  (Where blocks of 128 are just half as
+// many the rule can lose: 64 x 8 x 65 x 32 57 and 79 us, 45 and 67 with blocks of 64.)
 template <int CP, typename F>
 int by_rows(const Place& at, const SimtPair& pair, F&& f) {
     if constexpr (CP <= 128) {

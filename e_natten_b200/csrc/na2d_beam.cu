@@ -7,7 +7,8 @@
 // those go to shared memory, where at the end each counts the better ones.  The bound is formed anew behind 1, 2, 4 ... chunks.
 // select_beams_kernel joins an entry's segments: sums in 64 bits, candidates by the same bound.  (value, lowest beam, lowest word) is a
 // total order, so nothing depends on the order in which candidates arrive.  What a block keeps has room for 512: where more words reach
-// the bound (equal ones, ascending ones) it looks for the best below the last one, `count` times over.
+// the bound (equal ones, ascending ones; all of 513 to 1792 in 16 bits, 513 to 896 in 32, which leave a warp without a word and the bound at
+// nothing) it looks for the best below the last one, `count` times over.
 // Measured: 64 x 8 x 131072 fp32, 268 MB: 55 us, 74 % of the copy bandwidth (the rows 53, issue slots 54 %); 7 x 5 x 100003 fp16, rows on odd
 // places, 15 us, of which the rows are 8 and the joining 6; 16 x 4 x 32768 bf16 10.6, the host's time of the call.
 //

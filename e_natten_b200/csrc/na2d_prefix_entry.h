@@ -8,7 +8,8 @@ namespace na2d_prefix {
 
 constexpr int kTokenEntries = 4096;     // prefixes and batch entries on the line, at most
 // Steps that a unit counts for beside those of its keys: its queries' way in and its sums' way out.  64 x 8 caches of 1 to 1024 keys behind a prefix of
-// 16384: 73.3 us with 1, 72.1 with 3, 72.6 with 6; 16 x 4 prefixes with 256 short caches 49.2, 47.7, 47.7.
+// 16384: 73.1 us with 1, 70.8 with 3, 71.3 with 6; 16 x 4 prefixes of up to 8192 with 256 short caches 48.7, 47.6, 47.6, of up to 32768 130.0,
+// 130.1, 136.0.
 constexpr int kUnitSteps = 3;
 
 // One kind of keys: prefixes, or the entries' own.
